@@ -46,7 +46,7 @@ _NP2DT = {
     np.dtype(np.uint16): K.DATA_TYPE_U16, np.dtype(np.int16): K.DATA_TYPE_S16,
     np.dtype(np.int32): K.DATA_TYPE_S32, np.dtype(np.uint32): K.DATA_TYPE_U32, np.dtype(np.float32): K.DATA_TYPE_F32,
     np.dtype(np.float64): K.DATA_TYPE_F64, np.dtype(np.float16): K.DATA_TYPE_F16,
-    np.dtype(np.complex64): K.DATA_TYPE_C64, np.dtype(np.complex128): K.DATA_TYPE_C128,
+    np.dtype(np.complex64): K.DATA_TYPE_C64, np.dtype(np.complex128): K.DATA_TYPE_C128, np.dtype(np.int64): K.DATA_TYPE_S64,
 }
 _DT2NP = {v: k for k, v in _NP2DT.items()}
 _NP2TORCH = {
@@ -54,8 +54,12 @@ _NP2TORCH = {
     np.dtype(np.int16): torch.int16, np.dtype(np.int32): torch.int32, np.dtype(np.uint32): torch.uint32,
     np.dtype(np.float32): torch.float32,
     np.dtype(np.float64): torch.float64, np.dtype(np.float16): torch.float16,
-    np.dtype(np.complex64): torch.complex64, np.dtype(np.complex128): torch.complex128,
+    np.dtype(np.complex64): torch.complex64, np.dtype(np.complex128): torch.complex128, np.dtype(np.int64): torch.int64,
 }
+# numpy has no such type: here and where a dtype is asked for, torch's stands for it
+_NP2DT[torch.bfloat16] = K.DATA_TYPE_BF16
+_DT2NP[K.DATA_TYPE_BF16] = torch.bfloat16
+_NP2TORCH[torch.bfloat16] = torch.bfloat16
 
 
 def stream_ptr(stream=None):
@@ -177,7 +181,7 @@ class Tensor(_Handle):
     @classmethod
     def from_torch(cls, t, layout):
         """Zero-copy view of a torch CUDA tensor."""
-        npdt = np.dtype(str(t.dtype).replace("torch.", ""))
+        npdt = t.dtype if t.dtype is torch.bfloat16 else np.dtype(str(t.dtype).replace("torch.", ""))
         es = t.element_size()
         return cls.wrap(t.data_ptr(), list(t.shape), [s * es for s in t.stride()], npdt, layout, keep=t)
 
@@ -210,6 +214,8 @@ class Tensor(_Handle):
     def __cuda_array_interface__(self):
         d = self.export()
         npdt = _DT2NP[d.dtype]
+        if npdt is torch.bfloat16:
+            raise TypeError("the array interface has no bfloat16")
         return {"shape": tuple(d.shape[i] for i in range(d.rank)), "typestr": npdt.str,
                 "data": (int(d.buffer.basePtr or 0), False),
                 "strides": tuple(d.buffer.strides[i] for i in range(d.rank)), "version": 3}
@@ -279,7 +285,7 @@ class Tensor(_Handle):
 def _as_dtype(dtype):
     if isinstance(dtype, int):
         return dtype
-    return _NP2DT[np.dtype(dtype)]
+    return K.DATA_TYPE_BF16 if dtype is torch.bfloat16 else _NP2DT[np.dtype(dtype)]
 
 
 class Image(_Handle):
@@ -569,3 +575,84 @@ class WarpPerspective(_Operator):
             m = (C.c_float * 9)(*[float(v) for v in xform])
             check(_cv.cvcudaWarpPerspectiveSubmit(self.handle, stream_ptr(stream), _h(inp), _h(out), m, flags,
                                                   border, bv))
+
+
+class LayerNorm(_Operator):
+    """Extension: cvcuda/LayerNorm.h. None stands for a tensor that is left out."""
+    _create = "cvcudaxLayerNormCreate"
+
+    def __call__(self, stream, inp, gamma, beta, out, mean=None, rstd=None, epsilon=1e-5):
+        check(_cv.cvcudaxLayerNormSubmit(self.handle, stream_ptr(stream), _h(inp), _h(gamma), _h(beta), _h(out), _h(mean),
+                                         _h(rstd), epsilon))
+
+
+class LayerNormGrad(_Operator):
+    """Extension: cvcuda/LayerNorm.h, the gradient."""
+    _create = "cvcudaxLayerNormCreate"
+
+    @staticmethod
+    def workspace(rows, columns):
+        """Bytes of workspace of a call."""
+        n = C.c_int64()
+        check(_cv.cvcudaxLayerNormGradWorkspace(rows, columns, C.byref(n)))
+        return n.value
+
+    def __call__(self, stream, grad, inp, gamma, mean, rstd, grad_in, grad_gamma, grad_beta, workspace=None):
+        check(_cv.cvcudaxLayerNormGradSubmit(self.handle, stream_ptr(stream), _h(grad), _h(inp), _h(gamma), _h(mean), _h(rstd),
+                                             _h(grad_in), _h(grad_gamma), _h(grad_beta), _h(workspace)))
+
+
+class Embedding(_Operator):
+    """Extension: cvcuda/Embedding.h."""
+    _create = "cvcudaxEmbeddingCreate"
+
+    def __call__(self, stream, table, tokens, out, scale=1.0):
+        check(_cv.cvcudaxEmbeddingSubmit(self.handle, stream_ptr(stream), _h(table), _h(tokens), _h(out), scale))
+
+
+class EmbeddingGrad(_Operator):
+    """Extension: cvcuda/Embedding.h, the gradient. padding: a token, or -1 for none."""
+    _create = "cvcudaxEmbeddingCreate"
+
+    @staticmethod
+    def workspace(tokens, vocabulary, columns):
+        """Bytes of workspace of a call."""
+        n = C.c_int64()
+        check(_cv.cvcudaxEmbeddingGradWorkspace(tokens, vocabulary, columns, C.byref(n)))
+        return n.value
+
+    def __call__(self, stream, grad, tokens, grad_table, workspace=None, scale=1.0, padding=-1, accumulate=False):
+        check(_cv.cvcudaxEmbeddingGradSubmit(self.handle, stream_ptr(stream), _h(grad), _h(tokens), _h(grad_table), _h(workspace),
+                                             scale, padding, accumulate))
+
+
+def _handles(tensors, count):
+    """The handles of a list of tensors (None: no list; in it, no tensor)."""
+    if tensors is None:
+        return None
+    if len(tensors) != count:
+        raise ValueError("lists of %d and %d tensors" % (count, len(tensors)))
+    return (C.c_void_p * count)(*[_h(t) for t in tensors])
+
+
+class AdamW(_Operator):
+    """Extension: cvcuda/AdamW.h, over lists of tensors."""
+    _create = "cvcudaxAdamWCreate"
+
+    def __call__(self, stream, params, moments, variances, grads, copies, moment_scales, variance_scales, grad_scale, step, lr,
+                 beta1, beta2, epsilon, weight_decay):
+        n = len(params)
+        args = capi.AdamWArgs(lr, beta1, beta2, epsilon, weight_decay, step)
+        check(_cv.cvcudaxAdamWSubmit(self.handle, stream_ptr(stream), n, _handles(params, n), _handles(moments, n),
+                                     _handles(variances, n), _handles(grads, n), _handles(copies, n), _handles(moment_scales, n),
+                                     _handles(variance_scales, n), _h(grad_scale), C.byref(args)))
+
+
+class AdamWUnpack(_Operator):
+    """Extension: cvcuda/AdamW.h, the values of 8-bit states."""
+    _create = "cvcudaxAdamWCreate"
+
+    def __call__(self, stream, codes, scales, out):
+        n = len(codes)
+        check(_cv.cvcudaxAdamWUnpackSubmit(self.handle, stream_ptr(stream), n, _handles(codes, n), _handles(scales, n),
+                                           _handles(out, n)))

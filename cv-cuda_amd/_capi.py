@@ -357,3 +357,22 @@ declare_optional("cvcudaWarpAffineVarShapeSubmit", ST, H, C.c_void_p, H, H, H, C
 declare_optional("cvcudaWarpPerspectiveCreate", ST, P(H), C.c_int32)
 declare_optional("cvcudaWarpPerspectiveSubmit", ST, H, C.c_void_p, H, H, P(C.c_float), C.c_int32, C.c_int, Float4)
 declare_optional("cvcudaWarpPerspectiveVarShapeSubmit", ST, H, C.c_void_p, H, H, H, C.c_int32, C.c_int, Float4)
+
+
+class AdamWArgs(C.Structure):
+    """CVCUDAXAdamW (cvcuda/AdamW.h, extension)."""
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("epsilon", C.c_double),
+                ("weightDecay", C.c_double), ("step", C.c_int64)]
+
+
+_sig(cvcuda, "cvcudaxLayerNormCreate", ST, P(H))
+_sig(cvcuda, "cvcudaxLayerNormSubmit", ST, H, C.c_void_p, H, H, H, H, H, H, C.c_float)
+_sig(cvcuda, "cvcudaxLayerNormGradWorkspace", ST, C.c_int64, C.c_int64, P(C.c_int64))
+_sig(cvcuda, "cvcudaxLayerNormGradSubmit", ST, H, C.c_void_p, H, H, H, H, H, H, H, H, H)
+_sig(cvcuda, "cvcudaxEmbeddingCreate", ST, P(H))
+_sig(cvcuda, "cvcudaxEmbeddingSubmit", ST, H, C.c_void_p, H, H, H, C.c_float)
+_sig(cvcuda, "cvcudaxEmbeddingGradWorkspace", ST, C.c_int64, C.c_int64, C.c_int64, P(C.c_int64))
+_sig(cvcuda, "cvcudaxEmbeddingGradSubmit", ST, H, C.c_void_p, H, H, H, H, C.c_float, C.c_int64, C.c_int8)
+_sig(cvcuda, "cvcudaxAdamWCreate", ST, P(H))
+_sig(cvcuda, "cvcudaxAdamWSubmit", ST, H, C.c_void_p, C.c_int32, P(H), P(H), P(H), P(H), P(H), P(H), P(H), H, P(AdamWArgs))
+_sig(cvcuda, "cvcudaxAdamWUnpackSubmit", ST, H, C.c_void_p, C.c_int32, P(H), P(H), P(H))

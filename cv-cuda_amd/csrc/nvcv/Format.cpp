@@ -1000,6 +1000,7 @@ const char *nvcvDataTypeGetName(NVCVDataType type)
         T(2F16), T(3F16), T(4F16), T(F32), T(2F32), T(3F32), T(4F32), T(U64), T(2U64), T(3U64), T(4U64), T(S64), T(2S64),
         T(3S64), T(4S64), T(F64), T(2F64), T(3F64), T(4F64), T(C64), T(2C64), T(3C64), T(4C64), T(C128), T(2C128),
 #undef T
+        {NVCVX_DATA_TYPE_BF16, "NVCVX_DATA_TYPE_BF16"},
     };
     for (const auto &k : known)
     {

@@ -27,8 +27,9 @@ def main():
     src = ['#define CVCUDA_NO_HIP_HEADERS', '#include <stdio.h>', '#include <nvcv/Tensor.h>',
            '#include <nvcv/BorderType.h>', '#include <cvcuda/Types.h>', '#include <cvcuda/OpNormalize.h>',
            'int main(void){']
+    dts += names("nvcv/DataType.h", r"^#define (NVCVX_DATA_TYPE_\w+) ")
     for n in fmts + dts:
-        src.append('printf("%s = 0x%%016llx\\n", (unsigned long long)(%s));' % (n[5:], n))
+        src.append('printf("%s = 0x%%016llx\\n", (unsigned long long)(%s));' % (n.split("_", 1)[1], n))
     for n in enums + ["CVCUDA_NORMALIZE_SCALE_IS_STDDEV"]:
         short = n[5:] if n.startswith("NVCV_") else n
         src.append('printf("%s = %%lld\\n", (long long)(%s));' % (short, n))

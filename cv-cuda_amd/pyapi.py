@@ -25,8 +25,9 @@ import numpy as np
 import torch
 
 from . import _constants as K
-from . import (CenterCrop, ConvertTo, CropFlipNormalizeReformat, CustomCrop, CvtColor, Error, Flip, Normalize, Reformat,
-               Resize, ResizeCropConvertReformat, WarpAffine, WarpPerspective)
+from . import (AdamW, AdamWUnpack, CenterCrop, ConvertTo, CropFlipNormalizeReformat, CustomCrop, CvtColor, Embedding, EmbeddingGrad,
+               Error, Flip, LayerNorm, LayerNormGrad, Normalize, Reformat, Resize, ResizeCropConvertReformat, WarpAffine,
+               WarpPerspective)
 from . import Image as _Image
 from . import ImageBatchVarShape as _ImageBatchVarShape
 from . import Tensor as _Tensor
@@ -270,6 +271,8 @@ def _np_dtype(dtype):
         if int(dtype) not in _DT2NP:
             raise ValueError("data type 0x%x has no array element type" % int(dtype))
         return _DT2NP[int(dtype)]
+    if dtype is torch.bfloat16:
+        return dtype
     if isinstance(dtype, torch.dtype):
         return np.dtype(str(dtype).replace("torch.", ""))
     return np.dtype(dtype)
@@ -426,6 +429,8 @@ def clear_cache():
 def _result(shape, dtype, layout, stream):
     """A tensor for an operator's result. Only a call on the default stream takes one that is handed out again: another
     stream would have to wait for the default stream's last use of it, which one that is being captured cannot."""
+    if dtype is torch.bfloat16:
+        return Tensor(tuple(shape), dtype, layout)
     key = _native_stream_key() if stream is None else None
     if key is None and _default_stream_key(stream) is None:
         return Tensor(tuple(shape), dtype, layout)
@@ -1107,3 +1112,109 @@ def crop_flip_normalize_reformat(src, out_shape, out_dtype, out_layout, rect, fl
     dst = _result(out_shape, _np_dtype(out_dtype), out_layout, stream)
     return crop_flip_normalize_reformat_into(dst, src, rect, flip_code, base, scale, globalscale, globalshift, epsilon,
                                              flags, border, bvalue, stream=stream)
+
+
+# ---- rows of values: extensions, behind the image batches ------------------------------------------------------------
+def _given(*tensors):
+    return [t for t in tensors if t is not None]
+
+
+def _workspace(workspace, size, stream):
+    """The caller's workspace, or one for this call alone (None where none is needed)."""
+    return workspace if workspace is not None or size == 0 else _result((size,), np.uint8, None, stream)
+
+
+def _rows_of(tensor):
+    """(rows, elements in a row)"""
+    shape = tensor.shape
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    return rows, shape[-1]
+
+
+def layer_norm_into(dst, src, gamma=None, beta=None, epsilon=1e-5, *, mean=None, rstd=None, stream=None):
+    """Layer norm of the rows (last dimension) of `src`: F32, F16 or BF16, with weights of that type or F32 (none: 1 and 0).
+    `mean` and `rstd`: F32 tensors of an element per row that receive what the gradient needs. `dst` may be `src`."""
+    _run(stream, _given(src, gamma, beta), _given(dst, mean, rstd), _op(LayerNorm), src, gamma, beta, dst, mean, rstd, float(epsilon))
+    return dst
+
+
+def layer_norm(src, gamma=None, beta=None, epsilon=1e-5, *, mean=None, rstd=None, stream=None):
+    return layer_norm_into(_like(src, stream), src, gamma, beta, epsilon, mean=mean, rstd=rstd, stream=stream)
+
+
+def layer_norm_grad_into(grad_src, grad_gamma, grad_beta, grad, src, gamma, mean, rstd, *, workspace=None, stream=None):
+    """The gradients of layer_norm from `grad`, that of its result; `mean` and `rstd` as the forward call gave them.
+    `grad_gamma`, `grad_beta` and `gamma` may be None. `grad_src` may be `grad` or `src`."""
+    sums = grad_gamma is not None or grad_beta is not None
+    workspace = _workspace(workspace, LayerNormGrad.workspace(*_rows_of(src)) if sums else 0, stream)
+    _run(stream, _given(grad, src, gamma, mean, rstd), _given(grad_src, grad_gamma, grad_beta, workspace), _op(LayerNormGrad), grad, src,
+         gamma, mean, rstd, grad_src, grad_gamma, grad_beta, workspace)
+    return grad_src, grad_gamma, grad_beta
+
+
+def layer_norm_grad(grad, src, gamma, mean, rstd, *, stream=None):
+    """(gradient of src, of gamma, of beta); the latter have gamma's type, F32 without one."""
+    kind = np.dtype(np.float32) if gamma is None else gamma.dtype
+    made = [_result((src.shape[-1],), kind, None, stream) for _ in range(2)]
+    return layer_norm_grad_into(_like(src, stream), made[0], made[1], grad, src, gamma, mean, rstd, stream=stream)
+
+
+def embedding_into(dst, table, tokens, scale=1.0, *, stream=None):
+    """dst[i] = scale * table[tokens[i]]: rows of a table by tokens (int32 or int64); zeros for tokens that it does not have.
+    `dst` has the table's type, or F16 or BF16 beside a table of F32."""
+    _run(stream, [table, tokens], [dst], _op(Embedding), table, tokens, dst, float(scale))
+    return dst
+
+
+def embedding(table, tokens, scale=1.0, *, dtype=None, stream=None):
+    """The rows as a tensor of the tokens' shape and a row's elements, of `dtype` (none: the table's)."""
+    dst = _result(tuple(tokens.shape) + (table.shape[-1],), table.dtype if dtype is None else _np_dtype(dtype), None, stream)
+    return embedding_into(dst, table, tokens, scale, stream=stream)
+
+
+def embedding_grad_into(grad_table, grad, tokens, scale=1.0, *, padding=None, accumulate=False, workspace=None, stream=None):
+    """The gradient of embedding's table from `grad`, that of its result, in `grad`'s type or F32: written whole, or with
+    `accumulate` added to what `grad_table` holds. Tokens equal to `padding` have no part in it."""
+    if padding is not None and padding < 0:
+        raise ValueError("padding is a token, or None")
+    rows, columns = _rows_of(grad)
+    workspace = _workspace(workspace, EmbeddingGrad.workspace(rows, _rows_of(grad_table)[0], columns), stream)
+    reads, writes = [grad, tokens], _given(grad_table, workspace)
+    _run(stream, reads, writes, _op(EmbeddingGrad), grad, tokens, grad_table, workspace, float(scale), -1 if padding is None else int(padding),
+         bool(accumulate))
+    return grad_table
+
+
+def embedding_grad(grad, tokens, rows, scale=1.0, *, padding=None, dtype=None, stream=None):
+    """The gradient of a table of `rows` rows, of `dtype` (none: grad's)."""
+    dst = _result((int(rows), grad.shape[-1]), grad.dtype if dtype is None else _np_dtype(dtype), None, stream)
+    return embedding_grad_into(dst, grad, tokens, scale, padding=padding, stream=stream)
+
+
+def adamw_into(params, moments, variances, grads, step, lr=1e-3, betas=(0.9, 0.999), epsilon=1e-8, weight_decay=1e-2, *, copies=None,
+               moment_scales=None, variance_scales=None, grad_scale=None, stream=None):
+    """One step of AdamW over lists of dense tensors: `params` (F32, F16 or BF16) and their states are updated, `step` is 1 for
+    the first. States are F32, or in 8 bits: int8 moments and uint8 variances with F32 scales of an element for each 256.
+    `copies`: tensors of F16 or BF16 that receive the new params (None in the list: no copy of that one). `grad_scale`: an F32
+    tensor of one element that the gradients are multiplied with. What is computed exactly: cvcuda/AdamW.h."""
+    lists = [params, moments, variances, grads, copies, moment_scales, variance_scales]
+    for part in lists[1:]:
+        if part is not None and len(part) != len(params):
+            raise ValueError("lists of %d and %d tensors" % (len(params), len(part)))
+    writes = [t for part in (params, moments, variances, copies, moment_scales, variance_scales) if part is not None for t in part
+              if t is not None]
+    raw = [None if part is None else [t if t is None else t._t for t in part] for part in lists]
+    _run(stream, list(grads) + _given(grad_scale), writes, _op(AdamW), *raw, grad_scale, int(step), float(lr), float(betas[0]),
+         float(betas[1]), float(epsilon), float(weight_decay))
+    return params
+
+
+def adamw_unpack_into(dst, codes, scales, *, stream=None):
+    """The F32 values that 8-bit states stand for, over lists of tensors: moments (int8) or variances (uint8)."""
+    if not len(dst) == len(codes) == len(scales):
+        raise ValueError("lists of %d, %d and %d tensors" % (len(dst), len(codes), len(scales)))
+    _run(stream, list(codes) + list(scales), list(dst), _op(AdamWUnpack), [t._t for t in codes], [t._t for t in scales],
+         [t._t for t in dst])
+    return dst

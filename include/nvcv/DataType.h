@@ -80,6 +80,11 @@ typedef uint64_t NVCVDataType;
 #define NVCV_DATA_TYPE_C128   NVCV_DETAIL_DATA_TYPE(COMPLEX, X128)
 #define NVCV_DATA_TYPE_2C128  NVCV_DETAIL_DATA_TYPE(COMPLEX, X128_Y128)
 
+/* Extension (no counterpart in the reference): the upper 16 bits of a float32, which the row operators (cvcuda/LayerNorm.h,
+ * Embedding.h, AdamW.h) take beside F16. A data kind of its own: every operator on images refuses it. */
+#define NVCVX_DATA_KIND_BFLOAT 4
+#define NVCVX_DATA_TYPE_BF16   NVCV_DETAIL_MAKE_DATA_TYPE(NVCVX_DATA_KIND_BFLOAT, NVCV_PACKING_X16)
+
 NVCV_PUBLIC NVCVStatus nvcvMakeDataType(NVCVDataType *outDataType, NVCVDataKind dataKind, NVCVPacking packing);
 NVCV_PUBLIC NVCVStatus nvcvDataTypeGetPacking(NVCVDataType type, NVCVPacking *outPacking);
 NVCV_PUBLIC NVCVStatus nvcvDataTypeGetBitsPerPixel(NVCVDataType type, int32_t *outBPP);
