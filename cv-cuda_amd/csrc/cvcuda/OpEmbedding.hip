@@ -19,16 +19,6 @@ struct LookupArgs
     float       scale;
 };
 
-struct GradArgs
-{
-    RowPlaces   grad, table;
-    const void *tokens;
-    int32_t     wide, accumulate;
-    int32_t     count, vocabulary, columns;
-    int64_t     padding;
-    float       scale;
-};
-
 __device__ __forceinline__ int64_t TokenAt(const void *tokens, int wide, int64_t i)
 {
     return wide ? static_cast<const int64_t *>(tokens)[i] : static_cast<const int32_t *>(tokens)[i];
@@ -51,52 +41,540 @@ __global__ __launch_bounds__(256) void EmbeddingKernel(const LookupArgs a)
     }
 }
 
-// A workgroup per row of the table and 256 columns looks through all tokens and adds the rows of its own in their order.
-template<class T, class O>
-__global__ __launch_bounds__(256) void EmbeddingGradKernel(const GradArgs a)
+// ---- gradient: tokens in order ---------------------------------------------------------------------------------------
+// The positions of equal tokens have to stand together, in their order. Tokens become keys (one that has no part in the
+// gradient the key V, behind all others), and (key, position) are sorted by digits from the lowest up, each pass stable: the
+// place of an element is the number of those with a smaller digit, and of those before it with the same one. Within a wave that
+// number comes from the lanes that share the digit: a ballot for each bit of it.
+struct TokenSource
 {
-    __shared__ uint64_t found[4];
-    const uint32_t      tiles = (a.columns + 255) / 256;
-    for (uint64_t k = blockIdx.x; k < (uint64_t)a.vocabulary * tiles; k += gridDim.x)
+    const void *tokens;
+    int32_t     wide, count, vocabulary;
+    int64_t     padding;
+
+    __device__ __forceinline__ uint32_t key(uint32_t i) const
     {
-        const int64_t       v = k / tiles;
-        const int           c = (int)(k % tiles) * 256 + threadIdx.x;
-        float               s = 0;
-        bool                any = false;
-        for (int first = 0; first < a.count && v != a.padding; first += 256)
+        if (i >= (uint32_t)count)
         {
-            const int      i    = first + threadIdx.x;
-            const uint64_t mine = __ballot(i < a.count && TokenAt(a.tokens, a.wide, i) == v);
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0)
-            {
-                found[threadIdx.x >> 6] = mine;
-            }
-            __syncthreads();
-            for (int w = 0; w < 4; ++w)
-            {
-                for (uint64_t f = found[w]; f != 0; f &= f - 1)
-                {
-                    any = true;
-                    s += c < a.columns ? (float)reinterpret_cast<const T *>(a.grad.at(first + 64 * w + __ffsll((unsigned long long)f) - 1))[c] : 0.f;
-                }
-            }
+            return vocabulary;
         }
-        O *out = reinterpret_cast<O *>(a.table.at((uint32_t)v));
-        if (c < a.columns && (any || !a.accumulate))
+        const int64_t t = TokenAt(tokens, wide, i);
+        return t >= 0 && t < vocabulary && t != padding ? (uint32_t)t : (uint32_t)vocabulary;
+    }
+};
+
+// The lanes of the wave whose digit of BITS bits is this lane's.
+template<int BITS>
+__device__ __forceinline__ uint64_t LanesOfDigit(uint32_t digit)
+{
+    uint64_t same = ~0ull;
+#pragma unroll
+    for (int b = 0; b < BITS; ++b)
+    {
+        const bool     set = (digit >> b) & 1;
+        const uint64_t on  = __ballot(set);
+        same &= set ? on : ~on;
+    }
+    return same;
+}
+
+__device__ __forceinline__ int LanesBefore(uint64_t lanes)
+{
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+}
+
+// Counts this lane's digit in its wave's counters and gives the number of those before it. (the wave's lanes go through here
+// together and LDS serves a wave in order: all read before one of each digit writes)
+template<int BITS>
+__device__ __forceinline__ uint32_t CountDigit(volatile uint32_t *counters, uint32_t digit)
+{
+    const uint64_t same   = LanesOfDigit<BITS>(digit);
+    const int      before = LanesBefore(same);
+    const uint32_t had    = counters[digit];
+    __builtin_amdgcn_wave_barrier();
+    if (before == 0)
+    {
+        counters[digit] = had + (uint32_t)__popcll(same);
+    }
+    __builtin_amdgcn_wave_barrier();
+    return had + before;
+}
+
+// Inclusive sum over the lanes before and this one.
+__device__ __forceinline__ uint32_t WaveScan(uint32_t v)
+{
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1)
+    {
+        const uint32_t o = __shfl_up(v, s);
+        v += (int)(threadIdx.x & 63) >= s ? o : 0;
+    }
+    return v;
+}
+
+constexpr int kSmallThreads = 1024, kSmallBits = 6;
+constexpr int kMostSmall    = 16 * kSmallThreads; // 64 KiB of keys and 32 of positions in LDS
+
+// All of up to K * 1024 tokens by one workgroup, in LDS. A wave owns 64 K consecutive elements; 16 waves with 64 digits
+// each have a counter per thread.
+template<int K>
+__global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const TokenSource src, uint32_t *keys, uint32_t *places, int bits)
+{
+    __shared__ uint32_t s_key[K * kSmallThreads];
+    __shared__ uint16_t s_place[K * kSmallThreads];
+    __shared__ uint32_t s_count[16][1 << kSmallBits];
+    __shared__ uint32_t s_sum[16];
+    const uint32_t      wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = wave * 64 * K + lane;
+    uint32_t            key[K], place[K], rank[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+    {
+        place[k] = first + 64 * k;
+        key[k]   = src.key(place[k]);
+    }
+    for (int shift = 0; shift < bits; shift += kSmallBits)
+    {
+        s_count[wave][lane] = 0; // (a wave's own)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < K; ++k)
         {
-            out[c] = FromFloat<O>(a.accumulate ? (float)out[c] + s * a.scale : s * a.scale);
+            rank[k] = CountDigit<kSmallBits>(s_count[wave], (key[k] >> shift) & 63);
+        }
+        __syncthreads();
+        // what comes before each counter, by digit and then by wave: thread t holds digit t / 16 of wave t % 16
+        const uint32_t mine = s_count[threadIdx.x & 15][threadIdx.x >> 4], upTo = WaveScan(mine);
+        if (lane == 63)
+        {
+            s_sum[wave] = upTo;
+        }
+        __syncthreads();
+        uint32_t base = upTo - mine;
+        for (uint32_t w = 0; w < wave; ++w)
+        {
+            base += s_sum[w];
+        }
+        s_count[threadIdx.x & 15][threadIdx.x >> 4] = base;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            const uint32_t to = s_count[wave][(key[k] >> shift) & 63] + rank[k];
+            s_key[to]         = key[k];
+            s_place[to]       = (uint16_t)place[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            key[k]   = s_key[first + 64 * k];
+            place[k] = s_place[first + 64 * k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+    {
+        if (first + 64 * k < (uint32_t)src.count)
+        {
+            keys[first + 64 * k]   = key[k];
+            places[first + 64 * k] = place[k];
         }
     }
 }
 
+// More tokens: tiles of them, two launches for each digit. The first counts the digits of each tile, the second adds up what
+// comes before each digit of its tile and puts the tile's elements there.
+constexpr int kTileThreads = 512, kTileKeys = 8, kTile = kTileThreads * kTileKeys, kTileBits = 9, kDigits = 1 << kTileBits;
+
+struct TileArgs
+{
+    TokenSource     src;
+    const uint32_t *keys, *places; // nullptr: the tokens themselves, at their places
+    uint32_t       *toKeys, *toPlaces;
+    uint32_t       *counts; // [kDigits][tiles]
+    int32_t         tiles, shift;
+
+    __device__ __forceinline__ uint32_t key(uint32_t i) const
+    {
+        return keys == nullptr ? src.key(i) : i < (uint32_t)src.count ? keys[i] : (uint32_t)src.vocabulary;
+    }
+};
+
+__global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileArgs a)
+{
+    __shared__ uint32_t s_count[kDigits];
+    s_count[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTileKeys; ++k)
+    {
+        const uint32_t i = blockIdx.x * kTile + k * kTileThreads + threadIdx.x;
+        if (i < (uint32_t)a.src.count)
+        {
+            atomicAdd(&s_count[(a.key(i) >> a.shift) & (kDigits - 1)], 1u);
+        }
+    }
+    __syncthreads();
+    a.counts[(size_t)threadIdx.x * a.tiles + blockIdx.x] = s_count[threadIdx.x];
+}
+
+__global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileArgs a)
+{
+    constexpr int       kWaves = kTileThreads / 64;
+    __shared__ uint32_t s_count[kWaves][kDigits];
+    __shared__ uint32_t s_sum[kWaves];
+    const uint32_t      wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = blockIdx.x * kTile + wave * 64 * kTileKeys + lane;
+    uint32_t            key[kTileKeys], place[kTileKeys], rank[kTileKeys];
+#pragma unroll
+    for (int k = 0; k < kTileKeys; ++k)
+    {
+        const uint32_t i = first + 64 * k;
+        key[k]           = a.key(i);
+        place[k]         = a.keys == nullptr ? i : i < (uint32_t)a.src.count ? a.places[i] : 0;
+    }
+    for (int w = 0; w < kWaves; ++w)
+    {
+        s_count[w][threadIdx.x] = 0;
+    }
+    // thread d: the elements of digit d before this tile, and all of them
+    uint32_t before = 0, all = 0;
+    for (int t = 0; t < a.tiles; ++t)
+    {
+        const uint32_t c = a.counts[(size_t)threadIdx.x * a.tiles + t];
+        before += t < (int)blockIdx.x ? c : 0;
+        all += c;
+    }
+    const uint32_t upTo = WaveScan(all);
+    if (lane == 63)
+    {
+        s_sum[wave] = upTo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTileKeys; ++k)
+    {
+        // (past the last token: the highest digit, behind all others of the last tile)
+        const uint32_t digit = first + 64 * k < (uint32_t)a.src.count ? (key[k] >> a.shift) & (kDigits - 1) : kDigits - 1;
+        rank[k]              = CountDigit<kTileBits>(s_count[wave], digit);
+    }
+    uint32_t base = before + upTo - all;
+    for (uint32_t w = 0; w < wave; ++w)
+    {
+        base += s_sum[w];
+    }
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w)
+    {
+        const uint32_t c        = s_count[w][threadIdx.x];
+        s_count[w][threadIdx.x] = base;
+        base += c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTileKeys; ++k)
+    {
+        if (first + 64 * k < (uint32_t)a.src.count)
+        {
+            const uint32_t to = s_count[wave][(key[k] >> a.shift) & (kDigits - 1)] + rank[k];
+            a.toKeys[to]      = key[k];
+            a.toPlaces[to]    = place[k];
+        }
+    }
+}
+
+// ---- gradient: sums ----------------------------------------------------------------------------------------------------
+// The sorted positions are cut into pieces of kPiece, whatever their tokens: every wave adds up the same number of rows, of 64
+// lanes' columns. A token whose positions lie within a piece is done there; of one that reaches over a piece's end each
+// piece leaves a sum of its own in the workspace, and a second launch adds these up in their order. Rows of the table that no
+// token names are cleared beside that by waves that look for their keys among the sorted ones.
+constexpr int kPiece = 32;
+
+struct SumArgs
+{
+    RowPlaces       grad, table;
+    const uint32_t *keys, *places;
+    float          *partial; // [pieces][2][columns]: of the token that began before the piece, of the one that goes on behind it
+    int32_t         count, vocabulary, columns, accumulate;
+    uint32_t        pieces, columnTiles, joinTiles, sumGroups, clearGroups;
+    float           scale;
+};
+
+constexpr int kClearRows = 16; // of a wave
+
+// The first place among `n` sorted keys that holds `key` or more.
+__device__ __forceinline__ uint32_t FirstOf(const uint32_t *keys, uint32_t n, uint32_t key)
+{
+    uint32_t lo = 0; // keys before it are less
+    uint32_t len = n;
+    while (len > 0)
+    {
+        // 64 places of the rest at once
+        const uint32_t step = (len + 63) / 64, at = lo + (threadIdx.x & 63) * step;
+        const uint64_t less = __ballot(at < lo + len && keys[at] < key);
+        const uint32_t k    = (uint32_t)__popcll(less);
+        if (k == 0)
+        {
+            break;
+        }
+        const uint32_t end = min(lo + len, lo + k * step);
+        lo += (k - 1) * step + 1;
+        len = end - lo;
+    }
+    return lo;
+}
+
+template<class O, int N>
+__device__ __forceinline__ void PutRun(O *row, int c, int columns, const float (&s)[N], float scale, bool accumulate)
+{
+    if (c + N <= columns)
+    {
+        Run<O, N> *to = reinterpret_cast<Run<O, N> *>(row + c);
+        Run<O, N>  r;
+        if (accumulate)
+        {
+            r = *to;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            r.v[i] = FromFloat<O>(accumulate ? (float)r.v[i] + s[i] * scale : s[i] * scale);
+        }
+        *to = r;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+        if (c + i < columns)
+        {
+            row[c + i] = FromFloat<O>(accumulate ? (float)row[c + i] + s[i] * scale : s[i] * scale);
+        }
+    }
+}
+
+template<class T, int N>
+__device__ __forceinline__ void GetRun(const T *row, int c, int columns, T (&v)[N])
+{
+    if (c + N <= columns)
+    {
+        const Run<T, N> r = *reinterpret_cast<const Run<T, N> *>(row + c);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            v[i] = r.v[i];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+        v[i] = c + i < columns ? row[c + i] : (T)0.f;
+    }
+}
+
+template<class O>
+__device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
+{
+    const uint32_t lane = threadIdx.x & 63, row0 = wave * kClearRows, rows = min((uint32_t)kClearRows, (uint32_t)a.vocabulary - row0);
+    uint32_t       named = 0;
+    for (uint32_t at = FirstOf(a.keys, a.count, row0);; at += 64)
+    {
+        const uint32_t key  = at + lane < (uint32_t)a.count ? a.keys[at + lane] : 0xFFFFFFFFu;
+        const bool     here = key < row0 + rows;
+#pragma unroll
+        for (uint32_t r = 0; r < kClearRows; ++r)
+        {
+            named |= __ballot(here && key == row0 + r) != 0 ? 1u << r : 0;
+        }
+        if (__ballot(here) != ~0ull)
+        {
+            break;
+        }
+    }
+    constexpr int N = kRunOf<O>;
+    const float   zeros[N] = {};
+    for (uint32_t r = 0; r < rows; ++r)
+    {
+        if (!((named >> r) & 1))
+        {
+            O *row = reinterpret_cast<O *>(a.table.at(row0 + r));
+            for (int c = lane * N; c < a.columns; c += 64 * N)
+            {
+                PutRun<O, N>(row, c, a.columns, zeros, 0.f, false);
+            }
+        }
+    }
+}
+
+template<class T, class O>
+__device__ __forceinline__ void SumPiece(const SumArgs &a, uint32_t piece, uint32_t tile)
+{
+    constexpr int  N    = kRunOf<T>;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t first = piece * kPiece, many = min((uint32_t)kPiece, (uint32_t)a.count - first);
+    const int      c     = (int)(tile * 64 + lane) * N;
+    // lane k: the piece's k-th key and place; the keys before and behind the piece
+    const uint32_t myKey   = lane < many ? a.keys[first + lane] : 0;
+    const uint32_t myPlace = lane < many ? a.places[first + lane] : 0;
+    const uint32_t before  = first > 0 ? a.keys[first - 1] : 0xFFFFFFFFu;
+    const uint32_t behind  = first + many < (uint32_t)a.count ? a.keys[first + many] : 0xFFFFFFFFu;
+    float          s[N]    = {};
+    constexpr int  kAhead  = 4; // rows on their way
+    T              row[kAhead][N];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+    {
+        if ((uint32_t)k < many)
+        {
+            GetRun<T, N>(reinterpret_cast<const T *>(a.grad.at(__builtin_amdgcn_readlane(myPlace, k))), c, a.columns, row[k]);
+        }
+    }
+    bool open = (uint32_t)__builtin_amdgcn_readlane(myKey, 0) == before; // the sum began in an earlier piece
+    for (uint32_t k0 = 0; k0 < many; k0 += kAhead)
+    {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+        {
+            const uint32_t k = k0 + j;
+            if (k >= many)
+            {
+                break;
+            }
+            const uint32_t key = __builtin_amdgcn_readlane(myKey, k);
+            if (key == (uint32_t)a.vocabulary)
+            {
+                return; // all others are behind the last row's
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                s[i] += (float)row[j][i];
+            }
+            if (k + kAhead < many)
+            {
+                GetRun<T, N>(reinterpret_cast<const T *>(a.grad.at(__builtin_amdgcn_readlane(myPlace, k + kAhead))), c, a.columns, row[j]);
+            }
+            const uint32_t next = k + 1 < many ? __builtin_amdgcn_readlane(myKey, k + 1) : behind;
+            if (next == key && k + 1 < many)
+            {
+                continue;
+            }
+            if (!open && next != key)
+            {
+                PutRun<O, N>(reinterpret_cast<O *>(a.table.at(key)), c, a.columns, s, a.scale, a.accumulate);
+            }
+            else
+            {
+                PutRun<float, N>(a.partial + ((size_t)piece * 2 + (open ? 0 : 1)) * a.columns, c, a.columns, s, 1.f, false);
+            }
+            open = false;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                s[i] = 0;
+            }
+        }
+    }
+}
+
+// A workgroup is four waves of pieces, or of rows to clear.
+template<class T, class O>
+__global__ __launch_bounds__(256) void EmbeddingSumKernel(const SumArgs a)
+{
+    const uint32_t wave = threadIdx.x >> 6;
+    if (blockIdx.x >= a.sumGroups)
+    {
+        const uint64_t waves = ((uint64_t)a.vocabulary + kClearRows - 1) / kClearRows;
+        for (uint64_t w = (uint64_t)(blockIdx.x - a.sumGroups) * 4 + wave; w < waves; w += (uint64_t)a.clearGroups * 4)
+        {
+            ClearRows<O>(a, (uint32_t)w);
+        }
+        return;
+    }
+    for (uint64_t w = (uint64_t)blockIdx.x * 4 + wave; w < (uint64_t)a.pieces * a.columnTiles; w += (uint64_t)a.sumGroups * 4)
+    {
+        SumPiece<T, O>(a, (uint32_t)(w / a.columnTiles), (uint32_t)(w % a.columnTiles));
+    }
+}
+
+// The sum of a token that begins in a piece and goes on behind it.
+template<class O>
+__device__ __forceinline__ void JoinPieces(const SumArgs &a, uint32_t piece, uint32_t tile)
+{
+    const uint64_t first = (uint64_t)piece * kPiece, behind = first + kPiece;
+    const uint32_t key = a.keys[behind - 1];
+    if (key == (uint32_t)a.vocabulary || a.keys[behind] != key || (piece > 0 && a.keys[first] == key && a.keys[first - 1] == key))
+    {
+        return;
+    }
+    constexpr int N = 4;
+    const int     c = (int)(tile * 64 + (threadIdx.x & 63)) * N;
+    float         s[N];
+    GetRun<float, N>(a.partial + ((size_t)piece * 2 + 1) * a.columns, c, a.columns, s);
+    for (uint32_t p = piece + 1;; ++p)
+    {
+        float part[N];
+        GetRun<float, N>(a.partial + (size_t)p * 2 * a.columns, c, a.columns, part);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            s[i] += part[i];
+        }
+        const uint64_t end = ((uint64_t)p + 1) * kPiece;
+        if (end >= (uint64_t)a.count || a.keys[end - 1] != key || a.keys[end] != key)
+        {
+            break;
+        }
+    }
+    PutRun<O, N>(reinterpret_cast<O *>(a.table.at(key)), c, a.columns, s, a.scale, a.accumulate);
+}
+
+// A wave per piece but the last, which nothing follows.
+template<class O>
+__global__ __launch_bounds__(256) void EmbeddingJoinKernel(const SumArgs a)
+{
+    for (uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); w < (uint64_t)(a.pieces - 1) * a.joinTiles; w += (uint64_t)gridDim.x * 4)
+    {
+        JoinPieces<O>(a, (uint32_t)(w / a.joinTiles), (uint32_t)(w % a.joinTiles));
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
 // Workgroups of a launch: a dimension of the grid holds fewer than 2^32 threads.
 constexpr int kMostGroups = 1 << 20;
 
-// ---- host ----------------------------------------------------------------------------------------------------------
-int64_t GradWorkspace(int64_t, int64_t, int64_t)
+int64_t Parts(int64_t v, int64_t of)
 {
-    return 0;
+    return (v + of - 1) / of;
+}
+
+int64_t RoundUp(int64_t v, int64_t to)
+{
+    return Parts(v, to) * to;
+}
+
+// Parts of the workspace, each from a multiple of 256 bytes on.
+struct GradRoom
+{
+    int64_t keys, places, otherKeys, otherPlaces, counts, partial, bytes;
+
+    GradRoom(int64_t tokens, int64_t columns)
+    {
+        const int64_t list = RoundUp(tokens * 4, 256), tiles = tokens > kMostSmall ? Parts(tokens, kTile) : 0;
+        const int64_t pieces = Parts(tokens, kPiece);
+        keys        = 0;
+        places      = keys + list;
+        otherKeys   = places + list;
+        otherPlaces = otherKeys + (tiles > 0 ? list : 0);
+        counts      = otherPlaces + (tiles > 0 ? list : 0);
+        partial     = counts + RoundUp(tiles * kDigits * 4, 256);
+        bytes       = partial + (pieces > 1 ? pieces * 2 * columns * 4 : 0);
+    }
+};
+
+int64_t GradWorkspace(int64_t tokens, int64_t, int64_t columns)
+{
+    return GradRoom(tokens, columns).bytes;
 }
 
 template<class T, class O>
@@ -106,11 +584,70 @@ void LaunchLookup(const LookupArgs &a, hipStream_t stream)
     CheckLaunch("EmbeddingKernel");
 }
 
-template<class T, class O>
-void LaunchGrad(const GradArgs &a, hipStream_t stream)
+// Sorts into the workspace's keys and places.
+void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, hipStream_t stream)
 {
-    hipLaunchKernelGGL((EmbeddingGradKernel<T, O>), dim3((int)std::min<int64_t>((int64_t)a.vocabulary * DivUp(a.columns, 256), kMostGroups)), dim3(256), 0, stream, a);
-    CheckLaunch("EmbeddingGradKernel");
+    auto     part = [&](int64_t offset) { return reinterpret_cast<uint32_t *>(room + offset); };
+    uint32_t *keys = part(at.keys), *places = part(at.places);
+    const int bits = src.vocabulary > 0 ? 32 - __builtin_clz((uint32_t)src.vocabulary) : 1;
+    if (src.count <= kMostSmall)
+    {
+        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(1), dim3(kSmallThreads), 0, stream, src, keys, places, bits); };
+        if (src.count <= kSmallThreads)
+        {
+            launch(EmbeddingSortSmallKernel<1>);
+        }
+        else if (src.count <= 4 * kSmallThreads)
+        {
+            launch(EmbeddingSortSmallKernel<4>);
+        }
+        else
+        {
+            launch(EmbeddingSortSmallKernel<16>);
+        }
+        CheckLaunch("EmbeddingSortSmallKernel");
+        return;
+    }
+    TileArgs a      = {src, nullptr, nullptr, nullptr, nullptr, part(at.counts), (int32_t)Parts(src.count, kTile), 0};
+    int      passes = DivUp(bits, kTileBits);
+    for (int p = 0; p < passes; ++p)
+    {
+        // the last pass ends in keys and places
+        const bool to = (passes - 1 - p) % 2 == 0;
+        a.toKeys      = to ? keys : part(at.otherKeys);
+        a.toPlaces    = to ? places : part(at.otherPlaces);
+        a.shift       = p * kTileBits;
+        hipLaunchKernelGGL(EmbeddingCountKernel, dim3(a.tiles), dim3(kTileThreads), 0, stream, a);
+        CheckLaunch("EmbeddingCountKernel");
+        hipLaunchKernelGGL(EmbeddingPlaceKernel, dim3(a.tiles), dim3(kTileThreads), 0, stream, a);
+        CheckLaunch("EmbeddingPlaceKernel");
+        a.keys   = a.toKeys;
+        a.places = a.toPlaces;
+    }
+}
+
+uint32_t Groups(int64_t waves)
+{
+    return (uint32_t)std::min<int64_t>((waves + 3) / 4, kMostGroups);
+}
+
+template<class T, class O>
+void LaunchGrad(SumArgs &a, hipStream_t stream)
+{
+    a.columnTiles = (uint32_t)Parts(a.columns, 64 * kRunOf<T>);
+    a.joinTiles   = (uint32_t)Parts(a.columns, 64 * 4);
+    a.sumGroups   = Groups((int64_t)a.pieces * a.columnTiles);
+    a.clearGroups = a.accumulate ? 0 : Groups(Parts(a.vocabulary, kClearRows));
+    if (a.sumGroups + a.clearGroups > 0)
+    {
+        hipLaunchKernelGGL((EmbeddingSumKernel<T, O>), dim3(a.sumGroups + a.clearGroups), dim3(256), 0, stream, a);
+        CheckLaunch("EmbeddingSumKernel");
+    }
+    if (a.pieces > 1)
+    {
+        hipLaunchKernelGGL((EmbeddingJoinKernel<O>), dim3(Groups((int64_t)(a.pieces - 1) * a.joinTiles)), dim3(256), 0, stream, a);
+        CheckLaunch("EmbeddingJoinKernel");
+    }
 }
 
 struct Tokens
@@ -204,13 +741,19 @@ public:
         {
             throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Padding must be a token, or -1 for none, not %ld", (long)padding);
         }
-        (void)RequireWorkspace(hworkspace, GradWorkspace(tokens.count, table.rows, table.columns));
+        const GradRoom at(tokens.count, table.columns);
+        uint8_t       *room = RequireWorkspace(hworkspace, at.bytes);
         if (table.rows == 0 || table.columns == 0)
         {
             return;
         }
-        const GradArgs a = {RowPlaces(grad), RowPlaces(table), tokens.base, tokens.wide, accumulate, tokens.count, table.rows, table.columns,
-                            padding, scale};
+        if (tokens.count > 0)
+        {
+            SortTokens({tokens.base, tokens.wide, tokens.count, table.rows, padding}, room, at, stream);
+        }
+        SumArgs a = {RowPlaces(grad), RowPlaces(table), reinterpret_cast<const uint32_t *>(room + at.keys),
+                     reinterpret_cast<const uint32_t *>(room + at.places), reinterpret_cast<float *>(room + at.partial), tokens.count,
+                     table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, kPiece), 0, 0, 0, 0, scale};
         if (grad.elem == kRowF32)
         {
             LaunchGrad<float, float>(a, stream);

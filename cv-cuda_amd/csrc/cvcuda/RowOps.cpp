@@ -54,7 +54,7 @@ RowsView RequireRows(NVCVTensorHandle h, const char *what)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must have rows of elements that follow one another", what);
     }
-    if (columns > INT32_MAX)
+    if (columns > kMostColumns)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s has rows of too many elements", what);
     }

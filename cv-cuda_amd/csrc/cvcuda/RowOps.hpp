@@ -60,6 +60,9 @@ __device__ __forceinline__ float WaveSum(float v)
     return v;
 }
 
+// Elements of a row: a lane's first column stays a 32-bit number also behind the end of the row.
+constexpr int64_t kMostColumns = 1 << 30;
+
 // ---- rows of a tensor --------------------------------------------------------------------------------------------
 // Row r begins at base + (r / inner) * outerStride + (r % inner) * innerStride bytes.
 struct RowsView

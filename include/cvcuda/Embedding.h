@@ -13,7 +13,7 @@
  * padding         : a token, or -1 for none.
  * workspace       : U8, dense, at least as many elements as cvcudaxEmbeddingGradWorkspace gives, aligned to 16 bytes. It
  *                   belongs to the call until the stream has passed it; NULL where 0 bytes are needed.
- * n, V, D: below 2^31 each. Tensors may be larger than 2^32 bytes.
+ * n, V: below 2^31 each, D: 2^30 at most. Tensors may be larger than 2^32 bytes.
  * Status: INVALID_ARGUMENT for any type / shape / stride problem. */
 #ifndef CVCUDA_EMBEDDING_H
 #define CVCUDA_EMBEDDING_H

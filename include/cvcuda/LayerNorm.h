@@ -16,7 +16,7 @@
  *                           of the gradient.
  * workspace               : U8, dense, at least as many elements as cvcudaxLayerNormGradWorkspace gives, aligned to 16 bytes. It
  *                           belongs to the call until the stream has passed it; NULL where 0 bytes are needed.
- * Rows and row elements: below 2^31 each. Tensors may be larger than 2^32 bytes. Tensors without elements are allowed: sums
+ * Rows: below 2^31, row elements: 2^30 at most. Tensors may be larger than 2^32 bytes. Tensors without elements are allowed: sums
  * over no rows are 0.
  * Status: INVALID_ARGUMENT for any type / shape / stride problem. */
 #ifndef CVCUDA_LAYER_NORM_H
