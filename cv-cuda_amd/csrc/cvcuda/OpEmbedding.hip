@@ -54,12 +54,9 @@ struct TokenSource
 
     __device__ __forceinline__ uint32_t key(uint32_t i) const
     {
-        if (i >= (uint32_t)count)
-        {
-            return vocabulary;
-        }
-        const int64_t t = TokenAt(tokens, wide, i);
-        return t >= 0 && t < vocabulary && t != padding ? (uint32_t)t : (uint32_t)vocabulary;
+        // (past the last one a load of that: loads under a condition wait for one another)
+        const int64_t t = TokenAt(tokens, wide, min(i, (uint32_t)count - 1));
+        return t >= 0 && t < vocabulary && t != padding && i < (uint32_t)count ? (uint32_t)t : (uint32_t)vocabulary;
     }
 };
 
@@ -112,6 +109,19 @@ __device__ __forceinline__ uint32_t WaveScan(uint32_t v)
     return v;
 }
 
+// The sum of the first `n` of N numbers in LDS: all of them on their way at once.
+template<int N>
+__device__ __forceinline__ uint32_t SumOfFirst(const uint32_t (&v)[N], uint32_t n)
+{
+    uint32_t s = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+        s += (uint32_t)i < n ? v[i] : 0;
+    }
+    return s;
+}
+
 constexpr int kSmallThreads = 1024, kSmallBits = 6;
 constexpr int kMostSmall    = 16 * kSmallThreads; // 64 KiB of keys and 32 of positions in LDS
 
@@ -149,12 +159,7 @@ __global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const 
             s_sum[wave] = upTo;
         }
         __syncthreads();
-        uint32_t base = upTo - mine;
-        for (uint32_t w = 0; w < wave; ++w)
-        {
-            base += s_sum[w];
-        }
-        s_count[threadIdx.x & 15][threadIdx.x >> 4] = base;
+        s_count[threadIdx.x & 15][threadIdx.x >> 4] = upTo - mine + SumOfFirst(s_sum, wave);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -184,38 +189,51 @@ __global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const 
 
 // More tokens: tiles of them, two launches for each digit. The first counts the digits of each tile, the second adds up what
 // comes before each digit of its tile and puts the tile's elements there.
-constexpr int kTileThreads = 512, kTileKeys = 8, kTile = kTileThreads * kTileKeys, kTileBits = 9, kDigits = 1 << kTileBits;
+constexpr int kTileThreads = 512, kTileKeys = 4, kTile = kTileThreads * kTileKeys, kTileBits = 9, kDigits = 1 << kTileBits;
+
+constexpr int kCountsAtOnce = 16; // of tiles that a thread reads: a digit's counts are padded to as many
 
 struct TileArgs
 {
     TokenSource     src;
     const uint32_t *keys, *places; // nullptr: the tokens themselves, at their places
     uint32_t       *toKeys, *toPlaces;
-    uint32_t       *counts; // [kDigits][tiles]
-    int32_t         tiles, shift;
+    uint32_t       *counts; // [kDigits][pitch]
+    int32_t         tiles, pitch, shift;
 
     __device__ __forceinline__ uint32_t key(uint32_t i) const
     {
-        return keys == nullptr ? src.key(i) : i < (uint32_t)src.count ? keys[i] : (uint32_t)src.vocabulary;
+        if (keys == nullptr)
+        {
+            return src.key(i);
+        }
+        const uint32_t k = keys[min(i, (uint32_t)src.count - 1)];
+        return i < (uint32_t)src.count ? k : (uint32_t)src.vocabulary;
     }
 };
 
 __global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileArgs a)
 {
     __shared__ uint32_t s_count[kDigits];
+    const uint32_t      first = blockIdx.x * kTile + threadIdx.x;
+    uint32_t            key[kTileKeys];
     s_count[threadIdx.x] = 0;
+#pragma unroll
+    for (int k = 0; k < kTileKeys; ++k)
+    {
+        key[k] = a.key(first + k * kTileThreads);
+    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kTileKeys; ++k)
     {
-        const uint32_t i = blockIdx.x * kTile + k * kTileThreads + threadIdx.x;
-        if (i < (uint32_t)a.src.count)
+        if (first + k * kTileThreads < (uint32_t)a.src.count)
         {
-            atomicAdd(&s_count[(a.key(i) >> a.shift) & (kDigits - 1)], 1u);
+            atomicAdd(&s_count[(key[k] >> a.shift) & (kDigits - 1)], 1u);
         }
     }
     __syncthreads();
-    a.counts[(size_t)threadIdx.x * a.tiles + blockIdx.x] = s_count[threadIdx.x];
+    a.counts[(size_t)threadIdx.x * a.pitch + blockIdx.x] = s_count[threadIdx.x];
 }
 
 __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileArgs a)
@@ -230,19 +248,24 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
     {
         const uint32_t i = first + 64 * k;
         key[k]           = a.key(i);
-        place[k]         = a.keys == nullptr ? i : i < (uint32_t)a.src.count ? a.places[i] : 0;
+        place[k]         = a.keys == nullptr ? i : a.places[min(i, (uint32_t)a.src.count - 1)];
     }
     for (int w = 0; w < kWaves; ++w)
     {
         s_count[w][threadIdx.x] = 0;
     }
     // thread d: the elements of digit d before this tile, and all of them
-    uint32_t before = 0, all = 0;
-    for (int t = 0; t < a.tiles; ++t)
+    const uint32_t *row = a.counts + (size_t)threadIdx.x * a.pitch;
+    uint32_t        before = 0, all = 0;
+    for (int t = 0; t < a.pitch; t += kCountsAtOnce)
     {
-        const uint32_t c = a.counts[(size_t)threadIdx.x * a.tiles + t];
-        before += t < (int)blockIdx.x ? c : 0;
-        all += c;
+        const Run<uint32_t, kCountsAtOnce> c = *reinterpret_cast<const Run<uint32_t, kCountsAtOnce> *>(row + t);
+#pragma unroll
+        for (int i = 0; i < kCountsAtOnce; ++i)
+        {
+            before += t + i < (int)blockIdx.x ? c.v[i] : 0;
+            all += t + i < a.tiles ? c.v[i] : 0;
+        }
     }
     const uint32_t upTo = WaveScan(all);
     if (lane == 63)
@@ -257,11 +280,7 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
         const uint32_t digit = first + 64 * k < (uint32_t)a.src.count ? (key[k] >> a.shift) & (kDigits - 1) : kDigits - 1;
         rank[k]              = CountDigit<kTileBits>(s_count[wave], digit);
     }
-    uint32_t base = before + upTo - all;
-    for (uint32_t w = 0; w < wave; ++w)
-    {
-        base += s_sum[w];
-    }
+    uint32_t base = before + upTo - all + SumOfFirst(s_sum, wave);
     __syncthreads();
     for (int w = 0; w < kWaves; ++w)
     {
@@ -287,7 +306,7 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
 // lanes' columns. A token whose positions lie within a piece is done there; of one that reaches over a piece's end each
 // piece leaves a sum of its own in the workspace, and a second launch adds these up in their order. Rows of the table that no
 // token names are cleared beside that by waves that look for their keys among the sorted ones.
-constexpr int kPiece = 32;
+constexpr int kPiece = 32, kBatch = 16; // of which so many are loaded at once
 
 struct SumArgs
 {
@@ -323,52 +342,121 @@ __device__ __forceinline__ uint32_t FirstOf(const uint32_t *keys, uint32_t n, ui
     return lo;
 }
 
-template<class O, int N>
-__device__ __forceinline__ void PutRun(O *row, int c, int columns, const float (&s)[N], float scale, bool accumulate)
+// The columns of a lane: N from `first` on. It loads N from `from` on, which lies before `first` where the row ends within
+// them, so that every lane loads as all others do (loads under a condition wait for one another); the first `skip` are then not
+// its own. It stores what it loaded: twice the same sums, where another lane has these columns too. Not where they are added to
+// the table (ACCUMULATE): there it stores its own. NARROW: rows of fewer than N columns, one by one.
+template<int N, bool NARROW, bool ACCUMULATE>
+struct LaneColumns
 {
-    if (c + N <= columns)
+    int first, from, columns;
+
+    __device__ __forceinline__ LaneColumns(uint32_t tile, int of)
+        : first((int)(tile * 64 + (threadIdx.x & 63)) * N)
+        , from(max(0, min(first, of - N)))
+        , columns(of)
     {
-        Run<O, N> *to = reinterpret_cast<Run<O, N> *>(row + c);
-        Run<O, N>  r;
-        if (accumulate)
+    }
+
+    template<class T>
+    __device__ __forceinline__ Run<T, N> get(const T *row) const
+    {
+        if constexpr (!NARROW)
         {
-            r = *to;
+            return *reinterpret_cast<const Run<T, N> *>(row + from);
+        }
+        Run<T, N> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            r.v[i] = row[min(i, columns - 1)];
+        }
+        return r;
+    }
+
+    // s, which is not to be added to what is there
+    template<class O>
+    __device__ __forceinline__ void set(O *row, const float (&s)[N], float scale) const
+    {
+        if (first >= columns)
+        {
+            return;
+        }
+        if constexpr (!NARROW)
+        {
+            Run<O, N> r;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                r.v[i] = FromFloat<O>(s[i] * scale);
+            }
+            *reinterpret_cast<Run<O, N> *>(row + from) = r;
+            return;
         }
 #pragma unroll
         for (int i = 0; i < N; ++i)
         {
-            r.v[i] = FromFloat<O>(accumulate ? (float)r.v[i] + s[i] * scale : s[i] * scale);
+            if (i < columns)
+            {
+                row[i] = FromFloat<O>(s[i] * scale);
+            }
         }
-        *to = r;
-        return;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
+
+    template<class O>
+    __device__ __forceinline__ void put(O *row, const float (&s)[N], float scale) const
     {
-        if (c + i < columns)
+        if constexpr (!ACCUMULATE)
         {
-            row[c + i] = FromFloat<O>(accumulate ? (float)row[c + i] + s[i] * scale : s[i] * scale);
+            set(row, s, scale);
+            return;
+        }
+        if (first + N <= columns)
+        {
+            Run<O, N> *to = reinterpret_cast<Run<O, N> *>(row + first);
+            Run<O, N>  r  = *to;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                r.v[i] = FromFloat<O>((float)r.v[i] + s[i] * scale);
+            }
+            *to = r;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const int c = from + i;
+            if (c >= first && c < columns)
+            {
+                row[c] = FromFloat<O>((float)row[c] + s[i] * scale);
+            }
         }
     }
+};
+
+// The wave's number of a workgroup, as what it is to the compiler: the same in all lanes.
+__device__ __forceinline__ uint32_t WaveOfGroup()
+{
+    return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 }
 
-template<class T, int N>
-__device__ __forceinline__ void GetRun(const T *row, int c, int columns, T (&v)[N])
+// `bytes` from `p` on, which begins with an element of 2 or 4 bytes, by a wave: 16 bytes per lane from the first multiple of 16
+// on, as streaming stores.
+__device__ __forceinline__ void ClearBytes(uint8_t *p, int64_t bytes, int element)
 {
-    if (c + N <= columns)
+    typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+    const int64_t lane = threadIdx.x & 63, head = min((int64_t)(-reinterpret_cast<uintptr_t>(p) & 15), bytes);
+    const int64_t body = (bytes - head) / 16 * 16, tail = bytes - head - body;
+    for (int64_t i = lane * 16; i < body; i += 64 * 16)
     {
-        const Run<T, N> r = *reinterpret_cast<const Run<T, N> *>(row + c);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-        {
-            v[i] = r.v[i];
-        }
-        return;
+        __builtin_nontemporal_store(U32x4{0, 0, 0, 0}, reinterpret_cast<U32x4 *>(p + head + i));
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
+    // the ends: up to seven elements each
+    const int64_t at = lane < 16 ? lane * element : head + body + (lane - 16) * element;
+    if (lane < 16 ? at < head : at < head + body + tail)
     {
-        v[i] = c + i < columns ? row[c + i] : (T)0.f;
+        element == 4 ? (void)(*reinterpret_cast<uint32_t *>(p + at) = 0) : (void)(*reinterpret_cast<uint16_t *>(p + at) = 0);
     }
 }
 
@@ -391,81 +479,69 @@ __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
             break;
         }
     }
-    constexpr int N = kRunOf<O>;
-    const float   zeros[N] = {};
-    for (uint32_t r = 0; r < rows; ++r)
+    // rows that follow one another without a gap are cleared as one run of bytes
+    const bool whole = a.table.innerStride == (int64_t)a.columns * (int64_t)sizeof(O);
+    for (uint32_t r = 0; r < rows;)
     {
-        if (!((named >> r) & 1))
+        if ((named >> r) & 1)
         {
-            O *row = reinterpret_cast<O *>(a.table.at(row0 + r));
-            for (int c = lane * N; c < a.columns; c += 64 * N)
-            {
-                PutRun<O, N>(row, c, a.columns, zeros, 0.f, false);
-            }
+            ++r;
+            continue;
         }
+        const uint32_t many = whole ? min(rows - r, (uint32_t)__builtin_ctz((named >> r) | 1u << kClearRows)) : 1;
+        ClearBytes(a.table.at(row0 + r), (int64_t)many * a.columns * (int64_t)sizeof(O), (int)sizeof(O));
+        r += many;
     }
 }
 
-template<class T, class O>
+template<class T, class O, bool NARROW, bool ACCUMULATE>
 __device__ __forceinline__ void SumPiece(const SumArgs &a, uint32_t piece, uint32_t tile)
 {
     constexpr int  N    = kRunOf<T>;
-    const uint32_t lane = threadIdx.x & 63;
-    const uint32_t first = piece * kPiece, many = min((uint32_t)kPiece, (uint32_t)a.count - first);
-    const int      c     = (int)(tile * 64 + lane) * N;
-    // lane k: the piece's k-th key and place; the keys before and behind the piece
-    const uint32_t myKey   = lane < many ? a.keys[first + lane] : 0;
-    const uint32_t myPlace = lane < many ? a.places[first + lane] : 0;
-    const uint32_t before  = first > 0 ? a.keys[first - 1] : 0xFFFFFFFFu;
-    const uint32_t behind  = first + many < (uint32_t)a.count ? a.keys[first + many] : 0xFFFFFFFFu;
-    float          s[N]    = {};
-    constexpr int  kAhead  = 4; // rows on their way
-    T              row[kAhead][N];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
+    const uint32_t lane = threadIdx.x & 63, first = piece * kPiece, many = min((uint32_t)kPiece, (uint32_t)a.count - first);
+    // lane k: the piece's k-th key and place (behind its end the last one's); the keys before and behind the piece
+    const uint32_t mine  = first + min(lane, many - 1);
+    const uint32_t myKey = a.keys[mine], myPlace = a.places[mine];
+    const uint32_t before = first > 0 ? a.keys[first - 1] : 0xFFFFFFFFu;
+    const uint32_t behind = first + many < (uint32_t)a.count ? a.keys[first + many] : 0xFFFFFFFFu;
+    const LaneColumns<N, NARROW, ACCUMULATE> columns(tile, a.columns);
+
+    float s[N]  = {};
+    bool  open  = (uint32_t)__builtin_amdgcn_readlane(myKey, 0) == before; // the sum began in an earlier piece
+    for (uint32_t k0 = 0; k0 < many; k0 += kBatch)
     {
-        if ((uint32_t)k < many)
+        Run<T, N> row[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
         {
-            GetRun<T, N>(reinterpret_cast<const T *>(a.grad.at(__builtin_amdgcn_readlane(myPlace, k))), c, a.columns, row[k]);
+            row[j] = columns.get(reinterpret_cast<const T *>(a.grad.at(__builtin_amdgcn_readlane(myPlace, k0 + j))));
         }
-    }
-    bool open = (uint32_t)__builtin_amdgcn_readlane(myKey, 0) == before; // the sum began in an earlier piece
-    for (uint32_t k0 = 0; k0 < many; k0 += kAhead)
-    {
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
+        for (int j = 0; j < kBatch; ++j)
         {
-            const uint32_t k = k0 + j;
-            if (k >= many)
-            {
-                break;
-            }
+            const uint32_t k   = k0 + j;
             const uint32_t key = __builtin_amdgcn_readlane(myKey, k);
-            if (key == (uint32_t)a.vocabulary)
+            if (k >= many || key == (uint32_t)a.vocabulary)
             {
-                return; // all others are behind the last row's
+                return; // (all others are behind the table's last row)
             }
 #pragma unroll
             for (int i = 0; i < N; ++i)
             {
-                s[i] += (float)row[j][i];
+                s[i] += (float)row[j].v[i];
             }
-            if (k + kAhead < many)
-            {
-                GetRun<T, N>(reinterpret_cast<const T *>(a.grad.at(__builtin_amdgcn_readlane(myPlace, k + kAhead))), c, a.columns, row[j]);
-            }
-            const uint32_t next = k + 1 < many ? __builtin_amdgcn_readlane(myKey, k + 1) : behind;
+            const uint32_t next = k + 1 < many ? (uint32_t)__builtin_amdgcn_readlane(myKey, k + 1) : behind;
             if (next == key && k + 1 < many)
             {
                 continue;
             }
             if (!open && next != key)
             {
-                PutRun<O, N>(reinterpret_cast<O *>(a.table.at(key)), c, a.columns, s, a.scale, a.accumulate);
+                columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale);
             }
             else
             {
-                PutRun<float, N>(a.partial + ((size_t)piece * 2 + (open ? 0 : 1)) * a.columns, c, a.columns, s, 1.f, false);
+                columns.set(a.partial + ((size_t)piece * 2 + (open ? 0 : 1)) * a.columns, s, 1.f);
             }
             open = false;
 #pragma unroll
@@ -478,10 +554,10 @@ __device__ __forceinline__ void SumPiece(const SumArgs &a, uint32_t piece, uint3
 }
 
 // A workgroup is four waves of pieces, or of rows to clear.
-template<class T, class O>
+template<class T, class O, bool NARROW, bool ACCUMULATE>
 __global__ __launch_bounds__(256) void EmbeddingSumKernel(const SumArgs a)
 {
-    const uint32_t wave = threadIdx.x >> 6;
+    const uint32_t wave = WaveOfGroup();
     if (blockIdx.x >= a.sumGroups)
     {
         const uint64_t waves = ((uint64_t)a.vocabulary + kClearRows - 1) / kClearRows;
@@ -493,49 +569,62 @@ __global__ __launch_bounds__(256) void EmbeddingSumKernel(const SumArgs a)
     }
     for (uint64_t w = (uint64_t)blockIdx.x * 4 + wave; w < (uint64_t)a.pieces * a.columnTiles; w += (uint64_t)a.sumGroups * 4)
     {
-        SumPiece<T, O>(a, (uint32_t)(w / a.columnTiles), (uint32_t)(w % a.columnTiles));
+        SumPiece<T, O, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.columnTiles), (uint32_t)(w % a.columnTiles));
     }
 }
 
+constexpr int kJoinRun = 4; // columns of a lane
+
 // The sum of a token that begins in a piece and goes on behind it.
-template<class O>
+template<class O, bool NARROW, bool ACCUMULATE>
 __device__ __forceinline__ void JoinPieces(const SumArgs &a, uint32_t piece, uint32_t tile)
 {
     const uint64_t first = (uint64_t)piece * kPiece, behind = first + kPiece;
-    const uint32_t key = a.keys[behind - 1];
+    const uint32_t key = __builtin_amdgcn_readfirstlane(a.keys[behind - 1]);
     if (key == (uint32_t)a.vocabulary || a.keys[behind] != key || (piece > 0 && a.keys[first] == key && a.keys[first - 1] == key))
     {
         return;
     }
-    constexpr int N = 4;
-    const int     c = (int)(tile * 64 + (threadIdx.x & 63)) * N;
-    float         s[N];
-    GetRun<float, N>(a.partial + ((size_t)piece * 2 + 1) * a.columns, c, a.columns, s);
-    for (uint32_t p = piece + 1;; ++p)
+    constexpr int                            N = kJoinRun;
+    const LaneColumns<N, NARROW, ACCUMULATE> columns(tile, a.columns);
+    Run<float, N>                            sum = columns.get(a.partial + ((size_t)piece * 2 + 1) * a.columns);
+    // the piece of the last of them, first: sums whose number is known are on their way together
+    const uint32_t last = (FirstOf(a.keys, a.count, key + 1) - 1) / kPiece;
+    constexpr int  kAhead = 8;
+    for (uint32_t p = piece + 1; p <= last; p += kAhead)
     {
-        float part[N];
-        GetRun<float, N>(a.partial + (size_t)p * 2 * a.columns, c, a.columns, part);
+        Run<float, N> part[kAhead];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int j = 0; j < kAhead; ++j)
         {
-            s[i] += part[i];
+            part[j] = columns.get(a.partial + (size_t)min(p + j, last) * 2 * a.columns);
         }
-        const uint64_t end = ((uint64_t)p + 1) * kPiece;
-        if (end >= (uint64_t)a.count || a.keys[end - 1] != key || a.keys[end] != key)
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
         {
-            break;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                sum.v[i] += p + j <= last ? part[j].v[i] : 0.f;
+            }
         }
     }
-    PutRun<O, N>(reinterpret_cast<O *>(a.table.at(key)), c, a.columns, s, a.scale, a.accumulate);
+    float s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+        s[i] = sum.v[i];
+    }
+    columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale);
 }
 
 // A wave per piece but the last, which nothing follows.
-template<class O>
+template<class O, bool NARROW, bool ACCUMULATE>
 __global__ __launch_bounds__(256) void EmbeddingJoinKernel(const SumArgs a)
 {
-    for (uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); w < (uint64_t)(a.pieces - 1) * a.joinTiles; w += (uint64_t)gridDim.x * 4)
+    for (uint64_t w = (uint64_t)blockIdx.x * 4 + WaveOfGroup(); w < (uint64_t)(a.pieces - 1) * a.joinTiles; w += (uint64_t)gridDim.x * 4)
     {
-        JoinPieces<O>(a, (uint32_t)(w / a.joinTiles), (uint32_t)(w % a.joinTiles));
+        JoinPieces<O, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.joinTiles), (uint32_t)(w % a.joinTiles));
     }
 }
 
@@ -567,7 +656,7 @@ struct GradRoom
         otherKeys   = places + list;
         otherPlaces = otherKeys + (tiles > 0 ? list : 0);
         counts      = otherPlaces + (tiles > 0 ? list : 0);
-        partial     = counts + RoundUp(tiles * kDigits * 4, 256);
+        partial     = counts + RoundUp(tiles, kCountsAtOnce) * kDigits * 4;
         bytes       = partial + (pieces > 1 ? pieces * 2 * columns * 4 : 0);
     }
 };
@@ -608,7 +697,8 @@ void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, hipSt
         CheckLaunch("EmbeddingSortSmallKernel");
         return;
     }
-    TileArgs a      = {src, nullptr, nullptr, nullptr, nullptr, part(at.counts), (int32_t)Parts(src.count, kTile), 0};
+    TileArgs a      = {src, nullptr, nullptr, nullptr, nullptr, part(at.counts), (int32_t)Parts(src.count, kTile),
+                       (int32_t)RoundUp(Parts(src.count, kTile), kCountsAtOnce), 0};
     int      passes = DivUp(bits, kTileBits);
     for (int p = 0; p < passes; ++p)
     {
@@ -631,21 +721,31 @@ uint32_t Groups(int64_t waves)
     return (uint32_t)std::min<int64_t>((waves + 3) / 4, kMostGroups);
 }
 
+template<class K>
+void Launch(K plain, K accumulate, const SumArgs &a, dim3 grid, hipStream_t stream)
+{
+    hipLaunchKernelGGL(a.accumulate ? accumulate : plain, grid, dim3(256), 0, stream, a);
+}
+
 template<class T, class O>
 void LaunchGrad(SumArgs &a, hipStream_t stream)
 {
     a.columnTiles = (uint32_t)Parts(a.columns, 64 * kRunOf<T>);
-    a.joinTiles   = (uint32_t)Parts(a.columns, 64 * 4);
+    a.joinTiles   = (uint32_t)Parts(a.columns, 64 * kJoinRun);
     a.sumGroups   = Groups((int64_t)a.pieces * a.columnTiles);
     a.clearGroups = a.accumulate ? 0 : Groups(Parts(a.vocabulary, kClearRows));
     if (a.sumGroups + a.clearGroups > 0)
     {
-        hipLaunchKernelGGL((EmbeddingSumKernel<T, O>), dim3(a.sumGroups + a.clearGroups), dim3(256), 0, stream, a);
+        const dim3 grid(a.sumGroups + a.clearGroups);
+        a.columns < kRunOf<T> ? Launch(EmbeddingSumKernel<T, O, true, false>, EmbeddingSumKernel<T, O, true, true>, a, grid, stream)
+                              : Launch(EmbeddingSumKernel<T, O, false, false>, EmbeddingSumKernel<T, O, false, true>, a, grid, stream);
         CheckLaunch("EmbeddingSumKernel");
     }
     if (a.pieces > 1)
     {
-        hipLaunchKernelGGL((EmbeddingJoinKernel<O>), dim3(Groups((int64_t)(a.pieces - 1) * a.joinTiles)), dim3(256), 0, stream, a);
+        const dim3 grid(Groups((int64_t)(a.pieces - 1) * a.joinTiles));
+        a.columns < kJoinRun ? Launch(EmbeddingJoinKernel<O, true, false>, EmbeddingJoinKernel<O, true, true>, a, grid, stream)
+                             : Launch(EmbeddingJoinKernel<O, false, false>, EmbeddingJoinKernel<O, false, true>, a, grid, stream);
         CheckLaunch("EmbeddingJoinKernel");
     }
 }
