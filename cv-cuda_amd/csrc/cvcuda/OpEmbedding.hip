@@ -123,7 +123,7 @@ __device__ __forceinline__ uint32_t SumOfFirst(const uint32_t (&v)[N], uint32_t 
 }
 
 constexpr int kSmallThreads = 1024, kSmallBits = 6;
-constexpr int kMostSmall    = 16 * kSmallThreads; // 64 KiB of keys and 32 of positions in LDS
+constexpr int kMostSmall    = 4 * kSmallThreads;
 
 // All of up to K * 1024 tokens by one workgroup, in LDS. A wave owns 64 K consecutive elements; 16 waves with 64 digits
 // each have a counter per thread.
@@ -303,22 +303,26 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
 
 // ---- gradient: sums ----------------------------------------------------------------------------------------------------
 // The sorted positions are cut into pieces of kPiece, whatever their tokens: every wave adds up the same number of rows, of 64
-// lanes' columns. A token whose positions lie within a piece is done there; of one that reaches over a piece's end each
-// piece leaves a sum of its own in the workspace, and a second launch adds these up in their order. Rows of the table that no
-// token names are cleared beside that by waves that look for their keys among the sorted ones.
-constexpr int kPiece = 32, kBatch = 16; // of which so many are loaded at once
+// lanes' columns. A token whose positions lie within a piece is done there. What reaches over a piece's ends is joined by the
+// workgroup, whose waves have pieces that follow one another, and what reaches over the workgroup's is left in the workspace,
+// where a second launch adds it up: always in the order of the positions. Rows of the table that no token names are cleared
+// beside that by waves that look for their keys among the sorted ones.
+constexpr int kPiece = 32, kBatch = 16;                 // positions of a wave, of which so many rows are loaded at once
+constexpr int kSumWaves = 8, kGroup = kSumWaves * kPiece; // positions of a workgroup
 
 struct SumArgs
 {
     RowPlaces       grad, table;
     const uint32_t *keys, *places;
-    float          *partial; // [pieces][2][columns]: of the token that began before the piece, of the one that goes on behind it
+    float          *partial; // [groups][2][columns]: of the token that began before the group, of the one that goes on behind it
     int32_t         count, vocabulary, columns, accumulate;
-    uint32_t        pieces, columnTiles, joinTiles, sumGroups, clearGroups;
+    uint32_t        groups, columnTiles, joinTiles, sumGroups, clearGroups, clearRows;
     float           scale;
 };
 
-constexpr int kClearRows = 16; // of a wave
+// A wave clears as many rows as make 16 KiB, 32 at most: what all waves write lies close together at any time (16 rows of
+// 2048 floats each: 5.3 TB/s).
+constexpr int kMostClearRows = 32, kClearBytes = 16384;
 
 // The first place among `n` sorted keys that holds `key` or more.
 __device__ __forceinline__ uint32_t FirstOf(const uint32_t *keys, uint32_t n, uint32_t key)
@@ -463,16 +467,17 @@ __device__ __forceinline__ void ClearBytes(uint8_t *p, int64_t bytes, int elemen
 template<class O>
 __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
 {
-    const uint32_t lane = threadIdx.x & 63, row0 = wave * kClearRows, rows = min((uint32_t)kClearRows, (uint32_t)a.vocabulary - row0);
+    const uint32_t lane = threadIdx.x & 63, row0 = wave * a.clearRows, rows = min(a.clearRows, (uint32_t)a.vocabulary - row0);
     uint32_t       named = 0;
     for (uint32_t at = FirstOf(a.keys, a.count, row0);; at += 64)
     {
         const uint32_t key  = at + lane < (uint32_t)a.count ? a.keys[at + lane] : 0xFFFFFFFFu;
         const bool     here = key < row0 + rows;
-#pragma unroll
-        for (uint32_t r = 0; r < kClearRows; ++r)
+        for (uint64_t rest = __ballot(here); rest != 0;) // a key at a time
         {
-            named |= __ballot(here && key == row0 + r) != 0 ? 1u << r : 0;
+            const uint32_t one = (uint32_t)__builtin_amdgcn_readlane(key, __builtin_ctzll(rest));
+            named |= 1u << (one - row0);
+            rest &= ~__ballot(key == one);
         }
         if (__ballot(here) != ~0ull)
         {
@@ -488,26 +493,35 @@ __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
             ++r;
             continue;
         }
-        const uint32_t many = whole ? min(rows - r, (uint32_t)__builtin_ctz((named >> r) | 1u << kClearRows)) : 1;
+        const uint32_t many = whole ? min(rows - r, (uint32_t)__builtin_ctzll((named >> r) | 1ull << 32)) : 1;
         ClearBytes(a.table.at(row0 + r), (int64_t)many * a.columns * (int64_t)sizeof(O), (int)sizeof(O));
         r += many;
     }
 }
 
-template<class T, class O, bool NARROW, bool ACCUMULATE>
-__device__ __forceinline__ void SumPiece(const SumArgs &a, uint32_t piece, uint32_t tile)
+// What a piece leaves of the tokens that reach over its ends, and whether: its first one began before it, that one goes on
+// behind it as well, its last one goes on behind it.
+enum PieceFlags
 {
-    constexpr int  N    = kRunOf<T>;
+    kHead       = 1,
+    kHeadGoesOn = 2,
+    kTail       = 4
+};
+
+// Sums a piece: tokens within it into the table, the others into `head` and `tail`, a lane's N one after another. Returns the flags.
+template<class T, class O, class COLUMNS, int N>
+__device__ __forceinline__ uint32_t SumPiece(const SumArgs &a, uint32_t piece, const COLUMNS &columns, float (&head)[64][N], float (&tail)[64][N])
+{
     const uint32_t lane = threadIdx.x & 63, first = piece * kPiece, many = min((uint32_t)kPiece, (uint32_t)a.count - first);
     // lane k: the piece's k-th key and place (behind its end the last one's); the keys before and behind the piece
     const uint32_t mine  = first + min(lane, many - 1);
     const uint32_t myKey = a.keys[mine], myPlace = a.places[mine];
     const uint32_t before = first > 0 ? a.keys[first - 1] : 0xFFFFFFFFu;
     const uint32_t behind = first + many < (uint32_t)a.count ? a.keys[first + many] : 0xFFFFFFFFu;
-    const LaneColumns<N, NARROW, ACCUMULATE> columns(tile, a.columns);
 
-    float s[N]  = {};
-    bool  open  = (uint32_t)__builtin_amdgcn_readlane(myKey, 0) == before; // the sum began in an earlier piece
+    uint32_t flags = 0;
+    float    s[N]  = {};
+    bool     open  = (uint32_t)__builtin_amdgcn_readlane(myKey, 0) == before; // the sum began in an earlier piece
     for (uint32_t k0 = 0; k0 < many; k0 += kBatch)
     {
         Run<T, N> row[kBatch];
@@ -523,7 +537,7 @@ __device__ __forceinline__ void SumPiece(const SumArgs &a, uint32_t piece, uint3
             const uint32_t key = __builtin_amdgcn_readlane(myKey, k);
             if (k >= many || key == (uint32_t)a.vocabulary)
             {
-                return; // (all others are behind the table's last row)
+                return flags; // (all others are behind the table's last row)
             }
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -541,7 +555,13 @@ __device__ __forceinline__ void SumPiece(const SumArgs &a, uint32_t piece, uint3
             }
             else
             {
-                columns.set(a.partial + ((size_t)piece * 2 + (open ? 0 : 1)) * a.columns, s, 1.f);
+                float (&to)[N] = open ? head[lane] : tail[lane];
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    to[i] = s[i];
+                }
+                flags |= !open ? kTail : next == key ? kHead | kHeadGoesOn : kHead;
             }
             open = false;
 #pragma unroll
@@ -551,53 +571,122 @@ __device__ __forceinline__ void SumPiece(const SumArgs &a, uint32_t piece, uint3
             }
         }
     }
+    return flags;
 }
 
-// A workgroup is four waves of pieces, or of rows to clear.
+// kSumWaves pieces that follow one another, of 64 lanes' columns.
 template<class T, class O, bool NARROW, bool ACCUMULATE>
-__global__ __launch_bounds__(256) void EmbeddingSumKernel(const SumArgs a)
+__device__ __forceinline__ void SumGroup(const SumArgs &a, uint32_t group, uint32_t tile)
 {
-    const uint32_t wave = WaveOfGroup();
+    constexpr int       N = kRunOf<T>;
+    __shared__ float    s_head[kSumWaves][64][N], s_tail[kSumWaves][64][N];
+    __shared__ uint32_t s_flags[kSumWaves];
+    const LaneColumns<N, NARROW, ACCUMULATE> columns(tile, a.columns);
+
+    const uint32_t wave = WaveOfGroup(), lane = threadIdx.x & 63, piece = group * kSumWaves + wave;
+    uint32_t       flags = 0;
+    if ((uint64_t)piece * kPiece < (uint64_t)a.count)
+    {
+        flags = SumPiece<T, O>(a, piece, columns, s_head[wave], s_tail[wave]);
+    }
+    if (lane == 0)
+    {
+        s_flags[wave] = flags;
+    }
+    __syncthreads();
+    if (wave == 0)
+    {
+        bool  here = false, any = false; // of the sum that is open: began in this group; there is one
+        float s[N] = {};
+        for (uint32_t w = 0; w < kSumWaves; ++w)
+        {
+            const uint32_t f = __builtin_amdgcn_readfirstlane(s_flags[w]);
+            if (f & kHead)
+            {
+                any = true;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    s[i] += s_head[w][lane][i];
+                }
+                if (!(f & kHeadGoesOn))
+                {
+                    if (here)
+                    {
+                        const uint32_t key = __builtin_amdgcn_readfirstlane(a.keys[(size_t)(group * kSumWaves + w) * kPiece]);
+                        columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale);
+                    }
+                    else
+                    {
+                        columns.set(a.partial + (size_t)group * 2 * a.columns, s, 1.f);
+                    }
+                    any = false;
+                }
+            }
+            if (f & kTail)
+            {
+                here = any = true;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    s[i] = s_tail[w][lane][i];
+                }
+            }
+        }
+        if (any)
+        {
+            columns.set(a.partial + ((size_t)group * 2 + (here ? 1 : 0)) * a.columns, s, 1.f);
+        }
+    }
+    __syncthreads(); // (before the next group's)
+}
+
+// A workgroup is one of tokens, or waves that clear rows.
+template<class T, class O, bool NARROW, bool ACCUMULATE>
+__global__ __launch_bounds__(64 * kSumWaves) void EmbeddingSumKernel(const SumArgs a)
+{
     if (blockIdx.x >= a.sumGroups)
     {
-        const uint64_t waves = ((uint64_t)a.vocabulary + kClearRows - 1) / kClearRows;
-        for (uint64_t w = (uint64_t)(blockIdx.x - a.sumGroups) * 4 + wave; w < waves; w += (uint64_t)a.clearGroups * 4)
+        const uint64_t waves = ((uint64_t)a.vocabulary + a.clearRows - 1) / a.clearRows;
+        for (uint64_t w = (uint64_t)(blockIdx.x - a.sumGroups) * kSumWaves + WaveOfGroup(); w < waves; w += (uint64_t)a.clearGroups * kSumWaves)
         {
             ClearRows<O>(a, (uint32_t)w);
         }
         return;
     }
-    for (uint64_t w = (uint64_t)blockIdx.x * 4 + wave; w < (uint64_t)a.pieces * a.columnTiles; w += (uint64_t)a.sumGroups * 4)
+    for (uint64_t w = blockIdx.x; w < (uint64_t)a.groups * a.columnTiles; w += a.sumGroups)
     {
-        SumPiece<T, O, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.columnTiles), (uint32_t)(w % a.columnTiles));
+        SumGroup<T, O, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.columnTiles), (uint32_t)(w % a.columnTiles));
     }
 }
 
-constexpr int kJoinRun = 4; // columns of a lane
+constexpr int kJoinRun = 4, kJoinWaves = 4; // columns of a lane; each wave adds up a part of the groups
 
-// The sum of a token that begins in a piece and goes on behind it.
+// The sum of a token that begins in a group and goes on behind it.
 template<class O, bool NARROW, bool ACCUMULATE>
-__device__ __forceinline__ void JoinPieces(const SumArgs &a, uint32_t piece, uint32_t tile)
+__device__ __forceinline__ void JoinGroups(const SumArgs &a, uint32_t group, uint32_t tile)
 {
-    const uint64_t first = (uint64_t)piece * kPiece, behind = first + kPiece;
+    const uint64_t first = (uint64_t)group * kGroup, behind = first + kGroup;
     const uint32_t key = __builtin_amdgcn_readfirstlane(a.keys[behind - 1]);
-    if (key == (uint32_t)a.vocabulary || a.keys[behind] != key || (piece > 0 && a.keys[first] == key && a.keys[first - 1] == key))
+    if (key == (uint32_t)a.vocabulary || a.keys[behind] != key || (group > 0 && a.keys[first] == key && a.keys[first - 1] == key))
     {
         return;
     }
-    constexpr int                            N = kJoinRun;
+    constexpr int    N = kJoinRun, kAhead = 8;
+    __shared__ float s_part[kJoinWaves][64][N];
     const LaneColumns<N, NARROW, ACCUMULATE> columns(tile, a.columns);
-    Run<float, N>                            sum = columns.get(a.partial + ((size_t)piece * 2 + 1) * a.columns);
-    // the piece of the last of them, first: sums whose number is known are on their way together
-    const uint32_t last = (FirstOf(a.keys, a.count, key + 1) - 1) / kPiece;
-    constexpr int  kAhead = 8;
-    for (uint32_t p = piece + 1; p <= last; p += kAhead)
+    // the group of the last of them, first: sums whose number is known are on their way together
+    const uint32_t wave = WaveOfGroup(), lane = threadIdx.x & 63;
+    const uint32_t all = (FirstOf(a.keys, a.count, key + 1) - 1) / kGroup - group, each = (all + kJoinWaves - 1) / kJoinWaves;
+    const uint32_t from = group + 1 + wave * each, to = min(group + 1 + all, from + each);
+    float          s[N] = {};
+    for (uint32_t p = from; p < to; p += kAhead)
     {
         Run<float, N> part[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
         {
-            part[j] = columns.get(a.partial + (size_t)min(p + j, last) * 2 * a.columns);
+            part[j] = columns.get(a.partial + (size_t)min(p + j, to - 1) * 2 * a.columns);
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -605,32 +694,47 @@ __device__ __forceinline__ void JoinPieces(const SumArgs &a, uint32_t piece, uin
 #pragma unroll
             for (int i = 0; i < N; ++i)
             {
-                sum.v[i] += p + j <= last ? part[j].v[i] : 0.f;
+                s[i] += p + j < to ? part[j].v[i] : 0.f;
             }
         }
     }
-    float s[N];
 #pragma unroll
     for (int i = 0; i < N; ++i)
     {
-        s[i] = sum.v[i];
+        s_part[wave][lane][i] = s[i];
     }
-    columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale);
+    __syncthreads();
+    if (wave == 0)
+    {
+        const Run<float, N> began = columns.get(a.partial + ((size_t)group * 2 + 1) * a.columns);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            s[i] = began.v[i];
+#pragma unroll
+            for (int w = 0; w < kJoinWaves; ++w)
+            {
+                s[i] += s_part[w][lane][i];
+            }
+        }
+        columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale);
+    }
+    __syncthreads(); // (before the next group's)
 }
 
-// A wave per piece but the last, which nothing follows.
+// A workgroup per group but the last, which nothing follows, and 64 lanes' columns.
 template<class O, bool NARROW, bool ACCUMULATE>
-__global__ __launch_bounds__(256) void EmbeddingJoinKernel(const SumArgs a)
+__global__ __launch_bounds__(64 * kJoinWaves) void EmbeddingJoinKernel(const SumArgs a)
 {
-    for (uint64_t w = (uint64_t)blockIdx.x * 4 + WaveOfGroup(); w < (uint64_t)(a.pieces - 1) * a.joinTiles; w += (uint64_t)gridDim.x * 4)
+    for (uint64_t w = blockIdx.x; w < (uint64_t)(a.groups - 1) * a.joinTiles; w += gridDim.x)
     {
-        JoinPieces<O, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.joinTiles), (uint32_t)(w % a.joinTiles));
+        JoinGroups<O, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.joinTiles), (uint32_t)(w % a.joinTiles));
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-// Workgroups of a launch: a dimension of the grid holds fewer than 2^32 threads.
-constexpr int kMostGroups = 1 << 20;
+// Workgroups of one kind in a launch: a dimension of the grid holds fewer than 2^32 threads.
+constexpr int kMostGroups = 1 << 21;
 
 int64_t Parts(int64_t v, int64_t of)
 {
@@ -650,14 +754,14 @@ struct GradRoom
     GradRoom(int64_t tokens, int64_t columns)
     {
         const int64_t list = RoundUp(tokens * 4, 256), tiles = tokens > kMostSmall ? Parts(tokens, kTile) : 0;
-        const int64_t pieces = Parts(tokens, kPiece);
+        const int64_t groups = Parts(tokens, kGroup);
         keys        = 0;
         places      = keys + list;
         otherKeys   = places + list;
         otherPlaces = otherKeys + (tiles > 0 ? list : 0);
         counts      = otherPlaces + (tiles > 0 ? list : 0);
         partial     = counts + RoundUp(tiles, kCountsAtOnce) * kDigits * 4;
-        bytes       = partial + (pieces > 1 ? pieces * 2 * columns * 4 : 0);
+        bytes       = partial + (groups > 1 ? groups * 2 * columns * 4 : 0);
     }
 };
 
@@ -686,13 +790,9 @@ void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, hipSt
         {
             launch(EmbeddingSortSmallKernel<1>);
         }
-        else if (src.count <= 4 * kSmallThreads)
-        {
-            launch(EmbeddingSortSmallKernel<4>);
-        }
         else
         {
-            launch(EmbeddingSortSmallKernel<16>);
+            launch(EmbeddingSortSmallKernel<4>);
         }
         CheckLaunch("EmbeddingSortSmallKernel");
         return;
@@ -716,15 +816,15 @@ void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, hipSt
     }
 }
 
-uint32_t Groups(int64_t waves)
+uint32_t Groups(int64_t groups)
 {
-    return (uint32_t)std::min<int64_t>((waves + 3) / 4, kMostGroups);
+    return (uint32_t)std::min<int64_t>(groups, kMostGroups);
 }
 
 template<class K>
-void Launch(K plain, K accumulate, const SumArgs &a, dim3 grid, hipStream_t stream)
+void Launch(K plain, K accumulate, const SumArgs &a, uint32_t grid, int waves, hipStream_t stream)
 {
-    hipLaunchKernelGGL(a.accumulate ? accumulate : plain, grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(a.accumulate ? accumulate : plain, dim3(grid), dim3(64 * waves), 0, stream, a);
 }
 
 template<class T, class O>
@@ -732,20 +832,20 @@ void LaunchGrad(SumArgs &a, hipStream_t stream)
 {
     a.columnTiles = (uint32_t)Parts(a.columns, 64 * kRunOf<T>);
     a.joinTiles   = (uint32_t)Parts(a.columns, 64 * kJoinRun);
-    a.sumGroups   = Groups((int64_t)a.pieces * a.columnTiles);
-    a.clearGroups = a.accumulate ? 0 : Groups(Parts(a.vocabulary, kClearRows));
-    if (a.sumGroups + a.clearGroups > 0)
+    a.clearRows   = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(kMostClearRows, kClearBytes / (a.columns * (int64_t)sizeof(O))));
+    a.sumGroups   = Groups((int64_t)a.groups * a.columnTiles);
+    a.clearGroups = a.accumulate ? 0 : Groups(Parts(Parts(a.vocabulary, a.clearRows), kSumWaves));
+    if (const uint32_t grid = a.sumGroups + a.clearGroups)
     {
-        const dim3 grid(a.sumGroups + a.clearGroups);
-        a.columns < kRunOf<T> ? Launch(EmbeddingSumKernel<T, O, true, false>, EmbeddingSumKernel<T, O, true, true>, a, grid, stream)
-                              : Launch(EmbeddingSumKernel<T, O, false, false>, EmbeddingSumKernel<T, O, false, true>, a, grid, stream);
+        a.columns < kRunOf<T> ? Launch(EmbeddingSumKernel<T, O, true, false>, EmbeddingSumKernel<T, O, true, true>, a, grid, kSumWaves, stream)
+                              : Launch(EmbeddingSumKernel<T, O, false, false>, EmbeddingSumKernel<T, O, false, true>, a, grid, kSumWaves, stream);
         CheckLaunch("EmbeddingSumKernel");
     }
-    if (a.pieces > 1)
+    if (a.groups > 1)
     {
-        const dim3 grid(Groups((int64_t)(a.pieces - 1) * a.joinTiles));
-        a.columns < kJoinRun ? Launch(EmbeddingJoinKernel<O, true, false>, EmbeddingJoinKernel<O, true, true>, a, grid, stream)
-                             : Launch(EmbeddingJoinKernel<O, false, false>, EmbeddingJoinKernel<O, false, true>, a, grid, stream);
+        const uint32_t grid = Groups((int64_t)(a.groups - 1) * a.joinTiles);
+        a.columns < kJoinRun ? Launch(EmbeddingJoinKernel<O, true, false>, EmbeddingJoinKernel<O, true, true>, a, grid, kJoinWaves, stream)
+                             : Launch(EmbeddingJoinKernel<O, false, false>, EmbeddingJoinKernel<O, false, true>, a, grid, kJoinWaves, stream);
         CheckLaunch("EmbeddingJoinKernel");
     }
 }
@@ -853,7 +953,7 @@ public:
         }
         SumArgs a = {RowPlaces(grad), RowPlaces(table), reinterpret_cast<const uint32_t *>(room + at.keys),
                      reinterpret_cast<const uint32_t *>(room + at.places), reinterpret_cast<float *>(room + at.partial), tokens.count,
-                     table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, kPiece), 0, 0, 0, 0, scale};
+                     table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, kGroup), 0, 0, 0, 0, 0, scale};
         if (grad.elem == kRowF32)
         {
             LaunchGrad<float, float>(a, stream);
