@@ -8,12 +8,18 @@
 
 #include <algorithm>
 #include <cmath>
+#include <vector>
 
 namespace cvamd {
 
 namespace {
 
-constexpr int kBlock = CVCUDAX_ADAMW_BLOCK; // elements that share a scale: a tile
+constexpr int kBlock = CVCUDAX_ADAMW_BLOCK; // elements that share a scale: four for each lane of a wave
+constexpr int kRun   = 4;                   // elements that follow one another in a lane
+constexpr int kRuns  = 2;                   // of which a lane has so many, all on their way before the first is used
+constexpr int kTile  = 4 * kRuns * kBlock;  // elements of a workgroup of four waves
+
+static_assert(kBlock == 64 * kRun, "a wave's runs make a block");
 
 struct Entry
 {
@@ -21,7 +27,7 @@ struct Entry
     const void *grad;
     float      *momentScale, *varianceScale;
     int64_t     count;
-    uint8_t     paramElem, gradElem, copyElem;
+    int32_t     copyElem;
 };
 
 // Tensors of a launch: with the coefficients they stay within 4 KiB of arguments.
@@ -30,7 +36,7 @@ constexpr int kMostEntries = 48;
 struct StepArgs
 {
     Entry        entry[kMostEntries];
-    uint32_t     firstTile[kMostEntries];
+    uint32_t     firstTile[kMostEntries]; // behind the last entry: no tile's number
     uint32_t     tiles;
     int32_t      entries;
     const float *gradScale;
@@ -38,28 +44,6 @@ struct StepArgs
 };
 
 static_assert(sizeof(StepArgs) <= 4096, "arguments of a launch");
-
-__device__ __forceinline__ float LoadAs(const void *p, int elem, int64_t i)
-{
-    return elem == kRowF32 ? static_cast<const float *>(p)[i] : elem == kRowF16 ? (float)static_cast<const Half *>(p)[i]
-                                                                               : (float)static_cast<const Bf16 *>(p)[i];
-}
-
-__device__ __forceinline__ void StoreAs(void *p, int elem, int64_t i, float v)
-{
-    if (elem == kRowF32)
-    {
-        static_cast<float *>(p)[i] = v;
-    }
-    else if (elem == kRowF16)
-    {
-        static_cast<Half *>(p)[i] = FromFloat<Half>(v);
-    }
-    else
-    {
-        static_cast<Bf16 *>(p)[i] = FromFloat<Bf16>(v);
-    }
-}
 
 __device__ __forceinline__ float MomentOf(int q, float scale)
 {
@@ -74,94 +58,278 @@ __device__ __forceinline__ float VarianceOf(uint32_t q, float scale)
     return (t * t) * scale;
 }
 
-// The larger of two magnitudes; NaN where one is.
-__device__ __forceinline__ float Larger(float a, float b)
-{
-    return a != a || a > b ? a : b;
-}
-
-// Of a workgroup of 256, in every thread; NaN unless it is finite.
-__device__ __forceinline__ float BlockLargest(float v)
-{
-    __shared__ float part[4];
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1)
-    {
-        v = Larger(v, __shfl_xor(v, s));
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-    {
-        part[threadIdx.x >> 6] = v;
-    }
-    __syncthreads();
-    v = Larger(Larger(part[0], part[1]), Larger(part[2], part[3]));
-    return v < __builtin_inff() ? v : __builtin_nanf("");
-}
-
-// A code for |value| / scale = share: NaN gives 0.
+// A code as the formula gives it: NaN gives 0.
 __device__ __forceinline__ int CodeOf(float root, float most)
 {
     const float q = rintf(root * most);
     return q >= 0 ? (int)fminf(q, most) : 0;
 }
 
-__device__ __forceinline__ const Entry &EntryOf(const StepArgs &a, uint32_t tile, uint32_t &within)
+// Codes of magnitudes of a block with the largest `scale`. The formula's division and square roots are rounded to the nearest:
+// forty instructions and more for each. The hardware's approximations are within 2^-23 of them each, so that a code can differ
+// only where its root is within 6 * 2^-23 * 255 = 1.9e-4 of the middle between two: those are made again by the formula,
+// and so is a block whose scale has no reciprocal among the normal numbers.
+template<bool VARIANCE>
+__device__ __forceinline__ int Code(float magnitude, float scale, float reciprocal, bool ordinary)
 {
-    int e = 0;
-    for (int k = 1; k < a.entries; ++k)
+    constexpr float most = VARIANCE ? 255.f : 127.f;
+    float           root = __builtin_amdgcn_sqrtf(magnitude * reciprocal);
+    root                 = (VARIANCE ? __builtin_amdgcn_sqrtf(root) : root) * most;
+    const float q        = rintf(root);
+    int         code     = (int)q;
+    if (!ordinary || fabsf(root - q) > 0.5f - 2.5e-4f)
     {
-        e = tile >= a.firstTile[k] ? k : e;
+        root = sqrtf(scale > 0 ? magnitude / scale : 0.f);
+        code = CodeOf(VARIANCE ? sqrtf(root) : root, most);
     }
-    within = tile - a.firstTile[e];
-    return a.entry[e];
+    return VARIANCE ? max(code, magnitude > 0 ? 1 : 0) : code;
 }
 
-// A workgroup per tile, an element per thread.
-template<bool SHORT>
-__global__ __launch_bounds__(kBlock) void AdamWKernel(const StepArgs a)
+struct Moments
 {
+    float m, v;
+};
+
+// One element: the moments after the step, and p.
+__device__ __forceinline__ Moments Step(const StepArgs &a, float &p, float m, float v, float g, float gradScale)
+{
+    g = g * gradScale;
+    m = a.beta1 * m + g * a.gradPart1;
+    v = a.beta2 * v + g * a.gradPart2 * g;
+    p = p * a.keep - m / (sqrtf(v) * a.rootScale + a.epsilon) * a.step;
+    return {m, v};
+}
+
+template<class T>
+__device__ __forceinline__ Run<T, kRun> RunAt(const void *base, int64_t i)
+{
+    return *reinterpret_cast<const Run<T, kRun> *>(static_cast<const T *>(base) + i);
+}
+
+template<class T>
+__device__ __forceinline__ void PutRun(void *base, int64_t i, const float (&v)[kRun])
+{
+    Run<T, kRun> r;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k)
+    {
+        r.v[k] = FromFloat<T>(v[k]);
+    }
+    *reinterpret_cast<Run<T, kRun> *>(static_cast<T *>(base) + i) = r;
+}
+
+__device__ __forceinline__ void PutCopy(const Entry &e, int64_t i, const float (&v)[kRun])
+{
+    if (e.copy != nullptr) // (of the whole tensor)
+    {
+        e.copyElem == kRowF16 ? PutRun<Half>(e.copy, i, v) : PutRun<Bf16>(e.copy, i, v);
+    }
+}
+
+__device__ __forceinline__ void PutCopyOne(const Entry &e, int64_t i, float v)
+{
+    if (e.copy != nullptr)
+    {
+        e.copyElem == kRowF16 ? (void)(static_cast<Half *>(e.copy)[i] = FromFloat<Half>(v)) : (void)(static_cast<Bf16 *>(e.copy)[i] = FromFloat<Bf16>(v));
+    }
+}
+
+// The entry of a tile. All first tiles are compared at once: a search would wait for each of its loads.
+template<class Args>
+__device__ __forceinline__ int EntryOf(const Args &a, uint32_t tile)
+{
+    int e = 0;
+#pragma unroll
+    for (int k = 1; k < kMostEntries; ++k)
+    {
+        e += tile >= a.firstTile[k] ? 1 : 0;
+    }
+    return e;
+}
+
+// States of 32 bits. 28 bytes of an element and 40 instructions: bound by memory.
+template<class P, class G>
+__global__ __launch_bounds__(256) void AdamWKernel(const StepArgs a)
+{
+    const float gradScale = a.gradScale != nullptr ? *a.gradScale : 1.f;
     for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
     {
-        uint32_t      within;
-        const Entry  &e    = EntryOf(a, tile, within);
-        const int64_t i    = (int64_t)within * kBlock + threadIdx.x;
-        const bool    live = i < e.count;
-        float         p = 0, m = 0, v = 0;
-        if (live)
+        const int     n     = EntryOf(a, tile);
+        const Entry  &e     = a.entry[n];
+        const int64_t first = (int64_t)(tile - a.firstTile[n]) * kTile;
+        float        *ms = static_cast<float *>(e.moment), *vs = static_cast<float *>(e.variance);
+        if (first + kTile <= e.count)
         {
-            float g = LoadAs(e.grad, e.gradElem, i);
-            g       = a.gradScale != nullptr ? g * *a.gradScale : g;
-            p       = LoadAs(e.param, e.paramElem, i);
-            m       = SHORT ? MomentOf(static_cast<const int8_t *>(e.moment)[i], e.momentScale[within]) : static_cast<const float *>(e.moment)[i];
-            v = SHORT ? VarianceOf(static_cast<const uint8_t *>(e.variance)[i], e.varianceScale[within]) : static_cast<const float *>(e.variance)[i];
-            m = a.beta1 * m + g * a.gradPart1;
-            v = a.beta2 * v + g * a.gradPart2 * g;
-            p = p * a.keep - m / (sqrtf(v) * a.rootScale + a.epsilon) * a.step;
-            StoreAs(e.param, e.paramElem, i, p);
-            if (e.copy != nullptr)
+            Run<P, kRun>     p[kRuns];
+            Run<G, kRun>     g[kRuns];
+            Run<float, kRun> m[kRuns], v[kRuns];
+#pragma unroll
+            for (int r = 0; r < kRuns; ++r)
             {
-                StoreAs(e.copy, e.copyElem, i, p);
+                const int64_t i = first + (r * 256 + threadIdx.x) * kRun;
+                p[r]            = RunAt<P>(e.param, i);
+                g[r]            = RunAt<G>(e.grad, i);
+                m[r]            = RunAt<float>(ms, i);
+                v[r]            = RunAt<float>(vs, i);
             }
-            if (!SHORT)
+#pragma unroll
+            for (int r = 0; r < kRuns; ++r)
             {
-                static_cast<float *>(e.moment)[i]   = m;
-                static_cast<float *>(e.variance)[i] = v;
+                const int64_t i = first + (r * 256 + threadIdx.x) * kRun;
+                float         pn[kRun];
+#pragma unroll
+                for (int k = 0; k < kRun; ++k)
+                {
+                    pn[k]           = (float)p[r].v[k];
+                    const Moments s = Step(a, pn[k], m[r].v[k], v[r].v[k], (float)g[r].v[k], gradScale);
+                    m[r].v[k]       = s.m;
+                    v[r].v[k]       = s.v;
+                }
+                PutRun<P>(e.param, i, pn);
+                *reinterpret_cast<Run<float, kRun> *>(ms + i) = m[r];
+                *reinterpret_cast<Run<float, kRun> *>(vs + i) = v[r];
+                PutCopy(e, i, pn);
+            }
+            continue;
+        }
+        for (int64_t i = first + threadIdx.x; i < e.count; i += 256)
+        {
+            float         p = (float)static_cast<const P *>(e.param)[i];
+            const Moments s = Step(a, p, ms[i], vs[i], (float)static_cast<const G *>(e.grad)[i], gradScale);
+            static_cast<P *>(e.param)[i] = FromFloat<P>(p);
+            ms[i]                        = s.m;
+            vs[i]                        = s.v;
+            PutCopyOne(e, i, p);
+        }
+    }
+}
+
+// What a block's codes are made with.
+struct BlockScale
+{
+    float scale, reciprocal;
+    bool  ordinary;
+
+    // of the largest magnitude's bits
+    __device__ __forceinline__ explicit BlockScale(uint32_t largest)
+    {
+        scale      = largest < 0x7F800000u ? __uint_as_float(largest) : __builtin_nanf("");
+        reciprocal = __builtin_amdgcn_rcpf(scale);
+        ordinary   = scale > 1e-30f && scale < 1e30f;
+    }
+};
+
+// States of 8 bits: a wave takes whole blocks, whose largest magnitudes are found across its lanes.
+template<class P, class G>
+__global__ __launch_bounds__(256) void AdamWSmallKernel(const StepArgs a)
+{
+    const float    gradScale = a.gradScale != nullptr ? *a.gradScale : 1.f;
+    const uint32_t lane      = threadIdx.x & 63;
+    for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
+    {
+        const int     n     = EntryOf(a, tile);
+        const Entry  &e     = a.entry[n];
+        const int64_t block = (int64_t)(tile - a.firstTile[n]) * (kTile / kBlock) + WaveOfGroup() * kRuns, first = block * kBlock;
+        int8_t       *mq = static_cast<int8_t *>(e.moment);
+        uint8_t      *vq = static_cast<uint8_t *>(e.variance);
+        const bool    whole = first + kRuns * kBlock <= e.count;
+        Run<P, kRun>       p[kRuns] = {};
+        Run<G, kRun>       g[kRuns] = {};
+        Run<int8_t, kRun>  m[kRuns] = {};
+        Run<uint8_t, kRun> v[kRuns] = {};
+        float              ms[kRuns] = {}, vs[kRuns] = {};
+        if (whole)
+        {
+#pragma unroll
+            for (int r = 0; r < kRuns; ++r)
+            {
+                const int64_t i = first + r * kBlock + lane * kRun;
+                p[r]            = RunAt<P>(e.param, i);
+                g[r]            = RunAt<G>(e.grad, i);
+                m[r]            = RunAt<int8_t>(mq, i);
+                v[r]            = RunAt<uint8_t>(vq, i);
+                ms[r]           = e.momentScale[block + r];
+                vs[r]           = e.varianceScale[block + r];
             }
         }
-        if (SHORT)
+        else
         {
-            const float ms = BlockLargest(fabsf(m)), vs = BlockLargest(v);
-            if (live)
+#pragma unroll
+            for (int r = 0; r < kRuns; ++r)
             {
-                const int q                          = CodeOf(sqrtf(ms > 0 ? fabsf(m) / ms : 0.f), 127.f);
-                static_cast<int8_t *>(e.moment)[i]   = (int8_t)(m < 0 ? -q : q);
-                static_cast<uint8_t *>(e.variance)[i] = (uint8_t)max(CodeOf(sqrtf(sqrtf(vs > 0 ? v / vs : 0.f)), 255.f), v > 0 ? 1 : 0);
+                if (first + r * kBlock < e.count)
+                {
+                    ms[r] = e.momentScale[block + r];
+                    vs[r] = e.varianceScale[block + r];
+                }
+#pragma unroll
+                for (int k = 0; k < kRun; ++k)
+                {
+                    const int64_t i = first + r * kBlock + lane * kRun + k;
+                    if (i < e.count)
+                    {
+                        p[r].v[k] = static_cast<const P *>(e.param)[i];
+                        g[r].v[k] = static_cast<const G *>(e.grad)[i];
+                        m[r].v[k] = mq[i];
+                        v[r].v[k] = vq[i];
+                    }
+                }
             }
-            if (threadIdx.x == 0)
+        }
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r)
+        {
+            const int64_t i = first + r * kBlock + lane * kRun;
+            if (first + r * kBlock >= e.count)
             {
-                e.momentScale[within]   = ms;
-                e.varianceScale[within] = vs;
+                break;
+            }
+            float    pn[kRun], mn[kRun], vn[kRun];
+            uint32_t mMost = 0, vMost = 0;
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+            {
+                pn[k]           = (float)p[r].v[k];
+                const Moments s = Step(a, pn[k], MomentOf(m[r].v[k], ms[r]), VarianceOf(v[r].v[k], vs[r]), (float)g[r].v[k], gradScale);
+                const bool    in = whole || i + k < e.count; // (past the end nothing counts)
+                mn[k]            = in ? s.m : 0.f;
+                vn[k]            = in ? s.v : 0.f;
+                mMost            = max(mMost, __float_as_uint(fabsf(mn[k])));
+                vMost            = max(vMost, __float_as_uint(fabsf(vn[k])));
+            }
+            const BlockScale   mScale(WaveLargest(mMost)), vScale(WaveLargest(vMost));
+            Run<int8_t, kRun>  mCode;
+            Run<uint8_t, kRun> vCode;
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+            {
+                const int q = Code<false>(fabsf(mn[k]), mScale.scale, mScale.reciprocal, mScale.ordinary);
+                mCode.v[k]  = (int8_t)(mn[k] < 0 ? -q : q);
+                vCode.v[k]  = (uint8_t)Code<true>(vn[k], vScale.scale, vScale.reciprocal, vScale.ordinary);
+            }
+            if (lane == 0)
+            {
+                e.momentScale[block + r]   = mScale.scale;
+                e.varianceScale[block + r] = vScale.scale;
+            }
+            if (whole)
+            {
+                PutRun<P>(e.param, i, pn);
+                *reinterpret_cast<Run<int8_t, kRun> *>(mq + i)  = mCode;
+                *reinterpret_cast<Run<uint8_t, kRun> *>(vq + i) = vCode;
+                PutCopy(e, i, pn);
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+            {
+                if (i + k < e.count)
+                {
+                    static_cast<P *>(e.param)[i + k] = FromFloat<P>(pn[k]);
+                    mq[i + k]                        = mCode.v[k];
+                    vq[i + k]                        = vCode.v[k];
+                    PutCopyOne(e, i + k, pn[k]);
+                }
             }
         }
     }
@@ -186,22 +354,41 @@ struct UnpackArgs
 
 static_assert(sizeof(UnpackArgs) <= 4096, "arguments of a launch");
 
-__global__ __launch_bounds__(kBlock) void AdamWUnpackKernel(const UnpackArgs a)
+__global__ __launch_bounds__(256) void AdamWUnpackKernel(const UnpackArgs a)
 {
     for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
     {
-        int n = 0;
-        for (int k = 1; k < a.entries; ++k)
+        const int          n     = EntryOf(a, tile);
+        const UnpackEntry &e     = a.entry[n];
+        const int64_t      first = (int64_t)(tile - a.firstTile[n]) * kTile;
+        if (first + kTile <= e.count)
         {
-            n = tile >= a.firstTile[k] ? k : n;
+            Run<uint8_t, kRun> q[kRuns];
+            float              scale[kRuns];
+#pragma unroll
+            for (int r = 0; r < kRuns; ++r)
+            {
+                const int64_t i = first + (r * 256 + threadIdx.x) * kRun;
+                q[r]            = RunAt<uint8_t>(e.codes, i);
+                scale[r]        = e.scales[i / kBlock];
+            }
+#pragma unroll
+            for (int r = 0; r < kRuns; ++r)
+            {
+                float v[kRun];
+#pragma unroll
+                for (int k = 0; k < kRun; ++k)
+                {
+                    v[k] = e.variance ? VarianceOf(q[r].v[k], scale[r]) : MomentOf((int8_t)q[r].v[k], scale[r]);
+                }
+                PutRun<float>(e.out, first + (r * 256 + threadIdx.x) * kRun, v);
+            }
+            continue;
         }
-        const UnpackEntry &e      = a.entry[n];
-        const uint32_t     within = tile - a.firstTile[n];
-        const int64_t      i      = (int64_t)within * kBlock + threadIdx.x;
-        if (i < e.count)
+        for (int64_t i = first + threadIdx.x; i < e.count; i += 256)
         {
-            e.out[i] = e.variance ? VarianceOf(static_cast<const uint8_t *>(e.codes)[i], e.scales[within])
-                                  : MomentOf(static_cast<const int8_t *>(e.codes)[i], e.scales[within]);
+            e.out[i] = e.variance ? VarianceOf(static_cast<const uint8_t *>(e.codes)[i], e.scales[i / kBlock])
+                                  : MomentOf(static_cast<const int8_t *>(e.codes)[i], e.scales[i / kBlock]);
         }
     }
 }
@@ -212,7 +399,20 @@ constexpr uint32_t kMostGroups = 1 << 20;
 
 int64_t Tiles(int64_t count)
 {
+    return (count + kTile - 1) / kTile;
+}
+
+int64_t Blocks(int64_t count)
+{
     return (count + kBlock - 1) / kBlock;
+}
+
+template<class Args>
+void Clear(Args &a)
+{
+    a.tiles   = 0;
+    a.entries = 0;
+    std::fill_n(a.firstTile, kMostEntries, UINT32_MAX);
 }
 
 NVCVTensorHandle At(const NVCVTensorHandle *list, int i)
@@ -230,14 +430,14 @@ DenseView Take(NVCVTensorHandle h, const char *what, int64_t count, NVCVDataType
     return v;
 }
 
-uint8_t FloatElem(const DenseView &v, const char *what)
+RowElem FloatElem(const DenseView &v, const char *what)
 {
     const RowElem e = RowElemOf(v.dtype);
     if (e == kRowNone)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must hold F32, F16 or BF16 values", what);
     }
-    return (uint8_t)e;
+    return e;
 }
 
 void RequireCount(int32_t count, bool lists)
@@ -252,7 +452,7 @@ void RequireCount(int32_t count, bool lists)
 template<class Args, class E>
 bool Add(Args &a, const E &e, int64_t tiles)
 {
-    if (a.entries == kMostEntries || tiles > (int64_t)UINT32_MAX - a.tiles)
+    if (a.entries == kMostEntries || tiles >= (int64_t)UINT32_MAX - a.tiles)
     {
         return false;
     }
@@ -303,25 +503,37 @@ public:
         a.step      = (float)(s.lr / (1 - std::pow(s.beta1, (double)s.step)));
         a.rootScale = (float)(1 / std::sqrt(1 - std::pow(s.beta2, (double)s.step)));
         a.epsilon   = (float)s.epsilon;
-        // all of them are looked at before the first is changed
-        for (int pass = 0; pass < 2; ++pass)
+        // all of them are looked at before the first is changed; those of one pair of types go into a launch
+        std::vector<Given> given(count);
+        bool               there[kRowNone][kRowNone] = {};
+        for (int i = 0; i < count; ++i)
         {
-            for (int i = 0; i < count; ++i)
+            given[i] = EntryFor(i, params, moments, variances, grads, copies, momentScales, varianceScales);
+            if (Tiles(given[i].entry.count) >= UINT32_MAX)
             {
-                const Entry   e     = EntryFor(i, params, moments, variances, grads, copies, momentScales, varianceScales);
-                const int64_t tiles = Tiles(e.count);
-                if (tiles > UINT32_MAX)
+                throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Tensor %d has too many elements", i);
+            }
+            there[given[i].param][given[i].grad] = true;
+        }
+        for (int pair = 0; pair < kRowNone * kRowNone; ++pair)
+        {
+            const auto param = (RowElem)(pair / kRowNone), grad = (RowElem)(pair % kRowNone);
+            if (!there[param][grad])
+            {
+                continue;
+            }
+            Clear(a);
+            for (const Given &g : given)
+            {
+                const int64_t tiles = Tiles(g.entry.count);
+                if (g.param == param && g.grad == grad && tiles > 0 && !Add(a, g.entry, tiles))
                 {
-                    throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Tensor %d has too many elements", i);
-                }
-                if (pass == 1 && tiles > 0 && !Add(a, e, tiles))
-                {
-                    launch(a, small, stream);
-                    Add(a, e, tiles);
+                    launch(a, param, grad, small, stream);
+                    Add(a, g.entry, tiles);
                 }
             }
+            launch(a, param, grad, small, stream);
         }
-        launch(a, small, stream);
     }
 
     static void unpack(hipStream_t stream, int32_t count, const NVCVTensorHandle *codes, const NVCVTensorHandle *scales,
@@ -329,6 +541,7 @@ public:
     {
         RequireCount(count, codes != nullptr && scales != nullptr && out != nullptr);
         UnpackArgs a = {};
+        Clear(a);
         for (int pass = 0; pass < 2; ++pass)
         {
             for (int i = 0; i < count; ++i)
@@ -339,10 +552,10 @@ public:
                     throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Codes must be S8 or U8");
                 }
                 const int64_t     tiles = Tiles(c.count);
-                const UnpackEntry e     = {c.base, reinterpret_cast<const float *>(Take(scales[i], "Scales", tiles, NVCV_DATA_TYPE_F32).base),
+                const UnpackEntry e     = {c.base, reinterpret_cast<const float *>(Take(scales[i], "Scales", Blocks(c.count), NVCV_DATA_TYPE_F32).base),
                                            reinterpret_cast<float *>(Take(out[i], "Output", c.count, NVCV_DATA_TYPE_F32).base), c.count,
                                            c.dtype == NVCV_DATA_TYPE_U8};
-                if (tiles > UINT32_MAX)
+                if (tiles >= UINT32_MAX)
                 {
                     throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Tensor %d has too many elements", i);
                 }
@@ -357,25 +570,30 @@ public:
     }
 
 private:
-    static Entry EntryFor(int i, const NVCVTensorHandle *params, const NVCVTensorHandle *moments, const NVCVTensorHandle *variances,
+    struct Given
+    {
+        Entry   entry;
+        RowElem param, grad;
+    };
+
+    static Given EntryFor(int i, const NVCVTensorHandle *params, const NVCVTensorHandle *moments, const NVCVTensorHandle *variances,
                           const NVCVTensorHandle *grads, const NVCVTensorHandle *copies, const NVCVTensorHandle *momentScales,
                           const NVCVTensorHandle *varianceScales)
     {
         const bool      small = momentScales != nullptr;
         const DenseView p     = RequireDense(params[i], "Parameter", NVCV_DATA_TYPE_NONE);
         const DenseView g     = Take(grads[i], "Gradient", p.count);
-        Entry           e     = {};
+        Given           given = {{}, FloatElem(p, "Parameter"), FloatElem(g, "Gradient")};
+        Entry          &e     = given.entry;
         e.count               = p.count;
         e.param               = p.base;
-        e.paramElem           = FloatElem(p, "Parameter");
         e.grad                = g.base;
-        e.gradElem            = FloatElem(g, "Gradient");
         e.moment              = Take(moments[i], "Moment", p.count, small ? NVCV_DATA_TYPE_S8 : NVCV_DATA_TYPE_F32).base;
         e.variance            = Take(variances[i], "Variance", p.count, small ? NVCV_DATA_TYPE_U8 : NVCV_DATA_TYPE_F32).base;
         if (small)
         {
-            e.momentScale   = reinterpret_cast<float *>(Take(momentScales[i], "Moment's scales", Tiles(p.count), NVCV_DATA_TYPE_F32).base);
-            e.varianceScale = reinterpret_cast<float *>(Take(varianceScales[i], "Variance's scales", Tiles(p.count), NVCV_DATA_TYPE_F32).base);
+            e.momentScale   = reinterpret_cast<float *>(Take(momentScales[i], "Moment's scales", Blocks(p.count), NVCV_DATA_TYPE_F32).base);
+            e.varianceScale = reinterpret_cast<float *>(Take(varianceScales[i], "Variance's scales", Blocks(p.count), NVCV_DATA_TYPE_F32).base);
         }
         if (NVCVTensorHandle h = At(copies, i))
         {
@@ -387,37 +605,51 @@ private:
                 throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Copy must be F16 or BF16");
             }
         }
-        return e;
+        return given;
     }
 
-    static void launch(StepArgs &a, bool small, hipStream_t stream)
+    template<class P, class G>
+    static void launch(const StepArgs &a, bool small, hipStream_t stream)
+    {
+        const dim3 grid(std::min(a.tiles, kMostGroups));
+        if (small)
+        {
+            hipLaunchKernelGGL((AdamWSmallKernel<P, G>), grid, dim3(256), 0, stream, a);
+        }
+        else
+        {
+            hipLaunchKernelGGL((AdamWKernel<P, G>), grid, dim3(256), 0, stream, a);
+        }
+        CheckLaunch("AdamWKernel");
+    }
+
+    template<class P>
+    static void launch(const StepArgs &a, RowElem grad, bool small, hipStream_t stream)
+    {
+        grad == kRowF32   ? launch<P, float>(a, small, stream)
+        : grad == kRowF16 ? launch<P, Half>(a, small, stream)
+                          : launch<P, Bf16>(a, small, stream);
+    }
+
+    static void launch(StepArgs &a, RowElem param, RowElem grad, bool small, hipStream_t stream)
     {
         if (a.tiles > 0)
         {
-            const dim3 grid(std::min(a.tiles, kMostGroups));
-            if (small)
-            {
-                hipLaunchKernelGGL(AdamWKernel<true>, grid, dim3(kBlock), 0, stream, a);
-            }
-            else
-            {
-                hipLaunchKernelGGL(AdamWKernel<false>, grid, dim3(kBlock), 0, stream, a);
-            }
-            CheckLaunch("AdamWKernel");
+            param == kRowF32   ? launch<float>(a, grad, small, stream)
+            : param == kRowF16 ? launch<Half>(a, grad, small, stream)
+                               : launch<Bf16>(a, grad, small, stream);
         }
-        a.tiles   = 0;
-        a.entries = 0;
+        Clear(a);
     }
 
     static void launch(UnpackArgs &a, hipStream_t stream)
     {
         if (a.tiles > 0)
         {
-            hipLaunchKernelGGL(AdamWUnpackKernel, dim3(std::min(a.tiles, kMostGroups)), dim3(kBlock), 0, stream, a);
+            hipLaunchKernelGGL(AdamWUnpackKernel, dim3(std::min(a.tiles, kMostGroups)), dim3(256), 0, stream, a);
             CheckLaunch("AdamWUnpackKernel");
         }
-        a.tiles   = 0;
-        a.entries = 0;
+        Clear(a);
     }
 };
 

@@ -439,12 +439,6 @@ struct LaneColumns
     }
 };
 
-// The wave's number of a workgroup, as what it is to the compiler: the same in all lanes.
-__device__ __forceinline__ uint32_t WaveOfGroup()
-{
-    return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-}
-
 // `bytes` from `p` on, which begins with an element of 2 or 4 bytes, by a wave: 16 bytes per lane from the first multiple of 16
 // on, as streaming stores.
 __device__ __forceinline__ void ClearBytes(uint8_t *p, int64_t bytes, int element)

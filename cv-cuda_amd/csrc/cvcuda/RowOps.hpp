@@ -49,15 +49,43 @@ __device__ __forceinline__ T FromFloat(float v)
     return (T)v; // to the nearest even
 }
 
-// Sum over the 64 lanes, in every lane: halves of the wave in turn, so the order is the same in all of them.
+// What lane `of the step` has, 0 where there is none: the steps of a reduction over the wave by cross-lane moves alone (within
+// rows of 16 lanes, then from each row's last lane to the next row). After the last one lane 63 has it all.
+template<int STEP>
+__device__ __forceinline__ uint32_t LaneStep(uint32_t v)
+{
+    constexpr int ctrl[] = {0x111, 0x112, 0x114, 0x118, 0x142, 0x143}; // row_shr 1, 2, 4, 8, row_bcast 15, 31
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl[STEP], STEP == 4 ? 0xA : STEP == 5 ? 0xC : 0xF, 0xF, false);
+}
+
+// Sum over the 64 lanes, as one number.
 __device__ __forceinline__ float WaveSum(float v)
 {
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1)
-    {
-        v += __shfl_xor(v, s);
-    }
-    return v;
+    v += __uint_as_float(LaneStep<0>(__float_as_uint(v)));
+    v += __uint_as_float(LaneStep<1>(__float_as_uint(v)));
+    v += __uint_as_float(LaneStep<2>(__float_as_uint(v)));
+    v += __uint_as_float(LaneStep<3>(__float_as_uint(v)));
+    v += __uint_as_float(LaneStep<4>(__float_as_uint(v)));
+    v += __uint_as_float(LaneStep<5>(__float_as_uint(v)));
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+
+// The largest of the 64 lanes' numbers, as one. Of magnitudes by their bits: a NaN is larger than all others.
+__device__ __forceinline__ uint32_t WaveLargest(uint32_t v)
+{
+    v = max(v, LaneStep<0>(v));
+    v = max(v, LaneStep<1>(v));
+    v = max(v, LaneStep<2>(v));
+    v = max(v, LaneStep<3>(v));
+    v = max(v, LaneStep<4>(v));
+    v = max(v, LaneStep<5>(v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// The wave's number in its workgroup, as what it is to the compiler: the same in all lanes.
+__device__ __forceinline__ uint32_t WaveOfGroup()
+{
+    return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 }
 
 // Elements of a row: a lane's first column stays a 32-bit number also behind the end of the row.
