@@ -1,8 +1,10 @@
-// Layer norm of rows, and its gradient (formulas: cvcuda/LayerNorm.h).
+// Layer norm of rows, and its gradient (formulas: cvcuda/LayerNorm.h). Bound by memory: a row is read once and held in
+// registers by one, four or more waves, runs of 16 bytes of it in each lane.
 //
-// One workgroup per row: the mean, then the squares of what remains of each element without it (a sum of squares from
-// which the squared mean is taken would lose the variance of rows that lie far from 0), then the row itself. The gradient's
-// sums over rows are made by columns, in two steps whose order is fixed.
+// The variance is the mean of the squares of what remains of each element without the mean: the difference of the mean
+// square and the squared mean would lose it in rows that lie far from 0. The gradient's sums over rows stay in the registers of
+// workgroups that go through the rows in turn; each leaves its own in the workspace, a second launch adds them up: always in
+// the same order.
 #include "RowOps.hpp"
 
 #include <cvcuda/LayerNorm.h>
@@ -20,7 +22,7 @@ struct NormArgs
     const void *gamma, *beta; // nullptr: 1 and 0
     float      *mean, *rstd;  // nullptr: not wanted
     float       epsilon;
-    int32_t     rows, columns;
+    int32_t     rows, columns, firstRow;
 };
 
 struct GradArgs
@@ -32,6 +34,345 @@ struct GradArgs
     void        *gradGamma, *gradBeta;
     int32_t      rows, columns, parts;
 };
+
+// The runs of a lane in a row that WAVES waves hold: run k is N elements from `first(k)` on. It is loaded from `from(k)` on, which
+// lies before that where the row ends within or before the run, so that no load stands under a condition; of what is loaded
+// the elements from skip(k) on are its own. Stores are of whole runs too: twice the same values where runs overlap.
+template<int N, int WAVES>
+struct RowRuns
+{
+    int columns, lane0;
+
+    __device__ __forceinline__ explicit RowRuns(int of)
+        : columns(of)
+        , lane0((int)((WAVES == 1 ? 0 : WaveOfGroup() * 64) + (threadIdx.x & 63)) * N)
+    {
+    }
+
+    __device__ __forceinline__ int first(int k) const
+    {
+        return k * WAVES * 64 * N + lane0;
+    }
+
+    __device__ __forceinline__ int from(int k) const
+    {
+        return min(first(k), columns - N);
+    }
+
+    __device__ __forceinline__ int skip(int k) const
+    {
+        return first(k) - from(k);
+    }
+
+    // all lanes' runs lie within the row
+    __device__ __forceinline__ bool whole(int k) const
+    {
+        return (k + 1) * WAVES * 64 * N <= columns;
+    }
+
+    template<class T>
+    __device__ __forceinline__ Run<T, N> get(const void *row, int k) const
+    {
+        return *reinterpret_cast<const Run<T, N> *>(static_cast<const T *>(row) + from(k));
+    }
+
+    template<class T>
+    __device__ __forceinline__ void put(void *row, int k, const float (&v)[N]) const
+    {
+        if (first(k) < columns)
+        {
+            Run<T, N> r;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                r.v[i] = FromFloat<T>(v[i]);
+            }
+            *reinterpret_cast<Run<T, N> *>(static_cast<T *>(row) + from(k)) = r;
+        }
+    }
+};
+
+// Sum over the WAVES waves of a row, in all of them. `part`: room for a sum of each, not read by anyone at the time.
+template<int WAVES>
+__device__ __forceinline__ float RowSum(float v, float (&part)[WAVES])
+{
+    v = WaveSum(v);
+    if constexpr (WAVES > 1)
+    {
+        part[WaveOfGroup()] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+        {
+            v += part[w];
+        }
+    }
+    return v;
+}
+
+constexpr int GroupWaves(int waves)
+{
+    return waves == 1 ? 4 : waves; // narrow rows: four to a workgroup
+}
+
+// E: elements in a lane.
+template<class T, class W, int WAVES, int E>
+__global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const NormArgs a)
+{
+    constexpr int    N = kRunOf<T>, K = E / N;
+    constexpr bool   kWeightsFirst = E <= 16; // on their way beside the row; more of them would take registers from other rows
+    __shared__ float s_sum[WAVES], s_squares[WAVES];
+    const RowRuns<N, WAVES> runs(a.columns);
+    const uint32_t          row = a.firstRow + (WAVES == 1 ? blockIdx.x * 4 + WaveOfGroup() : blockIdx.x);
+    if (row >= (uint32_t)a.rows)
+    {
+        return;
+    }
+    const uint8_t *from = a.in.at(row);
+    Run<T, N>      x[K];
+    Run<W, N>      gamma[K], beta[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+    {
+        x[k] = runs.template get<T>(from, k);
+    }
+    auto loadWeights = [&]
+    {
+        if (a.gamma != nullptr)
+        {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+            {
+                gamma[k] = runs.template get<W>(a.gamma, k);
+            }
+        }
+        if (a.beta != nullptr)
+        {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+            {
+                beta[k] = runs.template get<W>(a.beta, k);
+            }
+        }
+    };
+    if (kWeightsFirst)
+    {
+        loadWeights();
+    }
+    float s = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+    {
+        const int skip = runs.whole(k) ? 0 : runs.skip(k);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            s += i >= skip ? (float)x[k].v[i] : 0.f;
+        }
+    }
+    const float mean = RowSum<WAVES>(s, s_sum) / (float)a.columns;
+    s                = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+    {
+        const int skip = runs.whole(k) ? 0 : runs.skip(k);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const float d = i >= skip ? (float)x[k].v[i] - mean : 0.f;
+            s += d * d;
+        }
+    }
+    const float rstd = 1.f / sqrtf(RowSum<WAVES>(s, s_squares) / (float)a.columns + a.epsilon);
+    uint8_t    *to   = a.out.at(row);
+    if (!kWeightsFirst)
+    {
+        loadWeights();
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+    {
+        float y[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            y[i] = ((float)x[k].v[i] - mean) * rstd;
+        }
+        if (a.gamma != nullptr)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                y[i] *= (float)gamma[k].v[i];
+            }
+        }
+        if (a.beta != nullptr)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                y[i] += (float)beta[k].v[i];
+            }
+        }
+        runs.template put<T>(to, k, y);
+    }
+    if (runs.lane0 == 0)
+    {
+        if (a.mean != nullptr)
+        {
+            a.mean[row] = mean;
+        }
+        if (a.rstd != nullptr)
+        {
+            a.rstd[row] = rstd;
+        }
+    }
+}
+
+// The rows' gradient, and the sums over the rows that a workgroup goes through: every parts-th (in narrow rows each of its
+// waves takes one).
+template<class T, class W, int WAVES, int E>
+__global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(const GradArgs a)
+{
+    constexpr int    N = kRunOf<T>, K = E / N, kRows = WAVES == 1 ? 4 : 1;
+    __shared__ float s_sum[2][2][WAVES]; // of one row and the next
+    const RowRuns<N, WAVES> runs(a.columns);
+    const uint32_t          step = (uint32_t)a.parts * kRows;
+    uint32_t                row  = blockIdx.x * kRows + (WAVES == 1 ? WaveOfGroup() : 0);
+    float                   gamma[K][N], toGamma[K][N] = {}, toBeta[K][N] = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            gamma[k][i] = 1;
+        }
+    }
+    if (a.gamma != nullptr)
+    {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            const Run<W, N> g = runs.template get<W>(a.gamma, k);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                gamma[k][i] = (float)g.v[i];
+            }
+        }
+    }
+    Run<T, N> x[K], dy[K];
+    auto      load = [&](uint32_t r)
+    {
+        const uint8_t *px = a.in.at(r), *pdy = a.grad.at(r);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            x[k]  = runs.template get<T>(px, k);
+            dy[k] = runs.template get<T>(pdy, k);
+        }
+    };
+    if (row < (uint32_t)a.rows)
+    {
+        load(row);
+    }
+    for (int turn = 0; row < (uint32_t)a.rows; row += step, turn ^= 1)
+    {
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float       w[K][N], h[K][N], s = 0, sh = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            const int skip = runs.whole(k) ? 0 : runs.skip(k);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                const float d = (float)dy[k].v[i];
+                h[k][i]       = ((float)x[k].v[i] - mean) * rstd;
+                w[k][i]       = d * gamma[k][i];
+                toGamma[k][i] += d * h[k][i];
+                toBeta[k][i] += d;
+                s += i >= skip ? w[k][i] : 0.f;
+                sh += i >= skip ? w[k][i] * h[k][i] : 0.f;
+            }
+        }
+        const uint32_t next = row + step;
+        if (next < (uint32_t)a.rows)
+        {
+            load(next);
+        }
+        s  = WaveSum(s);
+        sh = WaveSum(sh);
+        if constexpr (WAVES > 1)
+        {
+            s_sum[turn][0][WaveOfGroup()] = s;
+            s_sum[turn][1][WaveOfGroup()] = sh;
+            __syncthreads();
+            s = sh = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i)
+            {
+                s += s_sum[turn][0][i];
+                sh += s_sum[turn][1][i];
+            }
+        }
+        s /= (float)a.columns;
+        sh /= (float)a.columns;
+        uint8_t *to = a.out.at(row);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                w[k][i] = rstd * (w[k][i] - s - h[k][i] * sh);
+            }
+            runs.template put<T>(to, k, w[k]);
+        }
+    }
+    if (a.partial == nullptr)
+    {
+        return;
+    }
+    if constexpr (WAVES == 1)
+    {
+        // the workgroup's four waves hold the same columns
+        __shared__ float s_part[4][64][N];
+        const uint32_t   wave = WaveOfGroup(), lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < 2 * K; ++j)
+        {
+            float(&v)[N] = j < K ? toGamma[j] : toBeta[j - K];
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                s_part[wave][lane][i] = v[i];
+            }
+            __syncthreads();
+            if (wave == (uint32_t)j % 4)
+            {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    v[i] = s_part[0][lane][i] + s_part[1][lane][i] + s_part[2][lane][i] + s_part[3][lane][i];
+                }
+                runs.template put<float>(a.partial + ((size_t)blockIdx.x * 2 + j / K) * a.columns, j % K, v);
+            }
+            __syncthreads();
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            runs.template put<float>(a.partial + (size_t)blockIdx.x * 2 * a.columns, k, toGamma[k]);
+            runs.template put<float>(a.partial + ((size_t)blockIdx.x * 2 + 1) * a.columns, k, toBeta[k]);
+        }
+    }
+}
 
 // Sum over a workgroup of 256, in every thread.
 __device__ __forceinline__ float BlockSum(float v)
@@ -47,8 +388,9 @@ __device__ __forceinline__ float BlockSum(float v)
     return part[0] + part[1] + part[2] + part[3];
 }
 
+// Rows too wide for registers, or narrower than a run: one workgroup per row, element by element, three times over the row.
 template<class T, class W>
-__global__ __launch_bounds__(256) void LayerNormKernel(const NormArgs a)
+__global__ __launch_bounds__(256) void LayerNormAnyKernel(const NormArgs a)
 {
     for (uint32_t r = blockIdx.x; r < (uint32_t)a.rows; r += gridDim.x)
     {
@@ -86,7 +428,7 @@ __global__ __launch_bounds__(256) void LayerNormKernel(const NormArgs a)
 }
 
 template<class T, class W>
-__global__ __launch_bounds__(256) void LayerNormGradKernel(const GradArgs a)
+__global__ __launch_bounds__(256) void LayerNormGradAnyKernel(const GradArgs a)
 {
     for (uint32_t r = blockIdx.x; r < (uint32_t)a.rows; r += gridDim.x)
     {
@@ -112,9 +454,9 @@ __global__ __launch_bounds__(256) void LayerNormGradKernel(const GradArgs a)
     }
 }
 
-// A thread per column and part of the rows.
+// The same rows' sums: a thread per column and part of the rows.
 template<class T>
-__global__ __launch_bounds__(256) void LayerNormPartsKernel(const GradArgs a)
+__global__ __launch_bounds__(256) void LayerNormPartsAnyKernel(const GradArgs a)
 {
     const int c = blockIdx.x * 256 + threadIdx.x, D = a.columns;
     if (c >= D)
@@ -132,27 +474,44 @@ __global__ __launch_bounds__(256) void LayerNormPartsKernel(const GradArgs a)
     a.partial[(size_t)blockIdx.y * 2 * D + D + c] = b;
 }
 
+// Adds up the parts' sums: 16 columns to a workgroup, whose 64 rows of 16 lanes take every 64th part each.
+constexpr int kJoinColumns = 16;
+
 template<class W>
-__global__ __launch_bounds__(256) void LayerNormJoinKernel(const GradArgs a)
+__global__ __launch_bounds__(1024) void LayerNormJoinKernel(const GradArgs a)
 {
-    const int c = blockIdx.x * 256 + threadIdx.x, D = a.columns;
-    if (c >= D)
+    __shared__ float s_part[64][kJoinColumns + 1];
+    const int64_t    all = 2 * (int64_t)a.columns;
+    const int        l = threadIdx.x % kJoinColumns, r = threadIdx.x / kJoinColumns;
+    for (int64_t first = (int64_t)blockIdx.x * kJoinColumns; first < all; first += (int64_t)gridDim.x * kJoinColumns)
     {
-        return;
-    }
-    float g = 0, b = 0;
-    for (int p = 0; p < a.parts; ++p)
-    {
-        g += a.partial[(size_t)p * 2 * D + c];
-        b += a.partial[(size_t)p * 2 * D + D + c];
-    }
-    if (a.gradGamma != nullptr)
-    {
-        static_cast<W *>(a.gradGamma)[c] = FromFloat<W>(g);
-    }
-    if (a.gradBeta != nullptr)
-    {
-        static_cast<W *>(a.gradBeta)[c] = FromFloat<W>(b);
+        const int64_t c = min(first + l, all - 1);
+        float         s = 0;
+#pragma unroll 8
+        for (int p = r; p < a.parts; p += 64)
+        {
+            s += a.partial[(size_t)p * all + c];
+        }
+        s_part[r][l] = s;
+        __syncthreads();
+#pragma unroll
+        for (int n = 32; n > 0; n >>= 1)
+        {
+            if (r < n)
+            {
+                s_part[r][l] += s_part[r + n][l];
+            }
+            __syncthreads();
+        }
+        if (r == 0 && first + l < all)
+        {
+            void *to = c < a.columns ? a.gradGamma : a.gradBeta;
+            if (to != nullptr)
+            {
+                static_cast<W *>(to)[c < a.columns ? c : c - a.columns] = FromFloat<W>(s_part[0][l]);
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -160,9 +519,33 @@ __global__ __launch_bounds__(256) void LayerNormJoinKernel(const GradArgs a)
 constexpr int kMostGroups = 1 << 20;
 
 // ---- host ----------------------------------------------------------------------------------------------------------
+// What a kernel of rows is built for: waves to a row and elements to a lane. 0 waves: the kernels for any width.
+struct RowShape
+{
+    int waves, elements;
+};
+
+// The fewest waves whose lanes hold the row with 16 elements each, 32 where the widest workgroup needs them.
+RowShape ShapeOf(int64_t columns, int run, int widest)
+{
+    if (columns < run || columns > widest * 64 * 32)
+    {
+        return {0, 0};
+    }
+    const int waves = columns <= 64 * 16 ? 1 : columns <= 4 * 64 * 16 ? 4 : widest;
+    return {waves, columns <= waves * 64 * 8 ? 8 : columns <= waves * 64 * 16 ? 16 : 32};
+}
+
+// Waves of the widest workgroup. The gradient's lanes also hold two sums for each element: with sixteen waves, 128 registers
+// to a lane, they would not fit.
+constexpr int kNormWidest = 16, kGradWidest = 8;
+
+constexpr int kMostParts = 1024;
+
+// Workgroups that share the rows: one for four rows at least, four to a CU at most.
 int Parts(int64_t rows)
 {
-    return (int)std::min<int64_t>(rows, 256);
+    return (int)std::min<int64_t>((rows + 3) / 4, kMostParts);
 }
 
 int64_t GradWorkspace(int64_t rows, int64_t columns)
@@ -170,32 +553,87 @@ int64_t GradWorkspace(int64_t rows, int64_t columns)
     return (int64_t)Parts(rows) * 2 * columns * (int64_t)sizeof(float);
 }
 
+template<class T, class W, int WAVES, int E>
+void LaunchNormAs(const NormArgs &a, hipStream_t stream)
+{
+    const int64_t groups = WAVES == 1 ? ((int64_t)a.rows + 3) / 4 : a.rows;
+    // (rows beyond what a launch may hold go into further ones)
+    constexpr int64_t kMost = ((int64_t)1 << 32) / (64 * GroupWaves(WAVES)) - 1;
+    for (int64_t first = 0; first < groups; first += kMost)
+    {
+        NormArgs b = a;
+        b.firstRow = (int32_t)(first * (WAVES == 1 ? 4 : 1));
+        hipLaunchKernelGGL((LayerNormKernel<T, W, WAVES, E>), dim3((uint32_t)std::min(groups - first, kMost)), dim3(64 * GroupWaves(WAVES)), 0, stream, b);
+        CheckLaunch("LayerNormKernel");
+    }
+}
+
 template<class T, class W>
 void LaunchNorm(const NormArgs &a, hipStream_t stream)
 {
-    hipLaunchKernelGGL((LayerNormKernel<T, W>), dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, stream, a);
-    CheckLaunch("LayerNormKernel");
+    const RowShape s = ShapeOf(a.columns, kRunOf<T>, kNormWidest);
+    if (s.waves == 0)
+    {
+        hipLaunchKernelGGL((LayerNormAnyKernel<T, W>), dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, stream, a);
+        CheckLaunch("LayerNormAnyKernel");
+    }
+    else if (s.waves == 1)
+    {
+        s.elements == 8 ? LaunchNormAs<T, W, 1, 8>(a, stream) : LaunchNormAs<T, W, 1, 16>(a, stream);
+    }
+    else if (s.waves == 4)
+    {
+        s.elements == 8 ? LaunchNormAs<T, W, 4, 8>(a, stream) : LaunchNormAs<T, W, 4, 16>(a, stream);
+    }
+    else
+    {
+        s.elements <= 16 ? LaunchNormAs<T, W, kNormWidest, 16>(a, stream) : LaunchNormAs<T, W, kNormWidest, 32>(a, stream);
+    }
+}
+
+template<class T, class W, int WAVES, int E>
+void LaunchGradAs(const GradArgs &a, hipStream_t stream)
+{
+    hipLaunchKernelGGL((LayerNormGradKernel<T, W, WAVES, E>), dim3(a.parts), dim3(64 * GroupWaves(WAVES)), 0, stream, a);
+    CheckLaunch("LayerNormGradKernel");
 }
 
 template<class T, class W>
 void LaunchGrad(const GradArgs &a, hipStream_t stream)
 {
-    // gradIn may be written over gradOut or in: the sums over rows come first
-    if (a.gradGamma != nullptr || a.gradBeta != nullptr)
+    const RowShape s    = ShapeOf(a.columns, kRunOf<T>, kGradWidest);
+    const bool     sums = a.gradGamma != nullptr || a.gradBeta != nullptr;
+    if (a.rows == 0)
     {
-        const int tiles = DivUp(a.columns, 256);
-        if (a.parts > 0)
-        {
-            hipLaunchKernelGGL((LayerNormPartsKernel<T>), dim3(tiles, a.parts), dim3(256), 0, stream, a);
-            CheckLaunch("LayerNormPartsKernel");
-        }
-        hipLaunchKernelGGL((LayerNormJoinKernel<W>), dim3(tiles), dim3(256), 0, stream, a);
-        CheckLaunch("LayerNormJoinKernel");
     }
-    if (a.rows > 0)
+    else if (s.waves == 0)
     {
-        hipLaunchKernelGGL((LayerNormGradKernel<T, W>), dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, stream, a);
-        CheckLaunch("LayerNormGradKernel");
+        // gradIn may be written over gradOut or in: the sums over rows come first
+        if (sums)
+        {
+            hipLaunchKernelGGL((LayerNormPartsAnyKernel<T>), dim3(DivUp(a.columns, 256), a.parts), dim3(256), 0, stream, a);
+            CheckLaunch("LayerNormPartsAnyKernel");
+        }
+        hipLaunchKernelGGL((LayerNormGradAnyKernel<T, W>), dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, stream, a);
+        CheckLaunch("LayerNormGradAnyKernel");
+    }
+    else if (s.waves == 1)
+    {
+        s.elements == 8 ? LaunchGradAs<T, W, 1, 8>(a, stream) : LaunchGradAs<T, W, 1, 16>(a, stream);
+    }
+    else if (s.waves == 4)
+    {
+        s.elements == 8 ? LaunchGradAs<T, W, 4, 8>(a, stream) : LaunchGradAs<T, W, 4, 16>(a, stream);
+    }
+    else
+    {
+        s.elements <= 16 ? LaunchGradAs<T, W, kGradWidest, 16>(a, stream) : LaunchGradAs<T, W, kGradWidest, 32>(a, stream);
+    }
+    if (sums)
+    {
+        const int64_t groups = (2 * (int64_t)a.columns + kJoinColumns - 1) / kJoinColumns;
+        hipLaunchKernelGGL((LayerNormJoinKernel<W>), dim3((uint32_t)std::min<int64_t>(groups, kMostGroups)), dim3(1024), 0, stream, a);
+        CheckLaunch("LayerNormJoinKernel");
     }
 }
 
@@ -288,7 +726,7 @@ public:
         {
             return;
         }
-        const NormArgs a = {RowPlaces(in), RowPlaces(out), gamma, beta, mean, rstd, epsilon, in.rows, in.columns};
+        const NormArgs a = {RowPlaces(in), RowPlaces(out), gamma, beta, mean, rstd, epsilon, in.rows, in.columns, 0};
         Dispatch(in.elem, w.same(), [&](auto t, auto wt) { LaunchNorm<decltype(t), decltype(wt)>(a, stream); });
     }
 };
