@@ -580,6 +580,7 @@ class WarpPerspective(_Operator):
 class LayerNorm(_Operator):
     """Extension: cvcuda/LayerNorm.h. None stands for a tensor that is left out."""
     _create = "cvcudaxLayerNormCreate"
+    _native = 10
 
     def __call__(self, stream, inp, gamma, beta, out, mean=None, rstd=None, epsilon=1e-5):
         check(_cv.cvcudaxLayerNormSubmit(self.handle, stream_ptr(stream), _h(inp), _h(gamma), _h(beta), _h(out), _h(mean),
@@ -589,6 +590,7 @@ class LayerNorm(_Operator):
 class LayerNormGrad(_Operator):
     """Extension: cvcuda/LayerNorm.h, the gradient."""
     _create = "cvcudaxLayerNormCreate"
+    _native = 11
 
     @staticmethod
     def workspace(rows, columns):
@@ -605,6 +607,7 @@ class LayerNormGrad(_Operator):
 class Embedding(_Operator):
     """Extension: cvcuda/Embedding.h."""
     _create = "cvcudaxEmbeddingCreate"
+    _native = 12
 
     def __call__(self, stream, table, tokens, out, scale=1.0):
         check(_cv.cvcudaxEmbeddingSubmit(self.handle, stream_ptr(stream), _h(table), _h(tokens), _h(out), scale))
@@ -613,6 +616,7 @@ class Embedding(_Operator):
 class EmbeddingGrad(_Operator):
     """Extension: cvcuda/Embedding.h, the gradient. padding: a token, or -1 for none."""
     _create = "cvcudaxEmbeddingCreate"
+    _native = 13
 
     @staticmethod
     def workspace(tokens, vocabulary, columns):
@@ -638,6 +642,7 @@ def _handles(tensors, count):
 class AdamW(_Operator):
     """Extension: cvcuda/AdamW.h, over lists of tensors."""
     _create = "cvcudaxAdamWCreate"
+    _native = 14
 
     def __call__(self, stream, params, moments, variances, grads, copies, moment_scales, variance_scales, grad_scale, step, lr,
                  beta1, beta2, epsilon, weight_decay):
@@ -651,6 +656,7 @@ class AdamW(_Operator):
 class AdamWUnpack(_Operator):
     """Extension: cvcuda/AdamW.h, the values of 8-bit states."""
     _create = "cvcudaxAdamWCreate"
+    _native = 15
 
     def __call__(self, stream, codes, scales, out):
         n = len(codes)

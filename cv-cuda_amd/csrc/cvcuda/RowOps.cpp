@@ -110,8 +110,11 @@ DenseView RequireDense(NVCVTensorHandle h, const char *what, NVCVDataType dt)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must hold values of type %s", what, nvcvDataTypeGetName(dt));
     }
-    int32_t es = 0;
-    CheckCore(nvcvDataTypeGetStrideBytes(d.dtype, &es));
+    int32_t es = RowElemOf(d.dtype) != kRowNone ? RowElemSize(RowElemOf(d.dtype)) : 0; // (the others' sizes are looked up)
+    if (es == 0)
+    {
+        CheckCore(nvcvDataTypeGetStrideBytes(d.dtype, &es));
+    }
     DenseView v = {d.buffer.strided.basePtr, CountOf(d, what), d.dtype};
     int64_t   want = es;
     for (int i = d.rank - 1; i >= 0 && v.count > 0; --i)

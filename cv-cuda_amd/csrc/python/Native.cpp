@@ -1,5 +1,5 @@
 // The part of the Python interface that runs for every call: operators submitted on the default stream without a wait, the
-// planes of a list of torch tensors and batches of them, tensors of the library's own memory, the results that are handed out
+// planes of a list of torch tensors and batches of them, tensors over torch's memory and of the library's own, the results that are handed out
 // again and torch's views of them. In Python one call of an operator was 5.3 to 6.2 us of the interpreter beside 2 to 3 us of the
 // library, a result tensor 2.0 us, a batch of 61 images another 43 us.
 //
@@ -9,6 +9,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <cvcuda/AdamW.h>
+#include <cvcuda/Embedding.h>
+#include <cvcuda/LayerNorm.h>
 #include <cvcuda/OpConvertTo.h>
 #include <cvcuda/OpCropFlipNormalizeReformat.h>
 #include <cvcuda/OpCvtColor.h>
@@ -25,13 +28,14 @@
 #include <climits>
 #include <cstring>
 #include <memory>
+#include <vector>
 
 namespace {
 
 // names of pyapi and of the containers
 PyObject *s_submit, *s_Tensor, *s_ImageBatchVarShape, *s_lock, *s_followed, *s_tls, *s_stack, *s_check, *s_t, *s_handle, *s_wrote, *s_read,
     *s_kind, *s_acquire, *s_release, *s_torch, *s_C, *s_getDevice, *s_getStream, *s_value, *s_key, *s_meta, *s_nbytes, *s_np, *s_dtype, *s_made,
-    *s_sizeOf;
+    *s_sizeOf, *s_core, *s_voidp, *s_wrapped, *s_keep;
 
 // A new reference that goes with the scope.
 struct Ref
@@ -125,6 +129,27 @@ bool Pointer(PyObject *obj, void *&p)
     return true;
 }
 
+// The library's handle of a tensor of pyapi (`type`: that class), or of None where that may be: nullptr.
+bool TensorOf(PyObject *type, PyObject *obj, void *&handle, bool orNone = false)
+{
+    if (orNone && obj == Py_None)
+    {
+        handle = nullptr;
+        return true;
+    }
+    if (Py_TYPE(obj) != reinterpret_cast<PyTypeObject *>(type))
+    {
+        return false;
+    }
+    Ref inner(PyObject_GetAttr(obj, s_t));
+    if (!inner)
+    {
+        PyErr_Clear();
+        return false;
+    }
+    return Pointer(inner.o, handle) && handle != nullptr;
+}
+
 // The library's handle of a container of pyapi.
 Kind HandleOf(PyObject *api, PyObject *obj, void *&handle)
 {
@@ -152,6 +177,17 @@ bool Int(PyObject *o, int &v)
         return false;
     }
     return l >= INT_MIN && l <= INT_MAX;
+}
+
+bool Whole(PyObject *o, long long &v)
+{
+    v = PyLong_CheckExact(o) ? PyLong_AsLongLong(o) : 0;
+    if (v == -1 && PyErr_Occurred())
+    {
+        PyErr_Clear();
+        return false;
+    }
+    return PyLong_CheckExact(o);
 }
 
 bool Real(PyObject *o, double &v)
@@ -189,11 +225,58 @@ struct Call
 {
     int                kind;
     NVCVOperatorHandle op;
-    void              *h[5];
+    void              *h[9];
     bool               batch, flag;
     int                i[6];
-    double             d[4];
+    double             d[5];
     float              m[9], bv[4];
+    long long          whole;
+    std::vector<void *> lists[7];
+    bool                listed[7];
+
+    // `n` tensors into h, each or None where `optional` has its bit.
+    bool Tensors(PyObject *api, PyObject *const *a, int n, unsigned optional)
+    {
+        PyObject *type = Name(api, s_Tensor);
+        bool      ok   = type != nullptr;
+        for (int k = 0; ok && k < n; ++k)
+        {
+            ok = TensorOf(type, a[k], h[k], (optional >> k) & 1);
+        }
+        return ok;
+    }
+
+    // `n` lists of one length of tensors into `lists`; None instead, and in them, where `optional` has a list's bit.
+    bool Lists(PyObject *api, PyObject *const *a, int n, unsigned optional)
+    {
+        PyObject *type = Name(api, s_Tensor);
+        for (int k = 0; k < n; ++k)
+        {
+            listed[k] = a[k] != Py_None;
+            if (!listed[k] && ((optional >> k) & 1))
+            {
+                continue;
+            }
+            if (type == nullptr || !PyList_CheckExact(a[k]) || PyList_GET_SIZE(a[k]) != PyList_GET_SIZE(a[0]) || PyList_GET_SIZE(a[k]) > INT_MAX)
+            {
+                return false;
+            }
+            lists[k].resize((size_t)PyList_GET_SIZE(a[k]));
+            for (size_t i = 0; i < lists[k].size(); ++i)
+            {
+                if (!TensorOf(type, PyList_GET_ITEM(a[k], (Py_ssize_t)i), lists[k][i], (optional >> k) & 1))
+                {
+                    return false;
+                }
+            }
+        }
+        return true;
+    }
+
+    const NVCVTensorHandle *List(int k) const
+    {
+        return listed[k] ? reinterpret_cast<const NVCVTensorHandle *>(lists[k].data()) : nullptr;
+    }
 
     bool Parse(PyObject *api, PyObject *const *a, Py_ssize_t n)
     {
@@ -237,6 +320,20 @@ struct Call
         case 9: // WarpPerspective
             return n == 6 && handles({0, 1}) && (batch ? HandleOf(api, a[2], h[2]) != kNone : Reals(a[2], m, kind == 8 ? 6 : 9)) && Int(a[3], i[0])
                 && Int(a[4], i[1]) && Reals(a[5], bv, 4);
+        case 10: // LayerNorm
+            return n == 7 && Tensors(api, a, 6, 0b110110) && Real(a[6], d[0]);
+        case 11: // LayerNormGrad
+            return n == 9 && Tensors(api, a, 9, 0b111000100) && h[5] != nullptr;
+        case 12: // Embedding
+            return n == 4 && Tensors(api, a, 3, 0) && Real(a[3], d[0]);
+        case 13: // EmbeddingGrad
+            flag = n == 7 && a[6] == Py_True;
+            return n == 7 && Tensors(api, a, 4, 0b1000) && Real(a[4], d[0]) && Whole(a[5], whole) && PyBool_Check(a[6]);
+        case 14: // AdamW
+            return n == 14 && Lists(api, a, 7, 0b1110000) && Tensors(api, a + 7, 1, 1) && Whole(a[8], whole) && Real(a[9], d[0])
+                && Real(a[10], d[1]) && Real(a[11], d[2]) && Real(a[12], d[3]) && Real(a[13], d[4]);
+        case 15: // AdamWUnpack
+            return n == 3 && Lists(api, a, 3, 0);
         default:
             return false;
         }
@@ -285,6 +382,23 @@ struct Call
             return cvcudaCropFlipNormalizeReformatSubmit(op, nullptr, As<B>(0), As<T>(1), As<T>(2), (NVCVBorderType)i[0], (float)d[0],
                                                          As<T>(3), As<T>(4), reinterpret_cast<T>(h4), (float)d[1], (float)d[2], (float)d[3],
                                                          (uint32_t)i[1]);
+        case 10:
+            return cvcudaxLayerNormSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), As<T>(3), As<T>(4), As<T>(5), (float)d[0]);
+        case 11:
+            return cvcudaxLayerNormGradSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), As<T>(3), As<T>(4), As<T>(5), As<T>(6), As<T>(7),
+                                              As<T>(8));
+        case 12:
+            return cvcudaxEmbeddingSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), (float)d[0]);
+        case 13:
+            return cvcudaxEmbeddingGradSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), As<T>(3), (float)d[0], whole, flag);
+        case 14:
+        {
+            const CVCUDAXAdamW step = {d[0], d[1], d[2], d[3], d[4], whole};
+            return cvcudaxAdamWSubmit(op, nullptr, (int32_t)lists[0].size(), List(0), List(1), List(2), List(3), List(4), List(5), List(6),
+                                      As<T>(0), &step);
+        }
+        case 15:
+            return cvcudaxAdamWUnpackSubmit(op, nullptr, (int32_t)lists[0].size(), List(0), List(1), List(2));
         default:
         {
             const float4 c = {bv[0], bv[1], bv[2], bv[3]};
@@ -668,6 +782,112 @@ PyObject *TorchView(PyObject *, PyObject *args)
     }
 }
 
+// wrap(torch tensor, layout): a tensor of pyapi over its memory, which keeps it (pyapi.as_tensor); None where Python has to look
+// at it: no memory on the GPU, no elements, a type that has no other name here.
+PyObject *WrapTorch(PyObject *api, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 2 || !PyUnicode_Check(a[1]))
+    {
+        PyErr_SetString(PyExc_TypeError, "wrap(tensor, layout)");
+        return nullptr;
+    }
+    Py_ssize_t  letters = 0;
+    const char *layout  = PyUnicode_AsUTF8AndSize(a[1], &letters);
+    PyObject   *types = Name(api, s_wrapped), *core = Name(api, s_core), *type = Name(api, s_Tensor), *voidp = Name(api, s_voidp);
+    if (layout == nullptr || types == nullptr || core == nullptr || type == nullptr || voidp == nullptr || !PyType_Check(core) || !PyType_Check(type))
+    {
+        return PyErr_Occurred() ? nullptr : (PyErr_SetString(PyExc_RuntimeError, "pyapi is gone"), nullptr);
+    }
+    if (!THPVariable_Check(a[0]) || letters > NVCV_TENSOR_MAX_RANK)
+    {
+        Py_RETURN_NONE;
+    }
+    Ref dtype(PyObject_GetAttr(a[0], s_dtype));
+    if (!dtype)
+    {
+        return nullptr;
+    }
+    PyObject *known = PyDict_GetItemWithError(types, dtype.o); // (data type, element type)
+    if (known == nullptr)
+    {
+        return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
+    }
+    NVCVTensorData data  = {};
+    Ref            shape(nullptr);
+    try
+    {
+        const at::Tensor &t = THPVariable_Unpack(a[0]);
+        if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() < 1 || t.dim() > NVCV_TENSOR_MAX_RANK || t.numel() == 0)
+        {
+            Py_RETURN_NONE;
+        }
+        data.rank = (int32_t)t.dim();
+        shape.o   = PyTuple_New(data.rank);
+        if (!shape)
+        {
+            return nullptr;
+        }
+        const int64_t size = (int64_t)t.element_size();
+        for (int32_t k = 0; k < data.rank; ++k)
+        {
+            data.shape[k]                  = t.size(k);
+            data.buffer.strided.strides[k] = t.stride(k) * size;
+            PyObject *extent               = PyLong_FromLongLong(t.size(k));
+            if (extent == nullptr)
+            {
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(shape.o, k, extent);
+        }
+        data.buffer.strided.basePtr = static_cast<decltype(data.buffer.strided.basePtr)>(t.data_ptr());
+    }
+    catch (const std::exception &)
+    {
+        Py_RETURN_NONE; // (a tensor without memory of its own ...)
+    }
+    data.dtype       = PyTuple_CheckExact(known) && PyTuple_GET_SIZE(known) == 2 ? PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(known, 0)) : 0;
+    data.layout.rank = (int32_t)letters;
+    std::memcpy(data.layout.data, layout, (size_t)letters);
+    data.bufferType = NVCV_TENSOR_BUFFER_STRIDED_CUDA;
+    if (PyErr_Occurred())
+    {
+        return nullptr;
+    }
+    NVCVTensorHandle handle = nullptr;
+    const NVCVStatus status = nvcvTensorWrapDataConstruct(&data, nullptr, nullptr, &handle);
+    if (status != NVCV_SUCCESS)
+    {
+        PyObject *check = Name(api, s_check);
+        Ref       value(PyLong_FromLong((long)status));
+        Ref       raised(check != nullptr && value ? PyObject_CallOneArg(check, value.o) : nullptr);
+        if (!PyErr_Occurred())
+        {
+            PyErr_SetString(PyExc_RuntimeError, "the tensor cannot be wrapped");
+        }
+        return nullptr;
+    }
+    Ref none(PyTuple_New(0)), number(PyLong_FromVoidPtr(handle)), pointer(number ? PyObject_CallOneArg(voidp, number.o) : nullptr);
+    Ref raw(none ? reinterpret_cast<PyTypeObject *>(core)->tp_new(reinterpret_cast<PyTypeObject *>(core), none.o, nullptr) : nullptr);
+    Ref attributes(raw ? PyObject_GenericGetDict(raw.o, nullptr) : nullptr), kept(PyList_New(1));
+    if (!pointer || !attributes || !kept || PyDict_SetItem(attributes.o, s_handle, pointer.o) < 0)
+    {
+        (void)nvcvTensorDecRef(handle, nullptr);
+        return nullptr;
+    }
+    Py_INCREF(a[0]); // (from here on the handle is raw's)
+    PyList_SET_ITEM(kept.o, 0, a[0]);
+    Ref out(reinterpret_cast<PyTypeObject *>(type)->tp_new(reinterpret_cast<PyTypeObject *>(type), none.o, nullptr));
+    Ref own(out ? PyObject_GenericGetDict(out.o, nullptr) : nullptr);
+    Ref meta(PyTuple_Pack(3, shape.o, PyTuple_GET_ITEM(known, 1), letters > 0 ? a[1] : Py_None));
+    if (PyDict_SetItem(attributes.o, s_keep, kept.o) < 0 || !own || !meta || PyDict_SetItem(own.o, s_t, raw.o) < 0
+        || PyDict_SetItem(own.o, s_meta, meta.o) < 0)
+    {
+        return nullptr;
+    }
+    Py_INCREF(out.o);
+    return out.o;
+}
+
 // batch_alloc(capacity): (status, handle) of an image batch.
 PyObject *BatchAlloc(PyObject *, PyObject *capacity)
 {
@@ -1019,9 +1239,10 @@ PyType_Spec kOutputsSpec = {"_cvcuda_native.Outputs", sizeof(Outputs), 0, Py_TPF
 PyMethodDef kBound[] = {
     {"submit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Submit)), METH_FASTCALL, nullptr},
     {"default_stream_key", DefaultKey, METH_NOARGS, nullptr},
+    {"wrap", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(WrapTorch)), METH_FASTCALL, nullptr},
 };
 
-// bind(pyapi's dictionary): (submit, default_stream_key) for it.
+// bind(pyapi's dictionary): (submit, default_stream_key, wrap) for it.
 PyObject *Bind(PyObject *, PyObject *names)
 {
     if (!PyDict_Check(names))
@@ -1029,8 +1250,8 @@ PyObject *Bind(PyObject *, PyObject *names)
         PyErr_SetString(PyExc_TypeError, "bind(dict)");
         return nullptr;
     }
-    Ref submit(PyCFunction_New(&kBound[0], names)), key(PyCFunction_New(&kBound[1], names));
-    return submit && key ? PyTuple_Pack(2, submit.o, key.o) : nullptr;
+    Ref submit(PyCFunction_New(&kBound[0], names)), key(PyCFunction_New(&kBound[1], names)), wrap(PyCFunction_New(&kBound[2], names));
+    return submit && key && wrap ? PyTuple_Pack(3, submit.o, key.o, wrap.o) : nullptr;
 }
 
 PyMethodDef kMethods[] = {
@@ -1066,7 +1287,8 @@ PyMODINIT_FUNC PyInit__cvcuda_native(void)
         {&s_getStream, "_cuda_getCurrentRawStream"},
         {&s_value, "value"},      {&s_key, "_key"},        {&s_meta, "_meta"},
         {&s_nbytes, "_nbytes"},   {&s_np, "np"},           {&s_dtype, "dtype"},
-        {&s_made, "_new_result"}, {&s_sizeOf, "_bytes_of"},
+        {&s_made, "_new_result"}, {&s_sizeOf, "_bytes_of"}, {&s_core, "_CoreTensor"},
+        {&s_voidp, "_c_void_p"},  {&s_wrapped, "_WRAPPED"}, {&s_keep, "_keep"},
     };
     for (const auto &n : names)
     {

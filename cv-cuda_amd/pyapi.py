@@ -18,6 +18,7 @@ raised as the same types here.
 import ctypes as C
 import enum
 import functools
+import math
 import re
 import threading
 
@@ -31,7 +32,7 @@ from . import (AdamW, AdamWUnpack, CenterCrop, ConvertTo, CropFlipNormalizeRefor
 from . import Image as _Image
 from . import ImageBatchVarShape as _ImageBatchVarShape
 from . import Tensor as _Tensor
-from . import _DT2NP, check
+from . import _DT2NP, _NP2DT, _NP2TORCH, check
 from ._capi import native as _native, native_missing as _native_missing
 from ._capi import nvcv as _nv
 
@@ -378,6 +379,9 @@ class Tensor:
 
 
 _CoreTensor = _Tensor
+_c_void_p = C.c_void_p
+# (data type, element type) of a torch tensor's; others go through numpy's names
+_WRAPPED = {t: (_NP2DT[d], d) for d, t in _NP2TORCH.items()}
 _DIRECT_VIEW = {np.dtype(np.uint8): 0, np.dtype(np.float32): 1}
 
 
@@ -458,7 +462,8 @@ def as_tensor(obj, layout=None):
         wrapped._keep.append(obj)
         return Tensor(_wrap=wrapped)
     if isinstance(obj, torch.Tensor):
-        return Tensor(_wrap=_Tensor.from_torch(obj, layout or ""))
+        wrapped = _wrap_torch(obj, layout or "")
+        return wrapped if wrapped is not None else Tensor(_wrap=_Tensor.from_torch(obj, layout or ""))
     if hasattr(obj, "__cuda_array_interface__"):
         return Tensor(_wrap=_Tensor.from_cuda_array_interface(obj, layout or ""))
     return Tensor(_wrap=_Tensor.from_torch(torch.from_dlpack(obj), layout or ""))
@@ -827,7 +832,7 @@ def _same_images(src, fmt=None, sizes=None):
 
 
 # what every operator below goes through: _submit, in native code for calls on the default stream that wait for nothing
-_run, _native_stream_key = _native.bind(globals())
+_run, _native_stream_key, _wrap_torch = _native.bind(globals())
 
 
 def _image_axes(layout):
@@ -1127,10 +1132,11 @@ def _workspace(workspace, size, stream):
 def _rows_of(tensor):
     """(rows, elements in a row)"""
     shape = tensor.shape
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    return rows, shape[-1]
+    return math.prod(shape[:-1]), shape[-1]
+
+
+_layer_norm_workspace = functools.lru_cache(256)(LayerNormGrad.workspace)
+_embedding_workspace = functools.lru_cache(256)(EmbeddingGrad.workspace)
 
 
 def layer_norm_into(dst, src, gamma=None, beta=None, epsilon=1e-5, *, mean=None, rstd=None, stream=None):
@@ -1148,7 +1154,7 @@ def layer_norm_grad_into(grad_src, grad_gamma, grad_beta, grad, src, gamma, mean
     """The gradients of layer_norm from `grad`, that of its result; `mean` and `rstd` as the forward call gave them.
     `grad_gamma`, `grad_beta` and `gamma` may be None. `grad_src` may be `grad` or `src`."""
     sums = grad_gamma is not None or grad_beta is not None
-    workspace = _workspace(workspace, LayerNormGrad.workspace(*_rows_of(src)) if sums else 0, stream)
+    workspace = _workspace(workspace, _layer_norm_workspace(*_rows_of(src)) if sums else 0, stream)
     _run(stream, _given(grad, src, gamma, mean, rstd), _given(grad_src, grad_gamma, grad_beta, workspace), _op(LayerNormGrad), grad, src,
          gamma, mean, rstd, grad_src, grad_gamma, grad_beta, workspace)
     return grad_src, grad_gamma, grad_beta
@@ -1180,7 +1186,7 @@ def embedding_grad_into(grad_table, grad, tokens, scale=1.0, *, padding=None, ac
     if padding is not None and padding < 0:
         raise ValueError("padding is a token, or None")
     rows, columns = _rows_of(grad)
-    workspace = _workspace(workspace, EmbeddingGrad.workspace(rows, _rows_of(grad_table)[0], columns), stream)
+    workspace = _workspace(workspace, _embedding_workspace(rows, _rows_of(grad_table)[0], columns), stream)
     reads, writes = [grad, tokens], _given(grad_table, workspace)
     _run(stream, reads, writes, _op(EmbeddingGrad), grad, tokens, grad_table, workspace, float(scale), -1 if padding is None else int(padding),
          bool(accumulate))
@@ -1199,15 +1205,17 @@ def adamw_into(params, moments, variances, grads, step, lr=1e-3, betas=(0.9, 0.9
     the first. States are F32, or in 8 bits: int8 moments and uint8 variances with F32 scales of an element for each 256.
     `copies`: tensors of F16 or BF16 that receive the new params (None in the list: no copy of that one). `grad_scale`: an F32
     tensor of one element that the gradients are multiplied with. What is computed exactly: cvcuda/AdamW.h."""
-    lists = [params, moments, variances, grads, copies, moment_scales, variance_scales]
-    for part in lists[1:]:
+    lists = [part if part is None or type(part) is list else list(part)
+             for part in (params, moments, variances, grads, copies, moment_scales, variance_scales)]
+    params, moments, variances, grads, copies, moment_scales, variance_scales = lists
+    for part in lists:
         if part is not None and len(part) != len(params):
             raise ValueError("lists of %d and %d tensors" % (len(params), len(part)))
-    writes = [t for part in (params, moments, variances, copies, moment_scales, variance_scales) if part is not None for t in part
-              if t is not None]
-    raw = [None if part is None else [t if t is None else t._t for t in part] for part in lists]
-    _run(stream, list(grads) + _given(grad_scale), writes, _op(AdamW), *raw, grad_scale, int(step), float(lr), float(betas[0]),
-         float(betas[1]), float(epsilon), float(weight_decay))
+    writes = params + moments + variances + (moment_scales or []) + (variance_scales or [])
+    if copies is not None:
+        writes += [t for t in copies if t is not None]
+    _run(stream, grads if grad_scale is None else grads + [grad_scale], writes, _op(AdamW), *lists, grad_scale, int(step), float(lr),
+         float(betas[0]), float(betas[1]), float(epsilon), float(weight_decay))
     return params
 
 
@@ -1215,6 +1223,6 @@ def adamw_unpack_into(dst, codes, scales, *, stream=None):
     """The F32 values that 8-bit states stand for, over lists of tensors: moments (int8) or variances (uint8)."""
     if not len(dst) == len(codes) == len(scales):
         raise ValueError("lists of %d, %d and %d tensors" % (len(dst), len(codes), len(scales)))
-    _run(stream, list(codes) + list(scales), list(dst), _op(AdamWUnpack), [t._t for t in codes], [t._t for t in scales],
-         [t._t for t in dst])
+    codes, scales, made = list(codes), list(scales), list(dst)
+    _run(stream, codes + scales, made, _op(AdamWUnpack), codes, scales, made)
     return dst

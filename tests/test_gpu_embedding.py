@@ -20,6 +20,11 @@ def api(cv, gpu):
     return importlib.import_module("cvcuda_amd.pyapi")
 
 
+@pytest.fixture(autouse=True)
+def no_default_stream_is_followed(api, monkeypatch):
+    monkeypatch.setattr(api, "_followed", {})  # (a wait for the default stream has the calls after it record events)
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 

@@ -18,6 +18,11 @@ def api(cv, gpu):
     return importlib.import_module("cvcuda_amd.pyapi")
 
 
+@pytest.fixture(autouse=True)
+def no_default_stream_is_followed(api, monkeypatch):
+    monkeypatch.setattr(api, "_followed", {})  # (a wait for the default stream has the calls after it record events)
+
+
 def rows_of(shape, dtype, seed, offset=0.3, scale=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     return (torch.randn(shape, generator=g, device="cuda") * scale + offset).to(dtype)

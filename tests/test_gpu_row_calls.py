@@ -1,0 +1,115 @@
+"""The row operators' calls by native code do what pyapi._submit does, and torch tensors wrapped by native code are what
+Python makes of them."""
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def api(cv, gpu):
+    return importlib.import_module("cvcuda_amd.pyapi")
+
+
+@pytest.fixture(autouse=True)
+def no_default_stream_is_followed(api, monkeypatch):
+    monkeypatch.setattr(api, "_followed", {})
+
+
+def calls(api):
+    """(call, its results) of every form, on fresh tensors."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def t(*shape, dtype=torch.float32, scale=1.0):
+        return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+    wrap = api.as_tensor
+    x, dy, gamma, beta = wrap(t(7, 40)), wrap(t(7, 40)), wrap(t(40)), wrap(t(40))
+    out, mean, rstd, dx, dg, db = (wrap(t(*s)) for s in ((7, 40), (7,), (7,), (7, 40), (40,), (40,)))
+    table, tokens, rows, grad = wrap(t(9, 40)), wrap(torch.arange(7, device="cuda") % 3), wrap(t(7, 40)), wrap(t(9, 40))
+    stats = wrap(t(7)), wrap(t(7))
+    many = lambda *sizes, **kw: [wrap(t(n, **kw)) for n in sizes]
+    p, m, v, q = many(300, 5), many(300, 5), [wrap(t(n).abs()) for n in (300, 5)], many(300, 5, dtype=torch.bfloat16)
+    copies = [wrap(t(300, dtype=torch.float16)), None]
+    codes = [wrap(torch.randint(-127, 128, (n,), generator=g, device="cuda").to(torch.int8)) for n in (300, 5)]
+    squares = [wrap(torch.randint(0, 256, (n,), generator=g, device="cuda").to(torch.uint8)) for n in (300, 5)]
+    scales = [[wrap(t(n).abs()) for n in (2, 1)] for _ in range(2)]
+    p2, factor, values = many(300, 5), wrap(t(1)), many(300, 5)
+    return [
+        (lambda: api.layer_norm_into(out, x, gamma, beta, mean=mean, rstd=rstd), [out, mean, rstd]),
+        (lambda: api.layer_norm_into(out, x), [out]),
+        (lambda: api.layer_norm_grad_into(dx, dg, db, dy, x, gamma, *stats), [dx, dg, db]),
+        (lambda: api.layer_norm_grad_into(dx, None, None, dy, x, None, *stats), [dx]),
+        (lambda: api.embedding_into(rows, table, tokens, 2.0), [rows]),
+        (lambda: api.embedding_grad_into(grad, dy, tokens, 2.0, padding=1, accumulate=True), [grad]),
+        (lambda: api.embedding_grad_into(grad, dy, tokens), [grad]),
+        (lambda: api.adamw_into(p, m, v, q, 3, copies=copies), p + m + v + copies[:1]),
+        (lambda: api.adamw_into(p2, codes, squares, q, 3, moment_scales=scales[0], variance_scales=scales[1], grad_scale=factor),
+         p2 + codes + squares + scales[0] + scales[1]),
+        (lambda: api.adamw_unpack_into(values, codes, scales[0]), values),
+    ]
+
+
+def test_native_calls_do_what_submit_does(api, monkeypatch):
+    python = _Python(api)
+    for (native, got), (other, want) in zip(calls(api), calls(api)):
+        handed_on = []
+        monkeypatch.setattr(api, "_submit", lambda *a: handed_on.append(a))
+        native()
+        monkeypatch.undo()
+        assert not handed_on
+        assert all(t._wrote == (0, None) and t._read == {} for t in got)
+        monkeypatch.setattr(api, "_run", python)
+        other()
+        monkeypatch.undo()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.torch(), b.torch()) for a, b in zip(got, want))
+    assert python.calls == 10
+
+
+class _Python:
+    def __init__(self, api):
+        self.submit, self.calls = api._submit, 0
+
+    def __call__(self, *args):
+        self.calls += 1
+        self.submit(*args)
+
+
+def test_what_native_calls_raise(api, cv):
+    x, y = api.as_tensor(torch.zeros(4, 8, device="cuda")), api.as_tensor(torch.zeros(4, 9, device="cuda"))
+    for call in (lambda: api.layer_norm_into(y, x), lambda: api.embedding_into(y, x, x), lambda: api.adamw_into([x], [x], [x], [y], 1),
+                 lambda: api.adamw_into([x], [x], [x], [x], 0), lambda: api.adamw_into([x], [x], [x], [x], 1, copies=[y])):
+        with pytest.raises(cv.Error) as e:
+            call()
+        assert e.value.status == 2
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.float16, torch.bfloat16,
+                                   torch.float32, torch.float64, torch.complex64])
+def test_wrapped_torch_tensors(api, cv, dtype):
+    x = torch.arange(60, device="cuda").reshape(3, 4, 5).to(dtype)
+    for t, layout in ((x, None), (x[:, 1:], "HWC"), (x[0], "NW"), (torch.nn.Parameter(x, requires_grad=False), None)):
+        a, b = api.as_tensor(t, layout), api.Tensor(_wrap=cv.Tensor.from_torch(t, layout or ""))
+        assert a.shape == b.shape == tuple(t.shape) and a.dtype == b.dtype and a.layout == b.layout == layout and a._t.strides == b._t.strides
+        assert a._t.dtype == b._t.dtype and a._t._keep == [t]
+        assert torch.equal(a.torch(), t) and torch.equal(b.torch(), t) and a.torch().dtype == dtype and a.torch().data_ptr() == t.data_ptr()
+        handle = a._t
+        assert handle.refcount() == 1
+        del a
+        handle.close()
+
+
+def test_what_cannot_be_wrapped(api, cv):
+    with pytest.raises(cv.Error) as e:
+        api.as_tensor(torch.zeros(4, 8, device="cuda").t())  # its rows' elements do not follow one another
+    assert e.value.status == 2
+    with pytest.raises(cv.Error):
+        api.as_tensor(torch.zeros(0, 8, device="cuda"))
+    with pytest.raises(cv.Error):
+        api.as_tensor(torch.zeros(4, 8, device="cuda"), "NHWC")
+    with pytest.raises(TypeError):
+        api.as_tensor(torch.zeros(4, dtype=torch.bfloat16, device="cuda")).cuda()  # the array interface has no name for it
