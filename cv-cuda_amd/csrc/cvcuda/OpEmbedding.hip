@@ -1,4 +1,4 @@
-// Lookup of rows of a table by token, and the table's gradient (formulas: cvcuda/Embedding.h).
+// Lookup of rows of a table by token, and the table's gradient (formulas: cvcuda/Embedding.h). Both are bound by memory.
 #include "RowOps.hpp"
 
 #include <cvcuda/Embedding.h>
@@ -17,6 +17,7 @@ struct LookupArgs
     int32_t     wide; // tokens of 64 bits
     int32_t     count, vocabulary, columns;
     float       scale;
+    DivBy       runs; // of a row
 };
 
 __device__ __forceinline__ int64_t TokenAt(const void *tokens, int wide, int64_t i)
@@ -24,19 +25,179 @@ __device__ __forceinline__ int64_t TokenAt(const void *tokens, int wide, int64_t
     return wide ? static_cast<const int64_t *>(tokens)[i] : static_cast<const int32_t *>(tokens)[i];
 }
 
-// A workgroup per token.
+// The columns of a lane: N from `first` on. It loads N from `from` on, which lies before `first` where the row ends within
+// them, so that every lane loads as all others do (loads under a condition wait for one another); the first `skip` are then not
+// its own. It stores what it loaded: twice the same sums, where another lane has these columns too. Not where they are added to
+// the table (ACCUMULATE): there it stores its own. NARROW: rows of fewer than N columns, one by one.
+template<int N, bool NARROW, bool ACCUMULATE>
+struct LaneColumns
+{
+    int first, from, columns;
+
+    __device__ __forceinline__ LaneColumns(uint32_t tile, int of)
+        : first((int)(tile * 64 + (threadIdx.x & 63)) * N)
+        , from(max(0, min(first, of - N)))
+        , columns(of)
+    {
+    }
+
+    template<class T>
+    __device__ __forceinline__ Run<T, N> get(const T *row) const
+    {
+        if constexpr (!NARROW)
+        {
+            return *reinterpret_cast<const Run<T, N> *>(row + from);
+        }
+        Run<T, N> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            r.v[i] = row[min(i, columns - 1)];
+        }
+        return r;
+    }
+
+    // s, which is not to be added to what is there
+    template<class O>
+    __device__ __forceinline__ void set(O *row, const float (&s)[N], float scale) const
+    {
+        if (first >= columns)
+        {
+            return;
+        }
+        if constexpr (!NARROW)
+        {
+            Run<O, N> r;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                r.v[i] = FromFloat<O>(s[i] * scale);
+            }
+            *reinterpret_cast<Run<O, N> *>(row + from) = r;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            if (i < columns)
+            {
+                row[i] = FromFloat<O>(s[i] * scale);
+            }
+        }
+    }
+
+    template<class O>
+    __device__ __forceinline__ void put(O *row, const float (&s)[N], float scale) const
+    {
+        if constexpr (!ACCUMULATE)
+        {
+            set(row, s, scale);
+            return;
+        }
+        if (first + N <= columns)
+        {
+            Run<O, N> *to = reinterpret_cast<Run<O, N> *>(row + first);
+            Run<O, N>  r  = *to;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                r.v[i] = FromFloat<O>((float)r.v[i] + s[i] * scale);
+            }
+            *to = r;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const int c = from + i;
+            if (c >= first && c < columns)
+            {
+                row[c] = FromFloat<O>((float)row[c] + s[i] * scale);
+            }
+        }
+    }
+};
+
+// Columns of a lane of a lookup: what makes 16 bytes of the narrower type.
 template<class T, class O>
+constexpr int kLookupRun = sizeof(T) < sizeof(O) ? kRunOf<T> : kRunOf<O>;
+
+constexpr int kLookupRuns = 2, kLookupGroup = 256 * kLookupRuns; // of a lane, all on their way before the first is used; of a workgroup
+
+// The runs of all rows are numbered through, so that narrow rows fill the lanes as well. The last run of a row whose width is no
+// multiple begins earlier, as in LaneColumns. The token is read before its row: two waits for memory, which other waves fill.
+template<class T, class O, bool NARROW>
 __global__ __launch_bounds__(256) void EmbeddingKernel(const LookupArgs a)
 {
-    for (uint32_t i = blockIdx.x; i < (uint32_t)a.count; i += gridDim.x)
+    constexpr int  N    = kLookupRun<T, O>;
+    const uint32_t runs = a.runs.d; // of a row
+    for (uint64_t first = (uint64_t)blockIdx.x * kLookupGroup; first < (uint64_t)a.count * runs; first += (uint64_t)gridDim.x * kLookupGroup)
     {
-        const int64_t t = TokenAt(a.tokens, a.wide, i);
-        O            *y = reinterpret_cast<O *>(a.out.at(i));
-        const bool    known = t >= 0 && t < a.vocabulary;
-        const T      *row   = reinterpret_cast<const T *>(a.table.at(known ? (uint32_t)t : 0));
-        for (int c = threadIdx.x; c < a.columns; c += 256)
+        const uint32_t row0 = (uint32_t)(first / runs), run0 = (uint32_t)(first - (uint64_t)row0 * runs);
+        uint32_t       row[kLookupRuns];
+        int            from[kLookupRuns];
+        int64_t        token[kLookupRuns];
+#pragma unroll
+        for (int k = 0; k < kLookupRuns; ++k)
         {
-            y[c] = FromFloat<O>(known ? (float)row[c] * a.scale : 0.f);
+            const uint32_t at = run0 + k * 256 + threadIdx.x, rows = a.runs.Quotient(at);
+            row[k]   = row0 + rows;
+            from[k]  = max(0, min((int)(at - rows * runs) * N, a.columns - N));
+            token[k] = TokenAt(a.tokens, a.wide, min(row[k], (uint32_t)a.count - 1));
+        }
+        Run<T, N> r[kLookupRuns];
+        bool      known[kLookupRuns];
+#pragma unroll
+        for (int k = 0; k < kLookupRuns; ++k)
+        {
+            known[k] = token[k] >= 0 && token[k] < a.vocabulary;
+            r[k]     = {};
+            if (a.vocabulary > 0) // (of the whole launch)
+            {
+                const T *p = reinterpret_cast<const T *>(a.table.at(known[k] ? (uint32_t)token[k] : 0));
+                if constexpr (!NARROW)
+                {
+                    r[k] = *reinterpret_cast<const Run<T, N> *>(p + from[k]);
+                }
+                else
+                {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                    {
+                        r[k].v[i] = p[min(i, a.columns - 1)];
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kLookupRuns; ++k)
+        {
+            if (row[k] >= (uint32_t)a.count)
+            {
+                continue;
+            }
+            O        *to = reinterpret_cast<O *>(a.out.at(row[k]));
+            Run<O, N> o;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                o.v[i] = FromFloat<O>(known[k] ? (float)r[k].v[i] * a.scale : 0.f);
+            }
+            if constexpr (!NARROW)
+            {
+                *reinterpret_cast<Run<O, N> *>(to + from[k]) = o;
+            }
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    if (i < a.columns)
+                    {
+                        to[i] = o.v[i];
+                    }
+                }
+            }
         }
     }
 }
@@ -346,99 +507,6 @@ __device__ __forceinline__ uint32_t FirstOf(const uint32_t *keys, uint32_t n, ui
     return lo;
 }
 
-// The columns of a lane: N from `first` on. It loads N from `from` on, which lies before `first` where the row ends within
-// them, so that every lane loads as all others do (loads under a condition wait for one another); the first `skip` are then not
-// its own. It stores what it loaded: twice the same sums, where another lane has these columns too. Not where they are added to
-// the table (ACCUMULATE): there it stores its own. NARROW: rows of fewer than N columns, one by one.
-template<int N, bool NARROW, bool ACCUMULATE>
-struct LaneColumns
-{
-    int first, from, columns;
-
-    __device__ __forceinline__ LaneColumns(uint32_t tile, int of)
-        : first((int)(tile * 64 + (threadIdx.x & 63)) * N)
-        , from(max(0, min(first, of - N)))
-        , columns(of)
-    {
-    }
-
-    template<class T>
-    __device__ __forceinline__ Run<T, N> get(const T *row) const
-    {
-        if constexpr (!NARROW)
-        {
-            return *reinterpret_cast<const Run<T, N> *>(row + from);
-        }
-        Run<T, N> r;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-        {
-            r.v[i] = row[min(i, columns - 1)];
-        }
-        return r;
-    }
-
-    // s, which is not to be added to what is there
-    template<class O>
-    __device__ __forceinline__ void set(O *row, const float (&s)[N], float scale) const
-    {
-        if (first >= columns)
-        {
-            return;
-        }
-        if constexpr (!NARROW)
-        {
-            Run<O, N> r;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-            {
-                r.v[i] = FromFloat<O>(s[i] * scale);
-            }
-            *reinterpret_cast<Run<O, N> *>(row + from) = r;
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-        {
-            if (i < columns)
-            {
-                row[i] = FromFloat<O>(s[i] * scale);
-            }
-        }
-    }
-
-    template<class O>
-    __device__ __forceinline__ void put(O *row, const float (&s)[N], float scale) const
-    {
-        if constexpr (!ACCUMULATE)
-        {
-            set(row, s, scale);
-            return;
-        }
-        if (first + N <= columns)
-        {
-            Run<O, N> *to = reinterpret_cast<Run<O, N> *>(row + first);
-            Run<O, N>  r  = *to;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-            {
-                r.v[i] = FromFloat<O>((float)r.v[i] + s[i] * scale);
-            }
-            *to = r;
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-        {
-            const int c = from + i;
-            if (c >= first && c < columns)
-            {
-                row[c] = FromFloat<O>((float)row[c] + s[i] * scale);
-            }
-        }
-    }
-};
-
 // `bytes` from `p` on, which begins with an element of 2 or 4 bytes, by a wave: 16 bytes per lane from the first multiple of 16
 // on, as streaming stores.
 __device__ __forceinline__ void ClearBytes(uint8_t *p, int64_t bytes, int element)
@@ -462,21 +530,33 @@ template<class O>
 __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
 {
     const uint32_t lane = threadIdx.x & 63, row0 = wave * a.clearRows, rows = min(a.clearRows, (uint32_t)a.vocabulary - row0);
+    const uint32_t lo = FirstOf(a.keys, a.count, row0), key = lo + lane < (uint32_t)a.count ? a.keys[lo + lane] : 0xFFFFFFFFu;
+    const uint64_t here  = __ballot(key < row0 + rows);
     uint32_t       named = 0;
-    for (uint32_t at = FirstOf(a.keys, a.count, row0);; at += 64)
+    if (here != ~0ull)
     {
-        const uint32_t key  = at + lane < (uint32_t)a.count ? a.keys[at + lane] : 0xFFFFFFFFu;
-        const bool     here = key < row0 + rows;
-        for (uint64_t rest = __ballot(here); rest != 0;) // a key at a time
+        for (uint64_t rest = here; rest != 0;) // a key at a time
         {
             const uint32_t one = (uint32_t)__builtin_amdgcn_readlane(key, __builtin_ctzll(rest));
             named |= 1u << (one - row0);
             rest &= ~__ballot(key == one);
         }
-        if (__ballot(here) != ~0ull)
+    }
+    else
+    {
+        // more keys than lanes, of frequent tokens: lane r looks for row r's (64 at a time the first rows of 65536 words took 90 us)
+        uint32_t from = lo, many = (uint32_t)a.count - lo;
+        while (__ballot(many > 0) != 0)
         {
-            break;
+            const uint32_t half = many / 2;
+            if (many > 0)
+            {
+                const bool less = a.keys[from + half] < row0 + lane;
+                from            = less ? from + half + 1 : from;
+                many            = less ? many - half - 1 : half;
+            }
         }
+        named = (uint32_t)__ballot(lane < rows && from < (uint32_t)a.count && a.keys[min(from, (uint32_t)a.count - 1)] == row0 + lane);
     }
     // rows that follow one another without a gap are cleared as one run of bytes
     const bool whole = a.table.innerStride == (int64_t)a.columns * (int64_t)sizeof(O);
@@ -765,9 +845,19 @@ int64_t GradWorkspace(int64_t tokens, int64_t, int64_t columns)
 }
 
 template<class T, class O>
-void LaunchLookup(const LookupArgs &a, hipStream_t stream)
+void LaunchLookup(LookupArgs &a, hipStream_t stream)
 {
-    hipLaunchKernelGGL((EmbeddingKernel<T, O>), dim3(std::min(a.count, kMostGroups)), dim3(256), 0, stream, a);
+    constexpr int N = kLookupRun<T, O>;
+    a.runs          = DivBy((uint32_t)Parts(a.columns, N));
+    const dim3 grid((uint32_t)std::min<int64_t>(Parts((int64_t)a.count * a.runs.d, kLookupGroup), kMostGroups));
+    if (a.columns < N)
+    {
+        hipLaunchKernelGGL((EmbeddingKernel<T, O, true>), grid, dim3(256), 0, stream, a);
+    }
+    else
+    {
+        hipLaunchKernelGGL((EmbeddingKernel<T, O, false>), grid, dim3(256), 0, stream, a);
+    }
     CheckLaunch("EmbeddingKernel");
 }
 
@@ -893,7 +983,7 @@ public:
         {
             return;
         }
-        const LookupArgs a = {RowPlaces(table), RowPlaces(out), tokens.base, tokens.wide, tokens.count, table.rows, table.columns, scale};
+        LookupArgs a = {RowPlaces(table), RowPlaces(out), tokens.base, tokens.wide, tokens.count, table.rows, table.columns, scale, DivBy(1)};
         if (table.elem == kRowF16)
         {
             LaunchLookup<Half, Half>(a, stream);
