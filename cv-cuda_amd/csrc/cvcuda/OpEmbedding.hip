@@ -283,14 +283,70 @@ __device__ __forceinline__ uint32_t SumOfFirst(const uint32_t (&v)[N], uint32_t 
     return s;
 }
 
+// `bytes` from `p` on, which begins with an element of 2 or 4 bytes, by a wave: 16 bytes per lane from the first multiple of 16
+// on, as streaming stores.
+__device__ __forceinline__ void ClearBytes(uint8_t *p, int64_t bytes, int element)
+{
+    typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+    const int64_t lane = threadIdx.x & 63, head = min((int64_t)(-reinterpret_cast<uintptr_t>(p) & 15), bytes);
+    const int64_t body = (bytes - head) / 16 * 16, tail = bytes - head - body;
+    for (int64_t i = lane * 16; i < body; i += 64 * 16)
+    {
+        __builtin_nontemporal_store(U32x4{0, 0, 0, 0}, reinterpret_cast<U32x4 *>(p + head + i));
+    }
+    // the ends: up to seven elements each
+    const int64_t at = lane < 16 ? lane * element : head + body + (lane - 16) * element;
+    if (lane < 16 ? at < head : at < head + body + tail)
+    {
+        element == 4 ? (void)(*reinterpret_cast<uint32_t *>(p + at) = 0) : (void)(*reinterpret_cast<uint16_t *>(p + at) = 0);
+    }
+}
+
+// Rows of the table that are cleared beside the sort, whose few workgroups leave the card to others: by the workgroups of a
+// launch from the `sorting`-th on. What tokens name among them is written once more by the sums.
+struct ClearArgs
+{
+    RowPlaces table;
+    int64_t   rowBytes;
+    int32_t   element;
+    int32_t   dense; // rows follow one another without a gap: cleared as pieces of kClearBytes
+    uint32_t  row, rows;
+    uint32_t  sorting;
+};
+
+constexpr int kClearBytes = 16384;
+
+__device__ __forceinline__ void ClearBeside(const ClearArgs &a)
+{
+    const uint32_t waves = blockDim.x / 64;
+    const int64_t  bytes = a.rows * a.rowBytes, parts = a.dense ? (bytes + kClearBytes - 1) / kClearBytes : a.rows;
+    for (int64_t p = (int64_t)(blockIdx.x - a.sorting) * waves + WaveOfGroup(); p < parts; p += (int64_t)(gridDim.x - a.sorting) * waves)
+    {
+        if (a.dense)
+        {
+            ClearBytes(a.table.at(a.row) + p * kClearBytes, min((int64_t)kClearBytes, bytes - p * kClearBytes), a.element);
+        }
+        else
+        {
+            ClearBytes(a.table.at(a.row + (uint32_t)p), a.rowBytes, a.element);
+        }
+    }
+}
+
 constexpr int kSmallThreads = 1024, kSmallBits = 6;
 constexpr int kMostSmall    = 4 * kSmallThreads;
 
 // All of up to K * 1024 tokens by one workgroup, in LDS. A wave owns 64 K consecutive elements; 16 waves with 64 digits
 // each have a counter per thread.
 template<int K>
-__global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const TokenSource src, uint32_t *keys, uint32_t *places, int bits)
+__global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const TokenSource src, uint32_t *keys, uint32_t *places, int bits,
+                                                                         const ClearArgs clear)
 {
+    if (blockIdx.x > 0)
+    {
+        ClearBeside(clear);
+        return;
+    }
     __shared__ uint32_t s_key[K * kSmallThreads];
     __shared__ uint16_t s_place[K * kSmallThreads];
     __shared__ uint32_t s_count[16][1 << kSmallBits];
@@ -373,8 +429,13 @@ struct TileArgs
     }
 };
 
-__global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileArgs a)
+__global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileArgs a, const ClearArgs clear)
 {
+    if (blockIdx.x >= clear.sorting)
+    {
+        ClearBeside(clear);
+        return;
+    }
     __shared__ uint32_t s_count[kDigits];
     const uint32_t      first = blockIdx.x * kTile + threadIdx.x;
     uint32_t            key[kTileKeys];
@@ -397,8 +458,13 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileA
     a.counts[(size_t)threadIdx.x * a.pitch + blockIdx.x] = s_count[threadIdx.x];
 }
 
-__global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileArgs a)
+__global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileArgs a, const ClearArgs clear)
 {
+    if (blockIdx.x >= clear.sorting)
+    {
+        ClearBeside(clear);
+        return;
+    }
     constexpr int       kWaves = kTileThreads / 64;
     __shared__ uint32_t s_count[kWaves][kDigits];
     __shared__ uint32_t s_sum[kWaves];
@@ -478,12 +544,14 @@ struct SumArgs
     float          *partial; // [groups][2][columns]: of the token that began before the group, of the one that goes on behind it
     int32_t         count, vocabulary, columns, accumulate;
     uint32_t        groups, columnTiles, joinTiles, sumGroups, clearGroups, clearRows;
+    uint32_t        rowsToClear; // the others have been
+    int32_t         dense;       // the table's rows follow one another without a gap
     float           scale;
 };
 
 // A wave clears as many rows as make 16 KiB, 32 at most: what all waves write lies close together at any time (16 rows of
 // 2048 floats each: 5.3 TB/s).
-constexpr int kMostClearRows = 32, kClearBytes = 16384;
+constexpr int kMostClearRows = 32;
 
 // The first place among `n` sorted keys that holds `key` or more.
 __device__ __forceinline__ uint32_t FirstOf(const uint32_t *keys, uint32_t n, uint32_t key)
@@ -507,29 +575,10 @@ __device__ __forceinline__ uint32_t FirstOf(const uint32_t *keys, uint32_t n, ui
     return lo;
 }
 
-// `bytes` from `p` on, which begins with an element of 2 or 4 bytes, by a wave: 16 bytes per lane from the first multiple of 16
-// on, as streaming stores.
-__device__ __forceinline__ void ClearBytes(uint8_t *p, int64_t bytes, int element)
-{
-    typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
-    const int64_t lane = threadIdx.x & 63, head = min((int64_t)(-reinterpret_cast<uintptr_t>(p) & 15), bytes);
-    const int64_t body = (bytes - head) / 16 * 16, tail = bytes - head - body;
-    for (int64_t i = lane * 16; i < body; i += 64 * 16)
-    {
-        __builtin_nontemporal_store(U32x4{0, 0, 0, 0}, reinterpret_cast<U32x4 *>(p + head + i));
-    }
-    // the ends: up to seven elements each
-    const int64_t at = lane < 16 ? lane * element : head + body + (lane - 16) * element;
-    if (lane < 16 ? at < head : at < head + body + tail)
-    {
-        element == 4 ? (void)(*reinterpret_cast<uint32_t *>(p + at) = 0) : (void)(*reinterpret_cast<uint16_t *>(p + at) = 0);
-    }
-}
-
 template<class O>
 __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
 {
-    const uint32_t lane = threadIdx.x & 63, row0 = wave * a.clearRows, rows = min(a.clearRows, (uint32_t)a.vocabulary - row0);
+    const uint32_t lane = threadIdx.x & 63, row0 = wave * a.clearRows, rows = min(a.clearRows, a.rowsToClear - row0);
     const uint32_t lo = FirstOf(a.keys, a.count, row0), key = lo + lane < (uint32_t)a.count ? a.keys[lo + lane] : 0xFFFFFFFFu;
     const uint64_t here  = __ballot(key < row0 + rows);
     uint32_t       named = 0;
@@ -559,7 +608,6 @@ __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
         named = (uint32_t)__ballot(lane < rows && from < (uint32_t)a.count && a.keys[min(from, (uint32_t)a.count - 1)] == row0 + lane);
     }
     // rows that follow one another without a gap are cleared as one run of bytes
-    const bool whole = a.table.innerStride == (int64_t)a.columns * (int64_t)sizeof(O);
     for (uint32_t r = 0; r < rows;)
     {
         if ((named >> r) & 1)
@@ -567,7 +615,7 @@ __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
             ++r;
             continue;
         }
-        const uint32_t many = whole ? min(rows - r, (uint32_t)__builtin_ctzll((named >> r) | 1ull << 32)) : 1;
+        const uint32_t many = a.dense ? min(rows - r, (uint32_t)__builtin_ctzll((named >> r) | 1ull << 32)) : 1;
         ClearBytes(a.table.at(row0 + r), (int64_t)many * a.columns * (int64_t)sizeof(O), (int)sizeof(O));
         r += many;
     }
@@ -721,7 +769,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void EmbeddingSumKernel(const SumAr
 {
     if (blockIdx.x >= a.sumGroups)
     {
-        const uint64_t waves = ((uint64_t)a.vocabulary + a.clearRows - 1) / a.clearRows;
+        const uint64_t waves = ((uint64_t)a.rowsToClear + a.clearRows - 1) / a.clearRows;
         for (uint64_t w = (uint64_t)(blockIdx.x - a.sumGroups) * kSumWaves + WaveOfGroup(); w < waves; w += (uint64_t)a.clearGroups * kSumWaves)
         {
             ClearRows<O>(a, (uint32_t)w);
@@ -861,29 +909,58 @@ void LaunchLookup(LookupArgs &a, hipStream_t stream)
     CheckLaunch("EmbeddingKernel");
 }
 
+// Rows that are cleared beside the sort, the table's last ones: all where that writes a quarter of them again at most, else what
+// the card writes in the time that the sort takes (about 7 us for a workgroup's, 26 in four launches; the sums clear the others).
+uint32_t RowsBesideSort(int64_t tokens, int64_t vocabulary, int64_t rowBytes)
+{
+    if (tokens == 0)
+    {
+        return 0;
+    }
+    const int64_t bytes = tokens <= kMostSmall ? 32 << 20 : 128 << 20;
+    return (uint32_t)(tokens * 4 <= vocabulary ? vocabulary : std::min(vocabulary, bytes / rowBytes));
+}
+
+// Launches of a sort that clear rows beside it, each its share of those left.
+struct Clearing
+{
+    ClearArgs args;
+    uint32_t  left;   // rows
+    int       launches;
+
+    // The workgroups to add to `sorting`, each of `waves` waves.
+    uint32_t next(uint32_t sorting, int waves)
+    {
+        args.row += args.rows;
+        args.rows    = left / (uint32_t)launches + (left % (uint32_t)launches != 0 ? 1 : 0);
+        args.sorting = sorting;
+        left -= args.rows;
+        --launches;
+        const int64_t parts = args.dense ? Parts(args.rows * args.rowBytes, kClearBytes) : args.rows;
+        return (uint32_t)std::min<int64_t>(Parts(parts, waves), 1 << 20);
+    }
+};
+
 // Sorts into the workspace's keys and places.
-void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, hipStream_t stream)
+void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, Clearing clearing, hipStream_t stream)
 {
     auto     part = [&](int64_t offset) { return reinterpret_cast<uint32_t *>(room + offset); };
     uint32_t *keys = part(at.keys), *places = part(at.places);
     const int bits = src.vocabulary > 0 ? 32 - __builtin_clz((uint32_t)src.vocabulary) : 1;
     if (src.count <= kMostSmall)
     {
-        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(1), dim3(kSmallThreads), 0, stream, src, keys, places, bits); };
-        if (src.count <= kSmallThreads)
-        {
-            launch(EmbeddingSortSmallKernel<1>);
-        }
-        else
-        {
-            launch(EmbeddingSortSmallKernel<4>);
-        }
+        clearing.launches   = 1;
+        const uint32_t more = clearing.next(1, kSmallThreads / 64);
+        auto           launch = [&](auto kernel)
+        { hipLaunchKernelGGL(kernel, dim3(1 + more), dim3(kSmallThreads), 0, stream, src, keys, places, bits, clearing.args); };
+        src.count <= kSmallThreads ? launch(EmbeddingSortSmallKernel<1>) : launch(EmbeddingSortSmallKernel<4>);
         CheckLaunch("EmbeddingSortSmallKernel");
         return;
     }
     TileArgs a      = {src, nullptr, nullptr, nullptr, nullptr, part(at.counts), (int32_t)Parts(src.count, kTile),
                        (int32_t)RoundUp(Parts(src.count, kTile), kCountsAtOnce), 0};
     int      passes = DivUp(bits, kTileBits);
+    clearing.launches = 2 * passes;
     for (int p = 0; p < passes; ++p)
     {
         // the last pass ends in keys and places
@@ -891,9 +968,11 @@ void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, hipSt
         a.toKeys      = to ? keys : part(at.otherKeys);
         a.toPlaces    = to ? places : part(at.otherPlaces);
         a.shift       = p * kTileBits;
-        hipLaunchKernelGGL(EmbeddingCountKernel, dim3(a.tiles), dim3(kTileThreads), 0, stream, a);
+        uint32_t more = clearing.next(a.tiles, kTileThreads / 64);
+        hipLaunchKernelGGL(EmbeddingCountKernel, dim3(a.tiles + more), dim3(kTileThreads), 0, stream, a, clearing.args);
         CheckLaunch("EmbeddingCountKernel");
-        hipLaunchKernelGGL(EmbeddingPlaceKernel, dim3(a.tiles), dim3(kTileThreads), 0, stream, a);
+        more = clearing.next(a.tiles, kTileThreads / 64);
+        hipLaunchKernelGGL(EmbeddingPlaceKernel, dim3(a.tiles + more), dim3(kTileThreads), 0, stream, a, clearing.args);
         CheckLaunch("EmbeddingPlaceKernel");
         a.keys   = a.toKeys;
         a.places = a.toPlaces;
@@ -918,7 +997,7 @@ void LaunchGrad(SumArgs &a, hipStream_t stream)
     a.joinTiles   = (uint32_t)Parts(a.columns, 64 * kJoinRun);
     a.clearRows   = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(kMostClearRows, kClearBytes / (a.columns * (int64_t)sizeof(O))));
     a.sumGroups   = Groups((int64_t)a.groups * a.columnTiles);
-    a.clearGroups = a.accumulate ? 0 : Groups(Parts(Parts(a.vocabulary, a.clearRows), kSumWaves));
+    a.clearGroups = Groups(Parts(Parts(a.rowsToClear, a.clearRows), kSumWaves));
     if (const uint32_t grid = a.sumGroups + a.clearGroups)
     {
         a.columns < kRunOf<T> ? Launch(EmbeddingSumKernel<T, O, true, false>, EmbeddingSumKernel<T, O, true, true>, a, grid, kSumWaves, stream)
@@ -1031,13 +1110,18 @@ public:
         {
             return;
         }
+        const int64_t  rowBytes = table.columns * (int64_t)RowElemSize(table.elem);
+        const bool     dense    = table.inner == table.rows && table.innerStride == rowBytes;
+        const uint32_t beside   = accumulate ? 0 : RowsBesideSort(tokens.count, table.rows, rowBytes);
         if (tokens.count > 0)
         {
-            SortTokens({tokens.base, tokens.wide, tokens.count, table.rows, padding}, room, at, stream);
+            SortTokens({tokens.base, tokens.wide, tokens.count, table.rows, padding}, room, at,
+                       {{RowPlaces(table), rowBytes, RowElemSize(table.elem), dense, table.rows - beside, 0, 0}, beside, 0}, stream);
         }
         SumArgs a = {RowPlaces(grad), RowPlaces(table), reinterpret_cast<const uint32_t *>(room + at.keys),
                      reinterpret_cast<const uint32_t *>(room + at.places), reinterpret_cast<float *>(room + at.partial), tokens.count,
-                     table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, kGroup), 0, 0, 0, 0, 0, scale};
+                     table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, kGroup), 0, 0, 0, 0, 0,
+                     accumulate ? 0 : (uint32_t)table.rows - beside, dense, scale};
         if (grad.elem == kRowF32)
         {
             LaunchGrad<float, float>(a, stream);

@@ -178,6 +178,25 @@ def test_gradient_between_rows_with_gaps(api, in_type, out_type, d):
     assert torch.equal(dense, out[:, 2:d + 2])
 
 
+@pytest.mark.parametrize("n", [40, 3000, 30000])
+def test_gradient_into_rows_at_two_distances(api, n):
+    # a table of three parts with gaps between them: what is cleared ends where a part does
+    for rows, d in ((50, 64), (7, 515), (2000, 32)):
+        whole = torch.full((3, rows + 2, d), 9.0, device="cuda")
+        table = whole[:, 1:rows + 1]
+        tokens, dy = words(n, 3 * rows, n), normal((n, d), F32, 4)
+        api.embedding_grad_into(wrap(api, table), wrap(api, dy), wrap(api, tokens))
+        dense = api.embedding_grad(wrap(api, dy), wrap(api, tokens), 3 * rows).torch()
+        assert torch.equal(table.reshape(3 * rows, d), dense) and (whole[:, 0] == 9).all() and (whole[:, -1] == 9).all()
+        assert torch.equal(api.embedding(wrap(api, table), wrap(api, tokens)).torch(), dense[tokens])
+
+
+@pytest.mark.parametrize("n", [1, 300, 5000])
+def test_gradient_of_few_tokens_in_a_large_table(api, n):
+    check_gradient(api, normal((n, 48), F32, n), words(n, 40000, n), 40000, F32)
+    check_gradient(api, normal((n, 6), BF16, n), 39999 - words(n, 40000, n), 40000, BF16)
+
+
 def test_gradient_of_what_is_not_finite(api):
     tokens = words(2000, 60, 2)
     dy = normal((2000, 48), F32, 1)
