@@ -406,7 +406,14 @@ __global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const 
 
 // More tokens: tiles of them, two launches for each digit. The first counts the digits of each tile, the second adds up what
 // comes before each digit of its tile and puts the tile's elements there.
-constexpr int kTileThreads = 512, kTileKeys = 4, kTile = kTileThreads * kTileKeys, kTileBits = 9, kDigits = 1 << kTileBits;
+constexpr int kTileThreads = 512, kTileBits = 9, kDigits = 1 << kTileBits;
+
+// Keys of a thread. Small tiles are quick, but each reads the counts of all others: 64 small ones at most (16384 tokens' sort 30 us,
+// 35 with four keys), then 128 of eight, then sixteen.
+constexpr int KeysOf(int64_t tokens)
+{
+    return tokens <= 64 * 2 * kTileThreads ? 2 : tokens <= 128 * 8 * kTileThreads ? 8 : 16;
+}
 
 constexpr int kCountsAtOnce = 16; // of tiles that a thread reads: a digit's counts are padded to as many
 
@@ -429,6 +436,7 @@ struct TileArgs
     }
 };
 
+template<int KEYS>
 __global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileArgs a, const ClearArgs clear)
 {
     if (blockIdx.x >= clear.sorting)
@@ -437,17 +445,17 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileA
         return;
     }
     __shared__ uint32_t s_count[kDigits];
-    const uint32_t      first = blockIdx.x * kTile + threadIdx.x;
-    uint32_t            key[kTileKeys];
+    const uint32_t      first = blockIdx.x * (KEYS * kTileThreads) + threadIdx.x;
+    uint32_t            key[KEYS];
     s_count[threadIdx.x] = 0;
 #pragma unroll
-    for (int k = 0; k < kTileKeys; ++k)
+    for (int k = 0; k < KEYS; ++k)
     {
         key[k] = a.key(first + k * kTileThreads);
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kTileKeys; ++k)
+    for (int k = 0; k < KEYS; ++k)
     {
         if (first + k * kTileThreads < (uint32_t)a.src.count)
         {
@@ -458,6 +466,7 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingCountKernel(const TileA
     a.counts[(size_t)threadIdx.x * a.pitch + blockIdx.x] = s_count[threadIdx.x];
 }
 
+template<int KEYS>
 __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileArgs a, const ClearArgs clear)
 {
     if (blockIdx.x >= clear.sorting)
@@ -468,10 +477,10 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
     constexpr int       kWaves = kTileThreads / 64;
     __shared__ uint32_t s_count[kWaves][kDigits];
     __shared__ uint32_t s_sum[kWaves];
-    const uint32_t      wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = blockIdx.x * kTile + wave * 64 * kTileKeys + lane;
-    uint32_t            key[kTileKeys], place[kTileKeys], rank[kTileKeys];
+    const uint32_t      wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = blockIdx.x * (KEYS * kTileThreads) + wave * 64 * KEYS + lane;
+    uint32_t            key[KEYS], place[KEYS], rank[KEYS];
 #pragma unroll
-    for (int k = 0; k < kTileKeys; ++k)
+    for (int k = 0; k < KEYS; ++k)
     {
         const uint32_t i = first + 64 * k;
         key[k]           = a.key(i);
@@ -501,7 +510,7 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kTileKeys; ++k)
+    for (int k = 0; k < KEYS; ++k)
     {
         // (past the last token: the highest digit, behind all others of the last tile)
         const uint32_t digit = first + 64 * k < (uint32_t)a.src.count ? (key[k] >> a.shift) & (kDigits - 1) : kDigits - 1;
@@ -517,7 +526,7 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kTileKeys; ++k)
+    for (int k = 0; k < KEYS; ++k)
     {
         if (first + 64 * k < (uint32_t)a.src.count)
         {
@@ -529,13 +538,19 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
 }
 
 // ---- gradient: sums ----------------------------------------------------------------------------------------------------
-// The sorted positions are cut into pieces of kPiece, whatever their tokens: every wave adds up the same number of rows, of 64
+// The sorted positions are cut into pieces of PIECE, whatever their tokens: every wave adds up the same number of rows, of 64
 // lanes' columns. A token whose positions lie within a piece is done there. What reaches over a piece's ends is joined by the
 // workgroup, whose waves have pieces that follow one another, and what reaches over the workgroup's is left in the workspace,
 // where a second launch adds it up: always in the order of the positions. Rows of the table that no token names are cleared
 // beside that by waves that look for their keys among the sorted ones.
-constexpr int kPiece = 32, kBatch = 16;                 // positions of a wave, of which so many rows are loaded at once
-constexpr int kSumWaves = 8, kGroup = kSumWaves * kPiece; // positions of a workgroup
+constexpr int kSumWaves = 8, kSmallPiece = 8, kPiece = 32;
+
+// Small pieces where there are too few to fill the card (2^24 elements are 1024 waves of large ones): their time is that of
+// one wait after another (1003 tokens of width 515 28 -> 21.5 us, 16384 of 64 40 -> 32; 16384 of 4096 would take 141 for 135).
+constexpr int PieceOf(int64_t tokens, int64_t columns)
+{
+    return tokens * columns <= 1 << 24 ? kSmallPiece : kPiece;
+}
 
 struct SumArgs
 {
@@ -543,7 +558,8 @@ struct SumArgs
     const uint32_t *keys, *places;
     float          *partial; // [groups][2][columns]: of the token that began before the group, of the one that goes on behind it
     int32_t         count, vocabulary, columns, accumulate;
-    uint32_t        groups, columnTiles, joinTiles, sumGroups, clearGroups, clearRows;
+    uint32_t        groups, group; // workgroups' shares of the positions, and how many that is
+    uint32_t        columnTiles, joinTiles, sumGroups, clearGroups, clearRows;
     uint32_t        rowsToClear; // the others have been
     int32_t         dense;       // the table's rows follow one another without a gap
     float           scale;
@@ -631,10 +647,11 @@ enum PieceFlags
 };
 
 // Sums a piece: tokens within it into the table, the others into `head` and `tail`, a lane's N one after another. Returns the flags.
-template<class T, class O, class COLUMNS, int N>
+template<class T, class O, int PIECE, class COLUMNS, int N>
 __device__ __forceinline__ uint32_t SumPiece(const SumArgs &a, uint32_t piece, const COLUMNS &columns, float (&head)[64][N], float (&tail)[64][N])
 {
-    const uint32_t lane = threadIdx.x & 63, first = piece * kPiece, many = min((uint32_t)kPiece, (uint32_t)a.count - first);
+    constexpr int  kBatch = PIECE < 16 ? PIECE : 16; // rows that are loaded at once
+    const uint32_t lane = threadIdx.x & 63, first = piece * PIECE, many = min((uint32_t)PIECE, (uint32_t)a.count - first);
     // lane k: the piece's k-th key and place (behind its end the last one's); the keys before and behind the piece
     const uint32_t mine  = first + min(lane, many - 1);
     const uint32_t myKey = a.keys[mine], myPlace = a.places[mine];
@@ -697,7 +714,7 @@ __device__ __forceinline__ uint32_t SumPiece(const SumArgs &a, uint32_t piece, c
 }
 
 // kSumWaves pieces that follow one another, of 64 lanes' columns.
-template<class T, class O, bool NARROW, bool ACCUMULATE>
+template<class T, class O, int PIECE, bool NARROW, bool ACCUMULATE>
 __device__ __forceinline__ void SumGroup(const SumArgs &a, uint32_t group, uint32_t tile)
 {
     constexpr int       N = kRunOf<T>;
@@ -707,9 +724,9 @@ __device__ __forceinline__ void SumGroup(const SumArgs &a, uint32_t group, uint3
 
     const uint32_t wave = WaveOfGroup(), lane = threadIdx.x & 63, piece = group * kSumWaves + wave;
     uint32_t       flags = 0;
-    if ((uint64_t)piece * kPiece < (uint64_t)a.count)
+    if ((uint64_t)piece * PIECE < (uint64_t)a.count)
     {
-        flags = SumPiece<T, O>(a, piece, columns, s_head[wave], s_tail[wave]);
+        flags = SumPiece<T, O, PIECE>(a, piece, columns, s_head[wave], s_tail[wave]);
     }
     if (lane == 0)
     {
@@ -735,7 +752,7 @@ __device__ __forceinline__ void SumGroup(const SumArgs &a, uint32_t group, uint3
                 {
                     if (here)
                     {
-                        const uint32_t key = __builtin_amdgcn_readfirstlane(a.keys[(size_t)(group * kSumWaves + w) * kPiece]);
+                        const uint32_t key = __builtin_amdgcn_readfirstlane(a.keys[(size_t)(group * kSumWaves + w) * PIECE]);
                         columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale);
                     }
                     else
@@ -764,7 +781,7 @@ __device__ __forceinline__ void SumGroup(const SumArgs &a, uint32_t group, uint3
 }
 
 // A workgroup is one of tokens, or waves that clear rows.
-template<class T, class O, bool NARROW, bool ACCUMULATE>
+template<class T, class O, int PIECE, bool NARROW, bool ACCUMULATE>
 __global__ __launch_bounds__(64 * kSumWaves) void EmbeddingSumKernel(const SumArgs a)
 {
     if (blockIdx.x >= a.sumGroups)
@@ -778,7 +795,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void EmbeddingSumKernel(const SumAr
     }
     for (uint64_t w = blockIdx.x; w < (uint64_t)a.groups * a.columnTiles; w += a.sumGroups)
     {
-        SumGroup<T, O, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.columnTiles), (uint32_t)(w % a.columnTiles));
+        SumGroup<T, O, PIECE, NARROW, ACCUMULATE>(a, (uint32_t)(w / a.columnTiles), (uint32_t)(w % a.columnTiles));
     }
 }
 
@@ -788,7 +805,7 @@ constexpr int kJoinRun = 4, kJoinWaves = 4; // columns of a lane; each wave adds
 template<class O, bool NARROW, bool ACCUMULATE>
 __device__ __forceinline__ void JoinGroups(const SumArgs &a, uint32_t group, uint32_t tile)
 {
-    const uint64_t first = (uint64_t)group * kGroup, behind = first + kGroup;
+    const uint64_t first = (uint64_t)group * a.group, behind = first + a.group;
     const uint32_t key = __builtin_amdgcn_readfirstlane(a.keys[behind - 1]);
     if (key == (uint32_t)a.vocabulary || a.keys[behind] != key || (group > 0 && a.keys[first] == key && a.keys[first - 1] == key))
     {
@@ -799,7 +816,7 @@ __device__ __forceinline__ void JoinGroups(const SumArgs &a, uint32_t group, uin
     const LaneColumns<N, NARROW, ACCUMULATE> columns(tile, a.columns);
     // the group of the last of them, first: sums whose number is known are on their way together
     const uint32_t wave = WaveOfGroup(), lane = threadIdx.x & 63;
-    const uint32_t all = (FirstOf(a.keys, a.count, key + 1) - 1) / kGroup - group, each = (all + kJoinWaves - 1) / kJoinWaves;
+    const uint32_t all = (FirstOf(a.keys, a.count, key + 1) - 1) / a.group - group, each = (all + kJoinWaves - 1) / kJoinWaves;
     const uint32_t from = group + 1 + wave * each, to = min(group + 1 + all, from + each);
     float          s[N] = {};
     for (uint32_t p = from; p < to; p += kAhead)
@@ -875,8 +892,8 @@ struct GradRoom
 
     GradRoom(int64_t tokens, int64_t columns)
     {
-        const int64_t list = RoundUp(tokens * 4, 256), tiles = tokens > kMostSmall ? Parts(tokens, kTile) : 0;
-        const int64_t groups = Parts(tokens, kGroup);
+        const int64_t list = RoundUp(tokens * 4, 256), tiles = tokens > kMostSmall ? Parts(tokens, KeysOf(tokens) * kTileThreads) : 0;
+        const int64_t groups = Parts(tokens, kSumWaves * PieceOf(tokens, columns));
         keys        = 0;
         places      = keys + list;
         otherKeys   = places + list;
@@ -957,8 +974,8 @@ void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, Clear
         CheckLaunch("EmbeddingSortSmallKernel");
         return;
     }
-    TileArgs a      = {src, nullptr, nullptr, nullptr, nullptr, part(at.counts), (int32_t)Parts(src.count, kTile),
-                       (int32_t)RoundUp(Parts(src.count, kTile), kCountsAtOnce), 0};
+    const int64_t tiles = Parts(src.count, KeysOf(src.count) * kTileThreads);
+    TileArgs a      = {src, nullptr, nullptr, nullptr, nullptr, part(at.counts), (int32_t)tiles, (int32_t)RoundUp(tiles, kCountsAtOnce), 0};
     int      passes = DivUp(bits, kTileBits);
     clearing.launches = 2 * passes;
     for (int p = 0; p < passes; ++p)
@@ -968,12 +985,26 @@ void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, Clear
         a.toKeys      = to ? keys : part(at.otherKeys);
         a.toPlaces    = to ? places : part(at.otherPlaces);
         a.shift       = p * kTileBits;
-        uint32_t more = clearing.next(a.tiles, kTileThreads / 64);
-        hipLaunchKernelGGL(EmbeddingCountKernel, dim3(a.tiles + more), dim3(kTileThreads), 0, stream, a, clearing.args);
-        CheckLaunch("EmbeddingCountKernel");
-        more = clearing.next(a.tiles, kTileThreads / 64);
-        hipLaunchKernelGGL(EmbeddingPlaceKernel, dim3(a.tiles + more), dim3(kTileThreads), 0, stream, a, clearing.args);
-        CheckLaunch("EmbeddingPlaceKernel");
+        auto launch = [&](auto kernel)
+        {
+            const uint32_t more = clearing.next(a.tiles, kTileThreads / 64);
+            hipLaunchKernelGGL(kernel, dim3(a.tiles + more), dim3(kTileThreads), 0, stream, a, clearing.args);
+            CheckLaunch("EmbeddingSortKernel");
+        };
+        switch (KeysOf(src.count))
+        {
+        case 2:
+            launch(EmbeddingCountKernel<2>);
+            launch(EmbeddingPlaceKernel<2>);
+            break;
+        case 8:
+            launch(EmbeddingCountKernel<8>);
+            launch(EmbeddingPlaceKernel<8>);
+            break;
+        default:
+            launch(EmbeddingCountKernel<16>);
+            launch(EmbeddingPlaceKernel<16>);
+        }
         a.keys   = a.toKeys;
         a.places = a.toPlaces;
     }
@@ -990,6 +1021,14 @@ void Launch(K plain, K accumulate, const SumArgs &a, uint32_t grid, int waves, h
     hipLaunchKernelGGL(a.accumulate ? accumulate : plain, dim3(grid), dim3(64 * waves), 0, stream, a);
 }
 
+template<class T, class O, int PIECE>
+void LaunchSum(const SumArgs &a, uint32_t grid, hipStream_t stream)
+{
+    a.columns < kRunOf<T>
+        ? Launch(EmbeddingSumKernel<T, O, PIECE, true, false>, EmbeddingSumKernel<T, O, PIECE, true, true>, a, grid, kSumWaves, stream)
+        : Launch(EmbeddingSumKernel<T, O, PIECE, false, false>, EmbeddingSumKernel<T, O, PIECE, false, true>, a, grid, kSumWaves, stream);
+}
+
 template<class T, class O>
 void LaunchGrad(SumArgs &a, hipStream_t stream)
 {
@@ -1000,8 +1039,14 @@ void LaunchGrad(SumArgs &a, hipStream_t stream)
     a.clearGroups = Groups(Parts(Parts(a.rowsToClear, a.clearRows), kSumWaves));
     if (const uint32_t grid = a.sumGroups + a.clearGroups)
     {
-        a.columns < kRunOf<T> ? Launch(EmbeddingSumKernel<T, O, true, false>, EmbeddingSumKernel<T, O, true, true>, a, grid, kSumWaves, stream)
-                              : Launch(EmbeddingSumKernel<T, O, false, false>, EmbeddingSumKernel<T, O, false, true>, a, grid, kSumWaves, stream);
+        if (a.group == kSumWaves * kSmallPiece)
+        {
+            LaunchSum<T, O, kSmallPiece>(a, grid, stream);
+        }
+        else
+        {
+            LaunchSum<T, O, kPiece>(a, grid, stream);
+        }
         CheckLaunch("EmbeddingSumKernel");
     }
     if (a.groups > 1)
@@ -1118,9 +1163,10 @@ public:
             SortTokens({tokens.base, tokens.wide, tokens.count, table.rows, padding}, room, at,
                        {{RowPlaces(table), rowBytes, RowElemSize(table.elem), dense, table.rows - beside, 0, 0}, beside, 0}, stream);
         }
+        const uint32_t group = (uint32_t)(kSumWaves * PieceOf(tokens.count, table.columns));
         SumArgs a = {RowPlaces(grad), RowPlaces(table), reinterpret_cast<const uint32_t *>(room + at.keys),
                      reinterpret_cast<const uint32_t *>(room + at.places), reinterpret_cast<float *>(room + at.partial), tokens.count,
-                     table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, kGroup), 0, 0, 0, 0, 0,
+                     table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, group), group, 0, 0, 0, 0, 0,
                      accumulate ? 0 : (uint32_t)table.rows - beside, dense, scale};
         if (grad.elem == kRowF32)
         {

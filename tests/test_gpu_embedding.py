@@ -152,6 +152,14 @@ def test_gradient_of_one_token_and_of_different_ones(api, n):
     assert torch.equal(got[order], dy)  # each a sum of one
 
 
+@pytest.mark.parametrize("n,v", [(4096, 700), (4097, 700), (65536, 1 << 20), (65537, 3), (200000, 260000), (524289, 50000), (700000, 1 << 19)])
+def test_gradient_of_many_tokens(api, n, v):
+    # every size of the sort, one to three passes of it
+    tokens, dy = words(n, v, n), normal((n, 8), F32, n)
+    check_gradient(api, dy, tokens, v, F32, padding=1)
+    check_gradient(api, dy[:, :3], (v - 1 - tokens).int(), v, F32)
+
+
 def test_gradient_of_unknown_tokens(api):
     dy = normal((12, 40), F32, 1)
     tokens = torch.tensor([3, -1, 10, 9, 0, 1 << 40, -(1 << 40), (1 << 32) + 3, 5, 3, 1 << 31, 3], device="cuda")
