@@ -86,24 +86,24 @@ struct LaneColumns
         }
     }
 
+    // s into a row of the table, of which `old` is what get() gave: to add to where ACCUMULATE
     template<class O>
-    __device__ __forceinline__ void put(O *row, const float (&s)[N], float scale) const
+    __device__ __forceinline__ void put(O *row, const float (&s)[N], float scale, const Run<O, N> &old) const
     {
         if constexpr (!ACCUMULATE)
         {
             set(row, s, scale);
             return;
         }
+        Run<O, N> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            r.v[i] = FromFloat<O>((float)old.v[i] + s[i] * scale);
+        }
         if (first + N <= columns)
         {
-            Run<O, N> *to = reinterpret_cast<Run<O, N> *>(row + first);
-            Run<O, N>  r  = *to;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-            {
-                r.v[i] = FromFloat<O>((float)r.v[i] + s[i] * scale);
-            }
-            *to = r;
+            *reinterpret_cast<Run<O, N> *>(row + first) = r;
             return;
         }
 #pragma unroll
@@ -112,9 +112,15 @@ struct LaneColumns
             const int c = from + i;
             if (c >= first && c < columns)
             {
-                row[c] = FromFloat<O>((float)row[c] + s[i] * scale);
+                row[c] = r.v[i];
             }
         }
+    }
+
+    template<class O>
+    __device__ __forceinline__ void put(O *row, const float (&s)[N], float scale) const
+    {
+        put(row, s, scale, ACCUMULATE ? get(row) : Run<O, N>{});
     }
 };
 
@@ -647,10 +653,12 @@ enum PieceFlags
 };
 
 // Sums a piece: tokens within it into the table, the others into `head` and `tail`, a lane's N one after another. Returns the flags.
-template<class T, class O, int PIECE, class COLUMNS, int N>
+template<class T, class O, int PIECE, bool ACCUMULATE, class COLUMNS, int N>
 __device__ __forceinline__ uint32_t SumPiece(const SumArgs &a, uint32_t piece, const COLUMNS &columns, float (&head)[64][N], float (&tail)[64][N])
 {
-    constexpr int  kBatch = PIECE < 16 ? PIECE : 16; // rows that are loaded at once
+    // rows that are loaded at once; what they are added to comes with them (read where a sum is done it was a wait for each
+    // token: 20000 tokens of width 4096, BF16, 98 us, so 88; many rows of F32 178, so 188)
+    constexpr int  kBatch = PIECE < 16 || ACCUMULATE ? 8 : 16;
     const uint32_t lane = threadIdx.x & 63, first = piece * PIECE, many = min((uint32_t)PIECE, (uint32_t)a.count - first);
     // lane k: the piece's k-th key and place (behind its end the last one's); the keys before and behind the piece
     const uint32_t mine  = first + min(lane, many - 1);
@@ -664,10 +672,16 @@ __device__ __forceinline__ uint32_t SumPiece(const SumArgs &a, uint32_t piece, c
     for (uint32_t k0 = 0; k0 < many; k0 += kBatch)
     {
         Run<T, N> row[kBatch];
+        Run<O, N> old[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
         {
             row[j] = columns.get(reinterpret_cast<const T *>(a.grad.at(__builtin_amdgcn_readlane(myPlace, k0 + j))));
+            if constexpr (ACCUMULATE)
+            {
+                const uint32_t key = __builtin_amdgcn_readlane(myKey, k0 + j);
+                old[j]             = columns.get(reinterpret_cast<const O *>(a.table.at(min(key, (uint32_t)a.vocabulary - 1))));
+            }
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
@@ -690,7 +704,7 @@ __device__ __forceinline__ uint32_t SumPiece(const SumArgs &a, uint32_t piece, c
             }
             if (!open && next != key)
             {
-                columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale);
+                columns.put(reinterpret_cast<O *>(a.table.at(key)), s, a.scale, old[j]);
             }
             else
             {
@@ -726,7 +740,7 @@ __device__ __forceinline__ void SumGroup(const SumArgs &a, uint32_t group, uint3
     uint32_t       flags = 0;
     if ((uint64_t)piece * PIECE < (uint64_t)a.count)
     {
-        flags = SumPiece<T, O, PIECE>(a, piece, columns, s_head[wave], s_tail[wave]);
+        flags = SumPiece<T, O, PIECE, ACCUMULATE>(a, piece, columns, s_head[wave], s_tail[wave]);
     }
     if (lane == 0)
     {
