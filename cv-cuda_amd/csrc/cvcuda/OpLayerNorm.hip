@@ -111,9 +111,22 @@ __device__ __forceinline__ float RowSum(float v, float (&part)[WAVES])
     return v;
 }
 
+// Waves of the widest workgroup. The gradient's lanes also hold two sums for each element: with sixteen waves, 128 registers
+// to a lane, they would not fit.
+constexpr int kNormWidest = 16, kGradWidest = 8;
+
 constexpr int GroupWaves(int waves)
 {
     return waves == 1 ? 4 : waves; // narrow rows: four to a workgroup
+}
+
+// Workgroups of sixteen waves go through the rows in turn, each with the next row on its way: they are alone on their CU or nearly
+// so, and each sum would find all of its waves waiting (4000 rows of 8192 BF16 38 us, 52 with a workgroup to each row; with eight
+// waves 26 and 24, with four and 65536 rows of 4096 209 and 191). Not with 32 elements in a lane: two rows of them do not fit
+// in the registers (2000 rows of 24576 F32 144 us and 95).
+constexpr bool Turns(int waves, int elements)
+{
+    return waves == kNormWidest && elements <= 16;
 }
 
 // E: elements in a lane.
@@ -121,22 +134,27 @@ template<class T, class W, int WAVES, int E>
 __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const NormArgs a)
 {
     constexpr int    N = kRunOf<T>, K = E / N;
+    constexpr bool   kTurns        = Turns(WAVES, E);
     constexpr bool   kWeightsFirst = E <= 16; // on their way beside the row; more of them would take registers from other rows
     __shared__ float s_sum[WAVES], s_squares[WAVES];
     const RowRuns<N, WAVES> runs(a.columns);
-    const uint32_t          row = a.firstRow + (WAVES == 1 ? blockIdx.x * 4 + WaveOfGroup() : blockIdx.x);
+    uint32_t                row = a.firstRow + (WAVES == 1 ? blockIdx.x * 4 + WaveOfGroup() : blockIdx.x);
     if (row >= (uint32_t)a.rows)
     {
         return;
     }
-    const uint8_t *from = a.in.at(row);
-    Run<T, N>      x[K];
-    Run<W, N>      gamma[K], beta[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k)
+    Run<T, N> x[K];
+    Run<W, N> gamma[K], beta[K];
+    auto      load = [&](Run<T, N>(&to)[K], uint32_t r)
     {
-        x[k] = runs.template get<T>(from, k);
-    }
+        const uint8_t *from = a.in.at(r);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            to[k] = runs.template get<T>(from, k);
+        }
+    };
+    load(x, row);
     auto loadWeights = [&]
     {
         if (a.gamma != nullptr)
@@ -160,72 +178,90 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const 
     {
         loadWeights();
     }
-    float s = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (;;)
     {
-        const int skip = runs.whole(k) ? 0 : runs.skip(k);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
+        float s = 0;
+        Run<T, N> next[K];
+        if (kTurns && gridDim.x < (uint32_t)a.rows - row)
         {
-            s += i >= skip ? (float)x[k].v[i] : 0.f;
+            load(next, row + gridDim.x);
         }
-    }
-    const float mean = RowSum<WAVES>(s, s_sum) / (float)a.columns;
-    s                = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-    {
-        const int skip = runs.whole(k) ? 0 : runs.skip(k);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int k = 0; k < K; ++k)
         {
-            const float d = i >= skip ? (float)x[k].v[i] - mean : 0.f;
-            s += d * d;
-        }
-    }
-    const float rstd = 1.f / sqrtf(RowSum<WAVES>(s, s_squares) / (float)a.columns + a.epsilon);
-    uint8_t    *to   = a.out.at(row);
-    if (!kWeightsFirst)
-    {
-        loadWeights();
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-    {
-        float y[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-        {
-            y[i] = ((float)x[k].v[i] - mean) * rstd;
-        }
-        if (a.gamma != nullptr)
-        {
+            const int skip = runs.whole(k) ? 0 : runs.skip(k);
 #pragma unroll
             for (int i = 0; i < N; ++i)
             {
-                y[i] *= (float)gamma[k].v[i];
+                s += i >= skip ? (float)x[k].v[i] : 0.f;
             }
         }
-        if (a.beta != nullptr)
+        const float mean = RowSum<WAVES>(s, s_sum) / (float)a.columns;
+        s                = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
         {
+            const int skip = runs.whole(k) ? 0 : runs.skip(k);
 #pragma unroll
             for (int i = 0; i < N; ++i)
             {
-                y[i] += (float)beta[k].v[i];
+                const float d = i >= skip ? (float)x[k].v[i] - mean : 0.f;
+                s += d * d;
             }
         }
-        runs.template put<T>(to, k, y);
-    }
-    if (runs.lane0 == 0)
-    {
-        if (a.mean != nullptr)
+        const float rstd = 1.f / sqrtf(RowSum<WAVES>(s, s_squares) / (float)a.columns + a.epsilon);
+        uint8_t    *to   = a.out.at(row);
+        if (!kWeightsFirst)
         {
-            a.mean[row] = mean;
+            loadWeights();
         }
-        if (a.rstd != nullptr)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
         {
-            a.rstd[row] = rstd;
+            float y[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                y[i] = ((float)x[k].v[i] - mean) * rstd;
+            }
+            if (a.gamma != nullptr)
+            {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    y[i] *= (float)gamma[k].v[i];
+                }
+            }
+            if (a.beta != nullptr)
+            {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    y[i] += (float)beta[k].v[i];
+                }
+            }
+            runs.template put<T>(to, k, y);
+        }
+        if (runs.lane0 == 0)
+        {
+            if (a.mean != nullptr)
+            {
+                a.mean[row] = mean;
+            }
+            if (a.rstd != nullptr)
+            {
+                a.rstd[row] = rstd;
+            }
+        }
+        if (!kTurns || gridDim.x >= (uint32_t)a.rows - row)
+        {
+            break;
+        }
+        row += gridDim.x;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            x[k] = next[k];
         }
     }
 }
@@ -525,38 +561,44 @@ struct RowShape
     int waves, elements;
 };
 
-// The fewest waves whose lanes hold the row with 16 elements each, 32 where the widest workgroup needs them.
+// The fewest waves whose lanes hold the row with 16 elements each, 32 where the widest workgroup needs them. Eight where they
+// suffice: 40000 rows of 8192 BF16 258 us, 391 with sixteen of which half their runs lie behind the row.
 RowShape ShapeOf(int64_t columns, int run, int widest)
 {
     if (columns < run || columns > widest * 64 * 32)
     {
         return {0, 0};
     }
-    const int waves = columns <= 64 * 16 ? 1 : columns <= 4 * 64 * 16 ? 4 : widest;
+    const int waves = columns <= 64 * 16 ? 1 : columns <= 4 * 64 * 16 ? 4 : columns <= 8 * 64 * 16 ? 8 : widest;
     return {waves, columns <= waves * 64 * 8 ? 8 : columns <= waves * 64 * 16 ? 16 : 32};
 }
 
-// Waves of the widest workgroup. The gradient's lanes also hold two sums for each element: with sixteen waves, 128 registers
-// to a lane, they would not fit.
-constexpr int kNormWidest = 16, kGradWidest = 8;
-
-constexpr int kMostParts = 1024;
-
-// Workgroups that share the rows: one for four rows at least, four to a CU at most.
-int Parts(int64_t rows)
+// Workgroups that share the rows of a gradient. Each has the next row under way, so two waves on a SIMD are enough where a lane
+// has 16 elements or more, and fewer sums are left to add up: 65536 rows of 4096 BF16 293 us with 512 workgroups of four waves,
+// 317 with 768, 343 with 1024, 352 with 384; 4000 rows of 8192 56 with 256 of eight, 64 with 512. Lanes of 8 elements want as many
+// as fit, six: 60000 rows of 512 40 us with 1536, 52 with 512.
+int PartsOf(int64_t rows, int64_t columns)
 {
-    return (int)std::min<int64_t>((rows + 3) / 4, kMostParts);
+    const RowShape s    = ShapeOf(columns, 1, kGradWidest);
+    const int64_t  most = s.elements == 8 ? 1536 : 2048 / std::max(s.waves, 4);
+    return (int)std::min((rows + 3) / 4, most);
 }
 
 int64_t GradWorkspace(int64_t rows, int64_t columns)
 {
-    return (int64_t)Parts(rows) * 2 * columns * (int64_t)sizeof(float);
+    return (int64_t)PartsOf(rows, columns) * 2 * columns * (int64_t)sizeof(float);
 }
 
 template<class T, class W, int WAVES, int E>
 void LaunchNormAs(const NormArgs &a, hipStream_t stream)
 {
     const int64_t groups = WAVES == 1 ? ((int64_t)a.rows + 3) / 4 : a.rows;
+    if (Turns(WAVES, E))
+    {
+        hipLaunchKernelGGL((LayerNormKernel<T, W, WAVES, E>), dim3((uint32_t)std::min<int64_t>(groups, 256)), dim3(64 * WAVES), 0, stream, a);
+        CheckLaunch("LayerNormKernel");
+        return;
+    }
     // (rows beyond what a launch may hold go into further ones)
     constexpr int64_t kMost = ((int64_t)1 << 32) / (64 * GroupWaves(WAVES)) - 1;
     for (int64_t first = 0; first < groups; first += kMost)
@@ -584,6 +626,10 @@ void LaunchNorm(const NormArgs &a, hipStream_t stream)
     else if (s.waves == 4)
     {
         s.elements == 8 ? LaunchNormAs<T, W, 4, 8>(a, stream) : LaunchNormAs<T, W, 4, 16>(a, stream);
+    }
+    else if (s.waves == 8)
+    {
+        LaunchNormAs<T, W, 8, 16>(a, stream);
     }
     else
     {
@@ -752,7 +798,7 @@ public:
             return;
         }
         const GradArgs a = {RowPlaces(grad), RowPlaces(in), RowPlaces(out), gamma, mean, rstd, partial, gradGamma, gradBeta,
-                            in.rows, in.columns, Parts(in.rows)};
+                            in.rows, in.columns, PartsOf(in.rows, in.columns)};
         Dispatch(in.elem, w.same(), [&](auto t, auto wt) { LaunchGrad<decltype(t), decltype(wt)>(a, stream); });
     }
 };

@@ -118,6 +118,17 @@ def test_what_is_not_finite_stays_in_its_row(api, d):
         assert got[r].isnan().all() if r in (2, 5, 7) else torch.equal(got[r], clean[r])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [8200, 16383, 24000])
+def test_many_wide_rows(api, dtype, d):
+    """More rows than workgroups that hold one: some go through one row, some through two, some through three."""
+    gamma, beta = weights_of(d, dtype, 12)
+    x = rows_of((600, d), dtype, 13)
+    got, _, _ = check_forward(api, x, gamma, beta)
+    forward(api, x, gamma, beta, out=x)
+    assert torch.equal(x, got)
+
+
 def test_more_than_four_gigabytes(api):
     rows, d = 1100000, 2048
     x = torch.empty((rows, d), dtype=F16, device="cuda")
