@@ -133,7 +133,7 @@ constexpr bool Turns(int waves, int elements)
 template<class T, class W, int WAVES, int E>
 __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const NormArgs a)
 {
-    constexpr int    N = kRunOf<T>, K = E / N;
+    constexpr int    N = std::min(E, kRunOf<T>), K = E / N;
     constexpr bool   kTurns        = Turns(WAVES, E);
     constexpr bool   kWeightsFirst = E <= 16; // on their way beside the row; more of them would take registers from other rows
     __shared__ float s_sum[WAVES], s_squares[WAVES];
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const 
 template<class T, class W, int WAVES, int E>
 __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(const GradArgs a)
 {
-    constexpr int    N = kRunOf<T>, K = E / N, kRows = WAVES == 1 ? 4 : 1;
+    constexpr int    N = std::min(E, kRunOf<T>), K = E / N, kRows = WAVES == 1 ? 4 : 1;
     constexpr bool   kAhead = E * sizeof(T) <= 64;
     __shared__ float s_sum[2][2][WAVES]; // of one row and the next
     const RowRuns<N, WAVES> runs(a.columns);
@@ -433,7 +433,7 @@ __device__ __forceinline__ float BlockSum(float v)
     return part[0] + part[1] + part[2] + part[3];
 }
 
-// Rows too wide for registers, or narrower than a run: one workgroup per row, element by element, three times over the row.
+// Rows too wide for registers, or of fewer than four columns: one workgroup per row, element by element, three times over the row.
 template<class T, class W>
 __global__ __launch_bounds__(256) void LayerNormAnyKernel(const NormArgs a)
 {
@@ -570,26 +570,29 @@ struct RowShape
     int waves, elements;
 };
 
+constexpr int kNarrowest = 4; // columns, of a lane where they are few
+
 // The fewest waves whose lanes hold the row with 16 elements each, 32 where the widest workgroup needs them. Eight where they
-// suffice: 40000 rows of 8192 BF16 258 us, 391 with sixteen of which half their runs lie behind the row.
-RowShape ShapeOf(int64_t columns, int run, int widest)
+// suffice: 40000 rows of 8192 BF16 258 us, 391 with sixteen of which half their runs lie behind the row. Lanes of four where a
+// wave has enough: 60000 rows of 200 F32 17 us, 19 with runs of eight, the gradient 28 and 31.
+RowShape ShapeOf(int64_t columns, int widest)
 {
-    if (columns < run || columns > widest * 64 * 32)
+    if (columns < kNarrowest || columns > widest * 64 * 32)
     {
         return {0, 0};
     }
     const int waves = columns <= 64 * 16 ? 1 : columns <= 4 * 64 * 16 ? 4 : columns <= 8 * 64 * 16 ? 8 : widest;
-    return {waves, columns <= waves * 64 * 8 ? 8 : columns <= waves * 64 * 16 ? 16 : 32};
+    return {waves, columns <= 64 * 4 ? 4 : columns <= waves * 64 * 8 ? 8 : columns <= waves * 64 * 16 ? 16 : 32};
 }
 
 // Workgroups that share the rows of a gradient. Each has the next row under way, so two waves on a SIMD are enough where a lane
 // has 16 elements or more, and fewer sums are left to add up: 65536 rows of 4096 BF16 293 us with 512 workgroups of four waves,
-// 317 with 768, 343 with 1024, 352 with 384; 4000 rows of 8192 56 with 256 of eight, 64 with 512. Lanes of 8 elements want as many
-// as fit, six: 60000 rows of 512 40 us with 1536, 52 with 512.
+// 317 with 768, 343 with 1024, 352 with 384; 4000 rows of 8192 56 with 256 of eight, 64 with 512. Lanes of 8 or 4 elements want as
+// many as fit, six: 60000 rows of 512 40 us with 1536, 52 with 512.
 int PartsOf(int64_t rows, int64_t columns)
 {
-    const RowShape s    = ShapeOf(columns, 1, kGradWidest);
-    const int64_t  most = s.elements == 8 ? 1536 : 2048 / std::max(s.waves, 4);
+    const RowShape s    = ShapeOf(columns, kGradWidest);
+    const int64_t  most = s.elements <= 8 ? 1536 : 2048 / std::max(s.waves, 4);
     return (int)std::min((rows + 3) / 4, most);
 }
 
@@ -622,7 +625,7 @@ void LaunchNormAs(const NormArgs &a, hipStream_t stream)
 template<class T, class W>
 void LaunchNorm(const NormArgs &a, hipStream_t stream)
 {
-    const RowShape s = ShapeOf(a.columns, kRunOf<T>, kNormWidest);
+    const RowShape s = ShapeOf(a.columns, kNormWidest);
     if (s.waves == 0)
     {
         hipLaunchKernelGGL((LayerNormAnyKernel<T, W>), dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, stream, a);
@@ -630,7 +633,9 @@ void LaunchNorm(const NormArgs &a, hipStream_t stream)
     }
     else if (s.waves == 1)
     {
-        s.elements == 8 ? LaunchNormAs<T, W, 1, 8>(a, stream) : LaunchNormAs<T, W, 1, 16>(a, stream);
+        s.elements == 4   ? LaunchNormAs<T, W, 1, 4>(a, stream)
+        : s.elements == 8 ? LaunchNormAs<T, W, 1, 8>(a, stream)
+                          : LaunchNormAs<T, W, 1, 16>(a, stream);
     }
     else if (s.waves == 4)
     {
@@ -656,7 +661,7 @@ void LaunchGradAs(const GradArgs &a, hipStream_t stream)
 template<class T, class W>
 void LaunchGrad(const GradArgs &a, hipStream_t stream)
 {
-    const RowShape s    = ShapeOf(a.columns, kRunOf<T>, kGradWidest);
+    const RowShape s    = ShapeOf(a.columns, kGradWidest);
     const bool     sums = a.gradGamma != nullptr || a.gradBeta != nullptr;
     if (a.rows == 0)
     {
@@ -674,7 +679,9 @@ void LaunchGrad(const GradArgs &a, hipStream_t stream)
     }
     else if (s.waves == 1)
     {
-        s.elements == 8 ? LaunchGradAs<T, W, 1, 8>(a, stream) : LaunchGradAs<T, W, 1, 16>(a, stream);
+        s.elements == 4   ? LaunchGradAs<T, W, 1, 4>(a, stream)
+        : s.elements == 8 ? LaunchGradAs<T, W, 1, 8>(a, stream)
+                          : LaunchGradAs<T, W, 1, 16>(a, stream);
     }
     else if (s.waves == 4)
     {
