@@ -419,104 +419,213 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(co
     }
 }
 
-// Sum over a workgroup of 256, in every thread.
+// Rows too wide for registers, or of fewer than four columns: a workgroup goes over the row more than once, by runs of N (one for
+// narrow rows). 1000 rows of 50000 BF16 89 us, their gradient 198
+// (element by element 310 and 493): what the second time reads is in the cache.
+constexpr int kAnyThreads = 1024;
+
+// Sum over a workgroup of kAnyThreads, in every thread.
 __device__ __forceinline__ float BlockSum(float v)
 {
-    __shared__ float part[4];
-    v = WaveSum(v);
+    __shared__ float part[kAnyThreads / 64];
     __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-    {
-        part[threadIdx.x >> 6] = v;
-    }
-    __syncthreads();
-    return part[0] + part[1] + part[2] + part[3];
+    return RowSum(v, part);
 }
 
-// Rows too wide for registers, or of fewer than four columns: one workgroup per row, element by element, three times over the row.
-template<class T, class W>
-__global__ __launch_bounds__(256) void LayerNormAnyKernel(const NormArgs a)
+// The run from `first` on of D columns; it is loaded from `from` on, the first `skip` of what is loaded are not its own.
+template<int N>
+struct AnyRun
 {
-    for (uint32_t r = blockIdx.x; r < (uint32_t)a.rows; r += gridDim.x)
+    int from, skip;
+
+    __device__ __forceinline__ AnyRun(int first, int D)
+        : from(min(first, D - N))
+        , skip(first - from)
     {
-        const T  *x = reinterpret_cast<const T *>(a.in.at(r));
-        T        *y = reinterpret_cast<T *>(a.out.at(r));
-        const int D = a.columns;
-        float     s = 0;
-        for (int c = threadIdx.x; c < D; c += 256)
+    }
+
+    template<class T>
+    __device__ __forceinline__ Run<T, N> get(const void *row) const
+    {
+        return *reinterpret_cast<const Run<T, N> *>(static_cast<const T *>(row) + from);
+    }
+
+    // the weights of its columns: 1 or 0 where there are none
+    template<class W>
+    __device__ __forceinline__ void weights(float (&v)[N], const void *w, float none) const
+    {
+        if (w == nullptr)
         {
-            s += (float)x[c];
+            for (float &x : v)
+            {
+                x = none;
+            }
+            return;
+        }
+        const Run<W, N> r = get<W>(w);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            v[i] = (float)r.v[i];
+        }
+    }
+
+    // (its own alone: others' may be read from the same memory still)
+    template<class T>
+    __device__ __forceinline__ void put(void *row, const float (&v)[N]) const
+    {
+        T        *to = static_cast<T *>(row) + from;
+        Run<T, N> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            r.v[i] = FromFloat<T>(v[i]);
+        }
+        if (skip == 0)
+        {
+            *reinterpret_cast<Run<T, N> *>(to) = r;
+            return;
+        }
+#pragma unroll
+        for (int i = 1; i < N; ++i)
+        {
+            if (i >= skip)
+            {
+                to[i] = r.v[i];
+            }
+        }
+    }
+};
+
+template<class T, class W, int N>
+__global__ __launch_bounds__(kAnyThreads) void LayerNormAnyKernel(const NormArgs a)
+{
+    const int D = a.columns;
+    for (uint32_t row = blockIdx.x; row < (uint32_t)a.rows; row += gridDim.x)
+    {
+        const uint8_t *x = a.in.at(row);
+        uint8_t       *y = a.out.at(row);
+        float          s = 0;
+        for (int c = threadIdx.x * N; c < D; c += kAnyThreads * N)
+        {
+            const AnyRun<N> run(c, D);
+            const Run<T, N> v = run.template get<T>(x);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                s += i >= run.skip ? (float)v.v[i] : 0.f;
+            }
         }
         const float mean = BlockSum(s) / (float)D;
         s                = 0;
-        for (int c = threadIdx.x; c < D; c += 256)
+        for (int c = threadIdx.x * N; c < D; c += kAnyThreads * N)
         {
-            const float d = (float)x[c] - mean;
-            s += d * d;
+            const AnyRun<N> run(c, D);
+            const Run<T, N> v = run.template get<T>(x);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                const float d = i >= run.skip ? (float)v.v[i] - mean : 0.f;
+                s += d * d;
+            }
         }
         const float rstd = 1.f / sqrtf(BlockSum(s) / (float)D + a.epsilon);
-        for (int c = threadIdx.x; c < D; c += 256)
+        for (int c = threadIdx.x * N; c < D; c += kAnyThreads * N)
         {
-            const float g = a.gamma != nullptr ? (float)static_cast<const W *>(a.gamma)[c] : 1.f;
-            const float b = a.beta != nullptr ? (float)static_cast<const W *>(a.beta)[c] : 0.f;
-            y[c]          = FromFloat<T>(((float)x[c] - mean) * rstd * g + b);
+            const AnyRun<N> run(c, D);
+            const Run<T, N> v = run.template get<T>(x);
+            float           g[N], b[N], out[N];
+            run.template weights<W>(g, a.gamma, 1);
+            run.template weights<W>(b, a.beta, 0);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                out[i] = ((float)v.v[i] - mean) * rstd * g[i] + b[i];
+            }
+            run.template put<T>(y, out);
         }
         if (threadIdx.x == 0 && a.mean != nullptr)
         {
-            a.mean[r] = mean;
+            a.mean[row] = mean;
         }
         if (threadIdx.x == 0 && a.rstd != nullptr)
         {
-            a.rstd[r] = rstd;
+            a.rstd[row] = rstd;
         }
     }
 }
 
-template<class T, class W>
-__global__ __launch_bounds__(256) void LayerNormGradAnyKernel(const GradArgs a)
+template<class T, class W, int N>
+__global__ __launch_bounds__(kAnyThreads) void LayerNormGradAnyKernel(const GradArgs a)
 {
-    for (uint32_t r = blockIdx.x; r < (uint32_t)a.rows; r += gridDim.x)
+    const int D = a.columns;
+    for (uint32_t row = blockIdx.x; row < (uint32_t)a.rows; row += gridDim.x)
     {
-        const T    *dy = reinterpret_cast<const T *>(a.grad.at(r)), *x = reinterpret_cast<const T *>(a.in.at(r));
-        T          *dx   = reinterpret_cast<T *>(a.out.at(r));
-        const float mean = a.mean[r], rstd = a.rstd[r];
-        const int   D = a.columns;
-        float       s = 0, sh = 0;
-        for (int c = threadIdx.x; c < D; c += 256)
+        const uint8_t *dy = a.grad.at(row), *x = a.in.at(row);
+        uint8_t       *dx   = a.out.at(row);
+        const float    mean = a.mean[row], rstd = a.rstd[row];
+        float          s = 0, sh = 0;
+        for (int c = threadIdx.x * N; c < D; c += kAnyThreads * N)
         {
-            const float w = (float)dy[c] * (a.gamma != nullptr ? (float)static_cast<const W *>(a.gamma)[c] : 1.f);
-            s += w;
-            sh += w * (((float)x[c] - mean) * rstd);
+            const AnyRun<N> run(c, D);
+            const Run<T, N> v = run.template get<T>(x), d = run.template get<T>(dy);
+            float           g[N];
+            run.template weights<W>(g, a.gamma, 1);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                const float w = (float)d.v[i] * g[i];
+                s += i >= run.skip ? w : 0.f;
+                sh += i >= run.skip ? w * (((float)v.v[i] - mean) * rstd) : 0.f;
+            }
         }
         s  = BlockSum(s) / (float)D;
         sh = BlockSum(sh) / (float)D;
-        for (int c = threadIdx.x; c < D; c += 256)
+        for (int c = threadIdx.x * N; c < D; c += kAnyThreads * N)
         {
-            const float w = (float)dy[c] * (a.gamma != nullptr ? (float)static_cast<const W *>(a.gamma)[c] : 1.f);
-            const float h = ((float)x[c] - mean) * rstd;
-            dx[c]         = FromFloat<T>(rstd * (w - s - h * sh));
+            const AnyRun<N> run(c, D);
+            const Run<T, N> v = run.template get<T>(x), d = run.template get<T>(dy);
+            float           g[N], out[N];
+            run.template weights<W>(g, a.gamma, 1);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                const float w = (float)d.v[i] * g[i], h = ((float)v.v[i] - mean) * rstd;
+                out[i]        = rstd * (w - s - h * sh);
+            }
+            run.template put<T>(dx, out);
         }
     }
 }
 
-// The same rows' sums: a thread per column and part of the rows.
-template<class T>
-__global__ __launch_bounds__(256) void LayerNormPartsAnyKernel(const GradArgs a)
+// The same rows' sums: a thread for each run of columns and part of the rows.
+constexpr int kPartsThreads = 256;
+
+template<class T, int N>
+__global__ __launch_bounds__(kPartsThreads) void LayerNormPartsAnyKernel(const GradArgs a)
 {
-    const int c = blockIdx.x * 256 + threadIdx.x, D = a.columns;
+    const int64_t c = ((int64_t)blockIdx.x * kPartsThreads + threadIdx.x) * N;
+    const int     D = a.columns;
     if (c >= D)
     {
         return;
     }
-    float g = 0, b = 0;
+    const AnyRun<N> run((int)c, D);
+    float           g[N] = {}, b[N] = {};
+#pragma unroll 4
     for (uint32_t r = blockIdx.y; r < (uint32_t)a.rows; r += a.parts)
     {
-        const float dy = (float)reinterpret_cast<const T *>(a.grad.at(r))[c];
-        g += dy * (((float)reinterpret_cast<const T *>(a.in.at(r))[c] - a.mean[r]) * a.rstd[r]);
-        b += dy;
+        const float     mean = a.mean[r], rstd = a.rstd[r];
+        const Run<T, N> v = run.template get<T>(a.in.at(r)), d = run.template get<T>(a.grad.at(r));
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            g[i] += (float)d.v[i] * (((float)v.v[i] - mean) * rstd);
+            b[i] += (float)d.v[i];
+        }
     }
-    a.partial[(size_t)blockIdx.y * 2 * D + c]     = g;
-    a.partial[(size_t)blockIdx.y * 2 * D + D + c] = b;
+    run.template put<float>(a.partial + (size_t)blockIdx.y * 2 * D, g);
+    run.template put<float>(a.partial + ((size_t)blockIdx.y * 2 + 1) * D, b);
 }
 
 // Adds up the parts' sums: 16 columns to a workgroup, whose 64 rows of 16 lanes take every 64th part each.
@@ -628,7 +737,8 @@ void LaunchNorm(const NormArgs &a, hipStream_t stream)
     const RowShape s = ShapeOf(a.columns, kNormWidest);
     if (s.waves == 0)
     {
-        hipLaunchKernelGGL((LayerNormAnyKernel<T, W>), dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, stream, a);
+        const auto kernel = a.columns < kNarrowest ? LayerNormAnyKernel<T, W, 1> : LayerNormAnyKernel<T, W, kRunOf<T>>;
+        hipLaunchKernelGGL(kernel, dim3(std::min(a.rows, kMostGroups)), dim3(kAnyThreads), 0, stream, a);
         CheckLaunch("LayerNormAnyKernel");
     }
     else if (s.waves == 1)
@@ -669,12 +779,15 @@ void LaunchGrad(const GradArgs &a, hipStream_t stream)
     else if (s.waves == 0)
     {
         // gradIn may be written over gradOut or in: the sums over rows come first
+        const bool narrow = a.columns < kNarrowest;
         if (sums)
         {
-            hipLaunchKernelGGL((LayerNormPartsAnyKernel<T>), dim3(DivUp(a.columns, 256), a.parts), dim3(256), 0, stream, a);
+            const auto kernel = narrow ? LayerNormPartsAnyKernel<T, 1> : LayerNormPartsAnyKernel<T, kRunOf<T>>;
+            hipLaunchKernelGGL(kernel, dim3(DivUp(a.columns, kPartsThreads * (narrow ? 1 : kRunOf<T>)), a.parts), dim3(kPartsThreads), 0, stream, a);
             CheckLaunch("LayerNormPartsAnyKernel");
         }
-        hipLaunchKernelGGL((LayerNormGradAnyKernel<T, W>), dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, stream, a);
+        const auto kernel = narrow ? LayerNormGradAnyKernel<T, W, 1> : LayerNormGradAnyKernel<T, W, kRunOf<T>>;
+        hipLaunchKernelGGL(kernel, dim3(std::min(a.rows, kMostGroups)), dim3(kAnyThreads), 0, stream, a);
         CheckLaunch("LayerNormGradAnyKernel");
     }
     else if (s.waves == 1)

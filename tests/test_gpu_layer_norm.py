@@ -129,6 +129,24 @@ def test_many_wide_rows(api, dtype, d):
     assert torch.equal(x, got)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [2, 33001, 40003])
+def test_rows_read_more_than_once_in_place(api, dtype, d):
+    """Rows that do not fit the registers, their ends within a run: what is stored must not be read again."""
+    gamma, beta = weights_of(d, F32, 3)
+    x, dy = rows_of((5, d), dtype, 8), rows_of((5, d), dtype, 9)
+    got, mean, rstd = check_forward(api, x, gamma, beta)
+    dx = check_gradients(api, dy, x, gamma, mean, rstd)[0]
+    for over in (dy, x):
+        before = over.clone()
+        made = [torch.empty(d, device="cuda") for _ in range(2)]
+        api.layer_norm_grad_into(*[api.as_tensor(t) for t in (over, *made, dy, x, gamma, mean, rstd)])
+        assert torch.equal(over, dx)
+        over.copy_(before)
+    forward(api, x, gamma, beta, out=x)
+    assert torch.equal(x, got)
+
+
 def test_more_than_four_gigabytes(api):
     rows, d = 1100000, 2048
     x = torch.empty((rows, d), dtype=F16, device="cuda")
