@@ -161,7 +161,8 @@ __device__ __forceinline__ int EntryOf(const Args &a, uint32_t tile)
     return e;
 }
 
-// States of 32 bits. 28 bytes of an element and 40 instructions: bound by memory.
+// States of 32 bits. 24 bytes of an element and its gradient's, 40 instructions: bound by memory (134 M elements with BF16 gradients
+// 654 us, 5.3 TB/s; 772 thousand F32 ones 6.2 us).
 template<class P, class G>
 __global__ __launch_bounds__(256) void AdamWKernel(const StepArgs a)
 {
@@ -221,7 +222,7 @@ struct BlockScale
 };
 
 // States of 8 bits: a wave takes whole blocks, whose largest magnitudes are found across its lanes. Bound by its arithmetic: 110
-// instructions and six approximations of an element, 93 us for 30 M elements, which move their 14 bytes in 82 (measured: 101).
+// instructions and six approximations of an element, 410 us for 134 M elements, which move their 14 bytes in 370 (measured: 430).
 template<class P, class G>
 __global__ __launch_bounds__(256) void AdamWSmallKernel(const StepArgs a)
 {
@@ -359,6 +360,7 @@ struct UnpackArgs
 
 static_assert(sizeof(UnpackArgs) <= 4096, "arguments of a launch");
 
+// 5 bytes of an element, four of them written: 134 M elements 96 us, 7.0 TB/s, the rate of a fill.
 __global__ __launch_bounds__(256) void AdamWUnpackKernel(const UnpackArgs a)
 {
     for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)

@@ -132,6 +132,7 @@ constexpr int kLookupRuns = 2, kLookupGroup = 256 * kLookupRuns; // of a lane, a
 
 // The runs of all rows are numbered through, so that narrow rows fill the lanes as well. The last run of a row whose width is no
 // multiple begins earlier, as in LaneColumns. The token is read before its row: two waits for memory, which other waves fill.
+// 32768 rows of 2048 from F32 to BF16 45 us, 5.0 TB/s; eight rows of 4096 3 us.
 template<class T, class O, bool NARROW>
 __global__ __launch_bounds__(256) void EmbeddingKernel(const LookupArgs a)
 {
@@ -343,7 +344,7 @@ constexpr int kSmallThreads = 1024, kSmallBits = 6;
 constexpr int kMostSmall    = 4 * kSmallThreads;
 
 // All of up to K * 1024 tokens by one workgroup, in LDS. A wave owns 64 K consecutive elements; 16 waves with 64 digits
-// each have a counter per thread.
+// each have a counter per thread. 1003 tokens among 30011 7 us: three passes, one wait after another.
 template<int K>
 __global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const TokenSource src, uint32_t *keys, uint32_t *places, int bits,
                                                                          const ClearArgs clear)
@@ -411,7 +412,8 @@ __global__ __launch_bounds__(kSmallThreads) void EmbeddingSortSmallKernel(const 
 }
 
 // More tokens: tiles of them, two launches for each digit. The first counts the digits of each tile, the second adds up what
-// comes before each digit of its tile and puts the tile's elements there.
+// comes before each digit of its tile and puts the tile's elements there. 65536 tokens among 128000 38 us, the time in which 128 MiB
+// of the table are cleared beside it.
 constexpr int kTileThreads = 512, kTileBits = 9, kDigits = 1 << kTileBits;
 
 // Keys of a thread. Small tiles are quick, but each reads the counts of all others: 64 small ones at most (16384 tokens' sort 30 us,
@@ -794,7 +796,8 @@ __device__ __forceinline__ void SumGroup(const SumArgs &a, uint32_t group, uint3
     __syncthreads(); // (before the next group's)
 }
 
-// A workgroup is one of tokens, or waves that clear rows.
+// A workgroup is one of tokens, or waves that clear rows. 65536 tokens of width 2048, BF16, into 128000 rows of F32, of which the
+// sort has cleared some: 215 us, 5.3 TB/s.
 template<class T, class O, int PIECE, bool NARROW, bool ACCUMULATE>
 __global__ __launch_bounds__(64 * kSumWaves) void EmbeddingSumKernel(const SumArgs a)
 {
@@ -875,7 +878,7 @@ __device__ __forceinline__ void JoinGroups(const SumArgs &a, uint32_t group, uin
     __syncthreads(); // (before the next group's)
 }
 
-// A workgroup per group but the last, which nothing follows, and 64 lanes' columns.
+// A workgroup per group but the last, which nothing follows, and 64 lanes' columns (3 to 6 us).
 template<class O, bool NARROW, bool ACCUMULATE>
 __global__ __launch_bounds__(64 * kJoinWaves) void EmbeddingJoinKernel(const SumArgs a)
 {

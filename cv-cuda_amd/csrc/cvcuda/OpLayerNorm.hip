@@ -129,7 +129,8 @@ constexpr bool Turns(int waves, int elements)
     return waves == kNormWidest && elements <= 16;
 }
 
-// E: elements in a lane.
+// E: elements in a lane. 65536 rows of 4096 BF16 190 us, 5.6 TB/s; 12544 rows of 768 F16 11 us, 3.6 TB/s (half of that is the first
+// loads' and the last stores' time), one row 2.6.
 template<class T, class W, int WAVES, int E>
 __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const NormArgs a)
 {
@@ -269,6 +270,7 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const 
 // The rows' gradient, and the sums over the rows that a workgroup goes through: every parts-th (in narrow rows each of its
 // waves takes one). The next row and its statistics are on their way while the sums of one are awaited (8949 rows of 3328 F16 43
 // us, 49 where the statistics were not), unless two rows are too much for the registers (4000 rows of 12288 F32 124 us and 214).
+// 65536 rows of 4096 BF16 283 us, 5.7 TB/s; 12544 rows of 768 F16 15.6 us, 3.7 TB/s.
 template<class T, class W, int WAVES, int E>
 __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(const GradArgs a)
 {
@@ -628,7 +630,8 @@ __global__ __launch_bounds__(kPartsThreads) void LayerNormPartsAnyKernel(const G
     run.template put<float>(a.partial + ((size_t)blockIdx.y * 2 + 1) * D, b);
 }
 
-// Adds up the parts' sums: 16 columns to a workgroup, whose 64 rows of 16 lanes take every 64th part each.
+// Adds up the parts' sums: 16 columns to a workgroup, whose 64 rows of 16 lanes take every 64th part each (512 parts of 4096
+// columns 7.5 us, of 768 3.9, most of them one wait after another).
 constexpr int kJoinColumns = 16;
 
 template<class W>
