@@ -8,6 +8,8 @@ against the reference's `cvcuda` / `nvcv` modules for these operators runs with
     import cvcuda_amd.pyapi as cvcuda
     nvcv = cvcuda
 
+layer_norm, embedding, their gradients and adamw are additions of this module for models that train on its batches.
+
 Every function forwards to the C ABI through the operator classes of the package; `stream=None` means the current
 stream (`Stream.current`: the innermost `with stream:`, else the default stream). Containers keep the bindings'
 ordering across streams: a call on one stream waits for the work of other streams that wrote what it reads or
