@@ -271,8 +271,8 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormKernel(const 
 // waves takes one). The next row and its statistics are on their way while the sums of one are awaited (8949 rows of 3328 F16 43
 // us, 49 where the statistics were not), unless two rows are too much for the registers (4000 rows of 12288 F32 124 us and 214).
 // 65536 rows of 4096 BF16 283 us, 5.7 TB/s; 12544 rows of 768 F16 15.6 us, 3.7 TB/s.
-template<class T, class W, int WAVES, int E>
-__global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(const GradArgs a)
+template<class T, class W, int WAVES, int E, bool SUMS>
+__device__ __forceinline__ void GradRows(const GradArgs &a)
 {
     constexpr int    N = std::min(E, kRunOf<T>), K = E / N, kRows = WAVES == 1 ? 4 : 1;
     constexpr bool   kAhead = E * sizeof(T) <= 64;
@@ -335,8 +335,11 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(co
                 const float d = (float)dy[k].v[i];
                 h[k][i]       = ((float)x[k].v[i] - mean) * rstd;
                 w[k][i]       = d * gamma[k][i];
-                toGamma[k][i] += d * h[k][i];
-                toBeta[k][i] += d;
+                if constexpr (SUMS)
+                {
+                    toGamma[k][i] += d * h[k][i];
+                    toBeta[k][i] += d;
+                }
                 s += i >= skip ? w[k][i] : 0.f;
                 sh += i >= skip ? w[k][i] * h[k][i] : 0.f;
             }
@@ -379,7 +382,7 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(co
             load(next);
         }
     }
-    if (a.partial == nullptr)
+    if (!SUMS || a.partial == nullptr)
     {
         return;
     }
@@ -419,6 +422,12 @@ __global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(co
             runs.template put<float>(a.partial + ((size_t)blockIdx.x * 2 + 1) * a.columns, k, toBeta[k]);
         }
     }
+}
+
+template<class T, class W, int WAVES, int E>
+__global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradKernel(const GradArgs a)
+{
+    GradRows<T, W, WAVES, E, true>(a);
 }
 
 // Rows too wide for registers, or of fewer than four columns: a workgroup goes over the row more than once, by runs of N (one for
@@ -630,6 +639,88 @@ __global__ __launch_bounds__(kPartsThreads) void LayerNormPartsAnyKernel(const G
     run.template put<float>(a.partial + ((size_t)blockIdx.y * 2 + 1) * D, b);
 }
 
+// The sums over few rows, of as many columns as a workgroup holds for 32 rows at once, in runs of four.
+constexpr int kFewSlots = 32, kFewRun = 4;
+
+constexpr int FewColumns(int threads)
+{
+    return threads / kFewSlots * kFewRun;
+}
+
+template<class T, class W, int THREADS>
+__device__ __forceinline__ void SumColumns(const GradArgs &a, uint32_t tile)
+{
+    constexpr int    N = kFewRun, kColumns = FewColumns(THREADS), kLanes = kColumns / N, kAhead = 8; // rows of a lane on their way
+    __shared__ float s_gamma[kFewSlots][kColumns], s_beta[kFewSlots][kColumns];
+    const int        slot = threadIdx.x / kLanes, first = (int)tile * kColumns + (threadIdx.x % kLanes) * N;
+    const AnyRun<N>  run(first, a.columns);
+    float            g[N] = {}, b[N] = {};
+    for (int r0 = slot; r0 < a.rows; r0 += kFewSlots * kAhead)
+    {
+        Run<T, N> x[kAhead], dy[kAhead];
+        float     mean[kAhead], rstd[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+        {
+            const uint32_t r = min(r0 + j * kFewSlots, a.rows - 1);
+            x[j]             = run.template get<T>(a.in.at(r));
+            dy[j]            = run.template get<T>(a.grad.at(r));
+            mean[j]          = a.mean[r];
+            rstd[j]          = a.rstd[r];
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+        {
+            const bool there = r0 + j * kFewSlots < a.rows;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                const float d = (float)dy[j].v[i];
+                g[i] += there ? d * (((float)x[j].v[i] - mean[j]) * rstd[j]) : 0.f;
+                b[i] += there ? d : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+        if (i >= run.skip)
+        {
+            const int at     = run.from + i - (int)tile * kColumns;
+            s_gamma[slot][at] = g[i];
+            s_beta[slot][at]  = b[i];
+        }
+    }
+    __syncthreads();
+    const int c = threadIdx.x % kColumns, column = (int)tile * kColumns + c, which = threadIdx.x / kColumns;
+    W        *to = static_cast<W *>(which == 0 ? a.gradGamma : a.gradBeta);
+    if (which < 2 && column < a.columns && to != nullptr)
+    {
+        float s = 0;
+#pragma unroll
+        for (int k = 0; k < kFewSlots; ++k)
+        {
+            s += which == 0 ? s_gamma[k][c] : s_beta[k][c];
+        }
+        to[column] = FromFloat<W>(s);
+    }
+}
+
+// Few rows: all of the gradient in one launch, the sums from the rows themselves by workgroups behind those of the rows. 256 rows of
+// 768 BF16 4.2 us (in two launches 7.5, and a call 4 more), 512 rows of 4096 7.2 (13.9), 1024 of 768 9.0 (9.2).
+template<class T, class W, int WAVES, int E>
+__global__ __launch_bounds__(64 * GroupWaves(WAVES)) void LayerNormGradFewKernel(const GradArgs a)
+{
+    if (blockIdx.x < (uint32_t)a.parts)
+    {
+        GradRows<T, W, WAVES, E, false>(a);
+    }
+    else
+    {
+        SumColumns<T, W, 64 * GroupWaves(WAVES)>(a, blockIdx.x - a.parts);
+    }
+}
+
 // Adds up the parts' sums: 16 columns to a workgroup, whose 64 rows of 16 lanes take every 64th part each (512 parts of 4096
 // columns 7.5 us, of 768 3.9, most of them one wait after another).
 constexpr int kJoinColumns = 16;
@@ -695,6 +786,14 @@ RowShape ShapeOf(int64_t columns, int widest)
     }
     const int waves = columns <= 64 * 16 ? 1 : columns <= 4 * 64 * 16 ? 4 : columns <= 8 * 64 * 16 ? 8 : widest;
     return {waves, columns <= 64 * 4 ? 4 : columns <= waves * 64 * 8 ? 8 : columns <= waves * 64 * 16 ? 16 : 32};
+}
+
+// Rows whose gradient is one launch: the sums over 2048 of 768 would take 18 us, with a second launch 10.
+constexpr int kFewRows = 1024;
+
+bool Few(int64_t rows, int64_t columns)
+{
+    return rows > 0 && rows <= kFewRows && ShapeOf(columns, kGradWidest).waves != 0;
 }
 
 // Workgroups that share the rows of a gradient. Each has the next row under way, so two waves on a SIMD are enough where a lane
@@ -767,6 +866,29 @@ void LaunchNorm(const NormArgs &a, hipStream_t stream)
 template<class T, class W, int WAVES, int E>
 void LaunchGradAs(const GradArgs &a, hipStream_t stream)
 {
+    if (Few(a.rows, a.columns))
+    {
+        // gradIn may be written over gradOut or in: the sums over rows come first there
+        const bool     sums = a.gradGamma != nullptr || a.gradBeta != nullptr, over = a.out.base == a.grad.base || a.out.base == a.in.base;
+        const uint32_t tiles = sums ? DivUp(a.columns, FewColumns(64 * GroupWaves(WAVES))) : 0, rows = DivUp(a.rows, WAVES == 1 ? 4 : 1);
+        auto           launch = [&](uint32_t rowGroups, uint32_t columnGroups)
+        {
+            GradArgs b = a;
+            b.parts    = (int32_t)rowGroups;
+            hipLaunchKernelGGL((LayerNormGradFewKernel<T, W, WAVES, E>), dim3(rowGroups + columnGroups), dim3(64 * GroupWaves(WAVES)), 0, stream, b);
+            CheckLaunch("LayerNormGradFewKernel");
+        };
+        if (over && sums)
+        {
+            launch(0, tiles);
+            launch(rows, 0);
+        }
+        else
+        {
+            launch(rows, tiles);
+        }
+        return;
+    }
     hipLaunchKernelGGL((LayerNormGradKernel<T, W, WAVES, E>), dim3(a.parts), dim3(64 * GroupWaves(WAVES)), 0, stream, a);
     CheckLaunch("LayerNormGradKernel");
 }
@@ -807,7 +929,7 @@ void LaunchGrad(const GradArgs &a, hipStream_t stream)
     {
         s.elements <= 16 ? LaunchGradAs<T, W, kGradWidest, 16>(a, stream) : LaunchGradAs<T, W, kGradWidest, 32>(a, stream);
     }
-    if (sums)
+    if (sums && !Few(a.rows, a.columns))
     {
         const int64_t groups = (2 * (int64_t)a.columns + kJoinColumns - 1) / kJoinColumns;
         hipLaunchKernelGGL((LayerNormJoinKernel<W>), dim3((uint32_t)std::min<int64_t>(groups, kMostGroups)), dim3(1024), 0, stream, a);

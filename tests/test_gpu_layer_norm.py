@@ -222,6 +222,23 @@ def test_gradient_of_rows_with_gaps_and_in_place(api, dtype, d):
         over.copy_(before)
 
 
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 255, 256, 257, 1024, 1025])
+@pytest.mark.parametrize("d", [4, 31, 32, 33, 765, 1025, 4099, 8201])
+def test_gradient_of_few_rows(api, rows, d):
+    """One launch or two, whole and ragged tiles of columns and rows; over its inputs, and with NaN in one row."""
+    gamma, beta = weights_of(d, F32, 2)
+    x, dy = rows_of((rows, d), BF16, rows + d), rows_of((rows, d), BF16, rows * 3 + d, offset=0.01, scale=0.1)
+    _, mean, rstd = forward(api, x, gamma, beta)
+    got = check_gradients(api, dy, x, gamma, mean, rstd)
+    before = dy.clone()
+    again = gradients(api, dy, x, gamma, mean, rstd, out=dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    before[rows - 1, d - 1] = float("nan")
+    dx, dg, db = gradients(api, before, x, gamma, mean, rstd)
+    assert torch.equal(dx[:-1], got[0][:-1]) and dx[-1].isnan().all()
+    assert torch.equal(dg[:-1], got[1][:-1]) and torch.equal(db[:-1], got[2][:-1]) and dg[-1].isnan() and db[-1].isnan()
+
+
 def test_gradient_without_some_of_them(api):
     x, dy = rows_of((50, 300), BF16, 1), rows_of((50, 300), BF16, 2)
     gamma, beta = weights_of(300, BF16, 3)
