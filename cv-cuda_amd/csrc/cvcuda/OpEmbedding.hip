@@ -551,13 +551,13 @@ __global__ __launch_bounds__(kTileThreads) void EmbeddingPlaceKernel(const TileA
 // workgroup, whose waves have pieces that follow one another, and what reaches over the workgroup's is left in the workspace,
 // where a second launch adds it up: always in the order of the positions. Rows of the table that no token names are cleared
 // beside that by waves that look for their keys among the sorted ones.
-constexpr int kSumWaves = 8, kSmallPiece = 8, kPiece = 32;
+constexpr int kSumWaves = 8, kSmallPiece = 8, kPiece = 32, kFewTokens = kSumWaves * kSmallPiece;
 
 // Small pieces where there are too few to fill the card (2^24 elements are 1024 waves of large ones): their time is that of
 // one wait after another (1003 tokens of width 515 28 -> 21.5 us, 16384 of 64 40 -> 32; 16384 of 4096 would take 141 for 135).
 constexpr int PieceOf(int64_t tokens, int64_t columns)
 {
-    return tokens * columns <= 1 << 24 ? kSmallPiece : kPiece;
+    return tokens <= kFewTokens || tokens * columns <= 1 << 24 ? kSmallPiece : kPiece;
 }
 
 struct SumArgs
@@ -599,6 +599,23 @@ __device__ __forceinline__ uint32_t FirstOf(const uint32_t *keys, uint32_t n, ui
     return lo;
 }
 
+// Clears the rows from row0 on that have no bit in `named`; what follows one another without a gap as one run of bytes.
+template<class O>
+__device__ __forceinline__ void ClearNotNamed(const SumArgs &a, uint32_t row0, uint32_t rows, uint32_t named)
+{
+    for (uint32_t r = 0; r < rows;)
+    {
+        if ((named >> r) & 1)
+        {
+            ++r;
+            continue;
+        }
+        const uint32_t many = a.dense ? min(rows - r, (uint32_t)__builtin_ctzll((named >> r) | 1ull << 32)) : 1;
+        ClearBytes(a.table.at(row0 + r), (int64_t)many * a.columns * (int64_t)sizeof(O), (int)sizeof(O));
+        r += many;
+    }
+}
+
 template<class O>
 __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
 {
@@ -631,18 +648,7 @@ __device__ __forceinline__ void ClearRows(const SumArgs &a, uint32_t wave)
         }
         named = (uint32_t)__ballot(lane < rows && from < (uint32_t)a.count && a.keys[min(from, (uint32_t)a.count - 1)] == row0 + lane);
     }
-    // rows that follow one another without a gap are cleared as one run of bytes
-    for (uint32_t r = 0; r < rows;)
-    {
-        if ((named >> r) & 1)
-        {
-            ++r;
-            continue;
-        }
-        const uint32_t many = a.dense ? min(rows - r, (uint32_t)__builtin_ctzll((named >> r) | 1ull << 32)) : 1;
-        ClearBytes(a.table.at(row0 + r), (int64_t)many * a.columns * (int64_t)sizeof(O), (int)sizeof(O));
-        r += many;
-    }
+    ClearNotNamed<O>(a, row0, rows, named);
 }
 
 // What a piece leaves of the tokens that reach over its ends, and whether: its first one began before it, that one goes on
@@ -816,6 +822,65 @@ __global__ __launch_bounds__(64 * kSumWaves) void EmbeddingSumKernel(const SumAr
     }
 }
 
+// Few tokens, a group of small pieces: one launch and no workspace. The workgroups that sum put all of them in order by themselves:
+// the place of a key is the number of those that are less, and of the same ones before it. The waves that clear hold a key
+// in each lane. Three tokens of width 640 added to a table 7 us a call, 12 with the sort; 64 of 4544 into 4625 rows 16, 21.
+static_assert(kFewTokens == 64, "a key in each lane");
+
+// Larger tables are cleared whole by a launch of their own, whose waves wait for no token: 1.01 GB 175 us, so 187; 123 MB 29, so 22.
+constexpr int64_t kFewClearBytes = (int64_t)512 << 20;
+
+// Clears rows that no key names, region by region as ClearRows.
+template<class O>
+__device__ __forceinline__ void ClearFew(const SumArgs &a, uint32_t key)
+{
+    const uint32_t waves = (a.rowsToClear + a.clearRows - 1) / a.clearRows;
+    for (uint32_t w = (blockIdx.x - a.columnTiles) * kSumWaves + WaveOfGroup(); w < waves; w += a.clearGroups * kSumWaves)
+    {
+        const uint32_t row0 = w * a.clearRows, rows = min(a.clearRows, a.rowsToClear - row0);
+        uint32_t       named = 0;
+        for (uint64_t rest = __ballot(key - row0 < rows); rest != 0; rest &= rest - 1)
+        {
+            named |= 1u << ((uint32_t)__builtin_amdgcn_readlane(key, __builtin_ctzll(rest)) - row0);
+        }
+        ClearNotNamed<O>(a, row0, rows, named);
+    }
+}
+
+// Clears the rows of a table.
+__global__ __launch_bounds__(kSmallThreads) void EmbeddingClearKernel(const ClearArgs clear)
+{
+    ClearBeside(clear);
+}
+
+template<class T, class O, bool NARROW, bool ACCUMULATE>
+__global__ __launch_bounds__(64 * kSumWaves) void EmbeddingFewKernel(const TokenSource src, SumArgs a)
+{
+    __shared__ uint32_t s_keys[kFewTokens], s_places[kFewTokens];
+    const uint32_t      lane = threadIdx.x & 63, key = src.key(lane); // (behind the last one the table's length, as without a part in it)
+    if (blockIdx.x >= a.columnTiles)
+    {
+        ClearFew<O>(a, key);
+        return;
+    }
+    if (WaveOfGroup() == 0)
+    {
+        uint32_t place = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kFewTokens; ++j)
+        {
+            const uint32_t other = __builtin_amdgcn_readlane(key, j);
+            place += other < key || (other == key && j < lane) ? 1 : 0;
+        }
+        s_keys[place]   = key;
+        s_places[place] = lane;
+    }
+    __syncthreads();
+    a.keys   = s_keys;
+    a.places = s_places;
+    SumGroup<T, O, kSmallPiece, NARROW, ACCUMULATE>(a, 0, blockIdx.x);
+}
+
 constexpr int kJoinRun = 4, kJoinWaves = 4; // columns of a lane; each wave adds up a part of the groups
 
 // The sum of a token that begins in a group and goes on behind it.
@@ -917,7 +982,7 @@ struct GradRoom
         otherPlaces = otherKeys + (tiles > 0 ? list : 0);
         counts      = otherPlaces + (tiles > 0 ? list : 0);
         partial     = counts + RoundUp(tiles, kCountsAtOnce) * kDigits * 4;
-        bytes       = partial + (groups > 1 ? groups * 2 * columns * 4 : 0);
+        bytes       = tokens > kFewTokens ? partial + (groups > 1 ? groups * 2 * columns * 4 : 0) : 0;
     }
 };
 
@@ -1027,6 +1092,15 @@ void SortTokens(const TokenSource &src, uint8_t *room, const GradRoom &at, Clear
     }
 }
 
+// All of a gradient of few tokens.
+template<class T, class O, bool NARROW>
+void LaunchFew(const TokenSource &src, const SumArgs &a, hipStream_t stream)
+{
+    const auto kernel = a.accumulate ? EmbeddingFewKernel<T, O, NARROW, true> : EmbeddingFewKernel<T, O, NARROW, false>;
+    hipLaunchKernelGGL(kernel, dim3(a.columnTiles + a.clearGroups), dim3(64 * kSumWaves), 0, stream, src, a);
+    CheckLaunch("EmbeddingFewKernel");
+}
+
 uint32_t Groups(int64_t groups)
 {
     return (uint32_t)std::min<int64_t>(groups, kMostGroups);
@@ -1047,13 +1121,18 @@ void LaunchSum(const SumArgs &a, uint32_t grid, hipStream_t stream)
 }
 
 template<class T, class O>
-void LaunchGrad(SumArgs &a, hipStream_t stream)
+void LaunchGrad(const TokenSource &src, SumArgs &a, hipStream_t stream)
 {
     a.columnTiles = (uint32_t)Parts(a.columns, 64 * kRunOf<T>);
     a.joinTiles   = (uint32_t)Parts(a.columns, 64 * kJoinRun);
     a.clearRows   = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(kMostClearRows, kClearBytes / (a.columns * (int64_t)sizeof(O))));
     a.sumGroups   = Groups((int64_t)a.groups * a.columnTiles);
     a.clearGroups = Groups(Parts(Parts(a.rowsToClear, a.clearRows), kSumWaves));
+    if (a.count > 0 && a.count <= kFewTokens)
+    {
+        a.columns < kRunOf<T> ? LaunchFew<T, O, true>(src, a, stream) : LaunchFew<T, O, false>(src, a, stream);
+        return;
+    }
     if (const uint32_t grid = a.sumGroups + a.clearGroups)
     {
         if (a.group == kSumWaves * kSmallPiece)
@@ -1174,28 +1253,44 @@ public:
         }
         const int64_t  rowBytes = table.columns * (int64_t)RowElemSize(table.elem);
         const bool     dense    = table.inner == table.rows && table.innerStride == rowBytes;
-        const uint32_t beside   = accumulate ? 0 : RowsBesideSort(tokens.count, table.rows, rowBytes);
-        if (tokens.count > 0)
+        const bool     few      = tokens.count > 0 && tokens.count <= kFewTokens;
+        const uint32_t beside   = accumulate ? 0
+                                : few        ? (table.rows * rowBytes > kFewClearBytes ? table.rows : 0)
+                                             : RowsBesideSort(tokens.count, table.rows, rowBytes);
+        const TokenSource src      = {tokens.base, tokens.wide, tokens.count, table.rows, padding};
+        Clearing          clearing = {{RowPlaces(table), rowBytes, RowElemSize(table.elem), dense, table.rows - beside, 0, 0}, beside, 0};
+        if (tokens.count > kFewTokens)
         {
-            SortTokens({tokens.base, tokens.wide, tokens.count, table.rows, padding}, room, at,
-                       {{RowPlaces(table), rowBytes, RowElemSize(table.elem), dense, table.rows - beside, 0, 0}, beside, 0}, stream);
+            SortTokens(src, room, at, clearing, stream);
+        }
+        else if (beside > 0)
+        {
+            clearing.launches   = 1;
+            const uint32_t grid = clearing.next(0, kSmallThreads / 64);
+            hipLaunchKernelGGL(EmbeddingClearKernel, dim3(grid), dim3(kSmallThreads), 0, stream, clearing.args);
+            CheckLaunch("EmbeddingClearKernel");
         }
         const uint32_t group = (uint32_t)(kSumWaves * PieceOf(tokens.count, table.columns));
-        SumArgs a = {RowPlaces(grad), RowPlaces(table), reinterpret_cast<const uint32_t *>(room + at.keys),
-                     reinterpret_cast<const uint32_t *>(room + at.places), reinterpret_cast<float *>(room + at.partial), tokens.count,
+        SumArgs a = {RowPlaces(grad), RowPlaces(table), nullptr, nullptr, nullptr, tokens.count,
                      table.rows, table.columns, accumulate, (uint32_t)Parts(tokens.count, group), group, 0, 0, 0, 0, 0,
                      accumulate ? 0 : (uint32_t)table.rows - beside, dense, scale};
+        if (room != nullptr)
+        {
+            a.keys    = reinterpret_cast<const uint32_t *>(room + at.keys);
+            a.places  = reinterpret_cast<const uint32_t *>(room + at.places);
+            a.partial = reinterpret_cast<float *>(room + at.partial);
+        }
         if (grad.elem == kRowF32)
         {
-            LaunchGrad<float, float>(a, stream);
+            LaunchGrad<float, float>(src, a, stream);
         }
         else if (grad.elem == kRowF16)
         {
-            table.elem == kRowF32 ? LaunchGrad<Half, float>(a, stream) : LaunchGrad<Half, Half>(a, stream);
+            table.elem == kRowF32 ? LaunchGrad<Half, float>(src, a, stream) : LaunchGrad<Half, Half>(src, a, stream);
         }
         else
         {
-            table.elem == kRowF32 ? LaunchGrad<Bf16, float>(a, stream) : LaunchGrad<Bf16, Bf16>(a, stream);
+            table.elem == kRowF32 ? LaunchGrad<Bf16, float>(src, a, stream) : LaunchGrad<Bf16, Bf16>(src, a, stream);
         }
     }
 };

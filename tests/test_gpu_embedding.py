@@ -160,6 +160,30 @@ def test_gradient_of_many_tokens(api, n, v):
     check_gradient(api, dy[:, :3], (v - 1 - tokens).int(), v, F32)
 
 
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 63, 64, 65, 100])
+@pytest.mark.parametrize("in_type,out_type", [(F32, F32), (F16, F32), (BF16, BF16)])
+def test_gradient_of_few_tokens(api, n, in_type, out_type):
+    for v, d in ((1, 2), (30, 3), (40, 515), (1000, 4096), (70, 20000)):
+        tokens, dy = words(n, v + 3, n) - 1, normal((n, d), in_type, 5)  # (some are unknown)
+        got = check_gradient(api, dy, tokens, v, out_type, 3.0)
+        assert torch.equal(got, check_gradient(api, dy, tokens.int(), v, out_type, 3.0))
+        check_gradient(api, dy, tokens, v, out_type, 0.5, padding=0, accumulate=True, out=normal((v, d), out_type, 3))
+        check_gradient(api, dy, tokens, v, out_type, padding=v - 1)
+    dy = normal((n, 170001), in_type, 6)  # one group of large pieces, from 99 tokens on
+    check_gradient(api, dy, words(n, 5, n), 5, out_type)
+
+
+@pytest.mark.parametrize("gap", [0, 4])
+def test_gradient_of_few_tokens_into_a_large_table(api, gap):
+    v, d = 140000, 1024
+    table = torch.full((v, d + gap), 9.0, device="cuda")
+    tokens, dy = torch.tensor([v - 1, 5, v, 0, 5, 70000], device="cuda"), normal((6, d), F32, 7)
+    api.embedding_grad_into(wrap(api, table[:, :d]), wrap(api, dy), wrap(api, tokens), padding=0)
+    assert torch.equal(table[[v - 1, 5, 70000], :d], torch.stack([dy[0], dy[1] + dy[4], dy[5]]))
+    table[[v - 1, 5, 70000], :d] = 0
+    assert not table[:, :d].any() and (table[:, d:] == 9).all()
+
+
 def test_gradient_of_unknown_tokens(api):
     dy = normal((12, 40), F32, 1)
     tokens = torch.tensor([3, -1, 10, 9, 0, 1 << 40, -(1 << 40), (1 << 32) + 3, 5, 3, 1 << 31, 3], device="cuda")
