@@ -35,7 +35,7 @@ namespace {
 // names of pyapi and of the containers
 PyObject *s_submit, *s_Tensor, *s_ImageBatchVarShape, *s_lock, *s_followed, *s_tls, *s_stack, *s_check, *s_t, *s_handle, *s_wrote, *s_read,
     *s_kind, *s_acquire, *s_release, *s_torch, *s_C, *s_getDevice, *s_getStream, *s_value, *s_key, *s_meta, *s_nbytes, *s_np, *s_dtype, *s_made,
-    *s_sizeOf, *s_core, *s_voidp, *s_wrapped, *s_keep;
+    *s_sizeOf, *s_core, *s_voidp, *s_wrapped, *s_keep, *s_seen, *s_outputs, *s_put;
 
 // A new reference that goes with the scope.
 struct Ref
@@ -962,6 +962,46 @@ PyObject *Release(PyObject *, PyObject *handle)
     Py_RETURN_NONE;
 }
 
+// tensor_end(tensor): what the package's tensors do as they go (a method of theirs): the reference to the library's is given back.
+PyObject *TensorEnd(PyObject *, PyObject *obj)
+{
+    Ref       attributes(AttributesOf(obj));
+    PyObject *handle = attributes ? PyDict_GetItem(attributes.o, s_handle) : nullptr;
+    if (handle == nullptr || handle == Py_None)
+    {
+        Py_RETURN_NONE;
+    }
+    Ref   value(PyObject_GetAttr(handle, s_value));
+    void *p = value && PyLong_CheckExact(value.o) ? PyLong_AsVoidPtr(value.o) : nullptr;
+    PyErr_Clear();
+    if (p != nullptr && PyDict_SetItem(attributes.o, s_handle, Py_None) == 0)
+    {
+        Py_BEGIN_ALLOW_THREADS
+        (void)nvcvTensorDecRef(reinterpret_cast<NVCVTensorHandle>(p), nullptr);
+        Py_END_ALLOW_THREADS
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
+// end(tensor): what pyapi's tensors do as they go (a method of theirs): one that an operator made for its result and that nothing
+// outside has seen goes to pyapi._outputs, which is None where the interpreter is ending.
+PyObject *ResultEnd(PyObject *api, PyObject *obj)
+{
+    Ref       attributes(AttributesOf(obj));
+    PyObject *key = attributes ? PyDict_GetItem(attributes.o, s_key) : nullptr;
+    if (key == nullptr || key == Py_None)
+    {
+        Py_RETURN_NONE;
+    }
+    PyObject *seen = PyDict_GetItem(attributes.o, s_seen), *outputs = Name(api, s_outputs);
+    if ((seen != nullptr && PyObject_IsTrue(seen) != 0) || outputs == nullptr || outputs == Py_None)
+    {
+        Py_RETURN_NONE;
+    }
+    return PyObject_CallMethodOneArg(outputs, s_put, obj);
+}
+
 // ---- operators' results that are handed out again: see pyapi._Outputs, which is this type by another name. Its tables are
 // touched under the interpreter's lock alone, and no object is given up between a table and the numbers that go with it.
 struct Outputs
@@ -1240,9 +1280,19 @@ PyMethodDef kBound[] = {
     {"submit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Submit)), METH_FASTCALL, nullptr},
     {"default_stream_key", DefaultKey, METH_NOARGS, nullptr},
     {"wrap", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(WrapTorch)), METH_FASTCALL, nullptr},
+    {"end", ResultEnd, METH_O, nullptr},
 };
 
-// bind(pyapi's dictionary): (submit, default_stream_key, wrap) for it.
+PyMethodDef kTensorEnd = {"tensor_end", TensorEnd, METH_O, nullptr};
+
+// A function as a method of a class written in Python: it is given the object.
+PyObject *AsMethod(PyMethodDef *function, PyObject *self)
+{
+    Ref f(PyCFunction_New(function, self));
+    return f ? PyInstanceMethod_New(f.o) : nullptr;
+}
+
+// bind(pyapi's dictionary): (submit, default_stream_key, wrap, end) for it.
 PyObject *Bind(PyObject *, PyObject *names)
 {
     if (!PyDict_Check(names))
@@ -1251,7 +1301,8 @@ PyObject *Bind(PyObject *, PyObject *names)
         return nullptr;
     }
     Ref submit(PyCFunction_New(&kBound[0], names)), key(PyCFunction_New(&kBound[1], names)), wrap(PyCFunction_New(&kBound[2], names));
-    return submit && key && wrap ? PyTuple_Pack(3, submit.o, key.o, wrap.o) : nullptr;
+    Ref end(AsMethod(&kBound[3], names));
+    return submit && key && wrap && end ? PyTuple_Pack(4, submit.o, key.o, wrap.o, end.o) : nullptr;
 }
 
 PyMethodDef kMethods[] = {
@@ -1289,6 +1340,7 @@ PyMODINIT_FUNC PyInit__cvcuda_native(void)
         {&s_nbytes, "_nbytes"},   {&s_np, "np"},           {&s_dtype, "dtype"},
         {&s_made, "_new_result"}, {&s_sizeOf, "_bytes_of"}, {&s_core, "_CoreTensor"},
         {&s_voidp, "_c_void_p"},  {&s_wrapped, "_WRAPPED"}, {&s_keep, "_keep"},
+        {&s_seen, "_seen"},       {&s_outputs, "_outputs"}, {&s_put, "put"},
     };
     for (const auto &n : names)
     {
@@ -1298,7 +1350,9 @@ PyMODINIT_FUNC PyInit__cvcuda_native(void)
         }
     }
     Ref module(PyModule_Create(&kModule)), outputs(PyType_FromSpec(&kOutputsSpec));
-    if (!module || !outputs || PyModule_AddObjectRef(module.o, "Outputs", outputs.o) < 0)
+    Ref end(AsMethod(&kTensorEnd, nullptr));
+    if (!module || !outputs || !end || PyModule_AddObjectRef(module.o, "Outputs", outputs.o) < 0
+        || PyModule_AddObjectRef(module.o, "tensor_end", end.o) < 0)
     {
         return nullptr;
     }

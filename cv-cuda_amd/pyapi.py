@@ -375,9 +375,7 @@ class Tensor:
         view = _native.torch_view(raw.handle.value, form, torch._C._cuda_getDevice(), raw) if form is not None else None
         return raw.torch_view() if view is None else view
 
-    def __del__(self):
-        if self._key is not None and not self._seen and _outputs is not None:  # (None: the interpreter is ending)
-            _outputs.put(self)
+    # (__del__, below: a result that nothing outside this module has seen goes to _outputs)
 
 
 _CoreTensor = _Tensor
@@ -834,7 +832,7 @@ def _same_images(src, fmt=None, sizes=None):
 
 
 # what every operator below goes through: _submit, in native code for calls on the default stream that wait for nothing
-_run, _native_stream_key, _wrap_torch = _native.bind(globals())
+_run, _native_stream_key, _wrap_torch, Tensor.__del__ = _native.bind(globals())
 
 
 def _image_axes(layout):

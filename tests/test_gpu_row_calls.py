@@ -103,6 +103,32 @@ def test_wrapped_torch_tensors(api, cv, dtype):
         handle.close()
 
 
+def test_wrapped_tensors_go(api, cv):
+    import weakref
+    x = torch.zeros(4, 8, device="cuda")
+    kept, a, b = weakref.ref(x), api.as_tensor(x), api.as_tensor(x)
+    raw = a._t
+    del x, a
+    assert raw.refcount() == 1 and kept() is not None
+    raw.close()  # once; as it goes there is nothing left to give back
+    assert raw.handle is None
+    del raw
+    assert kept() is not None
+    del b
+    assert kept() is None
+
+
+def test_results_come_back(api):
+    made = api.layer_norm(api.as_tensor(torch.ones(4, 8, device="cuda")))
+    raw = made._t
+    del made
+    again = api.layer_norm(api.as_tensor(torch.ones(4, 8, device="cuda")))
+    assert again._t is raw
+    again.torch()  # seen: it does not come back
+    del again
+    assert api.layer_norm(api.as_tensor(torch.ones(4, 8, device="cuda")))._t is not raw
+
+
 def test_what_cannot_be_wrapped(api, cv):
     with pytest.raises(cv.Error) as e:
         api.as_tensor(torch.zeros(4, 8, device="cuda").t())  # its rows' elements do not follow one another
