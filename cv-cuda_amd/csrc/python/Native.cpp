@@ -34,7 +34,7 @@ namespace {
 
 // names of pyapi and of the containers
 PyObject *s_submit, *s_Tensor, *s_ImageBatchVarShape, *s_lock, *s_followed, *s_tls, *s_stack, *s_check, *s_t, *s_handle, *s_wrote, *s_read,
-    *s_kind, *s_acquire, *s_release, *s_torch, *s_C, *s_getDevice, *s_getStream, *s_value, *s_key, *s_meta, *s_nbytes, *s_np, *s_dtype, *s_made,
+    *s_kind, *s_acquire, *s_release, *s_torch, *s_C, *s_getDevice, *s_getStream, *s_key, *s_meta, *s_nbytes, *s_np, *s_dtype, *s_made,
     *s_sizeOf, *s_core, *s_voidp, *s_wrapped, *s_keep, *s_seen, *s_outputs, *s_put;
 
 // A new reference that goes with the scope.
@@ -111,22 +111,31 @@ enum Kind
     kBatch
 };
 
+// An attribute that an object itself has (borrowed), null without one. What the containers keep are such; looked up like this it is
+// a third of the time, and a call may have hundreds of them.
+PyObject *Own(PyObject *obj, PyObject *name)
+{
+    PyObject **dict = _PyObject_GetDictPtr(obj);
+    return dict != nullptr && *dict != nullptr ? PyDict_GetItem(*dict, name) : nullptr;
+}
+
 // The pointer that an object's `handle` (a ctypes.c_void_p) holds.
 bool Pointer(PyObject *obj, void *&p)
 {
-    Ref h(PyObject_GetAttr(obj, s_handle)), value(h ? PyObject_GetAttr(h.o, s_value) : nullptr);
-    if (!value || !PyLong_CheckExact(value.o))
+    PyObject *h = Own(obj, s_handle);
+    Py_buffer view;
+    if (h == nullptr || !PyObject_CheckBuffer(h) || PyObject_GetBuffer(h, &view, PyBUF_SIMPLE) < 0)
     {
         PyErr_Clear();
         return false;
     }
-    p = PyLong_AsVoidPtr(value.o);
-    if (PyErr_Occurred())
+    const bool ok = view.len == (Py_ssize_t)sizeof(p);
+    if (ok)
     {
-        PyErr_Clear();
-        return false;
+        std::memcpy(&p, view.buf, sizeof(p));
     }
-    return true;
+    PyBuffer_Release(&view);
+    return ok && p != nullptr;
 }
 
 // The library's handle of a tensor of pyapi (`type`: that class), or of None where that may be: nullptr.
@@ -141,13 +150,8 @@ bool TensorOf(PyObject *type, PyObject *obj, void *&handle, bool orNone = false)
     {
         return false;
     }
-    Ref inner(PyObject_GetAttr(obj, s_t));
-    if (!inner)
-    {
-        PyErr_Clear();
-        return false;
-    }
-    return Pointer(inner.o, handle) && handle != nullptr;
+    PyObject *inner = Own(obj, s_t);
+    return inner != nullptr && Pointer(inner, handle);
 }
 
 // The library's handle of a container of pyapi.
@@ -158,13 +162,8 @@ Kind HandleOf(PyObject *api, PyObject *obj, void *&handle)
     {
         return kNone;
     }
-    Ref inner(tensor ? PyObject_GetAttr(obj, s_t) : nullptr);
-    if (tensor && !inner)
-    {
-        PyErr_Clear();
-        return kNone;
-    }
-    return Pointer(tensor ? inner.o : obj, handle) && handle != nullptr ? (tensor ? kTensor : kBatch) : kNone;
+    PyObject *inner = tensor ? Own(obj, s_t) : obj;
+    return inner != nullptr && Pointer(inner, handle) ? (tensor ? kTensor : kBatch) : kNone;
 }
 
 bool Int(PyObject *o, int &v)
@@ -432,15 +431,15 @@ bool SameKey(PyObject *o, long key)
 }
 
 // Whether a mark (stream, event) is absent or of stream `key`.
-bool WroteBy(PyObject *attributes, long key)
+bool WroteBy(PyObject *obj, long key)
 {
-    PyObject *wrote = PyDict_GetItem(attributes, s_wrote);
+    PyObject *wrote = Own(obj, s_wrote);
     return wrote == nullptr || (PyTuple_CheckExact(wrote) && PyTuple_GET_SIZE(wrote) == 2 && SameKey(PyTuple_GET_ITEM(wrote, 0), key));
 }
 
-bool ReadBy(PyObject *attributes, long key)
+bool ReadBy(PyObject *obj, long key)
 {
-    PyObject *read = PyDict_GetItem(attributes, s_read);
+    PyObject *read = Own(obj, s_read);
     if (read == nullptr)
     {
         return true;
@@ -466,16 +465,14 @@ bool NothingToWaitFor(PyObject *reads, PyObject *writes, long key)
 {
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(reads); ++k)
     {
-        Ref attributes(AttributesOf(PyList_GET_ITEM(reads, k)));
-        if (!attributes || !WroteBy(attributes.o, key))
+        if (!WroteBy(PyList_GET_ITEM(reads, k), key))
         {
             return false;
         }
     }
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(writes); ++k)
     {
-        Ref attributes(AttributesOf(PyList_GET_ITEM(writes, k)));
-        if (!attributes || !WroteBy(attributes.o, key) || !ReadBy(attributes.o, key))
+        if (!WroteBy(PyList_GET_ITEM(writes, k), key) || !ReadBy(PyList_GET_ITEM(writes, k), key))
         {
             return false;
         }
@@ -488,8 +485,7 @@ bool Mark(PyObject *reads, PyObject *writes, PyObject *key)
 {
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(reads); ++k)
     {
-        Ref       attributes(AttributesOf(PyList_GET_ITEM(reads, k)));
-        PyObject *read = attributes ? PyDict_GetItem(attributes.o, s_read) : nullptr;
+        PyObject *read = Own(PyList_GET_ITEM(reads, k), s_read);
         if (read != nullptr)
         {
             if (PyDict_GetItem(read, key) != Py_None && PyDict_SetItem(read, key, Py_None) < 0)
@@ -507,8 +503,7 @@ bool Mark(PyObject *reads, PyObject *writes, PyObject *key)
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(writes); ++k)
     {
         PyObject *obj = PyList_GET_ITEM(writes, k);
-        Ref       attributes(AttributesOf(obj));
-        PyObject *was = attributes ? PyDict_GetItem(attributes.o, s_wrote) : nullptr, *read = attributes ? PyDict_GetItem(attributes.o, s_read) : nullptr;
+        PyObject *was = Own(obj, s_wrote), *read = Own(obj, s_read);
         // (marks that stand already stay; another thread may have set others meanwhile)
         const bool stands = was != nullptr && PyTuple_CheckExact(was) && PyTuple_GET_SIZE(was) == 2 && PyTuple_GET_ITEM(was, 1) == Py_None
                          && PyObject_RichCompareBool(PyTuple_GET_ITEM(was, 0), key, Py_EQ) == 1;
@@ -966,15 +961,8 @@ PyObject *Release(PyObject *, PyObject *handle)
 PyObject *TensorEnd(PyObject *, PyObject *obj)
 {
     Ref       attributes(AttributesOf(obj));
-    PyObject *handle = attributes ? PyDict_GetItem(attributes.o, s_handle) : nullptr;
-    if (handle == nullptr || handle == Py_None)
-    {
-        Py_RETURN_NONE;
-    }
-    Ref   value(PyObject_GetAttr(handle, s_value));
-    void *p = value && PyLong_CheckExact(value.o) ? PyLong_AsVoidPtr(value.o) : nullptr;
-    PyErr_Clear();
-    if (p != nullptr && PyDict_SetItem(attributes.o, s_handle, Py_None) == 0)
+    void     *p = nullptr;
+    if (attributes && Pointer(obj, p) && PyDict_SetItem(attributes.o, s_handle, Py_None) == 0)
     {
         Py_BEGIN_ALLOW_THREADS
         (void)nvcvTensorDecRef(reinterpret_cast<NVCVTensorHandle>(p), nullptr);
@@ -1207,7 +1195,7 @@ PyObject *OutputsPut(PyObject *self, PyObject *tensor)
         Py_RETURN_NONE;
     }
     const long by = -PyLong_AsLong(PyTuple_GET_ITEM(key, 3));
-    if (PyErr_Occurred() || !WroteBy(attributes.o, by) || !ReadBy(attributes.o, by))
+    if (PyErr_Occurred() || !WroteBy(tensor, by) || !ReadBy(tensor, by))
     {
         PyErr_Clear();
         Py_RETURN_NONE;
@@ -1336,7 +1324,7 @@ PyMODINIT_FUNC PyInit__cvcuda_native(void)
         {&s_kind, "_native"},     {&s_acquire, "acquire"}, {&s_release, "release"},
         {&s_torch, "torch"},      {&s_C, "_C"},            {&s_getDevice, "_cuda_getDevice"},
         {&s_getStream, "_cuda_getCurrentRawStream"},
-        {&s_value, "value"},      {&s_key, "_key"},        {&s_meta, "_meta"},
+        {&s_key, "_key"},        {&s_meta, "_meta"},
         {&s_nbytes, "_nbytes"},   {&s_np, "np"},           {&s_dtype, "dtype"},
         {&s_made, "_new_result"}, {&s_sizeOf, "_bytes_of"}, {&s_core, "_CoreTensor"},
         {&s_voidp, "_c_void_p"},  {&s_wrapped, "_WRAPPED"}, {&s_keep, "_keep"},
