@@ -279,11 +279,12 @@ HandlePool &TensorPool();
 HandlePool &ImagePool();
 HandlePool &ImageBatchPool();
 
+// T: what the pool's objects are (each pool holds those of one interface; a check of it was a third of a call that reads a
+// tensor, and operators over lists read hundreds).
 template<class T>
 T &Deref(HandlePool &pool, void *handle)
 {
-    CoreObject *o = pool.get(handle);
-    T          *t = dynamic_cast<T *>(o);
+    T *t = static_cast<T *>(pool.get(handle));
     if (t == nullptr)
     {
         throw Error(NVCV_ERROR_INVALID_ARGUMENT, "Handle does not refer to an object of the expected type");
