@@ -431,15 +431,13 @@ bool SameKey(PyObject *o, long key)
 }
 
 // Whether a mark (stream, event) is absent or of stream `key`.
-bool WroteBy(PyObject *obj, long key)
+bool WroteBy(PyObject *wrote, long key)
 {
-    PyObject *wrote = Own(obj, s_wrote);
     return wrote == nullptr || (PyTuple_CheckExact(wrote) && PyTuple_GET_SIZE(wrote) == 2 && SameKey(PyTuple_GET_ITEM(wrote, 0), key));
 }
 
-bool ReadBy(PyObject *obj, long key)
+bool ReadBy(PyObject *read, long key)
 {
-    PyObject *read = Own(obj, s_read);
     if (read == nullptr)
     {
         return true;
@@ -460,22 +458,34 @@ bool ReadBy(PyObject *obj, long key)
     return true;
 }
 
-// Whether no container of the call has a mark of another stream.
-bool NothingToWaitFor(PyObject *reads, PyObject *writes, long key)
+// Whether (key, None) is what a call on default stream `key` leaves as the mark of a write.
+bool Stands(PyObject *wrote, PyObject *key)
 {
+    return wrote != nullptr && PyTuple_CheckExact(wrote) && PyTuple_GET_SIZE(wrote) == 2 && PyTuple_GET_ITEM(wrote, 1) == Py_None
+        && PyObject_RichCompareBool(PyTuple_GET_ITEM(wrote, 0), key, Py_EQ) == 1;
+}
+
+// Whether no container of the call has a mark of another stream. `standing`: each has the marks already that the call would leave.
+bool NothingToWaitFor(PyObject *reads, PyObject *writes, PyObject *keyObject, long key, bool &standing)
+{
+    standing = true;
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(reads); ++k)
     {
-        if (!WroteBy(PyList_GET_ITEM(reads, k), key))
+        if (!WroteBy(Own(PyList_GET_ITEM(reads, k), s_wrote), key))
         {
             return false;
         }
+        PyObject *read = standing ? Own(PyList_GET_ITEM(reads, k), s_read) : nullptr;
+        standing       = read != nullptr && PyDict_CheckExact(read) && PyDict_GetItem(read, keyObject) == Py_None;
     }
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(writes); ++k)
     {
-        if (!WroteBy(PyList_GET_ITEM(writes, k), key) || !ReadBy(PyList_GET_ITEM(writes, k), key))
+        PyObject *wrote = Own(PyList_GET_ITEM(writes, k), s_wrote), *read = Own(PyList_GET_ITEM(writes, k), s_read);
+        if (!WroteBy(wrote, key) || !ReadBy(read, key))
         {
             return false;
         }
+        standing = standing && Stands(wrote, keyObject) && read != nullptr && PyDict_CheckExact(read) && PyDict_GET_SIZE(read) == 0;
     }
     return true;
 }
@@ -505,9 +515,7 @@ bool Mark(PyObject *reads, PyObject *writes, PyObject *key)
         PyObject *obj = PyList_GET_ITEM(writes, k);
         PyObject *was = Own(obj, s_wrote), *read = Own(obj, s_read);
         // (marks that stand already stay; another thread may have set others meanwhile)
-        const bool stands = was != nullptr && PyTuple_CheckExact(was) && PyTuple_GET_SIZE(was) == 2 && PyTuple_GET_ITEM(was, 1) == Py_None
-                         && PyObject_RichCompareBool(PyTuple_GET_ITEM(was, 0), key, Py_EQ) == 1;
-        if (!stands)
+        if (!Stands(was, key))
         {
             Ref wrote(PyTuple_Pack(2, key, Py_None));
             if (!wrote || PyObject_SetAttr(obj, s_wrote, wrote.o) < 0)
@@ -562,7 +570,8 @@ PyObject *Submit(PyObject *api, PyObject *const *a, Py_ssize_t n)
         return handOn();
     }
     PyObject  *calls = PyDict_GetItem(followed, keyObject.o);
-    const bool plain = (calls == nullptr || PyObject_IsTrue(calls) == 0) && NothingToWaitFor(a[1], a[2], key);
+    bool       standing;
+    const bool plain = (calls == nullptr || PyObject_IsTrue(calls) == 0) && NothingToWaitFor(a[1], a[2], keyObject.o, key, standing);
     Ref        released(PyObject_CallMethodNoArgs(lock, s_release));
     if (!plain)
     {
@@ -583,6 +592,10 @@ PyObject *Submit(PyObject *api, PyObject *const *a, Py_ssize_t n)
             PyErr_SetString(PyExc_RuntimeError, "the operator failed");
         }
         return nullptr;
+    }
+    if (standing) // (what another thread has made of them meanwhile, unordered with this call, may stay)
+    {
+        Py_RETURN_NONE;
     }
     Ref        held(PyObject_CallMethodNoArgs(lock, s_acquire));
     const bool ok = held && Mark(a[1], a[2], keyObject.o);
@@ -1195,7 +1208,7 @@ PyObject *OutputsPut(PyObject *self, PyObject *tensor)
         Py_RETURN_NONE;
     }
     const long by = -PyLong_AsLong(PyTuple_GET_ITEM(key, 3));
-    if (PyErr_Occurred() || !WroteBy(tensor, by) || !ReadBy(tensor, by))
+    if (PyErr_Occurred() || !WroteBy(Own(tensor, s_wrote), by) || !ReadBy(Own(tensor, s_read), by))
     {
         PyErr_Clear();
         Py_RETURN_NONE;

@@ -70,6 +70,25 @@ def test_native_calls_do_what_submit_does(api, monkeypatch):
     assert python.calls == 10
 
 
+def test_marks_that_stand_and_others(api):
+    x, out, other = (api.as_tensor(torch.randn(64, 512, device="cuda")) for _ in range(3))
+    for _ in range(3):  # the second time the first one's marks stand
+        api.layer_norm_into(out, x)
+        assert out._wrote == (0, None) and out._read == {} and x._read == {0: None}
+    api.layer_norm_into(other, out)
+    assert out._wrote == (0, None) and out._read == {0: None}
+    api.layer_norm_into(out, x)  # a read of what is written: the marks do not stand
+    assert out._wrote == (0, None) and out._read == {} and x._read == {0: None}
+    s = api.Stream()
+    api.layer_norm_into(out, other, stream=s)
+    assert out._wrote[0] == s.handle != 0 and set(other._read) == {s.handle}
+    api.layer_norm_into(other, out)  # waits for that
+    assert other._wrote[0] == 0 and other._read == {} and set(out._read) == {0}
+    torch.cuda.synchronize()
+    want = torch.nn.functional.layer_norm(x.torch(), (512,))
+    assert (out.torch() - torch.nn.functional.layer_norm(want, (512,))).abs().max() < 1e-4
+
+
 class _Python:
     def __init__(self, api):
         self.submit, self.calls = api._submit, 0
