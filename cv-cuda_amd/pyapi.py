@@ -1124,9 +1124,22 @@ def _given(*tensors):
     return [t for t in tensors if t is not None]
 
 
+def _capturing(stream):
+    """Whether what `stream` (None: the current one) is given is recorded for a graph. (A default stream's never is.)"""
+    if _default_stream_key(stream) is not None:
+        return False
+    with torch.cuda.stream(_torch_stream(stream)):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _workspace(workspace, size, stream):
-    """The caller's workspace, or one for this call alone (None where none is needed)."""
-    return workspace if workspace is not None or size == 0 else _result((size,), np.uint8, None, stream)
+    """The caller's workspace, or one for this call alone (None where none is needed). Not for a call that is captured: a graph
+    writes there in every replay, when others have the memory of what this call made."""
+    if workspace is not None or size == 0:
+        return workspace
+    if _capturing(stream):
+        raise Error(4, "a captured gradient needs workspace=, a tensor of %d bytes that lives as long as the graph" % size)  # INVALID_OPERATION
+    return _result((size,), np.uint8, None, stream)
 
 
 def _rows_of(tensor):
@@ -1152,7 +1165,8 @@ def layer_norm(src, gamma=None, beta=None, epsilon=1e-5, *, mean=None, rstd=None
 
 def layer_norm_grad_into(grad_src, grad_gamma, grad_beta, grad, src, gamma, mean, rstd, *, workspace=None, stream=None):
     """The gradients of layer_norm from `grad`, that of its result; `mean` and `rstd` as the forward call gave them.
-    `grad_gamma`, `grad_beta` and `gamma` may be None. `grad_src` may be `grad` or `src`."""
+    `grad_gamma`, `grad_beta` and `gamma` may be None. `grad_src` may be `grad` or `src`. `workspace`: a uint8 tensor of
+    LayerNormGrad.workspace(rows, columns) bytes, or None for one of this call's own, which a call that is captured cannot have."""
     sums = grad_gamma is not None or grad_beta is not None
     workspace = _workspace(workspace, _layer_norm_workspace(*_rows_of(src)) if sums else 0, stream)
     _run(stream, _given(grad, src, gamma, mean, rstd), _given(grad_src, grad_gamma, grad_beta, workspace), _op(LayerNormGrad), grad, src,
@@ -1160,11 +1174,12 @@ def layer_norm_grad_into(grad_src, grad_gamma, grad_beta, grad, src, gamma, mean
     return grad_src, grad_gamma, grad_beta
 
 
-def layer_norm_grad(grad, src, gamma, mean, rstd, *, stream=None):
+def layer_norm_grad(grad, src, gamma, mean, rstd, *, workspace=None, stream=None):
     """(gradient of src, of gamma, of beta); the latter have gamma's type, F32 without one."""
     kind = np.dtype(np.float32) if gamma is None else gamma.dtype
+    workspace = _workspace(workspace, _layer_norm_workspace(*_rows_of(src)), stream)  # (before anything is made)
     made = [_result((src.shape[-1],), kind, None, stream) for _ in range(2)]
-    return layer_norm_grad_into(_like(src, stream), made[0], made[1], grad, src, gamma, mean, rstd, stream=stream)
+    return layer_norm_grad_into(_like(src, stream), made[0], made[1], grad, src, gamma, mean, rstd, workspace=workspace, stream=stream)
 
 
 def embedding_into(dst, table, tokens, scale=1.0, *, stream=None):
@@ -1182,7 +1197,8 @@ def embedding(table, tokens, scale=1.0, *, dtype=None, stream=None):
 
 def embedding_grad_into(grad_table, grad, tokens, scale=1.0, *, padding=None, accumulate=False, workspace=None, stream=None):
     """The gradient of embedding's table from `grad`, that of its result, in `grad`'s type or F32: written whole, or with
-    `accumulate` added to what `grad_table` holds. Tokens equal to `padding` have no part in it."""
+    `accumulate` added to what `grad_table` holds. Tokens equal to `padding` have no part in it. `workspace`: a uint8 tensor of
+    EmbeddingGrad.workspace(tokens, rows of the table, columns) bytes, or None as for layer_norm_grad_into."""
     if padding is not None and padding < 0:
         raise ValueError("padding is a token, or None")
     rows, columns = _rows_of(grad)
@@ -1193,10 +1209,12 @@ def embedding_grad_into(grad_table, grad, tokens, scale=1.0, *, padding=None, ac
     return grad_table
 
 
-def embedding_grad(grad, tokens, rows, scale=1.0, *, padding=None, dtype=None, stream=None):
+def embedding_grad(grad, tokens, rows, scale=1.0, *, padding=None, dtype=None, workspace=None, stream=None):
     """The gradient of a table of `rows` rows, of `dtype` (none: grad's)."""
+    count, columns = _rows_of(grad)
+    workspace = _workspace(workspace, _embedding_workspace(count, int(rows), columns), stream)  # (before anything is made)
     dst = _result((int(rows), grad.shape[-1]), grad.dtype if dtype is None else _np_dtype(dtype), None, stream)
-    return embedding_grad_into(dst, grad, tokens, scale, padding=padding, stream=stream)
+    return embedding_grad_into(dst, grad, tokens, scale, padding=padding, workspace=workspace, stream=stream)
 
 
 def adamw_into(params, moments, variances, grads, step, lr=1e-3, betas=(0.9, 0.999), epsilon=1e-8, weight_decay=1e-2, *, copies=None,

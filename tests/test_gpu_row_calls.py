@@ -158,3 +158,37 @@ def test_what_cannot_be_wrapped(api, cv):
         api.as_tensor(torch.zeros(4, 8, device="cuda"), "NHWC")
     with pytest.raises(TypeError):
         api.as_tensor(torch.zeros(4, dtype=torch.bfloat16, device="cuda")).cuda()  # the array interface has no name for it
+
+
+def test_captured_gradients(api, cv):
+    """With a workspace of the caller's, which the calls take that make their results too; refused without one, and the capture goes on."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows, d, v = 4096, 96, 500
+    x, dy = (torch.randn((rows, d), generator=g, device="cuda") for _ in range(2))
+    mean, rstd, gamma = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda"), torch.ones(d, device="cuda")
+    tokens = torch.randint(0, v, (rows,), generator=g, device="cuda")
+    wrap = api.as_tensor
+    made = [torch.empty(s, device="cuda") for s in ((rows, d), (d,), (d,), (v, d), (v, d))]
+    sizes = api.LayerNormGrad.workspace(rows, d), api.EmbeddingGrad.workspace(rows, v, d)
+    rooms, others = ([wrap(torch.empty(n, dtype=torch.uint8, device="cuda")) for n in sizes] for _ in range(2))
+    dx, dg, db, table, few = map(wrap, made)
+    tx, tdy, tgamma, tmean, trstd, ttokens, tfew, ttfew = map(wrap, (x, dy, gamma, mean, rstd, tokens, dy[:64], tokens[:64]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: api.layer_norm_grad_into(dx, dg, db, tdy, tx, tgamma, tmean, trstd), lambda: api.layer_norm_grad(tdy, tx, tgamma, tmean, trstd),
+                     lambda: api.embedding_grad_into(table, tdy, ttokens), lambda: api.embedding_grad(tdy, ttokens, v)):
+            with pytest.raises(cv.Error) as e:
+                call()
+            assert e.value.status == 4
+        api.layer_norm_grad_into(dx, dg, db, tdy, tx, tgamma, tmean, trstd, workspace=rooms[0])
+        api.embedding_grad_into(table, tdy, ttokens, workspace=rooms[1])
+        api.embedding_grad_into(few, tfew, ttfew)  # needs none
+    for _ in range(4):
+        dy.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in made]
+        want = [*api.layer_norm_grad(tdy, tx, tgamma, tmean, trstd, workspace=others[0]), api.embedding_grad(tdy, ttokens, v, workspace=others[1]),
+                api.embedding_grad(tfew, ttfew, v)]
+        assert all(torch.equal(a, b.torch()) for a, b in zip(got, want))

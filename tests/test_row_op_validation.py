@@ -189,3 +189,40 @@ def test_lists_of_different_lengths(cv):
         api.adamw_unpack_into([t], [t], [t, t])
     with pytest.raises(ValueError):
         cv.AdamW()(0, [t._t], [], [t._t], [t._t], None, None, None, None, *HYPER)
+
+
+def test_a_captured_gradient_needs_a_workspace(cv, monkeypatch):
+    """Memory that only the call holds goes back to the allocator with it; a graph would write there in every replay."""
+    import contextlib
+
+    api = importlib.import_module("cvcuda_amd.pyapi")
+    calls, capturing = [], True
+    monkeypatch.setattr(api, "_default_stream_key", lambda stream: None)
+    monkeypatch.setattr(api, "_native_stream_key", lambda: None)
+    monkeypatch.setattr(api, "_torch_stream", lambda stream: stream)
+    monkeypatch.setattr(api.torch.cuda, "stream", lambda stream: contextlib.nullcontext())
+    monkeypatch.setattr(api.torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(api, "_run", lambda stream, reads, writes, op, *args: calls.append(writes))
+    monkeypatch.setattr(api, "_result", lambda shape, *args: api.Tensor(_wrap=fake(cv, shape, np.uint8)))
+    monkeypatch.setattr(api, "_like", lambda *args: api._result((1,)))
+    wrap = lambda *args, **kw: api.Tensor(_wrap=fake(cv, *args, **kw))
+    x, w, s, table, tokens = wrap([4096, 10]), wrap([10]), wrap([4096]), wrap([50, 10]), wrap([4096], np.int64)
+    norm, embedding = cv.LayerNormGrad.workspace(4096, 10), cv.EmbeddingGrad.workspace(4096, 50, 10)
+    assert norm > 0 and embedding > 0
+    forms = [(lambda **kw: api.layer_norm_grad_into(x, w, w, x, x, w, s, s, **kw), norm), (lambda **kw: api.layer_norm_grad(x, x, w, s, s, **kw), norm),
+             (lambda **kw: api.embedding_grad_into(table, x, tokens, **kw), embedding), (lambda **kw: api.embedding_grad(x, tokens, 50, **kw), embedding)]
+    for call, need in forms:
+        for stream in (None, "side"):
+            with pytest.raises(cv.Error) as e:
+                call(stream=stream)
+            assert e.value.status == 4 and "workspace=" in str(e.value) and str(need) in str(e.value) and not calls
+        room = wrap([need], np.uint8)
+        call(workspace=room)
+        assert calls.pop()[-1] is room
+    # what needs none is captured without one
+    api.layer_norm_grad_into(x, None, None, x, x, w, s, s)
+    api.embedding_grad_into(table, wrap([64, 10]), wrap([64], np.int64))
+    assert [len(writes) for writes in calls] == [1, 1]
+    capturing = False
+    forms[0][0]()
+    assert calls[-1][-1].shape == (norm,)
