@@ -800,10 +800,20 @@ bool Few(int64_t rows, int64_t columns)
 // has 16 elements or more, and fewer sums are left to add up: 65536 rows of 4096 BF16 293 us with 512 workgroups of four waves,
 // 317 with 768, 343 with 1024, 352 with 384; 4000 rows of 8192 56 with 256 of eight, 64 with 512. Lanes of 8 or 4 elements want as
 // many as fit, six: 60000 rows of 512 40 us with 1536, 52 with 512.
+constexpr int64_t kMostParts = 1536;
+
+// Rows that no workgroup holds have a launch of their own for the sums, of tiles of 1024 columns or more and parts: a million columns
+// in all parts together are 500 workgroups or more, and what they leave is 8 MiB, little beside the rows themselves. 6144 rows of 40000 BF16
+// 598 us, 585 with two million, 741 with half of one, 1153 with a part to four rows; 2000 rows of 20000 F32 201, 208, 204 and 238. Rows of
+// fewer than four columns have one tile, and so the most parts (100000 rows of 3 F32 270 us).
+constexpr int64_t kWideSums = 1 << 20;
+
 int PartsOf(int64_t rows, int64_t columns)
 {
     const RowShape s    = ShapeOf(columns, kGradWidest);
-    const int64_t  most = s.elements <= 8 ? 1536 : 2048 / std::max(s.waves, 4);
+    const int64_t  most = s.waves == 0      ? std::min(kMostParts, std::max<int64_t>(1, kWideSums / std::max<int64_t>(columns, 1)))
+                          : s.elements <= 8 ? kMostParts
+                                            : 2048 / std::max(s.waves, 4);
     return (int)std::min((rows + 3) / 4, most);
 }
 

@@ -191,6 +191,16 @@ def test_lists_of_different_lengths(cv):
         cv.AdamW()(0, [t._t], [], [t._t], [t._t], None, None, None, None, *HYPER)
 
 
+@pytest.mark.parametrize("columns", [16385, 20000, 40000, 70003, 1 << 20, 3000001, 1 << 30])
+def test_workspace_of_wide_rows(cv, columns):
+    """Rows that no workgroup holds ask for no more than the widest that one does, beyond the two sums of one part."""
+    most = max(cv.LayerNormGrad.workspace(6144, 16384), 2 * 4 * columns)
+    for rows in (1, 5, 1000, 6144, 100000, (1 << 31) - 1):
+        assert 2 * 4 * columns <= cv.LayerNormGrad.workspace(rows, columns) <= most
+    # little beside the input itself
+    assert cv.LayerNormGrad.workspace(6144, columns) <= 6144 * columns * 2 // 16
+
+
 def test_a_captured_gradient_needs_a_workspace(cv, monkeypatch):
     """Memory that only the call holds goes back to the allocator with it; a graph would write there in every replay."""
     import contextlib
