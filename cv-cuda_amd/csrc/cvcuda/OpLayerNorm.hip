@@ -817,9 +817,17 @@ int PartsOf(int64_t rows, int64_t columns)
     return (int)std::min((rows + 3) / 4, most);
 }
 
+// A gradient of one launch has no use for a workspace, and asks for the least: callers bring one, and learn that it is missing, at any
+// number of rows. What is touched is larger.
 int64_t GradWorkspace(int64_t rows, int64_t columns)
 {
-    return (int64_t)PartsOf(rows, columns) * 2 * columns * (int64_t)sizeof(float);
+    constexpr int64_t kUntouched = CVCUDAX_LAYER_NORM_UNTOUCHED_WORKSPACE;
+    if (Few(rows, columns))
+    {
+        return kUntouched;
+    }
+    const int64_t bytes = (int64_t)PartsOf(rows, columns) * 2 * columns * (int64_t)sizeof(float);
+    return bytes > 0 ? std::max(bytes, 2 * kUntouched) : 0;
 }
 
 template<class T, class W, int WAVES, int E>
@@ -1056,7 +1064,8 @@ public:
         void        *gradGamma = w.take(hgradGamma, "Gamma's gradient"), *gradBeta = w.take(hgradBeta, "Beta's gradient");
         const float *mean = TakeStatistics(hmean, "Mean", in.rows), *rstd = TakeStatistics(hrstd, "Rstd", in.rows);
         const bool   sums = gradGamma != nullptr || gradBeta != nullptr;
-        float       *partial = sums ? reinterpret_cast<float *>(RequireWorkspace(hworkspace, GradWorkspace(in.rows, in.columns))) : nullptr;
+        uint8_t     *room    = sums ? RequireWorkspace(hworkspace, GradWorkspace(in.rows, in.columns)) : nullptr;
+        float       *partial = Few(in.rows, in.columns) ? nullptr : reinterpret_cast<float *>(room);
         if (in.columns == 0)
         {
             return;

@@ -1132,11 +1132,24 @@ def _capturing(stream):
         return torch.cuda.is_current_stream_capturing()
 
 
+_UNTOUCHED_BYTES = 16  # CVCUDAX_LAYER_NORM_UNTOUCHED_WORKSPACE
+_untouched = {}        # device -> a workspace of that size, which no call reads or writes: it has no marks
+
+
+def _untouched_workspace():
+    device = torch._C._cuda_getDevice()
+    if device not in _untouched:
+        _untouched[device] = as_tensor(torch.empty(_UNTOUCHED_BYTES, dtype=torch.uint8, device="cuda"))
+    return _untouched[device]
+
+
 def _workspace(workspace, size, stream):
     """The caller's workspace, or one for this call alone (None where none is needed). Not for a call that is captured: a graph
     writes there in every replay, when others have the memory of what this call made."""
     if workspace is not None or size == 0:
         return workspace
+    if size <= _UNTOUCHED_BYTES:
+        return _untouched_workspace()
     if _capturing(stream):
         raise Error(4, "a captured gradient needs workspace=, a tensor of %d bytes that lives as long as the graph" % size)  # INVALID_OPERATION
     return _result((size,), np.uint8, None, stream)
@@ -1166,10 +1179,13 @@ def layer_norm(src, gamma=None, beta=None, epsilon=1e-5, *, mean=None, rstd=None
 def layer_norm_grad_into(grad_src, grad_gamma, grad_beta, grad, src, gamma, mean, rstd, *, workspace=None, stream=None):
     """The gradients of layer_norm from `grad`, that of its result; `mean` and `rstd` as the forward call gave them.
     `grad_gamma`, `grad_beta` and `gamma` may be None. `grad_src` may be `grad` or `src`. `workspace`: a uint8 tensor of
-    LayerNormGrad.workspace(rows, columns) bytes, or None for one of this call's own, which a call that is captured cannot have."""
+    LayerNormGrad.workspace(rows, columns) bytes, or None for one of this call's own, which a call that is captured cannot have
+    (unless it is one of few rows, which touches none)."""
     sums = grad_gamma is not None or grad_beta is not None
-    workspace = _workspace(workspace, _layer_norm_workspace(*_rows_of(src)) if sums else 0, stream)
-    _run(stream, _given(grad, src, gamma, mean, rstd), _given(grad_src, grad_gamma, grad_beta, workspace), _op(LayerNormGrad), grad, src,
+    need = _layer_norm_workspace(*_rows_of(src)) if sums else 0
+    workspace = _workspace(workspace, need, stream)
+    written = workspace if need > _UNTOUCHED_BYTES else None
+    _run(stream, _given(grad, src, gamma, mean, rstd), _given(grad_src, grad_gamma, grad_beta, written), _op(LayerNormGrad), grad, src,
          gamma, mean, rstd, grad_src, grad_gamma, grad_beta, workspace)
     return grad_src, grad_gamma, grad_beta
 

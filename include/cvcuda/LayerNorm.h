@@ -15,7 +15,9 @@
  * mean, rstd              : F32, one element per row, dense; outputs of the forward call (either may be NULL there), inputs
  *                           of the gradient.
  * workspace               : U8, dense, at least as many elements as cvcudaxLayerNormGradWorkspace gives, aligned to 16 bytes. It
- *                           belongs to the call until the stream has passed it; NULL where 0 bytes are needed.
+ *                           belongs to the call until the stream has passed it; NULL where 0 bytes are needed, or without gradGamma and
+ *                           gradBeta. Of CVCUDAX_LAYER_NORM_UNTOUCHED_WORKSPACE bytes (gradients of few rows, made in one launch) it has to be
+ *                           given, but is not touched: calls on any streams may share one.
  * Rows: below 2^31, row elements: 2^30 at most. Tensors may be larger than 2^32 bytes. Tensors without elements are allowed: sums
  * over no rows are 0.
  * Status: INVALID_ARGUMENT for any type / shape / stride problem. */
@@ -32,6 +34,8 @@
 extern "C"
 {
 #endif
+
+#define CVCUDAX_LAYER_NORM_UNTOUCHED_WORKSPACE 16
 
 CVCUDA_PUBLIC NVCVStatus cvcudaxLayerNormCreate(NVCVOperatorHandle *handle);
 

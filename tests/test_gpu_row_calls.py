@@ -192,3 +192,37 @@ def test_captured_gradients(api, cv):
         want = [*api.layer_norm_grad(tdy, tx, tgamma, tmean, trstd, workspace=others[0]), api.embedding_grad(tdy, ttokens, v, workspace=others[1]),
                 api.embedding_grad(tfew, ttfew, v)]
         assert all(torch.equal(a, b.torch()) for a, b in zip(got, want))
+
+
+def test_gradients_of_few_rows_make_no_workspace(api, monkeypatch):
+    """On any stream, and captured: the least workspace, which is not touched, is one tensor for all calls and carries no marks."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows, d = 256, 768
+    x, dy = (torch.randn((rows, d), generator=g, device="cuda") for _ in range(2))
+    mean, rstd, gamma = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda"), torch.ones(d, device="cuda")
+    made = [torch.empty(s, device="cuda") for s in ((rows, d), (d,), (d,))]
+    wrap = lambda: [api.as_tensor(t) for t in (*made, dy, x, gamma, mean, rstd)]
+
+    def none(*args):
+        raise AssertionError("a result of %s" % (args,))
+
+    monkeypatch.setattr(api, "_result", none)
+    results = []
+    api.layer_norm_grad_into(*wrap())
+    room = api._untouched_workspace()
+    results.append([t.clone() for t in made])
+    torch.cuda.synchronize()
+    api.layer_norm_grad_into(*wrap(), stream=api.Stream())
+    torch.cuda.synchronize()
+    results.append([t.clone() for t in made])
+    graph, captured = torch.cuda.CUDAGraph(), wrap()
+    with torch.cuda.graph(graph):
+        api.layer_norm_grad_into(*captured)
+    for _ in range(3):
+        for t in made:
+            t.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        results.append([t.clone() for t in made])
+    assert all(torch.equal(a, b) for got in results for a, b in zip(got, results[0]))
+    assert api._untouched_workspace() is room and not hasattr(room, "_wrote") and not hasattr(room, "_read")

@@ -201,6 +201,17 @@ def test_workspace_of_wide_rows(cv, columns):
     assert cv.LayerNormGrad.workspace(6144, columns) <= 6144 * columns * 2 // 16
 
 
+def test_workspace_of_few_rows(cv):
+    """A gradient of one launch makes its sums from the rows: it asks for the least, and nothing that is touched is as small."""
+    for columns in (4, 64, 1000, 8192, 16384):
+        for rows in (1, 6, 300, 1024):
+            assert cv.LayerNormGrad.workspace(rows, columns) == 16
+        assert cv.LayerNormGrad.workspace(1025, columns) >= 2 * 4 * columns
+    for rows, columns in ((1, 1), (4, 2), (3, 3), (1, 16385), (1025, 4)):
+        assert cv.LayerNormGrad.workspace(rows, columns) > 16
+    assert cv.LayerNormGrad.workspace(0, 100) == cv.LayerNormGrad.workspace(100, 0) == 0
+
+
 def test_a_captured_gradient_needs_a_workspace(cv, monkeypatch):
     """Memory that only the call holds goes back to the allocator with it; a graph would write there in every replay."""
     import contextlib
