@@ -23,6 +23,7 @@
 #include <cvcuda/OpWarpPerspective.h>
 #include <nvcv/Tensor.h>
 #include <structmember.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
@@ -1096,6 +1097,13 @@ PyObject *OutputsClear(PyObject *self, PyObject *)
     return all ? PyBool_FromLong(held) : nullptr;
 }
 
+// Whether it stands for itself as an element type: a numpy dtype, or torch's bfloat16, which numpy has not.
+bool IsElementType(PyObject *o, PyObject *numpyDtype)
+{
+    return PyObject_TypeCheck(o, reinterpret_cast<PyTypeObject *>(numpyDtype))
+        || (THPDtype_Check(o) && reinterpret_cast<THPDtype *>(o)->scalar_type == at::kBFloat16);
+}
+
 // get(shape, dtype, layout): a tensor for a result.
 PyObject *OutputsGet(PyObject *self, PyObject *const *a, Py_ssize_t n)
 {
@@ -1117,7 +1125,7 @@ PyObject *OutputsGet(PyObject *self, PyObject *const *a, Py_ssize_t n)
         return nullptr;
     }
     Ref dtype(nullptr);
-    if (PyObject_TypeCheck(a[1], reinterpret_cast<PyTypeObject *>(dtypes.o)))
+    if (IsElementType(a[1], dtypes.o))
     {
         Py_INCREF(a[1]);
         dtype.o = a[1];

@@ -433,8 +433,6 @@ def clear_cache():
 def _result(shape, dtype, layout, stream):
     """A tensor for an operator's result. Only a call on the default stream takes one that is handed out again: another
     stream would have to wait for the default stream's last use of it, which one that is being captured cannot."""
-    if dtype is torch.bfloat16:
-        return Tensor(tuple(shape), dtype, layout)
     key = _native_stream_key() if stream is None else None
     if key is None and _default_stream_key(stream) is None:
         return Tensor(tuple(shape), dtype, layout)

@@ -226,3 +226,19 @@ def test_gradients_of_few_rows_make_no_workspace(api, monkeypatch):
         results.append([t.clone() for t in made])
     assert all(torch.equal(a, b) for got in results for a, b in zip(got, results[0]))
     assert api._untouched_workspace() is room and not hasattr(room, "_wrote") and not hasattr(room, "_read")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_results_of_every_type_come_back(api, monkeypatch, dtype):
+    made, new = [], api._new_result
+    monkeypatch.setattr(api, "_new_result", lambda *args: made.append(args) or new(*args))
+    x, stats, gamma = (api.as_tensor(torch.ones(s, dtype=t, device="cuda")) for s, t in (((40, 24), dtype), (40, torch.float32), (24, dtype)))
+    tokens = api.as_tensor(torch.arange(40, device="cuda") % 7)
+    for _ in range(50):
+        api.layer_norm(api.layer_norm(x))
+        api.embedding(x, tokens)
+        api.layer_norm_grad(x, x, gamma, stats, stats)
+        api.embedding_grad(x, tokens, 9)
+    # (40, 24) twice at a time, two of (24,), one of (9, 24)
+    assert sorted(tuple(m[0]) for m in made) == [(9, 24), (24,), (24,), (40, 24), (40, 24)]
+    torch.cuda.synchronize()

@@ -247,3 +247,28 @@ def test_a_captured_gradient_needs_a_workspace(cv, monkeypatch):
     capturing = False
     forms[0][0]()
     assert calls[-1][-1].shape == (norm,)
+
+
+def test_results_of_bfloat16_are_handed_out_again(cv, monkeypatch):
+    """As those of every other type (no GPU: the library's tensors are stand-ins)."""
+    api, made = importlib.import_module("cvcuda_amd.pyapi"), []
+
+    def new(shape, dtype, layout):
+        made.append((shape, dtype))
+        return fake(cv, list(shape), dtype)
+
+    monkeypatch.setattr(api, "_new_result", new)
+    monkeypatch.setattr(api.torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(api, "_native_stream_key", lambda: 0)
+    monkeypatch.setattr(api, "_outputs", api._Outputs())
+    for dtype in (BF16, np.dtype(F16), np.dtype(np.int16)):
+        result = api._result((4, 8), dtype, None, None)
+        raw = result._t
+        assert result.dtype == dtype and result.shape == (4, 8)
+        result._wrote = (0, None)
+        del result
+        again, other = api._result((4, 8), dtype, None, None), api._result((4, 8), dtype, None, None)
+        assert again._t is raw and other._t is not raw
+    assert made == [((4, 8), t) for t in (BF16, F16, np.int16) for _ in range(2)]
+    with pytest.raises(TypeError):
+        api._outputs.get((4, 8), torch.float32, None)  # (numpy's types stand for the others)
