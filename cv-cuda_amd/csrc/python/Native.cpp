@@ -491,9 +491,20 @@ bool NothingToWaitFor(PyObject *reads, PyObject *writes, PyObject *keyObject, lo
     return true;
 }
 
+// How often marks were set, by calls here and in pyapi. (touched under the interpreter's lock)
+unsigned long s_markings;
+
+// marking(): a call is about to set its marks (pyapi._submit, under the marks' lock).
+PyObject *Marking(PyObject *, PyObject *)
+{
+    ++s_markings;
+    Py_RETURN_NONE;
+}
+
 // The marks of a call on default stream `key`: as pyapi._submit leaves them, without an event.
 bool Mark(PyObject *reads, PyObject *writes, PyObject *key)
 {
+    ++s_markings;
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(reads); ++k)
     {
         PyObject *read = Own(PyList_GET_ITEM(reads, k), s_read);
@@ -570,10 +581,11 @@ PyObject *Submit(PyObject *api, PyObject *const *a, Py_ssize_t n)
         PyErr_Clear();
         return handOn();
     }
-    PyObject  *calls = PyDict_GetItem(followed, keyObject.o);
-    bool       standing;
-    const bool plain = (calls == nullptr || PyObject_IsTrue(calls) == 0) && NothingToWaitFor(a[1], a[2], keyObject.o, key, standing);
-    Ref        released(PyObject_CallMethodNoArgs(lock, s_release));
+    PyObject           *calls    = PyDict_GetItem(followed, keyObject.o);
+    bool                standing = false;
+    const unsigned long markings = s_markings;
+    const bool          plain = (calls == nullptr || PyObject_IsTrue(calls) == 0) && NothingToWaitFor(a[1], a[2], keyObject.o, key, standing);
+    Ref released(PyObject_CallMethodNoArgs(lock, s_release));
     if (!plain)
     {
         PyErr_Clear();
@@ -594,7 +606,7 @@ PyObject *Submit(PyObject *api, PyObject *const *a, Py_ssize_t n)
         }
         return nullptr;
     }
-    if (standing) // (what another thread has made of them meanwhile, unordered with this call, may stay)
+    if (standing && markings == s_markings) // (another thread's marks, set meanwhile, would not wait for this call)
     {
         Py_RETURN_NONE;
     }
@@ -1316,6 +1328,7 @@ PyObject *Bind(PyObject *, PyObject *names)
 
 PyMethodDef kMethods[] = {
     {"bind", Bind, METH_O, nullptr},
+    {"marking", Marking, METH_NOARGS, nullptr},
     {"planes", Planes, METH_O, nullptr},
     {"tensor_alloc", TensorAlloc, METH_VARARGS, nullptr},
     {"torch_view", TorchView, METH_VARARGS, nullptr},

@@ -786,6 +786,7 @@ def _submit(stream, reads, writes, op, *args):
         mark = _new_event()
         mark.record(s)
     with _events_lock:
+        _marking()
         for obj in reads:
             if "_read" in obj.__dict__:
                 obj._read[key] = mark
@@ -795,6 +796,7 @@ def _submit(stream, reads, writes, op, *args):
             obj._wrote, obj._read = (key, mark), {}
 
 
+_marking = _native.marking  # (a native call that would leave the marks it found looks whether others were set meanwhile)
 _events_lock = threading.Lock()
 _FOLLOWED_CALLS = 256
 _followed = {}  # calls to come, per default stream, that record their events at once

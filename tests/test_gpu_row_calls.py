@@ -242,3 +242,46 @@ def test_results_of_every_type_come_back(api, monkeypatch, dtype):
     # (40, 24) twice at a time, two of (24,), one of (9, 24)
     assert sorted(tuple(m[0]) for m in made) == [(9, 24), (24,), (24,), (40, 24), (40, 24)]
     torch.cuda.synchronize()
+
+
+class _Between:
+    """The marks' lock; once, when it is given back the first time, another call runs: where another thread's may, after a call
+    has looked at the marks it found and before it is submitted."""
+
+    def __init__(self, lock, call):
+        self.lock, self.call = lock, call
+
+    def acquire(self, blocking=True):
+        return self.lock.acquire(blocking)
+
+    def release(self):
+        self.lock.release()
+        if self.call is not None:
+            call, self.call = self.call, None
+            call()
+
+    def __enter__(self):
+        self.acquire()
+
+    def __exit__(self, *exc):
+        self.release()
+
+
+def test_marks_that_another_call_sets_meanwhile(api, monkeypatch):
+    """A call whose marks stood when it looked leaves its own behind another's that came between: what follows on that one's stream
+    waits for it. (The other call's operator does nothing, so that nothing is written twice at a time.)"""
+    x, out = (api.as_tensor(torch.randn(64, 512, device="cuda")) for _ in range(2))
+    s = api.Stream()
+    for reads, writes in (([], [out]), ([], [x])):
+        for _ in range(2):
+            api.layer_norm_into(out, x)
+        monkeypatch.setattr(api, "_followed", {})
+        lock = _Between(api._events_lock, lambda: api._submit(s, reads, writes, lambda *args: None))
+        monkeypatch.setattr(api, "_events_lock", lock)
+        api.layer_norm_into(out, x)
+        monkeypatch.undo()
+        assert lock.call is None
+        assert out._wrote == (0, None) and out._read == {} and x._read[0] is None
+        monkeypatch.setattr(api, "_followed", {})
+        torch.cuda.synchronize()
+        x, out = api.as_tensor(x.torch()), api.as_tensor(out.torch())
