@@ -21,6 +21,7 @@ import time
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 PATCH, CROP, PADDING = 16, 224, 0
 
@@ -48,6 +49,7 @@ class LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable  # (the gradients have none of their own)
     def backward(ctx, grad):
         x, gamma, mean, rstd = ctx.saved_tensors
         grad = grad.contiguous()
@@ -66,6 +68,7 @@ class Embedding(torch.autograd.Function):
         return rows
 
     @staticmethod
+    @once_differentiable  # (the gradients have none of their own)
     def backward(ctx, grad):
         tokens, = ctx.saved_tensors
         grad = grad.contiguous()

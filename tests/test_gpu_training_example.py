@@ -71,3 +71,13 @@ def test_the_copies_follow_the_weights(example):
     optimizer.step(lr=1e-2)
     for w, c, b in zip(front.weights, front.copies, before):
         assert torch.equal(c.detach(), w.bfloat16()) and not torch.equal(w, b) and c.grad is None
+
+
+def test_second_derivatives_are_refused(example):
+    """The gradients are differentiated no further: a derivative of theirs is refused, not taken without their part in it."""
+    x, gamma, beta = (torch.randn(s, device="cuda", requires_grad=True) for s in ((5, 64), 64, 64))
+    table, tokens = torch.randn(9, 64, device="cuda", requires_grad=True), torch.tensor([3, 1, 3], device="cuda")
+    for out, of in ((example.LayerNorm.apply(x, gamma, beta), x), (example.Embedding.apply(table, tokens, 2.0), table)):
+        grad, = torch.autograd.grad((out * out).sum(), of, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (grad * grad).sum().backward()
