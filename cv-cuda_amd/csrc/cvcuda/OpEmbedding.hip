@@ -986,11 +986,6 @@ struct GradRoom
     }
 };
 
-int64_t GradWorkspace(int64_t tokens, int64_t, int64_t columns)
-{
-    return GradRoom(tokens, columns).bytes;
-}
-
 template<class T, class O>
 void LaunchLookup(LookupArgs &a, hipStream_t stream)
 {
@@ -1327,7 +1322,7 @@ CVCUDA_PUBLIC NVCVStatus cvcudaxEmbeddingGradWorkspace(int64_t tokens, int64_t v
                 throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Tokens, rows of the table and row elements must be in [0, %d], not %ld, %ld and %ld",
                               INT32_MAX, (long)tokens, (long)vocabulary, (long)columns);
             }
-            *bytes = GradWorkspace(tokens, vocabulary, columns);
+            *bytes = GradRoom(tokens, columns).bytes; // (whatever the vocabulary)
         });
 }
 

@@ -10,9 +10,8 @@
 
 namespace cvamd {
 
-using Half  = _Float16;
-using Bf16  = __bf16;
-using Bytes = const uint8_t *;
+using Half = _Float16;
+using Bf16 = __bf16;
 
 enum RowElem
 {
