@@ -788,7 +788,10 @@ RowShape ShapeOf(int64_t columns, int widest)
     return {waves, columns <= 64 * 4 ? 4 : columns <= waves * 64 * 8 ? 8 : columns <= waves * 64 * 16 ? 16 : 32};
 }
 
-// Rows whose gradient is one launch: the sums over 2048 of 768 would take 18 us, with a second launch 10.
+// Rows whose gradient is one launch: the sums over 2048 of 768 would take 18 us, with a second launch 10. At any width that a workgroup
+// holds: whole calls of 1024 rows of 8192 BF16 are 19 us, 21 with a second launch, of 16384 32 and 40, and the fewer rows the more (512 of
+// 16384 19 and 30, up to 4096 columns 15.5 and 17). Only the widest F32 rows, read a second time, are even: 1024 of 8192 27 and 26, of 12288 44
+// and 44, of 16384 60 and 58; 512 of 16384 30 and 33.
 constexpr int kFewRows = 1024;
 
 bool Few(int64_t rows, int64_t columns)
