@@ -23,6 +23,7 @@
 #include <cvcuda/OpWarpPerspective.h>
 #include <nvcv/Tensor.h>
 #include <structmember.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -639,6 +640,23 @@ PyObject *DefaultKey(PyObject *api, PyObject *)
         return nullptr;
     }
     Py_RETURN_NONE;
+}
+
+// capturing(handle): whether work given to this stream, which is no default stream, is recorded for a graph.
+PyObject *Capturing(PyObject *, PyObject *handle)
+{
+    void *stream = PyLong_AsVoidPtr(handle);
+    if (PyErr_Occurred())
+    {
+        return nullptr;
+    }
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status) != hipSuccess)
+    {
+        (void)hipGetLastError();
+        Py_RETURN_FALSE;
+    }
+    return PyBool_FromLong(status != hipStreamCaptureStatusNone);
 }
 
 // planes(buffers): (channels, packed NVCVImagePlaneStrided array) of torch tensors on the GPU of one element type and channel
@@ -1329,6 +1347,7 @@ PyObject *Bind(PyObject *, PyObject *names)
 PyMethodDef kMethods[] = {
     {"bind", Bind, METH_O, nullptr},
     {"marking", Marking, METH_NOARGS, nullptr},
+    {"capturing", Capturing, METH_O, nullptr},
     {"planes", Planes, METH_O, nullptr},
     {"tensor_alloc", TensorAlloc, METH_VARARGS, nullptr},
     {"torch_view", TorchView, METH_VARARGS, nullptr},

@@ -1126,10 +1126,13 @@ def _given(*tensors):
 
 def _capturing(stream):
     """Whether what `stream` (None: the current one) is given is recorded for a graph. (A default stream's never is.)"""
-    if _default_stream_key(stream) is not None:
-        return False
-    with torch.cuda.stream(_torch_stream(stream)):
-        return torch.cuda.is_current_stream_capturing()
+    stack = getattr(Stream._tls, "stack", None)
+    if stream is None and not stack:
+        handle = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    else:
+        stream = stack[-1] if stream is None else stream
+        handle = getattr(stream, "_s", stream).cuda_stream
+    return handle != 0 and _native.capturing(handle)
 
 
 _UNTOUCHED_BYTES = 16  # CVCUDAX_LAYER_NORM_UNTOUCHED_WORKSPACE

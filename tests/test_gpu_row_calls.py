@@ -285,3 +285,19 @@ def test_marks_that_another_call_sets_meanwhile(api, monkeypatch):
         monkeypatch.setattr(api, "_followed", {})
         torch.cuda.synchronize()
         x, out = api.as_tensor(x.torch()), api.as_tensor(out.torch())
+
+
+def test_what_is_captured(api):
+    """Streams that are captured, however they are given, and others beside them."""
+    side, other = api.Stream(), torch.cuda.Stream()
+    assert not any(api._capturing(s) for s in (None, side, other, api.Stream.default, api.as_stream(other.cuda_stream)))
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(8, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=other):
+        x.add_(1)
+        got = [api._capturing(s) for s in (None, other, api.as_stream(other), api.as_stream(other.cuda_stream), side)]
+        with side:
+            got.append(api._capturing(None))
+        with api.as_stream(other):
+            got.append(api._capturing(None))
+    assert got == [True, True, True, True, False, False, True] and not api._capturing(other)

@@ -214,15 +214,11 @@ def test_workspace_of_few_rows(cv):
 
 def test_a_captured_gradient_needs_a_workspace(cv, monkeypatch):
     """Memory that only the call holds goes back to the allocator with it; a graph would write there in every replay."""
-    import contextlib
-
     api = importlib.import_module("cvcuda_amd.pyapi")
     calls, capturing = [], True
     monkeypatch.setattr(api, "_default_stream_key", lambda stream: None)
     monkeypatch.setattr(api, "_native_stream_key", lambda: None)
-    monkeypatch.setattr(api, "_torch_stream", lambda stream: stream)
-    monkeypatch.setattr(api.torch.cuda, "stream", lambda stream: contextlib.nullcontext())
-    monkeypatch.setattr(api.torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(api, "_capturing", lambda stream: capturing)
     monkeypatch.setattr(api, "_run", lambda stream, reads, writes, op, *args: calls.append(writes))
     monkeypatch.setattr(api, "_result", lambda shape, *args: api.Tensor(_wrap=fake(cv, shape, np.uint8)))
     monkeypatch.setattr(api, "_like", lambda *args: api._result((1,)))
