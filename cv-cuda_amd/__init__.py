@@ -664,3 +664,70 @@ class AdamWUnpack(_Operator):
         n = len(codes)
         check(_cv.cvcudaxAdamWUnpackSubmit(self.handle, stream_ptr(stream), n, _handles(codes, n), _handles(scales, n),
                                            _handles(out, n)))
+
+
+class Rotary(_Operator):
+    """Extension: cvcuda/Rotary.h."""
+    _create = "cvcudaxRotaryCreate"
+    _native = 16
+
+    def __call__(self, stream, inp, positions, out, dims, base=10000.0, factor=1.0, original=0.0, low=0.0, high=0.0, magnitude=1.0,
+                 interleaved=False, inverse=False):
+        args = capi.RotaryArgs(base, factor, original, low, high, magnitude, dims, interleaved, inverse)
+        check(_cv.cvcudaxRotarySubmit(self.handle, stream_ptr(stream), _h(inp), _h(positions), _h(out), C.byref(args)))
+
+
+class Attention(_Operator):
+    """Extension: cvcuda/Attention.h. None stands for a tensor that is left out."""
+    _create = "cvcudaxAttentionCreate"
+    _native = 17
+
+    @staticmethod
+    def workspace(rows, keys, sequences, heads, key_heads, dims):
+        """Bytes of workspace of a call."""
+        n = C.c_int64()
+        check(_cv.cvcudaxAttentionWorkspace(rows, keys, sequences, heads, key_heads, dims, C.byref(n)))
+        return n.value
+
+    def __call__(self, stream, q, k, v, offsets, key_offsets, key_lengths, out, lse, workspace, scale, causal=True):
+        check(_cv.cvcudaxAttentionSubmit(self.handle, stream_ptr(stream), _h(q), _h(k), _h(v), _h(offsets), _h(key_offsets),
+                                         _h(key_lengths), _h(out), _h(lse), _h(workspace), scale, causal))
+
+
+class AttentionGrad(_Operator):
+    """Extension: cvcuda/Attention.h, the gradient."""
+    _create = "cvcudaxAttentionCreate"
+    _native = 18
+
+    @staticmethod
+    def workspace(rows, keys, sequences, heads, key_heads, dims):
+        """Bytes of workspace of a call."""
+        n = C.c_int64()
+        check(_cv.cvcudaxAttentionGradWorkspace(rows, keys, sequences, heads, key_heads, dims, C.byref(n)))
+        return n.value
+
+    def __call__(self, stream, grad, q, k, v, out, lse, offsets, key_offsets, key_lengths, grad_q, grad_k, grad_v, workspace, scale,
+                 causal=True):
+        check(_cv.cvcudaxAttentionGradSubmit(self.handle, stream_ptr(stream), _h(grad), _h(q), _h(k), _h(v), _h(out), _h(lse),
+                                             _h(offsets), _h(key_offsets), _h(key_lengths), _h(grad_q), _h(grad_k), _h(grad_v),
+                                             _h(workspace), scale, causal))
+
+
+class LogProbs(_Operator):
+    """Extension: cvcuda/LogProbs.h. None stands for a tensor that is left out."""
+    _create = "cvcudaxLogProbsCreate"
+    _native = 19
+
+    def __call__(self, stream, logits, tokens, out, entropy=None, lse=None, top_values=None, top_tokens=None, scale=1.0):
+        check(_cv.cvcudaxLogProbsSubmit(self.handle, stream_ptr(stream), _h(logits), _h(tokens), _h(out), _h(entropy), _h(lse),
+                                        _h(top_values), _h(top_tokens), scale))
+
+
+class LogProbsGrad(_Operator):
+    """Extension: cvcuda/LogProbs.h, the gradient."""
+    _create = "cvcudaxLogProbsCreate"
+    _native = 20
+
+    def __call__(self, stream, logits, tokens, lse, entropy, grad, grad_entropy, out, scale=1.0):
+        check(_cv.cvcudaxLogProbsGradSubmit(self.handle, stream_ptr(stream), _h(logits), _h(tokens), _h(lse), _h(entropy), _h(grad),
+                                            _h(grad_entropy), _h(out), scale))

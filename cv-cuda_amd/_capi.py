@@ -376,3 +376,21 @@ _sig(cvcuda, "cvcudaxEmbeddingGradSubmit", ST, H, C.c_void_p, H, H, H, H, C.c_fl
 _sig(cvcuda, "cvcudaxAdamWCreate", ST, P(H))
 _sig(cvcuda, "cvcudaxAdamWSubmit", ST, H, C.c_void_p, C.c_int32, P(H), P(H), P(H), P(H), P(H), P(H), P(H), H, P(AdamWArgs))
 _sig(cvcuda, "cvcudaxAdamWUnpackSubmit", ST, H, C.c_void_p, C.c_int32, P(H), P(H), P(H))
+
+
+class RotaryArgs(C.Structure):
+    """CVCUDAXRotary (cvcuda/Rotary.h, extension)."""
+    _fields_ = [("base", C.c_double), ("factor", C.c_double), ("original", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("magnitude", C.c_double), ("dims", C.c_int32), ("interleaved", C.c_int8), ("inverse", C.c_int8)]
+
+
+_sig(cvcuda, "cvcudaxRotaryCreate", ST, P(H))
+_sig(cvcuda, "cvcudaxRotarySubmit", ST, H, C.c_void_p, H, H, H, P(RotaryArgs))
+_sig(cvcuda, "cvcudaxAttentionCreate", ST, P(H))
+_sig(cvcuda, "cvcudaxAttentionWorkspace", ST, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, P(C.c_int64))
+_sig(cvcuda, "cvcudaxAttentionSubmit", ST, H, C.c_void_p, H, H, H, H, H, H, H, H, H, C.c_float, C.c_int8)
+_sig(cvcuda, "cvcudaxAttentionGradWorkspace", ST, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, P(C.c_int64))
+_sig(cvcuda, "cvcudaxAttentionGradSubmit", ST, H, C.c_void_p, H, H, H, H, H, H, H, H, H, H, H, H, H, C.c_float, C.c_int8)
+_sig(cvcuda, "cvcudaxLogProbsCreate", ST, P(H))
+_sig(cvcuda, "cvcudaxLogProbsSubmit", ST, H, C.c_void_p, H, H, H, H, H, H, H, C.c_float)
+_sig(cvcuda, "cvcudaxLogProbsGradSubmit", ST, H, C.c_void_p, H, H, H, H, H, H, H, C.c_float)

@@ -47,8 +47,16 @@ COMMON = [
 DEVICE = [
     "--offload-arch=" + ARCH, "-ffp-contract=off", "-fno-fast-math",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    "-Xclang", "-target-feature", "-Xclang", "-ashr-pk-insts",
 ]
+NO_SHIFTED_BYTES = ["-Xclang", "-target-feature", "-Xclang", "-ashr-pk-insts"]
+# Sources that clamp no shifted numbers to bytes: without that feature the compiler drops all of gfx950's own instructions,
+# the wide matrix instructions, transposed LDS reads and conversions to BF16 among them.
+OF_GFX950 = ("OpAttention.hip", "OpAttentionGrad.hip", "OpLogProbs.hip", "OpRotary.hip")
+
+
+def _device(source):
+    """Flags of a source's device code."""
+    return DEVICE + ([] if os.path.basename(source) in OF_GFX950 else NO_SHIFTED_BYTES)
 
 
 def _sources(sub, exts):
@@ -125,8 +133,8 @@ def build(force=False, jobs=8, verbose=True, sanitize=False):
     os.makedirs(objdir, exist_ok=True)
     newest_header = max(os.path.getmtime(h) for h in _headers())
     core = [(s, host_extra) for s in _sources("nvcv", (".cpp",))]
-    ops = [(s, DEVICE + hip_extra if s.endswith(".hip") else host_extra) for s in _sources("cvcuda", (".cpp", ".hip"))]
-    bench = [(s, DEVICE + hip_extra) for s in _sources("bench", (".hip",))]
+    ops = [(s, _device(s) + hip_extra if s.endswith(".hip") else host_extra) for s in _sources("cvcuda", (".cpp", ".hip"))]
+    bench = [(s, _device(s) + hip_extra) for s in _sources("bench", (".hip",))]
     tasks = []
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
         for group, items in (("nvcv", core), ("cvcuda", ops), ("bench", bench)):

@@ -1,0 +1,353 @@
+// What the kernels of attention and of its gradient share (formulas: cvcuda/Attention.h).
+//
+// All products are 32 x 32 x 16 matrix instructions. Scores are made transposed, keys times queries, so that a lane has the scores of ONE
+// query (column) and 16 keys of a tile's 32: their maximum and sum stay in the lane, but for one exchange with the lane that
+// has the other 16. And what a lane has of them is, rounded and packed, what the next product takes as its right operand,
+// without a move between lanes: of 16 keys the lower half wave has 0-3 and 8-11, the upper one 4-7 and 12-15, so the left operand's
+// keys are read in that order too (a sum's order does not matter to the instruction).
+//
+// Tiles of rows (keys and values, or queries and gradients) lie in LDS as they lie in memory, in units of 16 bytes that are exchanged within
+// a row by the row's number, so that neither eight rows' units of one column nor four rows' neighbouring units (a transposed read) meet
+// in a bank.
+#ifndef CVCUDA_AMD_ATTENTIONTILES_HPP
+#define CVCUDA_AMD_ATTENTIONTILES_HPP
+
+#include "HeadOps.hpp"
+
+#include <type_traits>
+
+namespace cvamd {
+
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Exponentials are kept in F16 times a power of two: a share of 2^-20 of the largest keeps all of its bits, one of 2^-30 one bit.
+// (BF16 has the exponents of F32.)
+template<class T>
+constexpr float kExpShift = std::is_same<T, Half>::value ? 6.f : 0.f;
+
+template<class T>
+using Vec8 = T __attribute__((ext_vector_type(8)));
+using Acc16 = float __attribute__((ext_vector_type(16)));
+using Vec4s = short __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void Multiply(Acc16 &acc, Vec8<Bf16> a, Vec8<Bf16> b)
+{
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ void Multiply(Acc16 &acc, Vec8<Half> a, Vec8<Half> b)
+{
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+}
+
+// The lane that has the same column's other rows.
+__device__ __forceinline__ float OtherHalf(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) != 0 ? r[0] : r[1]);
+}
+
+// Largest and sum of a lane's and the other half's.
+__device__ __forceinline__ float BothMax(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float BothSum(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------
+// Row r of DP elements (64 or 128), its unit u of 16 bytes at place u ^ Swap(r).
+__device__ __forceinline__ uint32_t Swap(uint32_t row)
+{
+    return ((row & 3) << 1) | ((row >> 2) & 1);
+}
+
+template<int DP>
+__device__ __forceinline__ uint32_t TileAt(uint32_t row, uint32_t unit)
+{
+    return row * (DP * 2) + ((unit ^ Swap(row)) << 4);
+}
+
+// Rows of a matrix as the instruction's left operand: lane l has row l % 32, elements 16 * step + 8 * (l / 32) to + 7.
+template<class T, int DP>
+__device__ __forceinline__ Vec8<T> RowsOperand(const uint8_t *tile, uint32_t firstRow, int step)
+{
+    const uint32_t lane = threadIdx.x & 63;
+    return *reinterpret_cast<const Vec8<T> *>(tile + TileAt<DP>(firstRow + (lane & 31), 2 * step + (lane >> 5)));
+}
+
+// Columns 32 * part to + 31 of 16 rows as the left operand: lane l has column 32 * part + l % 32 of the rows 4 * (l / 32) to + 3 and 8 + 4 *
+// (l / 32) to + 3. A transposed read gives each lane of 16 a column of the four rows that they read; firstRow is a multiple of 16.
+template<class T, int DP>
+__device__ __forceinline__ Vec8<T> ColumnsOperand(const uint8_t *tile, uint32_t firstRow, int part)
+{
+    using Place          = __attribute__((address_space(3))) Vec4s;
+    const uint32_t lane  = threadIdx.x & 63;
+    const uint32_t row   = firstRow + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const uint32_t unit  = 4 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const uint32_t place = (uint32_t)reinterpret_cast<uintptr_t>(tile) + TileAt<DP>(row, unit) + 8 * (lane & 1); // (Swap(row + 8) is Swap(row))
+    struct
+    {
+        Vec4s low, high;
+    } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Place *>(place)),
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Place *>(place + 8 * DP * 2))};
+    return __builtin_bit_cast(Vec8<T>, both);
+}
+
+// Eight of a lane's 16 numbers, rounded: rows 16 * half to + 15 of a product as the next one's right operand.
+template<class T>
+__device__ __forceinline__ Vec8<T> RoundedHalf(const Acc16 &v, int half)
+{
+    Vec8<T> r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        r[i] = (T)v[8 * half + i];
+    }
+    return r;
+}
+
+// The row that a lane's number i of a product lies in.
+__device__ __forceinline__ int RowOf(int i)
+{
+    return (i >> 2) * 8 + (int)((threadIdx.x & 63) >> 5) * 4 + (i & 3);
+}
+
+// A workgroup's part of a tile of ROWS rows on its way from memory to LDS: 16 bytes a piece, zeros for rows from `count` on and
+// elements from `dims` on. THREADS threads.
+template<int ROWS, int DP, int THREADS>
+struct TileLoad
+{
+    static constexpr int kUnits = DP / 8, kPieces = ROWS * kUnits / THREADS;
+    static_assert(ROWS * kUnits % THREADS == 0, "whole pieces");
+
+    uint4 piece[kPieces];
+
+    // `thread`: the caller's number among the THREADS. rowAt(r): where row r of the tile begins.
+    template<class F>
+    __device__ __forceinline__ void get(uint32_t thread, int count, int dims, F &&rowAt)
+    {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+        {
+            const int at = (int)thread + i * THREADS, row = at / kUnits, unit = at % kUnits;
+            piece[i] = make_uint4(0, 0, 0, 0);
+            if (row < count && unit * 8 < dims)
+            {
+                piece[i] = *reinterpret_cast<const uint4 *>(rowAt(row) + unit * 16);
+            }
+        }
+    }
+
+    // The same of rows at one distance from each other.
+    __device__ __forceinline__ void get(uint32_t thread, const uint8_t *base, int64_t rowStride, int count, int dims)
+    {
+        get(thread, count, dims, [&](int row) { return base + row * rowStride; });
+    }
+
+    __device__ __forceinline__ void put(uint32_t thread, uint8_t *tile) const
+    {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+        {
+            const int at = (int)thread + i * THREADS, row = at / kUnits, unit = at % kUnits;
+            *reinterpret_cast<uint4 *>(tile + TileAt<DP>(row, unit)) = piece[i];
+        }
+    }
+};
+
+// A row of a matrix as the right operand's column: element 16 * step + 8 * (l / 32) to + 7 of it; zeros where `there` is false and behind `dims`.
+template<class T, int DP>
+__device__ __forceinline__ void LoadColumn(Vec8<T> (&to)[DP / 16], const uint8_t *row, bool there, int dims)
+{
+    const int first = (int)((threadIdx.x & 63) >> 5) * 8;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+    {
+        to[s] = {};
+        if (there && 16 * s + first < dims)
+        {
+            to[s] = *reinterpret_cast<const Vec8<T> *>(row + (16 * s + first) * 2);
+        }
+    }
+}
+
+// A transposed product's columns to rows of memory: lane l's column is the row at `row`, times `factor`, rounded. Lanes exchange what they
+// have, so that each stores whole 16 bytes.
+template<class T, int DP>
+__device__ __forceinline__ void StoreColumn(const Acc16 (&acc)[DP / 32], float factor, uint8_t *row, bool there, int dims)
+{
+    const int upper = (int)((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int part = 0; part < DP / 32; ++part)
+    {
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+        {
+            uint32_t words[2][2]; // of the elements 16 * p + 4 * upper to + 3, and 8 + that
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+            {
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                {
+                    struct
+                    {
+                        T a, b;
+                    } two = {(T)(acc[part][8 * p + 4 * k + 2 * w] * factor), (T)(acc[part][8 * p + 4 * k + 2 * w + 1] * factor)};
+                    words[k][w] = __builtin_bit_cast(uint32_t, two);
+                }
+            }
+            const auto     x = __builtin_amdgcn_permlane32_swap(words[0][0], words[1][0], false, false);
+            const auto     y = __builtin_amdgcn_permlane32_swap(words[0][1], words[1][1], false, false);
+            const int      first = part * 32 + 16 * p + 8 * upper;
+            if (there && first < dims)
+            {
+                *reinterpret_cast<uint4 *>(row + first * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+            }
+        }
+    }
+}
+
+// ---- sequences -----------------------------------------------------------------------------------------------------
+struct AttentionSequences
+{
+    const int32_t *offsets, *keyOffsets, *keyLengths; // the latter two: nullptr as in cvcuda/Attention.h
+    int32_t        count, rows, keys;                 // sequences; tokens of q and of k
+
+    __device__ __forceinline__ int firstRow(int b) const
+    {
+        return min(max(offsets[b], 0), rows);
+    }
+
+    __device__ __forceinline__ int rowsOf(int b, int first) const
+    {
+        return max(min(max(offsets[b + 1], 0), rows) - first, 0);
+    }
+
+    __device__ __forceinline__ int firstKey(int b) const
+    {
+        return min(max((keyOffsets != nullptr ? keyOffsets : offsets)[b], 0), keys);
+    }
+
+    __device__ __forceinline__ int keysOf(int b, int first) const
+    {
+        const int n = max(min(max((keyOffsets != nullptr ? keyOffsets : offsets)[b + 1], 0), keys) - first, 0);
+        return keyLengths != nullptr ? min(max(keyLengths[b], 0), n) : n;
+    }
+};
+
+// A sequence and one of its tiles.
+struct SequenceTile
+{
+    int firstRow, rows, firstKey, keys; // of the sequence
+    int tile;                           // -1: there is none of that number
+};
+
+// Tile `t` of all sequences' tiles, of `size` rows each, a token having `each` rows (of keys: `ofKeys`). Every wave finds it by itself.
+__device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, uint32_t t, int size, int each, bool ofKeys)
+{
+    const int lane = (int)(threadIdx.x & 63);
+    uint32_t  before = 0; // tiles of the sequences that were looked at
+    for (int base = 0; base < s.count; base += 64)
+    {
+        const int b     = base + lane;
+        uint32_t  tiles = 0;
+        if (b < s.count)
+        {
+            const int first = ofKeys ? s.firstKey(b) : s.firstRow(b);
+            tiles           = ((uint32_t)(ofKeys ? s.keysOf(b, first) : s.rowsOf(b, first)) * (uint32_t)each + (uint32_t)size - 1) / (uint32_t)size;
+        }
+        uint32_t upTo = tiles; // this sequence's and those of the lanes before
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2)
+        {
+            const uint32_t v = __shfl_up(upTo, d);
+            upTo += lane >= d ? v : 0;
+        }
+        const uint64_t behind = __ballot(before + upTo > t);
+        if (behind != 0)
+        {
+            const int    at = (int)__builtin_ctzll(behind), found = base + at;
+            SequenceTile r;
+            r.tile     = (int)(t - before - ((uint32_t)__builtin_amdgcn_readlane((int)upTo, at) - (uint32_t)__builtin_amdgcn_readlane((int)tiles, at)));
+            r.firstRow = s.firstRow(found);
+            r.rows     = s.rowsOf(found, r.firstRow);
+            r.firstKey = s.firstKey(found);
+            r.keys     = s.keysOf(found, r.firstKey);
+            return r;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
+    }
+    return {0, 0, 0, 0, -1};
+}
+
+// The rows that a key head serves, as one matrix: row r of a sequence is head r % group of token r / group.
+struct GroupRows
+{
+    DivBy group;
+
+    __device__ __forceinline__ int size() const
+    {
+        return (int)group.d;
+    }
+
+    __device__ __forceinline__ int token(int r) const
+    {
+        return (int)group.Quotient((uint32_t)r);
+    }
+};
+
+// The last key that token i of a sequence sees.
+__device__ __forceinline__ int LimitOf(bool causal, const SequenceTile &s, int i)
+{
+    return causal ? i + s.keys - s.rows : s.keys - 1;
+}
+
+// Row r of that matrix. One behind the sequence's end counts as its last one, so that it changes no tile's borders.
+struct AttentionRow
+{
+    int  token, head; // in q and out
+    int  limit;
+    bool there;
+
+    __device__ __forceinline__ AttentionRow(const GroupRows &rows, bool causal, const SequenceTile &s, int keyHead, int r)
+    {
+        const int all = s.rows * rows.size(), at = min(r, all - 1), i = rows.token(at);
+        token = s.firstRow + i;
+        head  = keyHead * rows.size() + (at - i * rows.size());
+        limit = LimitOf(causal, s, i);
+        there = r < all;
+    }
+};
+
+// ---- the operator ------------------------------------------------------------------------------------------------
+class AttentionOperator final : public IOperator
+{
+};
+
+// ---- what the host has checked -----------------------------------------------------------------------------------
+struct AttentionInputs
+{
+    HeadsView          q, k, v;
+    AttentionSequences sequences;
+    float             *lse;
+};
+
+// Shared by the forward call and the gradient. Throws INVALID_ARGUMENT.
+AttentionInputs TakeAttention(NVCVTensorHandle q, NVCVTensorHandle k, NVCVTensorHandle v, NVCVTensorHandle offsets, NVCVTensorHandle keyOffsets,
+                              NVCVTensorHandle keyLengths, NVCVTensorHandle lse, bool lseOptional, float scale);
+
+// A tensor like `as`, aligned as attention's tensors are.
+HeadsView TakeHeadsLike(NVCVTensorHandle h, const HeadsView &as, const char *what);
+
+void RequireAttentionSizes(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t keyHeads, int64_t dims);
+
+} // namespace cvamd
+
+#endif // CVCUDA_AMD_ATTENTIONTILES_HPP

@@ -1,0 +1,543 @@
+// Attention over packed sequences (formulas: cvcuda/Attention.h; tiles and products: AttentionTiles.hpp).
+//
+// One pass over the keys, with the running maximum and sum of a softmax: a tile's scores live in registers from one product to the next. The
+// rows that a key head serves (all heads of its group, token by token) are one matrix, so that its keys and values are read once for
+// them, whatever the group.
+#include "AttentionTiles.hpp"
+
+#include <cvcuda/Attention.h>
+
+#include <algorithm>
+#include <cmath>
+
+namespace cvamd {
+
+namespace {
+
+struct AttentionArgs
+{
+    const uint8_t     *q, *k, *v;
+    uint8_t           *out;
+    int64_t            qToken, qHead, kToken, kHead, vToken, vHead, outToken, outHead;
+    AttentionSequences sequences;
+    float             *lse;                  // nullptr: not wanted
+    float             *partial, *partialLse; // [splits][heads][rows][dims], [splits][heads][rows]: where keys are split
+    GroupRows          rows;                 // of a key head
+    DivBy              keyHeads;
+    int32_t            heads, dims, splits;
+    uint32_t           tiles;
+    float              scale; // to the base 2
+    bool               causal;
+
+    // in lse
+    __device__ __forceinline__ int64_t number(const AttentionRow &row) const
+    {
+        return (int64_t)row.head * sequences.rows + row.token;
+    }
+};
+
+// A lane's row on its way through the keys: the largest score so far to the base 2, which exponentials are taken relative to, the sum of its
+// own keys' exponentials (the other half wave has the other keys') and the weighted values.
+template<class T, int DP>
+struct Running
+{
+    float top = -INFINITY, sum = 0;
+    Acc16 out[DP / 32] = {};
+
+    // KEYS / 32 products of scores; values: tile of KEYS rows in LDS.
+    template<int KEYS>
+    __device__ __forceinline__ void add(Acc16 (&scores)[KEYS / 32], const uint8_t *values, float scale)
+    {
+        float largest = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KEYS / 32; ++k)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                largest = fmaxf(largest, scores[k][i]); // (a NaN is left out here, and reaches the sums below)
+            }
+        }
+        largest = BothMax(largest) * scale;
+        if (__any(largest > top))
+        {
+            largest          = fmaxf(top, largest);
+            const float less = largest > top ? __builtin_amdgcn_exp2f(top - largest) : 1.f; // (0 for the first)
+            sum *= less;
+#pragma unroll
+            for (int p = 0; p < DP / 32; ++p)
+            {
+                out[p] *= less;
+            }
+            top = largest;
+        }
+        const float shift = kExpShift<T> - (top == -INFINITY ? 0.f : top);
+#pragma unroll
+        for (int k = 0; k < KEYS / 32; ++k)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                scores[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[k][i], scale, shift));
+                sum += scores[k][i];
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+            {
+                const Vec8<T> shares = RoundedHalf<T>(scores[k], half);
+#pragma unroll
+                for (int p = 0; p < DP / 32; ++p)
+                {
+                    Multiply(out[p], ColumnsOperand<T, DP>(values, 32 * k + 16 * half, p), shares);
+                }
+            }
+        }
+    }
+};
+
+// Scores of 32 * N keys, keys that a row does not see as -infinity.
+template<class T, int DP, int N>
+__device__ __forceinline__ void Scores(Acc16 (&scores)[N], const uint8_t *keys, const Vec8<T> (&q)[DP / 16], int firstKey, int limit, bool hide)
+{
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+    {
+        scores[k] = {};
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+        {
+            Multiply(scores[k], RowsOperand<T, DP>(keys, 32 * k, s), q[s]);
+        }
+    }
+    if (hide)
+    {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                scores[k][i] = firstKey + 32 * k + RowOf(i) <= limit ? scores[k][i] : -INFINITY;
+            }
+        }
+    }
+}
+
+// What a row has at the end: lse to the base 2.
+template<class T>
+__device__ __forceinline__ float LseOf(float top, float sum)
+{
+    return sum == 0 ? -INFINITY : top + (__builtin_amdgcn_logf(sum) - kExpShift<T>);
+}
+
+// ---- prompts: 128 rows to a workgroup, 32 to a wave ------------------------------------------------------------------
+constexpr int kManyRows = 128, kManyKeys = 64, kManyThreads = 256;
+
+template<class T, int DP>
+__global__ __launch_bounds__(kManyThreads) void AttentionKernel(const AttentionArgs a)
+{
+    __shared__ __attribute__((aligned(256))) uint8_t s_k[2][kManyKeys * DP * 2], s_v[2][kManyKeys * DP * 2];
+    const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
+    const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
+    // (with `causal` a sequence's last tiles have the most keys: they begin first)
+    const SequenceTile s = FindTile(a.sequences, a.causal ? a.tiles - 1 - t : t, kManyRows, a.rows.size(), false);
+    if (s.tile < 0)
+    {
+        return;
+    }
+    const int  first = s.tile * kManyRows, ownFirst = first + (int)WaveOfGroup() * 32, all = s.rows * a.rows.size();
+    const AttentionRow row(a.rows, a.causal, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
+    // keys of the tile, of the wave and those that all of the wave's rows see; this workgroup's part of the tile's
+    auto       limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
+    const int  tileKeys = max(limitAt(first + kManyRows - 1) + 1, 0), waveKeys = ownFirst < all ? limitAt(ownFirst + 31) + 1 : 0;
+    const int  seenKeys = limitAt(ownFirst) + 1;
+    const int  parts    = (tileKeys + kManyKeys - 1) / kManyKeys;
+    const int  from = (int)((int64_t)parts * blockIdx.y / a.splits), to = (int)((int64_t)parts * (blockIdx.y + 1) / a.splits);
+    const uint8_t *k = a.k + s.firstKey * a.kToken + keyHead * a.kHead, *v = a.v + s.firstKey * a.vToken + keyHead * a.vHead;
+
+    Vec8<T> q[DP / 16];
+    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, row.there, a.dims);
+    Running<T, DP>                         run;
+    TileLoad<kManyKeys, DP, kManyThreads> nextK, nextV;
+    auto load = [&](int part)
+    {
+        const int key = part * kManyKeys;
+        nextK.get(threadIdx.x, k + key * a.kToken, a.kToken, s.keys - key, a.dims);
+        nextV.get(threadIdx.x, v + key * a.vToken, a.vToken, s.keys - key, a.dims);
+    };
+    if (from < to)
+    {
+        load(from);
+    }
+    for (int part = from; part < to; ++part)
+    {
+        const int at = (part - from) & 1, key = part * kManyKeys;
+        nextK.put(threadIdx.x, s_k[at]);
+        nextV.put(threadIdx.x, s_v[at]);
+        __syncthreads(); // (all have done the part before, so that the one before that may be written over)
+        if (part + 1 < to)
+        {
+            load(part + 1);
+        }
+        if (key < waveKeys)
+        {
+            Acc16 scores[kManyKeys / 32];
+            Scores<T, DP>(scores, s_k[at], q, key, row.limit, key + kManyKeys > seenKeys);
+            run.template add<kManyKeys>(scores, s_v[at], a.scale);
+        }
+    }
+    const float   sum = BothSum(run.sum), factor = sum == 0 ? 0.f : 1.f / sum;
+    const float   lse = LseOf<T>(run.top, sum);
+    const int64_t number = a.number(row);
+    if (a.splits == 1)
+    {
+        StoreColumn<T, DP>(run.out, factor, a.out + row.token * a.outToken + row.head * a.outHead, row.there, a.dims);
+        if (a.lse != nullptr && row.there && (threadIdx.x & 32) == 0)
+        {
+            a.lse[number] = lse * kLn2;
+        }
+        return;
+    }
+    const int64_t at = (int64_t)blockIdx.y * a.heads * a.sequences.rows + number;
+    if (row.there)
+    {
+        float *partial = a.partial + at * a.dims;
+#pragma unroll
+        for (int p = 0; p < DP / 32; ++p)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+            {
+                const int d = 32 * p + RowOf(i);
+                if (d < a.dims)
+                {
+                    *reinterpret_cast<float4 *>(partial + d) = make_float4(run.out[p][i] * factor, run.out[p][i + 1] * factor,
+                                                                           run.out[p][i + 2] * factor, run.out[p][i + 3] * factor);
+                }
+            }
+        }
+        if ((threadIdx.x & 32) == 0)
+        {
+            a.partialLse[at] = lse;
+        }
+    }
+}
+
+// ---- few rows to a sequence (single tokens): 32 rows to a workgroup, every fourth 32 keys to each of its waves ------------
+constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4, kFewThreads = 64 * kFewWaves;
+
+template<class T, int DP>
+__global__ __launch_bounds__(kFewThreads) void AttentionFewKernel(const AttentionArgs a)
+{
+    // each wave's keys and values, later its weighted values in 32 bits
+    __shared__ __attribute__((aligned(256))) uint8_t s_tile[kFewWaves][2 * kFewKeys * DP * 2];
+    __shared__ float                                 s_top[kFewWaves][kFewRows], s_sum[kFewWaves][kFewRows];
+    const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
+    const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
+    const SequenceTile s       = FindTile(a.sequences, t, kFewRows, a.rows.size(), false);
+    if (s.tile < 0)
+    {
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 63, wave = WaveOfGroup();
+    const int      first = s.tile * kFewRows, all = s.rows * a.rows.size();
+    const AttentionRow row(a.rows, a.causal, s, keyHead, first + (int)(lane & 31));
+    auto           limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
+    const int      tileKeys = max(limitAt(first + kFewRows - 1) + 1, 0), seenKeys = limitAt(first) + 1;
+    const int      parts    = (tileKeys + kFewKeys - 1) / kFewKeys;
+    const int      from = (int)((int64_t)parts * blockIdx.y / a.splits) + (int)wave, to = (int)((int64_t)parts * (blockIdx.y + 1) / a.splits);
+    const uint8_t *k = a.k + s.firstKey * a.kToken + keyHead * a.kHead, *v = a.v + s.firstKey * a.vToken + keyHead * a.vHead;
+    uint8_t       *keys = s_tile[wave], *values = keys + kFewKeys * DP * 2;
+
+    TileLoad<kFewKeys, DP, 64> nextK, nextV;
+    auto load = [&](int part)
+    {
+        const int key = part * kFewKeys;
+        nextK.get(lane, k + key * a.kToken, a.kToken, s.keys - key, a.dims);
+        nextV.get(lane, v + key * a.vToken, a.vToken, s.keys - key, a.dims);
+    };
+    if (from < to)
+    {
+        load(from);
+    }
+    Vec8<T> q[DP / 16];
+    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, row.there, a.dims);
+    Running<T, DP> run;
+    for (int part = from; part < to; part += kFewWaves)
+    {
+        const int key = part * kFewKeys;
+        // (a wave's reads and writes of LDS take place in their order; the compiler is kept from changing it)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        nextK.put(lane, keys);
+        nextV.put(lane, values);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (part + kFewWaves < to)
+        {
+            load(part + kFewWaves);
+        }
+        Acc16 scores[1];
+        Scores<T, DP>(scores, keys, q, key, row.limit, key + kFewKeys > seenKeys);
+        run.template add<kFewKeys>(scores, values, a.scale);
+    }
+    // the waves' results joined: thread l has row l % 32, an eighth of its elements
+    const float sum = BothSum(run.sum);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float *own = reinterpret_cast<float *>(s_tile[wave]); // [DP][32]
+#pragma unroll
+    for (int p = 0; p < DP / 32; ++p)
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            own[(32 * p + RowOf(i)) * kFewRows + (lane & 31)] = run.out[p][i];
+        }
+    }
+    if (lane < 32)
+    {
+        s_top[wave][lane] = run.top;
+        s_sum[wave][lane] = sum;
+    }
+    __syncthreads();
+    const uint32_t r = threadIdx.x % kFewRows, d0 = threadIdx.x / kFewRows * (DP / 8);
+    float          top = -INFINITY, total = 0, weight[kFewWaves];
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w)
+    {
+        top = fmaxf(top, s_top[w][r]);
+    }
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w)
+    {
+        weight[w] = s_top[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_top[w][r] - top);
+        total += weight[w] * s_sum[w][r];
+    }
+    const float factor = total == 0 ? 0.f : 1.f / total, lse = LseOf<T>(top, total);
+    const AttentionRow its(a.rows, a.causal, s, keyHead, first + (int)r);
+    const int64_t number = a.number(its), at = (int64_t)blockIdx.y * a.heads * a.sequences.rows + number;
+    if (!its.there)
+    {
+        return;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 8; d += 8)
+    {
+        float v8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            v8[i] = 0;
+#pragma unroll
+            for (int w = 0; w < kFewWaves; ++w)
+            {
+                v8[i] += weight[w] * reinterpret_cast<const float *>(s_tile[w])[(d0 + d + i) * kFewRows + r];
+            }
+            v8[i] *= factor;
+        }
+        const int to8 = (int)d0 + d;
+        if (to8 < a.dims)
+        {
+            if (a.splits == 1)
+            {
+                Run<T, 8> made;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                {
+                    made.v[i] = FromFloat<T>(v8[i]);
+                }
+                *reinterpret_cast<Run<T, 8> *>(a.out + its.token * a.outToken + its.head * a.outHead + to8 * 2) = made;
+            }
+            else
+            {
+                float4 *partial = reinterpret_cast<float4 *>(a.partial + at * a.dims + to8);
+                partial[0]      = make_float4(v8[0], v8[1], v8[2], v8[3]);
+                partial[1]      = make_float4(v8[4], v8[5], v8[6], v8[7]);
+            }
+        }
+    }
+    if (d0 == 0)
+    {
+        if (a.splits > 1)
+        {
+            a.partialLse[at] = lse;
+        }
+        else if (a.lse != nullptr)
+        {
+            a.lse[number] = lse * kLn2;
+        }
+    }
+}
+
+// The parts of the keys joined: 16 lanes to a row, 8 elements to a lane.
+constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 16;
+
+template<class T>
+__global__ __launch_bounds__(kJoinThreads) void AttentionJoinKernel(const AttentionArgs a)
+{
+    const int64_t rows = (int64_t)a.heads * a.sequences.rows, number = (int64_t)blockIdx.x * kJoinRows + threadIdx.x / 16;
+    const int     head = (int)(number / a.sequences.rows), token = (int)(number - (int64_t)head * a.sequences.rows), d = (int)(threadIdx.x % 16) * 8;
+    if (number >= rows)
+    {
+        return;
+    }
+    // (rows of no sequence have no parts)
+    const int begin = a.sequences.firstRow(0), end = begin + a.sequences.rowsOf(a.sequences.count - 1, begin);
+    if (token < begin || token >= end || d >= a.dims)
+    {
+        return;
+    }
+    float top = -INFINITY, total = 0, out[8] = {};
+    for (int p = 0; p < a.splits; ++p)
+    {
+        top = fmaxf(top, a.partialLse[p * rows + number]);
+    }
+    for (int p = 0; p < a.splits; ++p)
+    {
+        const float lse = a.partialLse[p * rows + number], weight = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - top);
+        if (lse != -INFINITY)
+        {
+            const float *part = a.partial + (p * rows + number) * a.dims + d;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                out[i] += weight * part[i];
+            }
+            total += weight;
+        }
+    }
+    const float factor = total == 0 ? 0.f : 1.f / total;
+    Run<T, 8>   made;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        made.v[i] = FromFloat<T>(out[i] * factor);
+    }
+    *reinterpret_cast<Run<T, 8> *>(a.out + token * a.outToken + head * a.outHead + d * 2) = made;
+    if (d == 0 && a.lse != nullptr)
+    {
+        a.lse[number] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+    }
+}
+
+// How a call is made, by its sizes alone: the sequences' lengths are on the device.
+struct Plan
+{
+    bool     few;
+    int32_t  splits;
+    uint32_t tiles; // at most, of a key head
+
+    Plan(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t keyHeads)
+    {
+        const int64_t matrix = rows * (heads / keyHeads), most = std::max<int64_t>(sequences, 1);
+        few                  = matrix <= 48 * most;
+        const int64_t size = few ? kFewRows : kManyRows, whole = (matrix + size - 1) / size;
+        tiles              = (uint32_t)(whole + std::min(sequences, rows));
+        // as many workgroups as fill the card's CUs twice, each with 256 keys at least
+        const int64_t groups = std::max<int64_t>(std::max(whole, std::min(sequences, rows)) * keyHeads, 1), each = keys / most;
+        splits               = (int32_t)std::max<int64_t>(std::min<int64_t>({512 / groups, each / 256, 64}), 1);
+    }
+
+    int64_t partials(int64_t rows, int64_t heads) const
+    {
+        return splits > 1 ? splits * rows * heads : 0;
+    }
+
+    int64_t bytes(int64_t rows, int64_t heads, int64_t dims) const
+    {
+        return partials(rows, heads) * (dims + 1) * (int64_t)sizeof(float);
+    }
+};
+
+template<class T, int DP>
+void Launch(const AttentionArgs &a, bool few, hipStream_t stream)
+{
+    const dim3 grid(a.tiles * a.keyHeads.d, (uint32_t)a.splits);
+    if (few)
+    {
+        AttentionFewKernel<T, DP><<<grid, kFewThreads, 0, stream>>>(a);
+    }
+    else
+    {
+        AttentionKernel<T, DP><<<grid, kManyThreads, 0, stream>>>(a);
+    }
+    CheckLaunch("attention");
+    if (a.splits > 1)
+    {
+        const int64_t rows = (int64_t)a.heads * a.sequences.rows;
+        AttentionJoinKernel<T><<<(uint32_t)((rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, stream>>>(a);
+        CheckLaunch("attention's parts");
+    }
+}
+
+struct Attention
+{
+    static void submit(hipStream_t stream, NVCVTensorHandle hq, NVCVTensorHandle hk, NVCVTensorHandle hv, NVCVTensorHandle hoffsets,
+                       NVCVTensorHandle hkeyOffsets, NVCVTensorHandle hkeyLengths, NVCVTensorHandle hout, NVCVTensorHandle hlse,
+                       NVCVTensorHandle hworkspace, float scale, bool causal)
+    {
+        const AttentionInputs in  = TakeAttention(hq, hk, hv, hoffsets, hkeyOffsets, hkeyLengths, hlse, true, scale);
+        const HeadsView       out = TakeHeadsLike(hout, in.q, "Output");
+        const Plan            plan(in.q.tokens, in.k.tokens, in.sequences.count, in.q.heads, in.k.heads);
+        uint8_t              *room = RequireWorkspace(hworkspace, plan.bytes(in.q.tokens, in.q.heads, in.q.dims));
+        if (in.q.tokens == 0 || in.sequences.count == 0)
+        {
+            return;
+        }
+        if ((int64_t)plan.tiles * in.k.heads > INT32_MAX / kManyThreads * 2)
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Too many rows");
+        }
+        float              *partial = reinterpret_cast<float *>(room);
+        const AttentionArgs a = {in.q.base, in.k.base, in.v.base, out.base, in.q.tokenStride, in.q.headStride, in.k.tokenStride, in.k.headStride,
+                                 in.v.tokenStride, in.v.headStride, out.tokenStride, out.headStride, in.sequences, in.lse, partial,
+                                 partial + plan.partials(in.q.tokens, in.q.heads) * in.q.dims, {DivBy((uint32_t)(in.q.heads / in.k.heads))},
+                                 DivBy((uint32_t)in.k.heads), in.q.heads, in.q.dims, plan.splits, plan.tiles, scale * kLog2E, causal};
+        auto                launch = [&](auto t)
+        {
+            using T = decltype(t);
+            in.q.dims <= 64 ? Launch<T, 64>(a, plan.few, stream) : Launch<T, 128>(a, plan.few, stream);
+        };
+        in.q.elem == kRowF16 ? launch(Half{}) : launch(Bf16{});
+    }
+};
+
+} // namespace
+} // namespace cvamd
+
+using namespace cvamd;
+
+extern "C"
+{
+CVCUDA_PUBLIC NVCVStatus cvcudaxAttentionCreate(NVCVOperatorHandle *handle)
+{
+    return CreateOperator<AttentionOperator>(handle);
+}
+
+CVCUDA_PUBLIC NVCVStatus cvcudaxAttentionWorkspace(int64_t rows, int64_t keys, int64_t sequences, int32_t heads,
+                                                   int32_t keyHeads, int32_t dims, int64_t *bytes)
+{
+    return Protect(
+        [&]
+        {
+            if (bytes == nullptr)
+            {
+                throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Pointer to output must not be NULL");
+            }
+            RequireAttentionSizes(rows, keys, sequences, heads, keyHeads, dims);
+            *bytes = Plan(rows, keys, sequences, heads, keyHeads).bytes(rows, heads, dims);
+        });
+}
+
+CVCUDA_PUBLIC NVCVStatus cvcudaxAttentionSubmit(NVCVOperatorHandle handle, hipStream_t stream, NVCVTensorHandle q,
+                                                NVCVTensorHandle k, NVCVTensorHandle v, NVCVTensorHandle offsets,
+                                                NVCVTensorHandle keyOffsets, NVCVTensorHandle keyLengths,
+                                                NVCVTensorHandle out, NVCVTensorHandle lse, NVCVTensorHandle workspace,
+                                                float scale, int8_t causal)
+{
+    return Protect(
+        [&]
+        {
+            (void)ToOperator<AttentionOperator>(handle);
+            Attention::submit(stream, q, k, v, offsets, keyOffsets, keyLengths, out, lse, workspace, scale, causal != 0);
+        });
+}
+}

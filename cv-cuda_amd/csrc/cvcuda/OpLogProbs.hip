@@ -1,0 +1,590 @@
+// Log probabilities of tokens with entropy and top alternatives, and their gradient (formulas: cvcuda/LogProbs.h). Bound by memory: the
+// logits are read once.
+//
+// One pass over a row: each lane keeps the largest of its logits so far, m, and the sums of exp(z - scale * m) and of exp(z - scale * m) *
+// (x - m), rescaled whenever m grows; the workgroup joins its lanes' afterwards. The entropy is log(s) - scale * t / s, in which
+// nothing large is left to cancel. The top tokens come from what the pass has anyway: of the lanes' largest logits, by 64 groups, the K-th
+// largest is one that K logits of the row reach, so that the lanes which reach it, few in most rows, look through theirs again for those
+// that do. Where too many do, or the row has NaN, the whole row is gone over K times.
+#include "RowOps.hpp"
+
+#include <cvcuda/LogProbs.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+namespace cvamd {
+
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kFar   = -1e30f; // below any difference of logits whose exponential isn't 0; a sum of 2^31 of it is finite
+constexpr int   kGroups = 64, kCandidates = 512;
+static_assert(CVCUDAX_LOG_PROBS_MOST_TOP <= kGroups, "as many groups as top tokens");
+
+struct LogProbsArgs
+{
+    RowPlaces   logits;
+    const void *tokens;
+    float      *out, *entropy, *lse, *topValues; // all but out: nullptr where not wanted
+    int32_t    *topTokens;
+    float       scale;
+    int32_t     rows, columns, top, firstRow;
+    bool        wide; // tokens of 64 bits
+};
+
+__device__ __forceinline__ int64_t TokenAt(const void *tokens, bool wide, uint32_t row)
+{
+    return wide ? static_cast<const int64_t *>(tokens)[row] : static_cast<const int32_t *>(tokens)[row];
+}
+
+// Whole numbers in the order of the logits: NaN above all, -0 as +0.
+__device__ __forceinline__ uint32_t OrderOf(float x)
+{
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return x != x ? 0xFFFFFFFFu : (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
+}
+
+// A logit and its column: larger logits first, of equal ones the lower columns.
+__device__ __forceinline__ uint64_t KeyOf(float x, int column)
+{
+    return ((uint64_t)OrderOf(x) << 32) | (0xFFFFFFFFu - (uint32_t)column);
+}
+
+__device__ __forceinline__ int ColumnOf(uint64_t key)
+{
+    return (int)(0xFFFFFFFFu - (uint32_t)key);
+}
+
+// Run r of a row: N logits from N * r on, at the row's end the last N of it, of which those from `skip` on are its own.
+template<class T, int N>
+struct Logits
+{
+    Run<T, N> run;
+    int       from, skip;
+
+    __device__ __forceinline__ void get(const T *row, int columns, int r)
+    {
+        from = min(r * N, columns - N);
+        skip = r * N - from;
+        run  = *reinterpret_cast<const Run<T, N> *>(row + from);
+    }
+};
+
+template<int LANES>
+struct TopRoom
+{
+    uint32_t group[kGroups];
+    uint64_t key[kCandidates];
+    uint32_t count;
+};
+
+// The largest of the lanes' keys, in all of them. `part`: room that nobody reads or writes at the time, nor after the next barrier.
+template<int WAVES>
+__device__ __forceinline__ uint64_t LargestKey(uint64_t v, uint64_t (&part)[WAVES])
+{
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2)
+    {
+        const uint64_t o = ((uint64_t)__shfl_xor((uint32_t)(v >> 32), d) << 32) | __shfl_xor((uint32_t)v, d);
+        v                = o > v ? o : v;
+    }
+    if constexpr (WAVES > 1)
+    {
+        __syncthreads();
+        part[WaveOfGroup()] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+        {
+            v = part[w] > v ? part[w] : v;
+        }
+    }
+    return v;
+}
+
+// Entry `rank` of a row's top tokens.
+__device__ __forceinline__ void PutTop(const LogProbsArgs &a, uint32_t row, int rank, int column, float x, float largest, float logSum, bool nothing)
+{
+    const int64_t at = (int64_t)row * a.top + rank;
+    a.topTokens[at]  = column;
+    a.topValues[at]  = nothing ? -INFINITY : a.scale * (x - largest) - logSum;
+}
+
+// N: logits of a run (1 where rows are narrower than 16 bytes). One workgroup to a row.
+template<class T, int N, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs a)
+{
+    constexpr int       kLanes = 64 * WAVES, kAhead = 4;
+    __shared__ float    s_m[WAVES], s_s[WAVES], s_t[WAVES];
+    __shared__ uint64_t s_key[WAVES];
+    __shared__ TopRoom<kLanes> s_top;
+    const uint32_t row  = a.firstRow + blockIdx.x;
+    const T       *in   = reinterpret_cast<const T *>(a.logits.at(row));
+    const int      runs = (a.columns + N - 1) / N;
+    const float    c    = a.scale * kLog2E;
+    float          m = -FLT_MAX, s = 0, t = 0;
+    Logits<T, N>   x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+    {
+        x[k].get(in, a.columns, min((int)threadIdx.x + k * kLanes, runs - 1));
+    }
+    for (int r = (int)threadIdx.x; r < runs; r += kAhead * kLanes)
+    {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+        {
+            if (r + k * kLanes < runs)
+            {
+                float v[N], top = m;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    v[i] = i >= x[k].skip ? (float)x[k].run.v[i] : -INFINITY;
+                    top  = fmaxf(top, v[i]); // (a NaN is left out)
+                }
+                const float less = fmaxf(m - top, kFar), r2 = __builtin_amdgcn_exp2f(less * c);
+                t = r2 * __builtin_fmaf(s, less, t);
+                s *= r2;
+                m = top;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    const float d = v[i] - m, e = __builtin_amdgcn_exp2f(d * c);
+                    s += e;
+                    t = __builtin_fmaf(e, fmaxf(d, kFar), t); // (e is 0 where d is -infinity)
+                }
+            }
+            x[k].get(in, a.columns, min(r + (k + kAhead) * kLanes, runs - 1));
+        }
+    }
+    // the workgroup's m, s and t; a lane that has met nothing but -infinity, or nothing, has s = 0
+    const float own = m;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2)
+    {
+        const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d), t2 = __shfl_xor(t, d), top = fmaxf(m, m2);
+        const float less = fmaxf(m - top, kFar), less2 = fmaxf(m2 - top, kFar), r = __builtin_amdgcn_exp2f(less * c), r2 = __builtin_amdgcn_exp2f(less2 * c);
+        t = (s != 0 ? r * __builtin_fmaf(s, less, t) : 0.f) + (s2 != 0 ? r2 * __builtin_fmaf(s2, less2, t2) : 0.f);
+        s = (s != 0 ? s * r : 0.f) + (s2 != 0 ? s2 * r2 : 0.f);
+        m = top;
+    }
+    if constexpr (WAVES > 1)
+    {
+        if ((threadIdx.x & 63) == 0)
+        {
+            s_m[WaveOfGroup()] = m, s_s[WaveOfGroup()] = s, s_t[WaveOfGroup()] = t;
+        }
+    }
+    if (a.top > 0)
+    {
+        // groups of WAVES lanes that follow one another
+        float g = own;
+#pragma unroll
+        for (int d = 1; d < WAVES; d *= 2)
+        {
+            g = fmaxf(g, __shfl_xor(g, d));
+        }
+        if (threadIdx.x % WAVES == 0)
+        {
+            s_top.group[threadIdx.x / WAVES] = OrderOf(g);
+        }
+        if (threadIdx.x == 0)
+        {
+            s_top.count = 0;
+        }
+    }
+    __syncthreads();
+    if constexpr (WAVES > 1)
+    {
+        m = -FLT_MAX;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+        {
+            m = fmaxf(m, s_m[w]);
+        }
+        s = 0, t = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+        {
+            if (s_s[w] != 0)
+            {
+                const float less = fmaxf(s_m[w] - m, kFar), r = __builtin_amdgcn_exp2f(less * c);
+                t += r * __builtin_fmaf(s_s[w], less, s_t[w]);
+                s += r * s_s[w];
+            }
+        }
+    }
+    const bool  nothing = s == 0; // all logits are -infinity
+    const float logSum  = nothing ? 0.f : logf(s);
+    if (threadIdx.x == 0)
+    {
+        const int64_t token = TokenAt(a.tokens, a.wide, row);
+        float         p     = 0;
+        if (token >= 0 && token < a.columns)
+        {
+            p = nothing ? -INFINITY : a.scale * ((float)in[token] - m) - logSum;
+        }
+        a.out[row] = p;
+        if (a.entropy != nullptr)
+        {
+            a.entropy[row] = nothing ? 0.f : logSum - a.scale * (t / s);
+        }
+        if (a.lse != nullptr)
+        {
+            a.lse[row] = nothing ? -INFINITY : __builtin_fmaf(a.scale, m, logSum);
+        }
+    }
+    if (a.top == 0)
+    {
+        return;
+    }
+    // the K-th largest of the groups' largest logits
+    const uint32_t mine = s_top.group[threadIdx.x & 63];
+    int            rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < kGroups; ++j)
+    {
+        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+        rank += other > mine || (other == mine && j < (int)(threadIdx.x & 63)) ? 1 : 0;
+    }
+    const uint32_t least = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)__builtin_ctzll(__ballot(rank == a.top - 1)));
+    if (OrderOf(own) >= least && s == s)
+    {
+        for (int r = (int)threadIdx.x; r < runs; r += kLanes)
+        {
+            Logits<T, N> l;
+            l.get(in, a.columns, r);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                const float v = (float)l.run.v[i];
+                if (i >= l.skip && OrderOf(v) >= least)
+                {
+                    const uint32_t at = atomicAdd(&s_top.count, 1u);
+                    if (at < kCandidates)
+                    {
+                        s_top.key[at] = KeyOf(v, l.from + i);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int count = (int)s_top.count;
+    if (s == s && count >= a.top && count <= kCandidates)
+    {
+        for (int i = (int)threadIdx.x; i < count; i += kLanes)
+        {
+            const uint64_t key   = s_top.key[i];
+            int            above = 0;
+            for (int j = 0; j < count; ++j)
+            {
+                above += s_top.key[j] > key ? 1 : 0;
+            }
+            if (above < a.top)
+            {
+                PutTop(a, row, above, ColumnOf(key), (float)in[ColumnOf(key)], m, logSum, nothing);
+            }
+        }
+        return;
+    }
+    uint64_t before = ~0ull;
+    for (int k = 0; k < a.top; ++k)
+    {
+        uint64_t best = 0;
+        for (int r = (int)threadIdx.x; r < runs; r += kLanes)
+        {
+            Logits<T, N> l;
+            l.get(in, a.columns, r);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                const uint64_t key = KeyOf((float)l.run.v[i], l.from + i);
+                best               = key < before && key > best ? key : best;
+            }
+        }
+        before = LargestKey<WAVES>(best, s_key);
+        if (threadIdx.x == 0)
+        {
+            PutTop(a, row, k, ColumnOf(before), (float)in[ColumnOf(before)], m, logSum, nothing);
+        }
+    }
+}
+
+struct LogProbsGradArgs
+{
+    RowPlaces    logits, out;
+    const void  *tokens;
+    const float *lse, *entropy, *grad, *gradEntropy; // gradEntropy: nullptr for none
+    float        scale;
+    int32_t      rows, columns;
+    DivBy        parts; // workgroups of a row
+    bool         wide;
+};
+
+constexpr int kGradThreads = 256, kGradRuns = 4; // runs of a lane
+
+// A workgroup makes kGradRuns * kGradThreads runs of a row.
+template<class T, int N, bool ENTROPY>
+__global__ __launch_bounds__(kGradThreads) void LogProbsGradKernel(const LogProbsGradArgs a, uint32_t firstBlock)
+{
+    const uint32_t block = firstBlock + blockIdx.x, row = a.parts.Quotient(block), part = block - row * a.parts.d;
+    const T       *in    = reinterpret_cast<const T *>(a.logits.at(row));
+    T             *out   = reinterpret_cast<T *>(a.out.at(row));
+    const int      runs  = (a.columns + N - 1) / N, first = (int)(part * kGradRuns) * kGradThreads + (int)threadIdx.x;
+    Logits<T, N>   x[kGradRuns];
+#pragma unroll
+    for (int k = 0; k < kGradRuns; ++k)
+    {
+        x[k].get(in, a.columns, min(first + k * kGradThreads, runs - 1));
+    }
+    const int64_t token   = TokenAt(a.tokens, a.wide, row);
+    const bool    there   = token >= 0 && token < a.columns;
+    const float   lse     = a.lse[row], g = there ? a.grad[row] : 0.f, h = ENTROPY ? a.gradEntropy[row] : 0.f;
+    const float   entropy = ENTROPY ? a.entropy[row] : 0.f;
+    const bool    nothing = lse == -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kGradRuns; ++k)
+    {
+        if (first + k * kGradThreads >= runs)
+        {
+            break;
+        }
+        Run<T, N> made;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const float logp = a.scale * (float)x[k].run.v[i] - lse, p = __builtin_amdgcn_exp2f(logp * kLog2E);
+            float       v = -g * p;
+            if (ENTROPY)
+            {
+                v -= p == 0 ? 0.f : h * p * (logp + entropy);
+            }
+            v += there && x[k].from + i == (int)token ? g : 0.f;
+            made.v[i] = FromFloat<T>(nothing ? 0.f : a.scale * v);
+        }
+        if (x[k].skip == 0)
+        {
+            *reinterpret_cast<Run<T, N> *>(out + x[k].from) = made;
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                if (i >= x[k].skip)
+                {
+                    out[x[k].from + i] = made.v[i];
+                }
+            }
+        }
+    }
+}
+
+template<class T, int N, int WAVES>
+void LaunchRows(LogProbsArgs a, hipStream_t stream)
+{
+    constexpr int most = INT32_MAX / (64 * WAVES);
+    for (int64_t first = 0; first < a.rows; first += most)
+    {
+        a.firstRow = (int32_t)first;
+        LogProbsKernel<T, N, WAVES><<<(uint32_t)std::min<int64_t>(most, a.rows - first), 64 * WAVES, 0, stream>>>(a);
+        CheckLaunch("log probabilities");
+    }
+}
+
+template<class T, int N>
+void LaunchLogProbs(const LogProbsArgs &a, hipStream_t stream)
+{
+    a.columns <= 2048    ? LaunchRows<T, N, 1>(a, stream)
+    : a.columns <= 16384 ? LaunchRows<T, N, 4>(a, stream)
+    : a.rows > 512       ? LaunchRows<T, N, 8>(a, stream)
+                         : LaunchRows<T, N, 16>(a, stream);
+}
+
+template<class T, int N, bool ENTROPY>
+void LaunchLogProbsGrad(const LogProbsGradArgs &a, hipStream_t stream)
+{
+    const int64_t blocks = (int64_t)a.rows * a.parts.d, most = INT32_MAX / kGradThreads;
+    if (blocks > INT32_MAX)
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Logits have too many elements");
+    }
+    for (int64_t first = 0; first < blocks; first += most)
+    {
+        LogProbsGradKernel<T, N, ENTROPY><<<(uint32_t)std::min(most, blocks - first), kGradThreads, 0, stream>>>(a, (uint32_t)first);
+        CheckLaunch("log probabilities' gradient");
+    }
+}
+
+template<class F>
+void Dispatch(RowElem elem, F &&f)
+{
+    elem == kRowF32 ? f(float{}) : elem == kRowF16 ? f(Half{}) : f(Bf16{});
+}
+
+RowsView TakeLogits(NVCVTensorHandle h, const char *what)
+{
+    const RowsView v = RequireRows(h, what);
+    if (v.columns < 1 && v.rows > 0)
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must have rows of at least one element", what);
+    }
+    return v;
+}
+
+// A tensor of `count` elements; nullptr where there is none and it may be left out.
+float *TakeFloats(NVCVTensorHandle h, const char *what, int64_t count, bool optional)
+{
+    if (h == nullptr && optional)
+    {
+        return nullptr;
+    }
+    const DenseView v = RequireDense(h, what, NVCV_DATA_TYPE_F32);
+    if (v.count != count)
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must have %ld elements, not %ld", what, (long)count, (long)v.count);
+    }
+    return reinterpret_cast<float *>(v.base);
+}
+
+DenseView TakeTokens(NVCVTensorHandle h, int64_t count)
+{
+    const DenseView v = RequireDense(h, "Tokens", NVCV_DATA_TYPE_NONE);
+    if (v.dtype != NVCV_DATA_TYPE_S32 && v.dtype != NVCV_DATA_TYPE_S64)
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Tokens must hold S32 or S64 values");
+    }
+    if (v.count != count)
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Tokens must have one element for each of %ld rows, not %ld", (long)count, (long)v.count);
+    }
+    return v;
+}
+
+void RequireScale(float scale)
+{
+    if (!(scale > 0) || !std::isfinite(scale))
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Scale must be finite and positive, not %g", (double)scale);
+    }
+}
+
+class LogProbs final : public IOperator
+{
+public:
+    static void submit(hipStream_t stream, NVCVTensorHandle hlogits, NVCVTensorHandle htokens, NVCVTensorHandle hout, NVCVTensorHandle hentropy,
+                       NVCVTensorHandle hlse, NVCVTensorHandle htopValues, NVCVTensorHandle htopTokens, float scale)
+    {
+        const RowsView  logits = TakeLogits(hlogits, "Logits");
+        const DenseView tokens = TakeTokens(htokens, logits.rows);
+        float          *out = TakeFloats(hout, "Output", logits.rows, false), *entropy = TakeFloats(hentropy, "Entropy", logits.rows, true);
+        float          *lse = TakeFloats(hlse, "Lse", logits.rows, true), *topValues = nullptr;
+        int32_t        *topTokens = nullptr;
+        int64_t         top       = 0;
+        RequireScale(scale);
+        if ((htopValues == nullptr) != (htopTokens == nullptr))
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Top values and top tokens go together");
+        }
+        if (htopTokens != nullptr && logits.rows > 0)
+        {
+            const DenseView v = RequireDense(htopTokens, "Top tokens", NVCV_DATA_TYPE_S32);
+            top               = v.count / logits.rows;
+            if (top < 1 || top > CVCUDAX_LOG_PROBS_MOST_TOP || top > logits.columns || v.count % logits.rows != 0)
+            {
+                throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Top tokens must have 1 to %d elements for each of %d rows of %d logits, not %ld in all",
+                              CVCUDAX_LOG_PROBS_MOST_TOP, logits.rows, logits.columns, (long)v.count);
+            }
+            topTokens = reinterpret_cast<int32_t *>(v.base);
+            topValues = TakeFloats(htopValues, "Top values", v.count, false);
+        }
+        if (logits.rows == 0)
+        {
+            return;
+        }
+        const LogProbsArgs a = {RowPlaces(logits), tokens.base, out, entropy, lse, topValues, topTokens, scale, logits.rows, logits.columns,
+                                (int32_t)top, 0, tokens.dtype == NVCV_DATA_TYPE_S64};
+        Dispatch(logits.elem,
+                 [&](auto t)
+                 {
+                     using T = decltype(t);
+                     logits.columns >= kRunOf<T> ? LaunchLogProbs<T, kRunOf<T>>(a, stream) : LaunchLogProbs<T, 1>(a, stream);
+                 });
+    }
+
+    static void submitGrad(hipStream_t stream, NVCVTensorHandle hlogits, NVCVTensorHandle htokens, NVCVTensorHandle hlse, NVCVTensorHandle hentropy,
+                           NVCVTensorHandle hgrad, NVCVTensorHandle hgradEntropy, NVCVTensorHandle hout, float scale)
+    {
+        const RowsView logits = TakeLogits(hlogits, "Logits"), out = TakeLogits(hout, "Logits' gradient");
+        if (out.elem != logits.elem || out.rows != logits.rows || out.columns != logits.columns)
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Logits' gradient must have the type and shape of the logits");
+        }
+        const DenseView tokens = TakeTokens(htokens, logits.rows);
+        const float    *lse = TakeFloats(hlse, "Lse", logits.rows, false), *grad = TakeFloats(hgrad, "Output's gradient", logits.rows, false);
+        const float    *gradEntropy = TakeFloats(hgradEntropy, "Entropy's gradient", logits.rows, true);
+        const float    *entropy     = TakeFloats(hentropy, "Entropy", logits.rows, gradEntropy == nullptr);
+        RequireScale(scale);
+        if (logits.rows == 0)
+        {
+            return;
+        }
+        Dispatch(logits.elem,
+                 [&](auto t)
+                 {
+                     using T              = decltype(t);
+                     const auto run       = [&](auto n)
+                     {
+                         constexpr int          N     = decltype(n)::value;
+                         const int64_t          parts = ((int64_t)logits.columns + N * kGradRuns * kGradThreads - 1) / (N * kGradRuns * kGradThreads);
+                         const LogProbsGradArgs a     = {RowPlaces(logits), RowPlaces(out), tokens.base, lse, entropy, grad, gradEntropy, scale,
+                                                         logits.rows, logits.columns, DivBy((uint32_t)parts), tokens.dtype == NVCV_DATA_TYPE_S64};
+                         gradEntropy != nullptr ? LaunchLogProbsGrad<T, N, true>(a, stream) : LaunchLogProbsGrad<T, N, false>(a, stream);
+                     };
+                     logits.columns >= kRunOf<T> ? run(std::integral_constant<int, kRunOf<T>>()) : run(std::integral_constant<int, 1>());
+                 });
+    }
+};
+
+} // namespace
+} // namespace cvamd
+
+using namespace cvamd;
+
+extern "C"
+{
+CVCUDA_PUBLIC NVCVStatus cvcudaxLogProbsCreate(NVCVOperatorHandle *handle)
+{
+    return CreateOperator<LogProbs>(handle);
+}
+
+CVCUDA_PUBLIC NVCVStatus cvcudaxLogProbsSubmit(NVCVOperatorHandle handle, hipStream_t stream, NVCVTensorHandle logits,
+                                               NVCVTensorHandle tokens, NVCVTensorHandle out, NVCVTensorHandle entropy,
+                                               NVCVTensorHandle lse, NVCVTensorHandle topValues, NVCVTensorHandle topTokens,
+                                               float scale)
+{
+    return Protect(
+        [&]
+        {
+            (void)ToOperator<LogProbs>(handle);
+            LogProbs::submit(stream, logits, tokens, out, entropy, lse, topValues, topTokens, scale);
+        });
+}
+
+CVCUDA_PUBLIC NVCVStatus cvcudaxLogProbsGradSubmit(NVCVOperatorHandle handle, hipStream_t stream, NVCVTensorHandle logits,
+                                                   NVCVTensorHandle tokens, NVCVTensorHandle lse, NVCVTensorHandle entropy,
+                                                   NVCVTensorHandle gradOut, NVCVTensorHandle gradEntropy,
+                                                   NVCVTensorHandle gradLogits, float scale)
+{
+    return Protect(
+        [&]
+        {
+            (void)ToOperator<LogProbs>(handle);
+            LogProbs::submitGrad(stream, logits, tokens, lse, entropy, gradOut, gradEntropy, gradLogits, scale);
+        });
+}
+}

@@ -1,0 +1,299 @@
+// Rotary positions (formulas: cvcuda/Rotary.h). Bound by memory: each element is read and written once.
+//
+// A frequency is held as the fraction of a whole turn that one position makes, in units of 2^-64 turns. A position times it, modulo
+// 2^64, is the angle without its whole turns, exactly, however far the position; the eighth of a turn nearest to it is taken off as well,
+// and what is left, at most 1/8 turn, is small enough for the sine's and cosine's Taylor polynomials.
+#include "HeadOps.hpp"
+
+#include <cvcuda/Rotary.h>
+
+#include <algorithm>
+#include <cmath>
+
+namespace cvamd {
+
+namespace {
+
+constexpr int kMostPairs = 128, kRotaryThreads = 256;
+
+struct RotaryArgs
+{
+    const uint8_t *in;
+    uint8_t       *out;
+    const void    *positions;
+    int64_t        inToken, inHead, outToken, outHead;
+    double         step; // the logarithm to the base 2 of what a frequency is of the one before
+    double         factor, original, low, high;
+    float          magnitude;
+    int32_t        tokens, heads, dims, pairs;
+    int32_t        copied;        // elements of a row behind the pairs' (0 in place)
+    int32_t        headsOf;       // heads that a lane turns by the same angles
+    DivBy          units, groups; // of a head: runs of N pairs, then of N copied elements; of a token: headsOf heads each
+    bool           wide, inverse; // wide: positions of 64 bits
+};
+
+// The frequency of pair i (cvcuda/Rotary.h) in turns of 2^-64 each.
+__device__ __forceinline__ uint64_t TurnsOf(const RotaryArgs &a, int i)
+{
+    constexpr double kTurn = 0.15915494309189535; // 1 / (2 pi)
+    double           turns = exp2(a.step * (double)i) * kTurn;
+    if (a.original > 0)
+    {
+        const double g = fmin(fmax((a.original * turns - a.low) / (a.high - a.low), 0.), 1.);
+        turns *= g + (1. - g) / a.factor;
+    }
+    else
+    {
+        turns /= a.factor;
+    }
+    turns -= floor(turns);
+    return (uint64_t)(turns * 18446744073709549568.); // (the largest double below 2^64: a fraction next to 1 stays in range)
+}
+
+// Cosine and sine of an angle of `hi` * 2^-32 turns.
+__device__ __forceinline__ void CosSin(uint32_t hi, float &c, float &s)
+{
+    const uint32_t quarter = hi + 0x20000000u;                        // the nearest quarter turn in its upper two bits
+    const float    x       = (float)(int32_t)(hi - (quarter & 0xC0000000u)) * 1.46291807926715968e-9f; // 2 pi * 2^-32: at most pi / 4
+    const float    q       = x * x;
+    // terms up to x^9 and x^10: the next ones are below 2^-28
+    const float sine = __builtin_fmaf(
+        __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(2.7557319e-6f, q, -1.9841270e-4f), q, 8.3333333e-3f), q, -1.6666667e-1f), q * x, x);
+    const float cosine = __builtin_fmaf(
+        __builtin_fmaf(
+            __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(-2.7557319e-7f, q, 2.4801587e-5f), q, -1.3888889e-3f), q, 4.1666667e-2f), q, -0.5f),
+        q, 1.f);
+    const bool odd = (quarter & 0x40000000u) != 0;
+    c              = odd ? sine : cosine;
+    s              = odd ? cosine : sine;
+    // quarters 1 and 2: the cosine changes its sign, 2 and 3: the sine
+    c = __uint_as_float(__float_as_uint(c) ^ ((quarter + 0x40000000u) & 0x80000000u));
+    s = __uint_as_float(__float_as_uint(s) ^ (quarter & 0x80000000u));
+}
+
+// A lane turns N pairs, or copies up to N elements behind them, of `headsOf` heads of a token. Lanes that follow one another have a head's runs.
+template<class T, int N, bool INTERLEAVED>
+__global__ __launch_bounds__(kRotaryThreads) void RotaryKernel(const RotaryArgs a)
+{
+    __shared__ uint64_t s_turns[kMostPairs];
+    if (threadIdx.x < (uint32_t)a.pairs)
+    {
+        s_turns[threadIdx.x] = TurnsOf(a, (int)threadIdx.x);
+    }
+    __syncthreads();
+    const uint32_t item = blockIdx.x * kRotaryThreads + threadIdx.x, group = a.units.Quotient(item), unit = item - group * a.units.d;
+    const uint32_t token = a.groups.Quotient(group);
+    if (token >= (uint32_t)a.tokens)
+    {
+        return;
+    }
+    const int      first = (int)(group - token * a.groups.d) * a.headsOf, last = min(first + a.headsOf, a.heads);
+    const uint8_t *in  = a.in + (int64_t)token * a.inToken + (int64_t)first * a.inHead;
+    uint8_t       *out = a.out + (int64_t)token * a.outToken + (int64_t)first * a.outHead;
+    const int      pair = (int)unit * N;
+    if (pair >= a.pairs)
+    {
+        const int from = a.dims + (pair - a.pairs);
+        for (int h = first; h < last; ++h, in += a.inHead, out += a.outHead)
+        {
+            *reinterpret_cast<Run<T, N> *>(out + from * (int)sizeof(T)) = *reinterpret_cast<const Run<T, N> *>(in + from * (int)sizeof(T));
+        }
+        return;
+    }
+    const uint64_t position = a.wide ? static_cast<const uint64_t *>(a.positions)[token]
+                                     : (uint64_t)(int64_t)static_cast<const int32_t *>(a.positions)[token];
+    float c[N], s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+        CosSin((uint32_t)((position * s_turns[pair + i]) >> 32), c[i], s[i]);
+        c[i] *= a.magnitude;
+        s[i] *= a.inverse ? -a.magnitude : a.magnitude;
+    }
+    const int at = (INTERLEAVED ? 2 * pair : pair) * (int)sizeof(T), other = at + a.pairs * (int)sizeof(T);
+    for (int h = first; h < last; ++h, in += a.inHead, out += a.outHead)
+    {
+        float x[N], y[N];
+        if (INTERLEAVED)
+        {
+            const Run<T, 2 * N> r = *reinterpret_cast<const Run<T, 2 * N> *>(in + at);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                x[i] = (float)r.v[2 * i], y[i] = (float)r.v[2 * i + 1];
+            }
+        }
+        else
+        {
+            const Run<T, N> r = *reinterpret_cast<const Run<T, N> *>(in + at), t = *reinterpret_cast<const Run<T, N> *>(in + other);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                x[i] = (float)r.v[i], y[i] = (float)t.v[i];
+            }
+        }
+        Run<T, N> toX, toY;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            toX.v[i] = FromFloat<T>(x[i] * c[i] - y[i] * s[i]);
+            toY.v[i] = FromFloat<T>(x[i] * s[i] + y[i] * c[i]);
+        }
+        if (INTERLEAVED)
+        {
+            Run<T, 2 * N> r;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                r.v[2 * i] = toX.v[i], r.v[2 * i + 1] = toY.v[i];
+            }
+            *reinterpret_cast<Run<T, 2 * N> *>(out + at) = r;
+        }
+        else
+        {
+            *reinterpret_cast<Run<T, N> *>(out + at)    = toX;
+            *reinterpret_cast<Run<T, N> *>(out + other) = toY;
+        }
+    }
+}
+
+template<class T, int N>
+void Launch(const RotaryArgs &all, bool interleaved, hipStream_t stream)
+{
+    const int64_t ofToken = (int64_t)all.units.d * all.groups.d, most = std::max<int64_t>(1, INT32_MAX / ofToken);
+    for (int64_t first = 0; first < all.tokens; first += most)
+    {
+        RotaryArgs a = all;
+        a.tokens     = (int32_t)std::min(most, all.tokens - first);
+        a.in += first * a.inToken;
+        a.out += first * a.outToken;
+        a.positions           = static_cast<const uint8_t *>(a.positions) + first * (a.wide ? 8 : 4);
+        const uint32_t blocks = (uint32_t)((a.tokens * ofToken + kRotaryThreads - 1) / kRotaryThreads);
+        if (!interleaved)
+        {
+            RotaryKernel<T, N, false><<<blocks, kRotaryThreads, 0, stream>>>(a);
+        }
+        else if constexpr (2 * N <= kRunOf<T>)
+        {
+            RotaryKernel<T, N, true><<<blocks, kRotaryThreads, 0, stream>>>(a);
+        }
+        CheckLaunch("rotary");
+    }
+}
+
+template<class T>
+void Choose(RotaryArgs &a, bool interleaved, hipStream_t stream)
+{
+    // runs as wide as 16 bytes, of which a row's pairs and what is copied behind them have whole ones
+    int n = interleaved ? kRunOf<T> / 2 : kRunOf<T>;
+    while (a.pairs % n != 0 || a.copied % n != 0)
+    {
+        n /= 2;
+    }
+    const int units = a.pairs / n + a.copied / n;
+    a.headsOf       = 1;
+    a.units         = DivBy((uint32_t)units);
+    a.groups        = DivBy((uint32_t)DivUp(a.heads, a.headsOf));
+    if ((int64_t)a.units.d * a.groups.d > INT32_MAX)
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Input has too many elements in a token");
+    }
+    switch (n)
+    {
+    case 8:
+        if constexpr (kRunOf<T> >= 8)
+        {
+            Launch<T, 8>(a, interleaved, stream);
+        }
+        break;
+    case 4: Launch<T, 4>(a, interleaved, stream); break;
+    case 2: Launch<T, 2>(a, interleaved, stream); break;
+    default: Launch<T, 1>(a, interleaved, stream); break;
+    }
+}
+
+class Rotary final : public IOperator
+{
+public:
+    static void submit(hipStream_t stream, NVCVTensorHandle hin, NVCVTensorHandle hpositions, NVCVTensorHandle hout, const CVCUDAXRotary *args)
+    {
+        const HeadsView in = RequireHeads(hin, "Input", 0), out = RequireHeads(hout, "Output", 0);
+        RequireSameHeads(in, out, "Output");
+        const DenseView positions = RequireDense(hpositions, "Positions", NVCV_DATA_TYPE_NONE);
+        if (positions.dtype != NVCV_DATA_TYPE_S32 && positions.dtype != NVCV_DATA_TYPE_S64)
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Positions must hold S32 or S64 values");
+        }
+        if (positions.count != in.tokens)
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Positions must have one element for each of %d tokens, not %ld", in.tokens, (long)positions.count);
+        }
+        if (args == nullptr)
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Pointer to arguments must not be NULL");
+        }
+        if (args->dims < 2 || args->dims % 2 != 0 || args->dims > 2 * kMostPairs || args->dims > in.dims)
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Dims must be even, in [2, %d] and at most a head's %d, not %d", 2 * kMostPairs, in.dims, args->dims);
+        }
+        auto positive = [](double v, const char *what)
+        {
+            if (!(v > 0) || !std::isfinite(v))
+            {
+                throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must be finite and positive, not %g", what, v);
+            }
+        };
+        positive(args->base, "Base");
+        positive(args->factor, "Factor");
+        positive(args->magnitude, "Magnitude");
+        positive((float)args->magnitude, "Magnitude");
+        if (!(args->original >= 0) || !std::isfinite(args->original))
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Original must be finite and not negative, not %g", args->original);
+        }
+        if (args->original > 0 && (!(args->low >= 0) || !(args->high > args->low) || !std::isfinite(args->high)))
+        {
+            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Low and high must be finite, 0 <= low < high, not %g and %g", args->low, args->high);
+        }
+        if (in.tokens == 0 || in.heads == 0)
+        {
+            return;
+        }
+        const bool inPlace = in.base == out.base && in.tokenStride == out.tokenStride && in.headStride == out.headStride;
+        RotaryArgs a = {in.base, out.base, positions.base, in.tokenStride, in.headStride, out.tokenStride, out.headStride,
+                        std::log2(args->base) * -2. / args->dims, args->factor, args->original, args->low, args->high, (float)args->magnitude,
+                        in.tokens, in.heads, args->dims, args->dims / 2, inPlace ? 0 : in.dims - args->dims, 1, DivBy(1), DivBy(1),
+                        positions.dtype == NVCV_DATA_TYPE_S64, args->inverse != 0};
+        const bool interleaved = args->interleaved != 0;
+        switch (in.elem)
+        {
+        case kRowF32: Choose<float>(a, interleaved, stream); break;
+        case kRowF16: Choose<Half>(a, interleaved, stream); break;
+        default: Choose<Bf16>(a, interleaved, stream); break;
+        }
+    }
+};
+
+} // namespace
+} // namespace cvamd
+
+using namespace cvamd;
+
+extern "C"
+{
+CVCUDA_PUBLIC NVCVStatus cvcudaxRotaryCreate(NVCVOperatorHandle *handle)
+{
+    return CreateOperator<Rotary>(handle);
+}
+
+CVCUDA_PUBLIC NVCVStatus cvcudaxRotarySubmit(NVCVOperatorHandle handle, hipStream_t stream, NVCVTensorHandle in,
+                                             NVCVTensorHandle positions, NVCVTensorHandle out, const CVCUDAXRotary *args)
+{
+    return Protect(
+        [&]
+        {
+            (void)ToOperator<Rotary>(handle);
+            Rotary::submit(stream, in, positions, out, args);
+        });
+}
+}

@@ -10,8 +10,10 @@
 
 #include <ATen/ATen.h>
 #include <cvcuda/AdamW.h>
+#include <cvcuda/Attention.h>
 #include <cvcuda/Embedding.h>
 #include <cvcuda/LayerNorm.h>
+#include <cvcuda/LogProbs.h>
 #include <cvcuda/OpConvertTo.h>
 #include <cvcuda/OpCropFlipNormalizeReformat.h>
 #include <cvcuda/OpCvtColor.h>
@@ -21,6 +23,7 @@
 #include <cvcuda/OpResizeCropConvertReformat.h>
 #include <cvcuda/OpWarpAffine.h>
 #include <cvcuda/OpWarpPerspective.h>
+#include <cvcuda/Rotary.h>
 #include <nvcv/Tensor.h>
 #include <structmember.h>
 #include <hip/hip_runtime_api.h>
@@ -226,10 +229,10 @@ struct Call
 {
     int                kind;
     NVCVOperatorHandle op;
-    void              *h[9];
+    void              *h[13];
     bool               batch, flag;
     int                i[6];
-    double             d[5];
+    double             d[6];
     float              m[9], bv[4];
     long long          whole;
     std::vector<void *> lists[7];
@@ -335,6 +338,21 @@ struct Call
                 && Real(a[10], d[1]) && Real(a[11], d[2]) && Real(a[12], d[3]) && Real(a[13], d[4]);
         case 15: // AdamWUnpack
             return n == 3 && Lists(api, a, 3, 0);
+        case 16: // Rotary
+            flag = n == 12 && a[11] == Py_True;
+            i[1] = n == 12 && a[10] == Py_True;
+            return n == 12 && Tensors(api, a, 3, 0) && Int(a[3], i[0]) && Real(a[4], d[0]) && Real(a[5], d[1]) && Real(a[6], d[2]) && Real(a[7], d[3])
+                && Real(a[8], d[4]) && Real(a[9], d[5]) && PyBool_Check(a[10]) && PyBool_Check(a[11]);
+        case 17: // Attention
+            flag = n == 11 && a[10] == Py_True;
+            return n == 11 && Tensors(api, a, 9, 0b110110000) && Real(a[9], d[0]) && PyBool_Check(a[10]);
+        case 18: // AttentionGrad
+            flag = n == 15 && a[14] == Py_True;
+            return n == 15 && Tensors(api, a, 13, 0b1000110000000) && Real(a[13], d[0]) && PyBool_Check(a[14]);
+        case 19: // LogProbs
+            return n == 8 && Tensors(api, a, 7, 0b1111000) && Real(a[7], d[0]);
+        case 20: // LogProbsGrad
+            return n == 8 && Tensors(api, a, 7, 0b0101000) && Real(a[7], d[0]);
         default:
             return false;
         }
@@ -400,6 +418,21 @@ struct Call
         }
         case 15:
             return cvcudaxAdamWUnpackSubmit(op, nullptr, (int32_t)lists[0].size(), List(0), List(1), List(2));
+        case 16:
+        {
+            const CVCUDAXRotary args = {d[0], d[1], d[2], d[3], d[4], d[5], i[0], (int8_t)i[1], flag};
+            return cvcudaxRotarySubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), &args);
+        }
+        case 17:
+            return cvcudaxAttentionSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), As<T>(3), As<T>(4), As<T>(5), As<T>(6), As<T>(7), As<T>(8),
+                                          (float)d[0], flag);
+        case 18:
+            return cvcudaxAttentionGradSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), As<T>(3), As<T>(4), As<T>(5), As<T>(6), As<T>(7),
+                                              As<T>(8), As<T>(9), As<T>(10), As<T>(11), As<T>(12), (float)d[0], flag);
+        case 19:
+            return cvcudaxLogProbsSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), As<T>(3), As<T>(4), As<T>(5), As<T>(6), (float)d[0]);
+        case 20:
+            return cvcudaxLogProbsGradSubmit(op, nullptr, As<T>(0), As<T>(1), As<T>(2), As<T>(3), As<T>(4), As<T>(5), As<T>(6), (float)d[0]);
         default:
         {
             const float4 c = {bv[0], bv[1], bv[2], bv[3]};

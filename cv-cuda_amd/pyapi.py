@@ -8,7 +8,8 @@ against the reference's `cvcuda` / `nvcv` modules for these operators runs with
     import cvcuda_amd.pyapi as cvcuda
     nvcv = cvcuda
 
-layer_norm, embedding, their gradients and adamw are additions of this module for models that train on its batches.
+layer_norm, embedding, rotary, attention, log_probs, their gradients and adamw are additions of this module for models that
+train on its batches or answer from them.
 
 Every function forwards to the C ABI through the operator classes of the package; `stream=None` means the current
 stream (`Stream.current`: the innermost `with stream:`, else the default stream). Containers keep the bindings'
@@ -23,14 +24,15 @@ import functools
 import math
 import re
 import threading
+import typing
 
 import numpy as np
 import torch
 
 from . import _constants as K
-from . import (AdamW, AdamWUnpack, CenterCrop, ConvertTo, CropFlipNormalizeReformat, CustomCrop, CvtColor, Embedding, EmbeddingGrad,
-               Error, Flip, LayerNorm, LayerNormGrad, Normalize, Reformat, Resize, ResizeCropConvertReformat, WarpAffine,
-               WarpPerspective)
+from . import (AdamW, AdamWUnpack, Attention, AttentionGrad, CenterCrop, ConvertTo, CropFlipNormalizeReformat, CustomCrop, CvtColor,
+               Embedding, EmbeddingGrad, Error, Flip, LayerNorm, LayerNormGrad, LogProbs, LogProbsGrad, Normalize, Reformat, Resize,
+               ResizeCropConvertReformat, Rotary, WarpAffine, WarpPerspective)
 from . import Image as _Image
 from . import ImageBatchVarShape as _ImageBatchVarShape
 from . import Tensor as _Tensor
@@ -1154,7 +1156,7 @@ def _workspace(workspace, size, stream):
     if size <= _UNTOUCHED_BYTES:
         return _untouched_workspace()
     if _capturing(stream):
-        raise Error(4, "a captured gradient needs workspace=, a tensor of %d bytes that lives as long as the graph" % size)  # INVALID_OPERATION
+        raise Error(4, "a captured call of this kind needs workspace=, a tensor of %d bytes that lives as long as the graph" % size)  # INVALID_OPERATION
     return _result((size,), np.uint8, None, stream)
 
 
@@ -1263,3 +1265,115 @@ def adamw_unpack_into(dst, codes, scales, *, stream=None):
     codes, scales, made = list(codes), list(scales), list(dst)
     _run(stream, codes + scales, made, _op(AdamWUnpack), codes, scales, made)
     return dst
+
+
+class RotaryScaling(typing.NamedTuple):
+    """How rotary positions are scaled for contexts of `factor` times the `original` length: pairs that turn at least `high` times
+    over it are left as they are, those of at most `low` turns are slowed down by `factor`, those between by a part of it; with
+    original=0 all are. Results are multiplied with `magnitude`."""
+    factor: float = 1.0
+    original: float = 0.0
+    low: float = 1.0
+    high: float = 4.0
+    magnitude: float = 1.0
+
+
+_NOT_SCALED = RotaryScaling()
+
+
+def rotary_into(dst, src, positions, dims=None, *, base=10000.0, interleaved=False, scaling=None, inverse=False, stream=None):
+    """Turns the first `dims` elements (none: all) of the rows of `src`, [tokens, heads, elements] of F32, F16 or BF16, by the tokens'
+    positions (int32 or int64): in pairs of neighbours (`interleaved`) or of the two halves, of frequencies base^(-2 i / dims), changed by
+    `scaling`, a RotaryScaling. `inverse` turns back: the gradient of `src` from that of `dst`. `dst` may be `src`."""
+    factor, original, low, high, magnitude = _NOT_SCALED if scaling is None else scaling
+    _run(stream, [src, positions], [dst], _op(Rotary), src, positions, dst, int(src.shape[-1] if dims is None else dims), float(base),
+         float(factor), float(original), float(low), float(high), float(magnitude), bool(interleaved), bool(inverse))
+    return dst
+
+
+def rotary(src, positions, dims=None, *, base=10000.0, interleaved=False, scaling=None, inverse=False, stream=None):
+    return rotary_into(_like(src, stream), src, positions, dims, base=base, interleaved=interleaved, scaling=scaling, inverse=inverse,
+                       stream=stream)
+
+
+_attention_workspace = functools.lru_cache(256)(Attention.workspace)
+_attention_grad_workspace = functools.lru_cache(256)(AttentionGrad.workspace)
+
+
+def _attention_sizes(q, k, offsets):
+    """(rows, keys, sequences, heads, key heads, elements); what is wrong with them is found by the call."""
+    if len(q.shape) != 3 or len(k.shape) != 3:
+        raise Error(2, "queries, keys and values have three dimensions (tokens, heads, elements)")  # INVALID_ARGUMENT
+    return q.shape[0], k.shape[0], math.prod(offsets.shape) - 1, q.shape[1], k.shape[1], q.shape[2]
+
+
+def _scale_of(scale, q):
+    return q.shape[-1] ** -0.5 if scale is None else float(scale)
+
+
+def attention_into(dst, q, k, v, offsets, *, key_offsets=None, key_lengths=None, causal=True, scale=None, lse=None, workspace=None,
+                   stream=None):
+    """Attention of packed sequences: `q` and `dst` [rows, heads, elements], `k` and `v` [keys, key heads, elements], F16 or BF16,
+    parts of one tensor if need be. `offsets`: int32, where each sequence begins, and the end of the last; `key_offsets`: the same for
+    the keys where they are others than the rows', and `key_lengths` how many of its keys' places each sequence has filled (none: all). The last row of
+    a sequence sees all its keys, with `causal` each row before it one less. `scale`: of the scores (none: 1 / sqrt(elements)). `lse`: an
+    F32 tensor [heads, rows] that receives what the gradient needs. Rows of no sequence are left as they are. `workspace`: a uint8
+    tensor of Attention.workspace(rows, keys, sequences, heads, key heads, elements) bytes, or None for one of this call's own, which
+    a call that is captured cannot have (unless it needs none)."""
+    workspace = _workspace(workspace, _attention_workspace(*_attention_sizes(q, k, offsets)), stream)
+    _run(stream, _given(q, k, v, offsets, key_offsets, key_lengths), _given(dst, lse, workspace), _op(Attention), q, k, v, offsets, key_offsets,
+         key_lengths, dst, lse, workspace, _scale_of(scale, q), bool(causal))
+    return dst
+
+
+def attention(q, k, v, offsets, *, key_offsets=None, key_lengths=None, causal=True, scale=None, lse=None, workspace=None, stream=None):
+    """As attention_into; rows of no sequence have no defined values."""
+    workspace = _workspace(workspace, _attention_workspace(*_attention_sizes(q, k, offsets)), stream)  # (before anything is made)
+    return attention_into(_like(q, stream), q, k, v, offsets, key_offsets=key_offsets, key_lengths=key_lengths, causal=causal, scale=scale,
+                          lse=lse, workspace=workspace, stream=stream)
+
+
+def attention_grad_into(grad_q, grad_k, grad_v, grad, q, k, v, out, lse, offsets, *, key_offsets=None, key_lengths=None, causal=True,
+                        scale=None, workspace=None, stream=None):
+    """The gradients of attention from `grad`, that of its result `out`, with the `lse` that the forward call gave. Rows of no sequence,
+    and places of keys that none has filled, are left as they are. `workspace`: as for attention_into, by AttentionGrad.workspace."""
+    workspace = _workspace(workspace, _attention_grad_workspace(*_attention_sizes(q, k, offsets)), stream)
+    _run(stream, _given(grad, q, k, v, out, lse, offsets, key_offsets, key_lengths), _given(grad_q, grad_k, grad_v, workspace), _op(AttentionGrad),
+         grad, q, k, v, out, lse, offsets, key_offsets, key_lengths, grad_q, grad_k, grad_v, workspace, _scale_of(scale, q), bool(causal))
+    return grad_q, grad_k, grad_v
+
+
+def attention_grad(grad, q, k, v, out, lse, offsets, *, key_offsets=None, key_lengths=None, causal=True, scale=None, workspace=None,
+                   stream=None):
+    """(gradient of q, of k, of v); those of rows of no sequence, and of places that none has filled, have no defined values."""
+    workspace = _workspace(workspace, _attention_grad_workspace(*_attention_sizes(q, k, offsets)), stream)  # (before anything is made)
+    return attention_grad_into(_like(q, stream), _like(k, stream), _like(v, stream), grad, q, k, v, out, lse, offsets, key_offsets=key_offsets,
+                               key_lengths=key_lengths, causal=causal, scale=scale, workspace=workspace, stream=stream)
+
+
+def log_probs_into(dst, logits, tokens, scale=1.0, *, entropy=None, lse=None, top_values=None, top_tokens=None, stream=None):
+    """The log probabilities of `tokens` (int32 or int64) by the softmax of scale * logits over the last dimension (F32, F16 or BF16); 0
+    for tokens that it does not have (padding). `entropy`, `lse`: F32 tensors of an element per row that receive the entropy and the logarithm
+    of the sum of exponentials; `top_tokens` (int32) and `top_values` (F32), both of K more elements per row: the K most likely tokens, the
+    first of equal ones first, and their log probabilities."""
+    _run(stream, [logits, tokens], _given(dst, entropy, lse, top_values, top_tokens), _op(LogProbs), logits, tokens, dst, entropy, lse, top_values,
+         top_tokens, float(scale))
+    return dst
+
+
+def log_probs(logits, tokens, scale=1.0, *, entropy=None, lse=None, top_values=None, top_tokens=None, stream=None):
+    """As log_probs_into, in a new tensor of the tokens' shape."""
+    dst = _result(tuple(tokens.shape), np.dtype(np.float32), None, stream)
+    return log_probs_into(dst, logits, tokens, scale, entropy=entropy, lse=lse, top_values=top_values, top_tokens=top_tokens, stream=stream)
+
+
+def log_probs_grad_into(grad_logits, logits, tokens, lse, grad, scale=1.0, *, entropy=None, grad_entropy=None, stream=None):
+    """The gradient of the logits from `grad`, that of log_probs' result, and `grad_entropy`, that of `entropy` (none: 0), with the `lse` and
+    `entropy` that the forward call gave. `grad_logits` may be `logits`."""
+    _run(stream, _given(logits, tokens, lse, entropy, grad, grad_entropy), [grad_logits], _op(LogProbsGrad), logits, tokens, lse, entropy, grad,
+         grad_entropy, grad_logits, float(scale))
+    return grad_logits
+
+
+def log_probs_grad(logits, tokens, lse, grad, scale=1.0, *, entropy=None, grad_entropy=None, stream=None):
+    return log_probs_grad_into(_like(logits, stream), logits, tokens, lse, grad, scale, entropy=entropy, grad_entropy=grad_entropy, stream=stream)
