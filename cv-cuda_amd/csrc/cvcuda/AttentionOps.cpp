@@ -1,4 +1,4 @@
-#include "AttentionTiles.hpp"
+#include "AttentionOps.hpp"
 
 #include <cmath>
 
@@ -24,6 +24,10 @@ HeadsView TakeHeads(NVCVTensorHandle h, const char *what)
     if (v.elem == kRowF32)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must hold F16 or BF16 values", what);
+    }
+    if (v.tokenStride > kMostStride || v.headStride * v.heads > kMostStride)
+    {
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must have tokens, and all heads, within %ld bytes of one another", what, (long)kMostStride);
     }
     return v;
 }

@@ -12,7 +12,7 @@
 #ifndef CVCUDA_AMD_ATTENTIONTILES_HPP
 #define CVCUDA_AMD_ATTENTIONTILES_HPP
 
-#include "HeadOps.hpp"
+#include "AttentionOps.hpp"
 
 #include <type_traits>
 
@@ -90,12 +90,11 @@ __device__ __forceinline__ Vec8<T> ColumnsOperand(const uint8_t *tile, uint32_t 
     const uint32_t lane  = threadIdx.x & 63;
     const uint32_t row   = firstRow + 4 * (lane >> 5) + ((lane & 15) >> 2);
     const uint32_t unit  = 4 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const uint32_t place = (uint32_t)reinterpret_cast<uintptr_t>(tile) + TileAt<DP>(row, unit) + 8 * (lane & 1); // (Swap(row + 8) is Swap(row))
+    const uint8_t *place = tile + TileAt<DP>(row, unit) + 8 * (lane & 1); // (Swap(row + 8) is Swap(row))
     struct
     {
         Vec4s low, high;
-    } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Place *>(place)),
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Place *>(place + 8 * DP * 2))};
+    } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Place *)(place)), __builtin_amdgcn_ds_read_tr16_b64_v4i16((Place *)(place + 8 * DP * 2))};
     return __builtin_bit_cast(Vec8<T>, both);
 }
 
@@ -161,19 +160,71 @@ struct TileLoad
     }
 };
 
-// A row of a matrix as the right operand's column: element 16 * step + 8 * (l / 32) to + 7 of it; zeros where `there` is false and behind `dims`.
+// ROWS rows from memory to a tile in LDS, without a stop in registers, by WAVES waves. Each instruction moves 64 units to 64 places that
+// follow one another: the lanes' addresses make the exchange of units. The buffer ends behind the last row, and what lies behind
+// a buffer's end reads as zeros; lanes of units behind `dims` read there too.
+template<int ROWS, int DP, int WAVES>
+struct TileCopy
+{
+    static constexpr int kUnits = DP / 8, kOfOne = 64 / kUnits, kCount = ROWS / (kOfOne * WAVES);
+    static_assert(ROWS % (kOfOne * WAVES) == 0, "whole instructions");
+    static constexpr uint32_t kNowhere = 0x80000000u; // (tiles are smaller: kMostStride)
+
+    // The lane's row of the tile and its unit in the wave's copy i.
+    __device__ __forceinline__ static int rowOf(uint32_t wave, int i)
+    {
+        return (int)((uint32_t)(i * WAVES) + wave) * kOfOne + (int)((threadIdx.x & 63) / kUnits);
+    }
+
+    __device__ __forceinline__ static uint32_t unitOf(int row)
+    {
+        return ((threadIdx.x & 63) % kUnits) ^ Swap((uint32_t)row);
+    }
+
+    __device__ __forceinline__ static void copy(uint32_t wave, int i, uint8_t *tile, __amdgpu_buffer_rsrc_t from, uint32_t at, uint32_t atAll)
+    {
+        using Place = __attribute__((address_space(3))) void;
+        uint8_t *to = tile + ((uint32_t)(i * WAVES) + wave) * 1024;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Place *)to, 16, (int)at, (int)atAll, 0, 0);
+    }
+
+    // Rows `stride` apart from `base` on, of which there are `count`, one at least.
+    __device__ __forceinline__ static void rows(uint32_t wave, uint8_t *tile, const uint8_t *base, uint32_t stride, int count, int dims)
+    {
+        const uint32_t bytes = (uint32_t)(min(count, ROWS) - 1) * stride + (uint32_t)dims * 2;
+        const auto     from  = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, (int)bytes, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+        {
+            const int      row  = rowOf(wave, i) - i * WAVES * kOfOne;
+            const uint32_t unit = unitOf(rowOf(wave, i));
+            copy(wave, i, tile, from, (int)unit * 8 < dims ? (uint32_t)row * stride + unit * 16 : kNowhere, (uint32_t)(i * WAVES * kOfOne) * stride);
+        }
+    }
+};
+
+// All waves' copies to LDS have arrived, and their reads of it are done. (A barrier alone waits for no copy.)
+__device__ __forceinline__ void CopiesAndBarrier()
+{
+    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
+    __syncthreads();
+}
+
+// A row of a matrix as the right operand's column: elements 16 * step + 8 * (l / 32) to + 7 of it, zeros behind `dims`. Loads stand
+// under no condition.
 template<class T, int DP>
-__device__ __forceinline__ void LoadColumn(Vec8<T> (&to)[DP / 16], const uint8_t *row, bool there, int dims)
+__device__ __forceinline__ void LoadColumn(Vec8<T> (&to)[DP / 16], const uint8_t *row, int dims)
 {
     const int first = (int)((threadIdx.x & 63) >> 5) * 8;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
     {
-        to[s] = {};
-        if (there && 16 * s + first < dims)
-        {
-            to[s] = *reinterpret_cast<const Vec8<T> *>(row + (16 * s + first) * 2);
-        }
+        to[s] = *reinterpret_cast<const Vec8<T> *>(row + min(16 * s + first, dims - 8) * 2);
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+    {
+        to[s] = 16 * s + first < dims ? to[s] : Vec8<T>{};
     }
 }
 
@@ -215,33 +266,6 @@ __device__ __forceinline__ void StoreColumn(const Acc16 (&acc)[DP / 32], float f
 }
 
 // ---- sequences -----------------------------------------------------------------------------------------------------
-struct AttentionSequences
-{
-    const int32_t *offsets, *keyOffsets, *keyLengths; // the latter two: nullptr as in cvcuda/Attention.h
-    int32_t        count, rows, keys;                 // sequences; tokens of q and of k
-
-    __device__ __forceinline__ int firstRow(int b) const
-    {
-        return min(max(offsets[b], 0), rows);
-    }
-
-    __device__ __forceinline__ int rowsOf(int b, int first) const
-    {
-        return max(min(max(offsets[b + 1], 0), rows) - first, 0);
-    }
-
-    __device__ __forceinline__ int firstKey(int b) const
-    {
-        return min(max((keyOffsets != nullptr ? keyOffsets : offsets)[b], 0), keys);
-    }
-
-    __device__ __forceinline__ int keysOf(int b, int first) const
-    {
-        const int n = max(min(max((keyOffsets != nullptr ? keyOffsets : offsets)[b + 1], 0), keys) - first, 0);
-        return keyLengths != nullptr ? min(max(keyLengths[b], 0), n) : n;
-    }
-};
-
 // A sequence and one of its tiles.
 struct SequenceTile
 {
@@ -325,28 +349,6 @@ struct AttentionRow
         there = r < all;
     }
 };
-
-// ---- the operator ------------------------------------------------------------------------------------------------
-class AttentionOperator final : public IOperator
-{
-};
-
-// ---- what the host has checked -----------------------------------------------------------------------------------
-struct AttentionInputs
-{
-    HeadsView          q, k, v;
-    AttentionSequences sequences;
-    float             *lse;
-};
-
-// Shared by the forward call and the gradient. Throws INVALID_ARGUMENT.
-AttentionInputs TakeAttention(NVCVTensorHandle q, NVCVTensorHandle k, NVCVTensorHandle v, NVCVTensorHandle offsets, NVCVTensorHandle keyOffsets,
-                              NVCVTensorHandle keyLengths, NVCVTensorHandle lse, bool lseOptional, float scale);
-
-// A tensor like `as`, aligned as attention's tensors are.
-HeadsView TakeHeadsLike(NVCVTensorHandle h, const HeadsView &as, const char *what);
-
-void RequireAttentionSizes(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t keyHeads, int64_t dims);
 
 } // namespace cvamd
 

@@ -134,9 +134,10 @@ __device__ __forceinline__ float LseOf(float top, float sum)
 constexpr int kManyRows = 128, kManyKeys = 64, kManyThreads = 256;
 
 template<class T, int DP>
-__global__ __launch_bounds__(kManyThreads) void AttentionKernel(const AttentionArgs a)
+__global__ __launch_bounds__(kManyThreads, 2) void AttentionKernel(const AttentionArgs a)
 {
-    __shared__ __attribute__((aligned(256))) uint8_t s_k[2][kManyKeys * DP * 2], s_v[2][kManyKeys * DP * 2];
+    __shared__ __attribute__((aligned(256))) uint8_t s_k0[kManyKeys * DP * 2], s_k1[kManyKeys * DP * 2];
+    __shared__ __attribute__((aligned(256))) uint8_t s_v0[kManyKeys * DP * 2], s_v1[kManyKeys * DP * 2];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
     const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
     // (with `causal` a sequence's last tiles have the most keys: they begin first)
@@ -145,7 +146,8 @@ __global__ __launch_bounds__(kManyThreads) void AttentionKernel(const AttentionA
     {
         return;
     }
-    const int  first = s.tile * kManyRows, ownFirst = first + (int)WaveOfGroup() * 32, all = s.rows * a.rows.size();
+    const uint32_t wave = WaveOfGroup();
+    const int  first = s.tile * kManyRows, ownFirst = first + (int)wave * 32, all = s.rows * a.rows.size();
     const AttentionRow row(a.rows, a.causal, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
     // keys of the tile, of the wave and those that all of the wave's rows see; this workgroup's part of the tile's
     auto       limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
@@ -155,35 +157,42 @@ __global__ __launch_bounds__(kManyThreads) void AttentionKernel(const AttentionA
     const int  from = (int)((int64_t)parts * blockIdx.y / a.splits), to = (int)((int64_t)parts * (blockIdx.y + 1) / a.splits);
     const uint8_t *k = a.k + s.firstKey * a.kToken + keyHead * a.kHead, *v = a.v + s.firstKey * a.vToken + keyHead * a.vHead;
 
-    Vec8<T> q[DP / 16];
-    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, row.there, a.dims);
-    Running<T, DP>                         run;
-    TileLoad<kManyKeys, DP, kManyThreads> nextK, nextV;
-    auto load = [&](int part)
+    using Copy = TileCopy<kManyKeys, DP, kManyThreads / 64>;
+    auto load  = [&](int part, uint8_t *toK, uint8_t *toV)
     {
         const int key = part * kManyKeys;
-        nextK.get(threadIdx.x, k + key * a.kToken, a.kToken, s.keys - key, a.dims);
-        nextV.get(threadIdx.x, v + key * a.vToken, a.vToken, s.keys - key, a.dims);
+        Copy::rows(wave, toK, k + key * a.kToken, (uint32_t)a.kToken, s.keys - key, a.dims);
+        Copy::rows(wave, toV, v + key * a.vToken, (uint32_t)a.vToken, s.keys - key, a.dims);
     };
     if (from < to)
     {
-        load(from);
+        load(from, s_k0, s_v0);
     }
-    for (int part = from; part < to; ++part)
+    Vec8<T> q[DP / 16];
+    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
+    Running<T, DP> run;
+    auto           take = [&](int part, const uint8_t *fromK, const uint8_t *fromV, uint8_t *nextK, uint8_t *nextV)
     {
-        const int at = (part - from) & 1, key = part * kManyKeys;
-        nextK.put(threadIdx.x, s_k[at]);
-        nextV.put(threadIdx.x, s_v[at]);
-        __syncthreads(); // (all have done the part before, so that the one before that may be written over)
+        const int key = part * kManyKeys;
+        CopiesAndBarrier(); // (all have done the part before: its place may be written over)
         if (part + 1 < to)
         {
-            load(part + 1);
+            load(part + 1, nextK, nextV);
         }
         if (key < waveKeys)
         {
             Acc16 scores[kManyKeys / 32];
-            Scores<T, DP>(scores, s_k[at], q, key, row.limit, key + kManyKeys > seenKeys);
-            run.template add<kManyKeys>(scores, s_v[at], a.scale);
+            Scores<T, DP>(scores, fromK, q, key, row.limit, key + kManyKeys > seenKeys);
+            run.template add<kManyKeys>(scores, fromV, a.scale);
+        }
+    };
+    // (by turns of their own, so that the compiler sees that what is read is not what is on its way)
+    for (int part = from; part < to; part += 2)
+    {
+        take(part, s_k0, s_v0, s_k1, s_v1);
+        if (part + 1 < to)
+        {
+            take(part + 1, s_k1, s_v1, s_k0, s_v0);
         }
     }
     const float   sum = BothSum(run.sum), factor = sum == 0 ? 0.f : 1.f / sum;
@@ -227,7 +236,7 @@ __global__ __launch_bounds__(kManyThreads) void AttentionKernel(const AttentionA
 constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4, kFewThreads = 64 * kFewWaves;
 
 template<class T, int DP>
-__global__ __launch_bounds__(kFewThreads) void AttentionFewKernel(const AttentionArgs a)
+__global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const AttentionArgs a)
 {
     // each wave's keys and values, later its weighted values in 32 bits
     __shared__ __attribute__((aligned(256))) uint8_t s_tile[kFewWaves][2 * kFewKeys * DP * 2];
@@ -261,7 +270,7 @@ __global__ __launch_bounds__(kFewThreads) void AttentionFewKernel(const Attentio
         load(from);
     }
     Vec8<T> q[DP / 16];
-    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, row.there, a.dims);
+    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
     Running<T, DP> run;
     for (int part = from; part < to; part += kFewWaves)
     {

@@ -183,7 +183,7 @@ __device__ __forceinline__ float ShareBase(float lse, bool there)
 constexpr int kGradRows = 128, kGradKeys = 64, kGradThreads = 256;
 
 template<class T, int DP>
-__global__ __launch_bounds__(kGradThreads) void AttentionGradQKernel(const AttentionGradArgs a)
+__global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const AttentionGradArgs a)
 {
     __shared__ __attribute__((aligned(256))) uint8_t s_k[2][kGradKeys * DP * 2], s_v[2][kGradKeys * DP * 2];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
@@ -212,8 +212,8 @@ __global__ __launch_bounds__(kGradThreads) void AttentionGradQKernel(const Atten
         load(0);
     }
     Vec8<T> q[DP / 16], grad[DP / 16];
-    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, row.there, a.dims);
-    LoadColumn<T, DP>(grad, a.grad + row.token * a.gradToken + row.head * a.gradHead, row.there, a.dims);
+    LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
+    LoadColumn<T, DP>(grad, a.grad + row.token * a.gradToken + row.head * a.gradHead, a.dims);
     const float factor = GradFactor<T>(a), base = ShareBase<T>(a.lse[a.number(row)], row.there);
     const float scale = a.scale * kLog2E, of = factor * __builtin_amdgcn_exp2f(-kShareShift<T>), delta = a.delta[a.number(row)] * of;
     Acc16       sum[DP / 32] = {};
@@ -320,8 +320,9 @@ __global__ __launch_bounds__(kGradThreads) void AttentionGradKVKernel(const Atte
         load(begin);
     }
     Vec8<T> k[DP / 16], v[DP / 16];
-    LoadColumn<T, DP>(k, a.k + (s.firstKey + key) * a.kToken + keyHead * a.kHead, there, a.dims);
-    LoadColumn<T, DP>(v, a.v + (s.firstKey + key) * a.vToken + keyHead * a.vHead, there, a.dims);
+    const int own = s.firstKey + min(key, s.keys - 1); // (columns behind the last key are made of it, and not stored)
+    LoadColumn<T, DP>(k, a.k + own * a.kToken + keyHead * a.kHead, a.dims);
+    LoadColumn<T, DP>(v, a.v + own * a.vToken + keyHead * a.vHead, a.dims);
     const float scale = a.scale * kLog2E;
     Acc16       sumK[DP / 32] = {}, sumV[DP / 32] = {};
     for (int at = begin, turn = 0; at < all; at += kOfRows, turn ^= 1)
