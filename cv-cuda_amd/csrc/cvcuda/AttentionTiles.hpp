@@ -60,17 +60,25 @@ __device__ __forceinline__ float BothSum(float v)
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Keeps the compiler from making what stands in a branch in every case, and choosing afterwards.
+__device__ __forceinline__ void KeepBranch()
+{
+    asm volatile("");
+}
+
 // ---- tiles in LDS ------------------------------------------------------------------------------------------------
-// Row r of DP elements (64 or 128), its unit u of 16 bytes at place u ^ Swap(r).
+// Row r of DP elements (64 or 128), its unit u of 16 bytes at place u ^ Swap(r). Of eleven exchanges that were tried these are the ones
+// with which a wave's read of rows takes 7.0 clocks and a transposed one 5.5 (without any 32 and 5.5, 64 and 8.1).
+template<int DP>
 __device__ __forceinline__ uint32_t Swap(uint32_t row)
 {
-    return ((row & 3) << 1) | ((row >> 2) & 1);
+    return DP == 64 ? (row >> 1) & 7 : ((row & 7) << 1) | ((row >> 3) & 1);
 }
 
 template<int DP>
 __device__ __forceinline__ uint32_t TileAt(uint32_t row, uint32_t unit)
 {
-    return row * (DP * 2) + ((unit ^ Swap(row)) << 4);
+    return row * (DP * 2) + ((unit ^ Swap<DP>(row)) << 4);
 }
 
 // Rows of a matrix as the instruction's left operand: lane l has row l % 32, elements 16 * step + 8 * (l / 32) to + 7.
@@ -90,11 +98,11 @@ __device__ __forceinline__ Vec8<T> ColumnsOperand(const uint8_t *tile, uint32_t 
     const uint32_t lane  = threadIdx.x & 63;
     const uint32_t row   = firstRow + 4 * (lane >> 5) + ((lane & 15) >> 2);
     const uint32_t unit  = 4 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const uint8_t *place = tile + TileAt<DP>(row, unit) + 8 * (lane & 1); // (Swap(row + 8) is Swap(row))
+    const uint8_t *first = tile + TileAt<DP>(row, unit) + 8 * (lane & 1), *second = tile + TileAt<DP>(row + 8, unit) + 8 * (lane & 1);
     struct
     {
         Vec4s low, high;
-    } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Place *)(place)), __builtin_amdgcn_ds_read_tr16_b64_v4i16((Place *)(place + 8 * DP * 2))};
+    } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Place *)first), __builtin_amdgcn_ds_read_tr16_b64_v4i16((Place *)second)};
     return __builtin_bit_cast(Vec8<T>, both);
 }
 
@@ -178,7 +186,7 @@ struct TileCopy
 
     __device__ __forceinline__ static uint32_t unitOf(int row)
     {
-        return ((threadIdx.x & 63) % kUnits) ^ Swap((uint32_t)row);
+        return ((threadIdx.x & 63) % kUnits) ^ Swap<DP>((uint32_t)row);
     }
 
     __device__ __forceinline__ static void copy(uint32_t wave, int i, uint8_t *tile, __amdgpu_buffer_rsrc_t from, uint32_t at, uint32_t atAll)
@@ -186,6 +194,15 @@ struct TileCopy
         using Place = __attribute__((address_space(3))) void;
         uint8_t *to = tile + ((uint32_t)(i * WAVES) + wave) * 1024;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Place *)to, 16, (int)at, (int)atAll, 0, 0);
+    }
+
+    // `tokens` tokens of `heads` heads from `base` on: as a buffer that ends behind the last one's last element, or after as many bytes as a tile's
+    // addresses reach.
+    __device__ __forceinline__ static __amdgpu_buffer_rsrc_t buffer(const uint8_t *base, int tokens, int64_t tokenStride, int heads, int64_t headStride,
+                                                                    int dims)
+    {
+        const uint32_t bytes = (uint32_t)(min(tokens, ROWS) - 1) * (uint32_t)tokenStride + (uint32_t)(heads - 1) * (uint32_t)headStride + (uint32_t)dims * 2;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, (int)bytes, 0x00027000);
     }
 
     // Rows `stride` apart from `base` on, of which there are `count`, one at least.
@@ -203,10 +220,12 @@ struct TileCopy
     }
 };
 
-// All waves' copies to LDS have arrived, and their reads of it are done. (A barrier alone waits for no copy.)
+// All waves' copies to LDS but each one's last LEFT have arrived, and their reads of it are done. (A barrier alone waits for no copy.)
+template<int LEFT = 0>
 __device__ __forceinline__ void CopiesAndBarrier()
 {
-    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
+    static_assert(LEFT < 64, "the counter's range");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (LEFT & 15) | (LEFT >> 4) << 14); // vmcnt(LEFT)
     __syncthreads();
 }
 
@@ -273,21 +292,67 @@ struct SequenceTile
     int tile;                           // -1: there is none of that number
 };
 
-// Tile `t` of all sequences' tiles, of `size` rows each, a token having `each` rows (of keys: `ofKeys`). Every wave finds it by itself.
-__device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, uint32_t t, int size, int each, bool ofKeys)
+// Sum over the 64 lanes, as one number.
+__device__ __forceinline__ uint32_t WaveTotal(uint32_t v)
 {
-    const int lane = (int)(threadIdx.x & 63);
-    uint32_t  before = 0; // tiles of the sequences that were looked at
+    v += LaneStep<0>(v);
+    v += LaneStep<1>(v);
+    v += LaneStep<2>(v);
+    v += LaneStep<3>(v);
+    v += LaneStep<4>(v);
+    v += LaneStep<5>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// Tile `t` of all sequences' tiles, of `size` rows each, a token having `each` rows (of keys: `ofKeys`). Every wave finds it by itself.
+// With `causal` a sequence's last tiles of rows have the most keys, its first tiles of keys the most rows. They come first, of all
+// sequences (up to 64 of them), so that the workgroups that begin last are short ones (long_attention_grad 863 us, 835 with it).
+__device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, uint32_t t, uint32_t most, int size, int each, bool ofKeys, bool causal)
+{
+    const int lane    = (int)(threadIdx.x & 63);
+    auto      tilesOf = [&](int b)
+    {
+        const int first = ofKeys ? s.firstKey(b) : s.firstRow(b);
+        return ((uint32_t)(ofKeys ? s.keysOf(b, first) : s.rowsOf(b, first)) * (uint32_t)each + (uint32_t)size - 1) / (uint32_t)size;
+    };
+    auto found = [&](int b, uint32_t tile)
+    {
+        SequenceTile r;
+        r.tile     = (int)tile;
+        r.firstRow = s.firstRow(b);
+        r.rows     = s.rowsOf(b, r.firstRow);
+        r.firstKey = s.firstKey(b);
+        r.keys     = s.keysOf(b, r.firstKey);
+        return r;
+    };
+    if (causal && s.count <= 64)
+    {
+        const uint32_t tiles = tilesOf(min(lane, s.count - 1)), own = lane < s.count ? tiles : 0;
+        // of the tiles that have at least `low` less heavy ones in their sequence there are more than t
+        auto     of  = [&](uint32_t less) { return WaveTotal(own > less ? own - less : 0); };
+        uint32_t low = 0, high = WaveLargest(own);
+        if (of(0) <= t)
+        {
+            return {0, 0, 0, 0, -1};
+        }
+        while (high - low > 1)
+        {
+            const uint32_t middle = (low + high) / 2;
+            of(middle) > t ? low = middle : high = middle;
+        }
+        const uint32_t rank = t - of(low + 1);
+        const uint64_t some = __ballot(own > low);
+        const uint32_t at   = __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+        const int      b    = (int)__builtin_ctzll(__ballot(own > low && at == rank));
+        return found(b, ofKeys ? (uint32_t)__builtin_amdgcn_readlane((int)own, b) - 1 - low : low);
+    }
+    t               = causal && !ofKeys ? most - 1 - t : t;
+    uint32_t before = 0; // tiles of the sequences that were looked at
     for (int base = 0; base < s.count; base += 64)
     {
-        const int b     = base + lane;
-        uint32_t  tiles = 0;
-        if (b < s.count)
-        {
-            const int first = ofKeys ? s.firstKey(b) : s.firstRow(b);
-            tiles           = ((uint32_t)(ofKeys ? s.keysOf(b, first) : s.rowsOf(b, first)) * (uint32_t)each + (uint32_t)size - 1) / (uint32_t)size;
-        }
-        uint32_t upTo = tiles; // this sequence's and those of the lanes before
+        const int      b = base + lane;
+        const uint32_t all = tilesOf(min(b, s.count - 1)), tiles = b < s.count ? all : 0;
+        uint32_t       upTo = tiles; // this sequence's and those of the lanes before
 #pragma unroll
         for (int d = 1; d < 64; d *= 2)
         {
@@ -297,14 +362,9 @@ __device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, ui
         const uint64_t behind = __ballot(before + upTo > t);
         if (behind != 0)
         {
-            const int    at = (int)__builtin_ctzll(behind), found = base + at;
-            SequenceTile r;
-            r.tile     = (int)(t - before - ((uint32_t)__builtin_amdgcn_readlane((int)upTo, at) - (uint32_t)__builtin_amdgcn_readlane((int)tiles, at)));
-            r.firstRow = s.firstRow(found);
-            r.rows     = s.rowsOf(found, r.firstRow);
-            r.firstKey = s.firstKey(found);
-            r.keys     = s.keysOf(found, r.firstKey);
-            return r;
+            const int at = (int)__builtin_ctzll(behind);
+            return found(base + at,
+                         t - before - ((uint32_t)__builtin_amdgcn_readlane((int)upTo, at) - (uint32_t)__builtin_amdgcn_readlane((int)tiles, at)));
         }
         before += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
     }

@@ -34,9 +34,9 @@ HeadsView RequireHeads(NVCVTensorHandle h, const char *what, int align)
     v.tokens = (int32_t)d.shape[0];
     v.heads  = (int32_t)d.shape[1];
     v.dims   = (int32_t)d.shape[2];
-    // (distances between one and the same are never gone)
-    v.tokenStride = v.tokens > 1 ? st[0] : 0;
+    // (distances between one and the same are never gone; a token behind the only one is still another place)
     v.headStride  = v.heads > 1 ? st[1] : 0;
+    v.tokenStride = v.tokens > 1 ? st[0] : v.heads > 1 ? v.headStride * v.heads : v.dims * es;
     if (v.tokenStride % whole != 0 || v.headStride % whole != 0)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must have tokens and heads at distances of whole %ld bytes", what, (long)whole);

@@ -23,20 +23,20 @@ struct AttentionGradArgs
     int64_t            gradQToken, gradQHead, gradKToken, gradKHead, gradVToken, gradVHead;
     AttentionSequences sequences;
     const float       *lse;
-    float             *delta;   // [heads][rows]: gradOut . out
+    float             *base, *delta; // [rows][heads]: ShareBase and gradOut . out
     float2            *largest; // F16: of each of the first kernel's workgroups, the largest squares of rows of gradOut and of v
     int32_t            largestCount;
     GroupRows          rows; // of a key head
-    DivBy              keyHeads;
+    DivBy              keyHeads, queryHeads;
     int32_t            heads, dims;
-    uint32_t           tiles, keyTiles;
+    uint32_t           tiles, keyTiles, boundTiles;
     float              scale;
     bool               causal;
 
-    // in lse and delta
+    // in base and delta
     __device__ __forceinline__ int64_t number(const AttentionRow &row) const
     {
-        return (int64_t)row.head * sequences.rows + row.token;
+        return (int64_t)row.token * heads + row.head;
     }
 };
 
@@ -44,32 +44,15 @@ struct AttentionGradArgs
 template<class T>
 constexpr float kShareShift = std::is_same<T, Half>::value ? 15.f : 0.f;
 
-// ---- gradOut . out, and for F16 what bounds the shares' gradients ------------------------------------------------------
-constexpr int kDeltaThreads = 1024, kDeltaRows = kDeltaThreads / 16, kDeltaBlocks = 512;
-
-__device__ __forceinline__ float SumOf16(float v)
-{
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2)
-    {
-        v += __shfl_xor(v, d);
-    }
-    return v;
-}
-
-// The sum of the products of 8 elements of two rows, in 32 bits.
+// What a row's scores are taken relative to: lse to the base 2, less the shift; a row without a key has no share.
 template<class T>
-__device__ __forceinline__ float Dot8(const uint8_t *a, const uint8_t *b)
+__device__ __forceinline__ float ShareBase(float lse)
 {
-    const Run<T, 8> x = *reinterpret_cast<const Run<T, 8> *>(a), y = *reinterpret_cast<const Run<T, 8> *>(b);
-    float           s = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-    {
-        s = __builtin_fmaf((float)x.v[i], (float)y.v[i], s);
-    }
-    return s;
+    return lse == -INFINITY ? INFINITY : __builtin_fmaf(lse, kLog2E, -kShareShift<T>);
 }
+
+// ---- F16: what bounds the shares' gradients ------------------------------------------------------------------------------
+constexpr int kBoundThreads = 1024, kBoundBlocks = 512, kBoundTokens = 4; // the last: of keys, to a wave
 
 // The larger of two sums of squares; one that is not finite (its sequence's gradients aren't either) counts for nothing.
 __device__ __forceinline__ float Larger(float a, float b)
@@ -77,76 +60,73 @@ __device__ __forceinline__ float Larger(float a, float b)
     return b < INFINITY ? fmaxf(a, b) : a;
 }
 
-// 16 lanes to a row, 8 elements to a lane.
-template<class T>
-__global__ __launch_bounds__(kDeltaThreads) void AttentionDeltaKernel(const AttentionGradArgs a)
+// The largest square of rows of `tokens` tokens from `base` on, of which the wave takes every `step`-th LANES-th of a wave from `first` on. LANES
+// lanes to a row, 8 elements to a lane.
+template<class T, int LANES>
+__device__ __forceinline__ float LargestSquare(const uint8_t *base, int64_t tokenStride, int64_t headStride, const DivBy &heads, uint32_t tokens, int dims,
+                                               uint32_t first, uint32_t step)
 {
-    constexpr bool kBounds = std::is_same<T, Half>::value;
-    const int      begin = a.sequences.firstRow(0), end = begin + a.sequences.rowsOf(a.sequences.count - 1, begin);
-    const int      d = (int)(threadIdx.x % 16) * 8;
-    const int64_t  first = (int64_t)blockIdx.x * kDeltaRows + threadIdx.x / 16, step = (int64_t)gridDim.x * kDeltaRows;
-    float          ofGrad = 0, ofValues = 0;
-    // (heads next to each other: rows of one token follow one another in memory)
-    for (int64_t at = first, all = (int64_t)(end - begin) * a.heads; at < all; at += step)
+    const uint32_t lane = threadIdx.x & 63, rows = tokens * heads.d;
+    const int      d       = (int)(lane % LANES) * 8, from = min(d, dims - 8);
+    float          largest = 0;
+#pragma unroll 4
+    for (uint32_t r = first * (64 / LANES) + lane / LANES; r < rows; r += step * (64 / LANES))
     {
-        const int token = begin + (int)(at / a.heads), head = (int)(at - (int64_t)(token - begin) * a.heads);
-        float     dot = 0, square = 0;
-        if (d < a.dims)
+        const uint32_t  token = heads.Quotient(r), head = r - token * heads.d;
+        const Run<T, 8> x      = *reinterpret_cast<const Run<T, 8> *>(base + token * tokenStride + head * headStride + from * 2);
+        float           square = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
         {
-            const uint8_t *grad = a.grad + token * a.gradToken + head * a.gradHead + d * 2;
-            dot                 = Dot8<T>(grad, a.out + token * a.outToken + head * a.outHead + d * 2);
-            square              = kBounds ? Dot8<T>(grad, grad) : 0.f;
+            square = __builtin_fmaf((float)x.v[i], (float)x.v[i], square);
         }
-        dot = SumOf16(dot);
-        if (kBounds)
+        square = d < dims ? square : 0.f;
+#pragma unroll
+        for (int n = 1; n < LANES; n *= 2)
         {
-            ofGrad = Larger(ofGrad, SumOf16(square));
+            square += __shfl_xor(square, n);
         }
-        if (d == 0)
-        {
-            a.delta[(int64_t)head * a.sequences.rows + token] = dot;
-        }
+        largest = Larger(largest, square);
     }
-    if constexpr (kBounds)
+    return largest;
+}
+
+template<class T, int DP>
+__global__ __launch_bounds__(kBoundThreads) void AttentionBoundKernel(const AttentionGradArgs a)
+{
+    __shared__ float2 s_largest[kBoundThreads / 64];
+    const uint32_t    wave = blockIdx.x * (kBoundThreads / 64) + WaveOfGroup(), waves = gridDim.x * (kBoundThreads / 64);
+    // the sequences' rows lie one behind the other, their keys may lie in places of a cache, which hold anything behind them
+    const int begin = a.sequences.firstRow(0), end = begin + a.sequences.rowsOf(a.sequences.count - 1, begin);
+    float     ofGrad = LargestSquare<T, DP / 8>(a.grad + begin * a.gradToken, a.gradToken, a.gradHead, a.queryHeads, (uint32_t)(end - begin), a.dims, wave,
+                                            waves);
+    float     ofValues = 0;
+    for (uint32_t t = wave; t < a.boundTiles; t += waves)
     {
-        // values of sequences alone: a cache's places behind them hold anything
-        const int32_t *starts = a.sequences.keyOffsets != nullptr ? a.sequences.keyOffsets : a.sequences.offsets;
-        const int      heads  = (int)a.keyHeads.d;
-        for (int64_t at = first, all = (int64_t)a.sequences.keys * heads; at < all; at += step)
+        const SequenceTile s = FindTile(a.sequences, t, 0, kBoundTokens, 1, true, false);
+        if (s.tile < 0)
         {
-            const int token = (int)(at / heads), head = (int)(at - (int64_t)token * heads);
-            int       low = 0, high = a.sequences.count; // the last sequence that begins at or before it lies between them
-            while (high - low > 1)
-            {
-                const int middle = (low + high) / 2;
-                (starts[middle] <= token ? low : high) = middle;
-            }
-            const int key = a.sequences.firstKey(low);
-            float     square = 0;
-            if (token >= key && token - key < a.sequences.keysOf(low, key) && d < a.dims)
-            {
-                const uint8_t *value = a.v + token * a.vToken + head * a.vHead + d * 2;
-                square               = Dot8<T>(value, value);
-            }
-            ofValues = Larger(ofValues, SumOf16(square));
+            break;
         }
-        __shared__ float2 s_largest[kDeltaThreads / 64];
-        ofGrad   = __uint_as_float(WaveLargest(__float_as_uint(ofGrad)));
-        ofValues = __uint_as_float(WaveLargest(__float_as_uint(ofValues)));
-        if ((threadIdx.x & 63) == 0)
+        const int first = s.tile * kBoundTokens;
+        ofValues = fmaxf(ofValues, LargestSquare<T, DP / 8>(a.v + (s.firstKey + first) * a.vToken, a.vToken, a.vHead, a.keyHeads,
+                                                            (uint32_t)min(s.keys - first, kBoundTokens), a.dims, 0, 1));
+    }
+    ofGrad                     = __uint_as_float(WaveLargest(__float_as_uint(ofGrad)));
+    ofValues                   = __uint_as_float(WaveLargest(__float_as_uint(ofValues)));
+    if ((threadIdx.x & 63) == 0)
+    {
+        s_largest[WaveOfGroup()] = make_float2(ofGrad, ofValues);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+    {
+        float2 largest = s_largest[0];
+        for (int w = 1; w < kBoundThreads / 64; ++w)
         {
-            s_largest[WaveOfGroup()] = make_float2(ofGrad, ofValues);
+            largest = make_float2(Larger(largest.x, s_largest[w].x), Larger(largest.y, s_largest[w].y));
         }
-        __syncthreads();
-        if (threadIdx.x == 0)
-        {
-            float2 largest = s_largest[0];
-            for (int w = 1; w < kDeltaThreads / 64; ++w)
-            {
-                largest = make_float2(Larger(largest.x, s_largest[w].x), Larger(largest.y, s_largest[w].y));
-            }
-            a.largest[blockIdx.x] = largest;
-        }
+        a.largest[blockIdx.x] = largest;
     }
 }
 
@@ -172,64 +152,79 @@ __device__ __forceinline__ float GradFactor(const AttentionGradArgs &a)
     return bound == 0 ? 1.f : ldexpf(1.f, min(max(12 - ilogbf(bound), -100), 100));
 }
 
-// What a row's scores are taken relative to: lse to the base 2, less the shift; a row without a key, or behind the end, has no share.
-template<class T>
-__device__ __forceinline__ float ShareBase(float lse, bool there)
-{
-    return !there || lse == -INFINITY ? INFINITY : __builtin_fmaf(lse, kLog2E, -kShareShift<T>);
-}
-
 // ---- the queries' gradient: 128 rows to a workgroup, 32 to a wave --------------------------------------------------------
 constexpr int kGradRows = 128, kGradKeys = 64, kGradThreads = 256;
 
 template<class T, int DP>
 __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const AttentionGradArgs a)
 {
-    __shared__ __attribute__((aligned(256))) uint8_t s_k[2][kGradKeys * DP * 2], s_v[2][kGradKeys * DP * 2];
+    __shared__ __attribute__((aligned(256))) uint8_t s_k0[kGradKeys * DP * 2], s_k1[kGradKeys * DP * 2];
+    __shared__ __attribute__((aligned(256))) uint8_t s_v0[kGradKeys * DP * 2], s_v1[kGradKeys * DP * 2];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
     const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
-    const SequenceTile s       = FindTile(a.sequences, a.causal ? a.tiles - 1 - t : t, kGradRows, a.rows.size(), false);
+    const SequenceTile s       = FindTile(a.sequences, t, a.tiles, kGradRows, a.rows.size(), false, a.causal);
     if (s.tile < 0)
     {
         return;
     }
-    const int first = s.tile * kGradRows, ownFirst = first + (int)WaveOfGroup() * 32, all = s.rows * a.rows.size();
+    const uint32_t wave = WaveOfGroup();
+    const int      first = s.tile * kGradRows, ownFirst = first + (int)wave * 32, all = s.rows * a.rows.size();
     const AttentionRow row(a.rows, a.causal, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
     auto               limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
     const int          tileKeys = max(limitAt(first + kGradRows - 1) + 1, 0), waveKeys = ownFirst < all ? limitAt(ownFirst + 31) + 1 : 0;
     const int          seenKeys = limitAt(ownFirst) + 1, parts = (tileKeys + kGradKeys - 1) / kGradKeys;
     const uint8_t     *k = a.k + s.firstKey * a.kToken + keyHead * a.kHead, *v = a.v + s.firstKey * a.vToken + keyHead * a.vHead;
 
-    TileLoad<kGradKeys, DP, kGradThreads> nextK, nextV;
-    auto load = [&](int part)
+    using Copy = TileCopy<kGradKeys, DP, kGradThreads / 64>;
+    auto load  = [&](int part, uint8_t *toK, uint8_t *toV)
     {
         const int key = part * kGradKeys;
-        nextK.get(threadIdx.x, k + key * a.kToken, a.kToken, s.keys - key, a.dims);
-        nextV.get(threadIdx.x, v + key * a.vToken, a.vToken, s.keys - key, a.dims);
+        Copy::rows(wave, toK, k + key * a.kToken, (uint32_t)a.kToken, s.keys - key, a.dims);
+        Copy::rows(wave, toV, v + key * a.vToken, (uint32_t)a.vToken, s.keys - key, a.dims);
     };
     if (parts > 0)
     {
-        load(0);
+        load(0, s_k0, s_v0);
     }
     Vec8<T> q[DP / 16], grad[DP / 16];
     LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
     LoadColumn<T, DP>(grad, a.grad + row.token * a.gradToken + row.head * a.gradHead, a.dims);
-    const float factor = GradFactor<T>(a), base = ShareBase<T>(a.lse[a.number(row)], row.there);
-    const float scale = a.scale * kLog2E, of = factor * __builtin_amdgcn_exp2f(-kShareShift<T>), delta = a.delta[a.number(row)] * of;
-    Acc16       sum[DP / 32] = {};
-    for (int part = 0; part < parts; ++part)
+    const float factor = GradFactor<T>(a), base = ShareBase<T>(a.lse[(int64_t)row.head * a.sequences.rows + row.token]);
+    const float scale = a.scale * kLog2E, of = factor * __builtin_amdgcn_exp2f(-kShareShift<T>);
+    // gradOut . out, here and for the other kernel
+    float dot = 0;
     {
-        const int at = part & 1, key = part * kGradKeys;
-        nextK.put(threadIdx.x, s_k[at]);
-        nextV.put(threadIdx.x, s_v[at]);
-        __syncthreads();
+        Vec8<T> out[DP / 16];
+        LoadColumn<T, DP>(out, a.out + row.token * a.outToken + row.head * a.outHead, a.dims);
+#pragma unroll
+        for (int step = 0; step < DP / 16; ++step)
+        {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                dot = __builtin_fmaf((float)out[step][i], (float)grad[step][i], dot);
+            }
+        }
+        dot = BothSum(dot);
+    }
+    if (row.there && (threadIdx.x & 32) == 0)
+    {
+        a.base[a.number(row)]  = base;
+        a.delta[a.number(row)] = dot;
+    }
+    const float delta = dot * of;
+    Acc16       sum[DP / 32] = {};
+    auto        take = [&](int part, const uint8_t *fromK, const uint8_t *fromV, uint8_t *nextK, uint8_t *nextV)
+    {
+        const int key = part * kGradKeys;
+        CopiesAndBarrier(); // (all have done the part before: its place may be written over)
         if (part + 1 < parts)
         {
-            load(part + 1);
+            load(part + 1, nextK, nextV);
         }
         if (key >= waveKeys)
         {
-            continue;
+            return;
         }
         const bool hide = key + kGradKeys > seenKeys;
 #pragma unroll
@@ -239,8 +234,8 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
 #pragma unroll
             for (int step = 0; step < DP / 16; ++step)
             {
-                Multiply(shares, RowsOperand<T, DP>(s_k[at], 32 * half, step), q[step]);
-                Multiply(grads, RowsOperand<T, DP>(s_v[at], 32 * half, step), grad[step]);
+                Multiply(shares, RowsOperand<T, DP>(fromK, 32 * half, step), q[step]);
+                Multiply(grads, RowsOperand<T, DP>(fromV, 32 * half, step), grad[step]);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -250,6 +245,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
             }
             if (hide)
             {
+                KeepBranch();
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                 {
@@ -263,9 +259,18 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
 #pragma unroll
                 for (int p = 0; p < DP / 32; ++p)
                 {
-                    Multiply(sum[p], ColumnsOperand<T, DP>(s_k[at], 32 * half + 16 * k16, p), rounded);
+                    Multiply(sum[p], ColumnsOperand<T, DP>(fromK, 32 * half + 16 * k16, p), rounded);
                 }
             }
+        }
+    };
+    // (by turns of their own, so that the compiler sees that what is read is not what is on its way)
+    for (int part = 0; part < parts; part += 2)
+    {
+        take(part, s_k0, s_v0, s_k1, s_v1);
+        if (part + 1 < parts)
+        {
+            take(part + 1, s_k1, s_v1, s_k0, s_v0);
         }
     }
     StoreColumn<T, DP>(sum, a.scale / factor, a.gradQ + row.token * a.gradQToken + row.head * a.gradQHead, row.there, a.dims);
@@ -274,103 +279,163 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
 // ---- the keys' and values' gradients: 128 keys to a workgroup, 32 to a wave ------------------------------------------------
 constexpr int kOfKeys = 128, kOfRows = 64;
 
-template<class T, int DP>
-__global__ __launch_bounds__(kGradThreads) void AttentionGradKVKernel(const AttentionGradArgs a)
+// With heads of 128 elements two gradients, keys and values would be 192 registers of the 256 that two waves to a SIMD have: keys and values
+// stay in LDS, and eight waves go with them, of which two have the same keys and halves of each tile of rows, so that the
+// workgroup of a long sequence's first keys, which all rows see, is done in half the time. (With 64 elements such pairs are slower:
+// pairs_attention_grad's kernel 64 us, 43 with four waves that take whole tiles.)
+template<int DP>
+constexpr bool kInPairs = DP > 64;
+template<int DP>
+constexpr int kOfThreads = kInPairs<DP> ? 512 : 256;
+
+// A tile of rows: queries, gradients, and what their shares are made with.
+template<int DP>
+struct RowsPlace
 {
-    __shared__ __attribute__((aligned(256))) uint8_t s_q[2][kOfRows * DP * 2], s_grad[2][kOfRows * DP * 2];
-    __shared__ __attribute__((aligned(16))) float    s_base[2][kOfRows], s_delta[2][kOfRows];
-    __shared__ int                                   s_limit[2][kOfRows];
+    uint8_t *q, *grad;
+    float   *base, *delta;
+};
+
+template<class T, int DP>
+__global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const AttentionGradArgs a)
+{
+    constexpr int kWaves = kOfThreads<DP> / 64, kBytes = kOfRows * DP * 2;
+    using Copy           = TileCopy<kOfRows, DP, kWaves>;
+    __shared__ __attribute__((aligned(256))) uint8_t s_q0[kBytes], s_q1[kBytes], s_grad0[kBytes], s_grad1[kBytes];
+    __shared__ __attribute__((aligned(256))) float   s_base0[kOfRows], s_base1[kOfRows], s_delta0[kOfRows], s_delta1[kOfRows];
+    __shared__ __attribute__((aligned(256))) uint8_t s_k[kInPairs<DP> ? kOfKeys * DP * 2 : 16], s_v[kInPairs<DP> ? kOfKeys * DP * 2 : 16];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
     const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
-    const SequenceTile s       = FindTile(a.sequences, t, kOfKeys, 1, true);
+    const SequenceTile s       = FindTile(a.sequences, t, a.keyTiles, kOfKeys, 1, true, a.causal);
     if (s.tile < 0)
     {
         return;
     }
-    const int  first = s.tile * kOfKeys, ownFirst = first + (int)WaveOfGroup() * 32, key = ownFirst + (int)(threadIdx.x & 31);
-    const bool there = key < s.keys;
-    const int  all   = s.rows * a.rows.size();
+    const uint32_t wave = WaveOfGroup(), ofKeys = wave % 4;
+    const int      first = s.tile * kOfKeys, ownFirst = first + (int)ofKeys * 32, key = ownFirst + (int)(threadIdx.x & 31);
+    const bool     there = key < s.keys;
+    const int      group = a.rows.size(), all = s.rows * group;
     // the first row that sees one of these keys
-    const int  begin = a.causal ? min(max(first - (s.keys - s.rows), 0), s.rows) * a.rows.size() : 0;
-    auto       limitAt = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
+    const int begin = a.causal ? min(max(first - (s.keys - s.rows), 0), s.rows) * group : 0;
+    auto      limitAt = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
 
-    TileLoad<kOfRows, DP, kGradThreads> nextQ, nextGrad;
-    float                               nextBase = INFINITY, nextDelta = 0;
-    int                                 nextLimit = -1;
-    const float                         factor = GradFactor<T>(a), of = factor * __builtin_amdgcn_exp2f(-kShareShift<T>);
-    auto load = [&](int at)
+    Vec8<T> k[kInPairs<DP> ? 1 : DP / 16], v[kInPairs<DP> ? 1 : DP / 16];
+    if constexpr (kInPairs<DP>)
     {
-        auto place = [&](const uint8_t *base, int64_t tokenStride, int64_t headStride, int r)
+        using Keys = TileCopy<kOfKeys, DP, kWaves>;
+        Keys::rows(wave, s_k, a.k + (s.firstKey + first) * a.kToken + keyHead * a.kHead, (uint32_t)a.kToken, s.keys - first, a.dims);
+        Keys::rows(wave, s_v, a.v + (s.firstKey + first) * a.vToken + keyHead * a.vHead, (uint32_t)a.vToken, s.keys - first, a.dims);
+    }
+    else
+    {
+        const int own = s.firstKey + min(key, s.keys - 1); // (columns behind the last key are made of it, and not stored)
+        LoadColumn<T, DP>(k, a.k + own * a.kToken + keyHead * a.kHead, a.dims);
+        LoadColumn<T, DP>(v, a.v + own * a.vToken + keyHead * a.vHead, a.dims);
+    }
+    auto keyOperand = [&](int step) { return kInPairs<DP> ? RowsOperand<T, DP>(s_k, 32 * ofKeys, step) : k[kInPairs<DP> ? 0 : step]; };
+    auto valueOperand = [&](int step) { return kInPairs<DP> ? RowsOperand<T, DP>(s_v, 32 * ofKeys, step) : v[kInPairs<DP> ? 0 : step]; };
+    const float factor = GradFactor<T>(a), of = factor * __builtin_amdgcn_exp2f(-kShareShift<T>), scale = a.scale * kLog2E;
+
+    // the lane's places in a tile, from its first token's on
+    uint32_t placeQ[Copy::kCount], placeGrad[Copy::kCount], placeValue;
+    auto     places = [&](int at)
+    {
+        const int i0 = a.rows.token(at);
+#pragma unroll
+        for (int c = 0; c < Copy::kCount; ++c)
         {
-            const int i = a.rows.token(at + r);
-            return base + (s.firstRow + i) * tokenStride + (keyHead * a.rows.size() + (at + r - i * a.rows.size())) * headStride;
-        };
-        nextQ.get(threadIdx.x, all - at, a.dims, [&](int r) { return place(a.q, a.qToken, a.qHead, r); });
-        nextGrad.get(threadIdx.x, all - at, a.dims, [&](int r) { return place(a.grad, a.gradToken, a.gradHead, r); });
-        if (threadIdx.x < kOfRows)
+            const int      r = Copy::rowOf(wave, c), i = a.rows.token(at + r);
+            const uint32_t unit = Copy::unitOf(r), token = (uint32_t)(i - i0), head = (uint32_t)(at + r - i * group);
+            const bool     some = (int)unit * 8 < a.dims;
+            placeQ[c]           = some ? token * (uint32_t)a.qToken + head * (uint32_t)a.qHead + unit * 16 : Copy::kNowhere;
+            placeGrad[c]        = some ? token * (uint32_t)a.gradToken + head * (uint32_t)a.gradHead + unit * 16 : Copy::kNowhere;
+        }
+        const int r = (int)(threadIdx.x & 63), i = a.rows.token(at + r);
+        placeValue  = ((uint32_t)(i - i0) * (uint32_t)a.heads + (uint32_t)(at + r - i * group)) * 4;
+    };
+    // Rows from `at` on to LDS. Their buffers end with the sequence: rows behind it are zeros, which add nothing to any sum.
+    auto load = [&](int at, const RowsPlace<DP> &to)
+    {
+        using Place = __attribute__((address_space(3))) void;
+        if (kOfRows % group != 0) // (where tiles have whole tokens, places are the same in all of them)
         {
-            const AttentionRow row(a.rows, a.causal, s, keyHead, at + (int)threadIdx.x);
-            nextBase  = ShareBase<T>(a.lse[a.number(row)], row.there);
-            nextDelta = row.there ? a.delta[a.number(row)] * of : 0.f;
-            nextLimit = row.there ? row.limit : -1;
+            places(at);
+        }
+        const int      i0 = a.rows.token(at), tokens = s.rows - i0, token = s.firstRow + i0, head = keyHead * group;
+        const int64_t  number = (int64_t)token * a.heads + head;
+        const uint32_t bytes  = ((uint32_t)(min(tokens, kOfRows) - 1) * (uint32_t)a.heads + (uint32_t)group) * 4;
+        // (every wave makes one of these two copies, so that all have as many on their way)
+        const bool odd  = (wave & 1) != 0;
+        const auto from = __builtin_amdgcn_make_buffer_rsrc((odd ? a.delta : a.base) + number, 0, (int)bytes, 0x00027000);
+        const auto q    = Copy::buffer(a.q + token * a.qToken + head * a.qHead, tokens, a.qToken, group, a.qHead, a.dims);
+        const auto grad = Copy::buffer(a.grad + token * a.gradToken + head * a.gradHead, tokens, a.gradToken, group, a.gradHead, a.dims);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Place *)(odd ? to.delta : to.base), 4, (int)placeValue, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < Copy::kCount; ++c)
+        {
+            Copy::copy(wave, c, to.q, q, placeQ[c], 0);
+            Copy::copy(wave, c, to.grad, grad, placeGrad[c], 0);
         }
     };
+    const RowsPlace<DP> place0 = {s_q0, s_grad0, s_base0, s_delta0}, place1 = {s_q1, s_grad1, s_base1, s_delta1};
     if (begin < all)
     {
-        load(begin);
+        places(begin);
+        load(begin, place0);
     }
-    Vec8<T> k[DP / 16], v[DP / 16];
-    const int own = s.firstKey + min(key, s.keys - 1); // (columns behind the last key are made of it, and not stored)
-    LoadColumn<T, DP>(k, a.k + own * a.kToken + keyHead * a.kHead, a.dims);
-    LoadColumn<T, DP>(v, a.v + own * a.vToken + keyHead * a.vHead, a.dims);
-    const float scale = a.scale * kLog2E;
-    Acc16       sumK[DP / 32] = {}, sumV[DP / 32] = {};
-    for (int at = begin, turn = 0; at < all; at += kOfRows, turn ^= 1)
+    Acc16 sumK[DP / 32] = {}, sumV[DP / 32] = {};
+    auto  take = [&](int at, const RowsPlace<DP> &place, const RowsPlace<DP> &next)
     {
-        nextQ.put(threadIdx.x, s_q[turn]);
-        nextGrad.put(threadIdx.x, s_grad[turn]);
-        if (threadIdx.x < kOfRows)
-        {
-            s_base[turn][threadIdx.x]  = nextBase;
-            s_delta[turn][threadIdx.x] = nextDelta;
-            s_limit[turn][threadIdx.x] = nextLimit;
-        }
-        __syncthreads();
+        CopiesAndBarrier(); // (all have done the tile before: its place may be written over)
         if (at + kOfRows < all)
         {
-            load(at + kOfRows);
+            load(at + kOfRows, next);
         }
-        if (limitAt(at + kOfRows - 1) < ownFirst)
-        {
-            continue;
-        }
-        const bool hide = limitAt(at) < ownFirst + 31;
 #pragma unroll
-        for (int half = 0; half < kOfRows / 32; ++half)
+        for (int part = 0; part < (kInPairs<DP> ? 1 : 2); ++part)
         {
-            Acc16 shares = {}, grads = {};
+            const int half = kInPairs<DP> ? (int)wave / 4 : part, from = at + 32 * half;
+            if (from >= all || limitAt(from + 31) < ownFirst)
+            {
+                continue;
+            }
+            Acc16 shares = {}, grads;
 #pragma unroll
             for (int step = 0; step < DP / 16; ++step)
             {
-                Multiply(shares, RowsOperand<T, DP>(s_q[turn], 32 * half, step), k[step]);
-                Multiply(grads, RowsOperand<T, DP>(s_grad[turn], 32 * half, step), v[step]);
+                Multiply(shares, RowsOperand<T, DP>(place.q, 32 * half, step), keyOperand(step));
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+            {
+                const float4 base = *reinterpret_cast<const float4 *>(place.base + 32 * half + RowOf(i));
+                const float4 delta = *reinterpret_cast<const float4 *>(place.delta + 32 * half + RowOf(i));
+                const float  b[4] = {base.x, base.y, base.z, base.w}, d[4] = {delta.x, delta.y, delta.z, delta.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                {
+                    shares[i + n] = __builtin_amdgcn_exp2f(__builtin_fmaf(shares[i + n], scale, -b[n]));
+                    grads[i + n]  = -d[n];
+                }
+            }
+            if (limitAt(from) < ownFirst + 31)
+            {
+                KeepBranch();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    shares[i] = key <= limitAt(from + RowOf(i)) ? shares[i] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int step = 0; step < DP / 16; ++step)
+            {
+                Multiply(grads, RowsOperand<T, DP>(place.grad, 32 * half, step), valueOperand(step));
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
             {
-                const int r = 32 * half + RowOf(i);
-                shares[i]   = __builtin_amdgcn_exp2f(__builtin_fmaf(shares[i], scale, -s_base[turn][r]));
-                grads[i]    = shares[i] * __builtin_fmaf(grads[i], of, -s_delta[turn][r]);
-            }
-            if (hide)
-            {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                {
-                    const bool seen = key <= s_limit[turn][32 * half + RowOf(i)];
-                    shares[i]       = seen ? shares[i] : 0.f;
-                    grads[i]        = seen ? grads[i] : 0.f;
-                }
+                grads[i] = shares[i] * (std::is_same<T, Half>::value ? grads[i] * of : grads[i]);
             }
 #pragma unroll
             for (int r16 = 0; r16 < 2; ++r16)
@@ -379,10 +444,50 @@ __global__ __launch_bounds__(kGradThreads) void AttentionGradKVKernel(const Atte
 #pragma unroll
                 for (int p = 0; p < DP / 32; ++p)
                 {
-                    Multiply(sumV[p], ColumnsOperand<T, DP>(s_grad[turn], 32 * half + 16 * r16, p), share);
-                    Multiply(sumK[p], ColumnsOperand<T, DP>(s_q[turn], 32 * half + 16 * r16, p), grad);
+                    Multiply(sumV[p], ColumnsOperand<T, DP>(place.grad, 32 * half + 16 * r16, p), share);
+                    Multiply(sumK[p], ColumnsOperand<T, DP>(place.q, 32 * half + 16 * r16, p), grad);
                 }
             }
+        }
+    };
+    for (int at = begin; at < all; at += 2 * kOfRows)
+    {
+        take(at, place0, place1);
+        if (at + kOfRows < all)
+        {
+            take(at + kOfRows, place1, place0);
+        }
+    }
+    if constexpr (kInPairs<DP>)
+    {
+        // the second half's sums are added to the first's, by way of the tiles' places: a wave's sum of one gradient fits one of them
+        float *place = reinterpret_cast<float *>(ofKeys == 0 ? s_q0 : ofKeys == 1 ? s_q1 : ofKeys == 2 ? s_grad0 : s_grad1) + (threadIdx.x & 63);
+        auto   join  = [&](Acc16(&sum)[DP / 32])
+        {
+            __syncthreads();
+            if (wave >= 4)
+            {
+#pragma unroll
+                for (int i = 0; i < DP / 2; ++i)
+                {
+                    place[i * 64] = sum[i / 16][i % 16];
+                }
+            }
+            __syncthreads();
+            if (wave < 4)
+            {
+#pragma unroll
+                for (int i = 0; i < DP / 2; ++i)
+                {
+                    sum[i / 16][i % 16] += place[i * 64];
+                }
+            }
+        };
+        join(sumK);
+        join(sumV);
+        if (wave >= 4)
+        {
+            return;
         }
     }
     StoreColumn<T, DP>(sumK, a.scale / factor, a.gradK + (s.firstKey + key) * a.gradKToken + keyHead * a.gradKHead, there, a.dims);
@@ -392,7 +497,7 @@ __global__ __launch_bounds__(kGradThreads) void AttentionGradKVKernel(const Atte
 
 int64_t GradBytes(int64_t rows, int64_t heads)
 {
-    return kDeltaBlocks * (int64_t)sizeof(float2) + rows * heads * (int64_t)sizeof(float);
+    return kBoundBlocks * (int64_t)sizeof(float2) + 2 * rows * heads * (int64_t)sizeof(float);
 }
 
 template<class T, int DP>
@@ -400,14 +505,17 @@ void Launch(const AttentionGradArgs &a, hipStream_t stream)
 {
     if (a.tiles > 0)
     {
-        AttentionDeltaKernel<T><<<(uint32_t)a.largestCount, kDeltaThreads, 0, stream>>>(a);
-        CheckLaunch("attention's gradient (sums)");
+        if (std::is_same<T, Half>::value)
+        {
+            AttentionBoundKernel<T, DP><<<(uint32_t)a.largestCount, kBoundThreads, 0, stream>>>(a);
+            CheckLaunch("attention's gradient (bounds)");
+        }
         AttentionGradQKernel<T, DP><<<a.tiles * a.keyHeads.d, kGradThreads, 0, stream>>>(a);
         CheckLaunch("attention's gradient (queries)");
     }
     if (a.keyTiles > 0)
     {
-        AttentionGradKVKernel<T, DP><<<a.keyTiles * a.keyHeads.d, kGradThreads, 0, stream>>>(a);
+        AttentionGradKVKernel<T, DP><<<a.keyTiles * a.keyHeads.d, kOfThreads<DP>, 0, stream>>>(a);
         CheckLaunch("attention's gradient (keys)");
     }
 }
@@ -432,15 +540,16 @@ void SubmitGrad(hipStream_t stream, NVCVTensorHandle hgrad, NVCVTensorHandle hq,
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Too many rows or keys");
     }
-    const int64_t  all = std::max(rows * in.q.heads, keys * in.k.heads);
+    const int64_t  bounds = (std::max(rows, keys) + kBoundTokens * kBoundThreads / 64 - 1) / (kBoundTokens * kBoundThreads / 64);
     float2        *largest = reinterpret_cast<float2 *>(room);
     const AttentionGradArgs a = {
         in.q.base, in.k.base, in.v.base, out.base, grad.base, gradQ.base, gradK.base, gradV.base, in.q.tokenStride, in.q.headStride,
         in.k.tokenStride, in.k.headStride, in.v.tokenStride, in.v.headStride, out.tokenStride, out.headStride, grad.tokenStride, grad.headStride,
         gradQ.tokenStride, gradQ.headStride, gradK.tokenStride, gradK.headStride, gradV.tokenStride, gradV.headStride, in.sequences, in.lse,
-        reinterpret_cast<float *>(largest + kDeltaBlocks), largest,
-        (int32_t)std::min<int64_t>((all + kDeltaRows - 1) / kDeltaRows, kDeltaBlocks), {DivBy((uint32_t)group)}, DivBy((uint32_t)in.k.heads),
-        in.q.heads, in.q.dims, (uint32_t)tiles, (uint32_t)keyTiles, scale, causal};
+        reinterpret_cast<float *>(largest + kBoundBlocks), reinterpret_cast<float *>(largest + kBoundBlocks) + rows * in.q.heads, largest,
+        (int32_t)std::max<int64_t>(std::min<int64_t>(bounds, kBoundBlocks), 1), {DivBy((uint32_t)group)}, DivBy((uint32_t)in.k.heads), DivBy((uint32_t)in.q.heads),
+        in.q.heads, in.q.dims, (uint32_t)tiles, (uint32_t)keyTiles,
+        (uint32_t)((keys + kBoundTokens - 1) / kBoundTokens + std::min(sequences, keys)), scale, causal};
     auto launch = [&](auto t)
     {
         using T = decltype(t);

@@ -259,7 +259,7 @@ public:
         {
             return;
         }
-        const bool inPlace = in.base == out.base && in.tokenStride == out.tokenStride && in.headStride == out.headStride;
+        const bool inPlace = in.base == out.base && (in.tokens == 1 || in.tokenStride == out.tokenStride) && in.headStride == out.headStride;
         RotaryArgs a = {in.base, out.base, positions.base, in.tokenStride, in.headStride, out.tokenStride, out.headStride,
                         std::log2(args->base) * -2. / args->dims, args->factor, args->original, args->low, args->high, (float)args->magnitude,
                         in.tokens, in.heads, args->dims, args->dims / 2, inPlace ? 0 : in.dims - args->dims, 1, DivBy(1), DivBy(1),
