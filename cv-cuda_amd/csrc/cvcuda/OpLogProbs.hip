@@ -1,11 +1,13 @@
 // Log probabilities of tokens with entropy and top alternatives, and their gradient (formulas: cvcuda/LogProbs.h). Bound by memory: the
 // logits are read once.
 //
-// One pass over a row: each lane keeps the largest of its logits so far, m, and the sums of exp(z - scale * m) and of exp(z - scale * m) *
-// (x - m), rescaled whenever m grows; the workgroup joins its lanes' afterwards. The entropy is log(s) - scale * t / s, in which
-// nothing large is left to cancel. The top tokens come from what the pass has anyway: of the lanes' largest logits, by 64 groups, the K-th
-// largest is one that K logits of the row reach, so that the lanes which reach it, few in most rows, look through theirs again for those
-// that do. Where too many do, or the row has NaN, the whole row is gone over K times.
+// One pass over a row: each lane has a number b that it takes exponentials relative to, and the sums of e = exp(z - b) and of e * (z - b).
+// b is the lane's first large z, and grows, the sums being rescaled, where a z lies more than kSlack above it: the sums have room for
+// e^kSlack, and most lanes never do. The workgroup joins its lanes' afterwards. The entropy is log(s) - t / s, in which nothing
+// large is left to cancel. The top tokens come from what the pass has
+// anyway: of the lanes' largest logits, by 64 groups, the K-th largest is one that K logits of the row reach, so that the lanes
+// which reach it, few in most rows, look through theirs again for those that do. Where too many do, or the row has NaN, the whole row is
+// gone over K times.
 #include "RowOps.hpp"
 
 #include <cvcuda/LogProbs.h>
@@ -19,7 +21,14 @@ namespace cvamd {
 namespace {
 
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr float kFar   = -1e30f; // below any difference of logits whose exponential isn't 0; a sum of 2^31 of it is finite
+constexpr float kLn2   = 0.6931471805599453f;
+constexpr float kFar   = -1e30f; // below any difference whose exponential isn't 0; a sum of 2^31 of it is finite
+constexpr float kSlack = 20.f;
+
+__device__ __forceinline__ float Exp(float x)
+{
+    return __builtin_amdgcn_exp2f(x * kLog2E);
+}
 constexpr int   kGroups = 64, kCandidates = 512;
 static_assert(CVCUDAX_LOG_PROBS_MOST_TOP <= kGroups, "as many groups as top tokens");
 
@@ -44,6 +53,11 @@ __device__ __forceinline__ uint32_t OrderOf(float x)
 {
     const uint32_t b = __float_as_uint(x + 0.f);
     return x != x ? 0xFFFFFFFFu : (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ float ValueOf(uint32_t order)
+{
+    return order == 0xFFFFFFFFu ? NAN : __uint_as_float((order & 0x80000000u) != 0 ? order & 0x7FFFFFFFu : ~order);
 }
 
 // A logit and its column: larger logits first, of equal ones the lower columns.
@@ -72,10 +86,9 @@ struct Logits
     }
 };
 
-template<int LANES>
 struct TopRoom
 {
-    uint32_t group[kGroups];
+    uint32_t group[kGroups], rank[kGroups];
     uint64_t key[kCandidates];
     uint32_t count;
 };
@@ -104,84 +117,151 @@ __device__ __forceinline__ uint64_t LargestKey(uint64_t v, uint64_t (&part)[WAVE
     return v;
 }
 
+// What the row's log probabilities are taken relative to: that of x is scale * x - base - logSum.
+struct Total
+{
+    float scale, base, logSum;
+    bool  nothing; // all logits are -infinity
+
+    __device__ __forceinline__ float of(float x) const
+    {
+        return nothing ? -INFINITY : __builtin_fmaf(x, scale, -base) - logSum;
+    }
+};
+
 // Entry `rank` of a row's top tokens.
-__device__ __forceinline__ void PutTop(const LogProbsArgs &a, uint32_t row, int rank, int column, float x, float largest, float logSum, bool nothing)
+__device__ __forceinline__ void PutTop(const LogProbsArgs &a, uint32_t row, int rank, uint64_t key, const Total &total)
 {
     const int64_t at = (int64_t)row * a.top + rank;
-    a.topTokens[at]  = column;
-    a.topValues[at]  = nothing ? -INFINITY : a.scale * (x - largest) - logSum;
+    a.topTokens[at]  = ColumnOf(key);
+    a.topValues[at]  = total.of(ValueOf((uint32_t)(key >> 32)));
 }
 
-// N: logits of a run (1 where rows are narrower than 16 bytes). One workgroup to a row.
-template<class T, int N, int WAVES>
+// A lane's sums on their way through the row.
+struct Sums
+{
+    float base, s, t, top; // top: the largest logit
+
+    __device__ __forceinline__ explicit Sums()
+        : base(-INFINITY)
+        , s(0)
+        , t(0)
+        , top(-INFINITY)
+    {
+    }
+
+    // N logits; (a NaN among them is left out of `top`, and reaches the sums)
+    template<int N>
+    __device__ __forceinline__ void add(const float (&v)[N], float scale)
+    {
+        float largest = v[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i)
+        {
+            largest = fmaxf(largest, v[i]);
+        }
+        top = fmaxf(top, largest);
+        if (largest * scale > base + kSlack)
+        {
+            const float to = largest * scale, less = fmaxf(base - to, kFar), r = Exp(less);
+            t    = r * __builtin_fmaf(s, less, t);
+            s    = s * r;
+            base = to;
+        }
+        const float from = base == -INFINITY ? 0.f : base; // (all were -infinity so far)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const float d = __builtin_fmaf(v[i], scale, -from), e = Exp(d);
+            s += e;
+            t = __builtin_fmaf(e, fmaxf(d, kFar), t); // (e is 0 where d is -infinity)
+        }
+    }
+};
+
+// N: logits of a run (1 where rows are narrower than 16 bytes). One workgroup to a row. HELD: the row fits the registers of runs on their
+// way, and is looked through again there.
+template<class T, int N, int WAVES, int AHEAD, bool HELD>
 __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs a)
 {
-    constexpr int       kLanes = 64 * WAVES, kAhead = 4;
-    __shared__ float    s_m[WAVES], s_s[WAVES], s_t[WAVES];
+    constexpr int       kLanes = 64 * WAVES;
+    __shared__ float    s_base[WAVES], s_s[WAVES], s_t[WAVES];
     __shared__ uint64_t s_key[WAVES];
-    __shared__ TopRoom<kLanes> s_top;
+    __shared__ TopRoom  s_top;
     const uint32_t row  = a.firstRow + blockIdx.x;
     const T       *in   = reinterpret_cast<const T *>(a.logits.at(row));
-    const int      runs = (a.columns + N - 1) / N;
-    const float    c    = a.scale * kLog2E;
-    float          m = -FLT_MAX, s = 0, t = 0;
-    Logits<T, N>   x[kAhead];
+    const int      runs = (a.columns + N - 1) / N, whole = a.columns / N;
+    Sums           sums;
+    Logits<T, N>   x[AHEAD];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
+    for (int k = 0; k < AHEAD; ++k)
     {
         x[k].get(in, a.columns, min((int)threadIdx.x + k * kLanes, runs - 1));
     }
-    for (int r = (int)threadIdx.x; r < runs; r += kAhead * kLanes)
+    // the token's own logit, on its way beside them
+    const int64_t token = TokenAt(a.tokens, a.wide, row);
+    const bool    there = token >= 0 && token < a.columns;
+    const float   its   = (float)in[there ? token : 0];
+    auto          take  = [&](const Logits<T, N> &l, int r)
+    {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            v[i] = (float)l.run.v[i];
+        }
+        if (r >= whole) // (the row's last run, where it is not a whole one)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+            {
+                v[i] = i >= l.skip ? v[i] : -INFINITY;
+            }
+        }
+        sums.add(v, a.scale);
+    };
+    for (int r = (int)threadIdx.x; r < runs; r += AHEAD * kLanes)
     {
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
+        for (int k = 0; k < AHEAD; ++k)
         {
             if (r + k * kLanes < runs)
             {
-                float v[N], top = m;
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                {
-                    v[i] = i >= x[k].skip ? (float)x[k].run.v[i] : -INFINITY;
-                    top  = fmaxf(top, v[i]); // (a NaN is left out)
-                }
-                const float less = fmaxf(m - top, kFar), r2 = __builtin_amdgcn_exp2f(less * c);
-                t = r2 * __builtin_fmaf(s, less, t);
-                s *= r2;
-                m = top;
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                {
-                    const float d = v[i] - m, e = __builtin_amdgcn_exp2f(d * c);
-                    s += e;
-                    t = __builtin_fmaf(e, fmaxf(d, kFar), t); // (e is 0 where d is -infinity)
-                }
+                take(x[k], r + k * kLanes);
             }
-            x[k].get(in, a.columns, min(r + (k + kAhead) * kLanes, runs - 1));
+            if (!HELD)
+            {
+                x[k].get(in, a.columns, min(r + (k + AHEAD) * kLanes, runs - 1));
+            }
         }
     }
-    // the workgroup's m, s and t; a lane that has met nothing but -infinity, or nothing, has s = 0
-    const float own = m;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2)
+    // the workgroup's sums; a lane that has met nothing but -infinity, or nothing, has s = 0
+    auto join = [&](float &base, float &s, float &t, float to)
     {
-        const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d), t2 = __shfl_xor(t, d), top = fmaxf(m, m2);
-        const float less = fmaxf(m - top, kFar), less2 = fmaxf(m2 - top, kFar), r = __builtin_amdgcn_exp2f(less * c), r2 = __builtin_amdgcn_exp2f(less2 * c);
-        t = (s != 0 ? r * __builtin_fmaf(s, less, t) : 0.f) + (s2 != 0 ? r2 * __builtin_fmaf(s2, less2, t2) : 0.f);
-        s = (s != 0 ? s * r : 0.f) + (s2 != 0 ? s2 * r2 : 0.f);
-        m = top;
-    }
+        const float less = fmaxf(base - to, kFar), r = Exp(less);
+        t    = s != 0 ? r * __builtin_fmaf(s, less, t) : 0.f;
+        s    = s != 0 ? r * s : 0.f;
+        base = to;
+    };
+    float base, s, t;
+    auto  ofWave = [&](float b, float sb, float tb)
+    {
+        base = ValueOf(WaveLargest(OrderOf(b)));
+        join(b, sb, tb, base);
+        s = WaveSum(sb), t = WaveSum(tb);
+    };
+    ofWave(sums.base, sums.s, sums.t);
     if constexpr (WAVES > 1)
     {
         if ((threadIdx.x & 63) == 0)
         {
-            s_m[WaveOfGroup()] = m, s_s[WaveOfGroup()] = s, s_t[WaveOfGroup()] = t;
+            s_base[WaveOfGroup()] = base, s_s[WaveOfGroup()] = s, s_t[WaveOfGroup()] = t;
         }
     }
     if (a.top > 0)
     {
         // groups of WAVES lanes that follow one another
-        float g = own;
+        float g = sums.top;
 #pragma unroll
         for (int d = 1; d < WAVES; d *= 2)
         {
@@ -191,6 +271,10 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         {
             s_top.group[threadIdx.x / WAVES] = OrderOf(g);
         }
+        if (threadIdx.x < kGroups)
+        {
+            s_top.rank[threadIdx.x] = 0;
+        }
         if (threadIdx.x == 0)
         {
             s_top.count = 0;
@@ -199,74 +283,88 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     __syncthreads();
     if constexpr (WAVES > 1)
     {
-        m = -FLT_MAX;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w)
-        {
-            m = fmaxf(m, s_m[w]);
-        }
-        s = 0, t = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w)
-        {
-            if (s_s[w] != 0)
-            {
-                const float less = fmaxf(s_m[w] - m, kFar), r = __builtin_amdgcn_exp2f(less * c);
-                t += r * __builtin_fmaf(s_s[w], less, s_t[w]);
-                s += r * s_s[w];
-            }
-        }
+        const uint32_t w = threadIdx.x % 64 % WAVES;
+        const bool     one = threadIdx.x % 64 < WAVES;
+        ofWave(one ? s_base[w] : -INFINITY, one ? s_s[w] : 0.f, one ? s_t[w] : 0.f);
     }
-    const bool  nothing = s == 0; // all logits are -infinity
-    const float logSum  = nothing ? 0.f : logf(s);
+    const Total total = {a.scale, base, s == 0 ? 0.f : __builtin_amdgcn_logf(s) * kLn2, s == 0};
     if (threadIdx.x == 0)
     {
-        const int64_t token = TokenAt(a.tokens, a.wide, row);
-        float         p     = 0;
-        if (token >= 0 && token < a.columns)
-        {
-            p = nothing ? -INFINITY : a.scale * ((float)in[token] - m) - logSum;
-        }
-        a.out[row] = p;
+        a.out[row] = there ? total.of(its) : 0.f;
         if (a.entropy != nullptr)
         {
-            a.entropy[row] = nothing ? 0.f : logSum - a.scale * (t / s);
+            a.entropy[row] = total.nothing ? 0.f : total.logSum - t / s;
         }
         if (a.lse != nullptr)
         {
-            a.lse[row] = nothing ? -INFINITY : __builtin_fmaf(a.scale, m, logSum);
+            a.lse[row] = total.nothing ? -INFINITY : base + total.logSum;
         }
     }
     if (a.top == 0)
     {
         return;
     }
-    // the K-th largest of the groups' largest logits
+    // the K-th largest of the groups' largest logits: each wave counts for some of them how many groups they lie before
     const uint32_t mine = s_top.group[threadIdx.x & 63];
-    int            rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < kGroups; ++j)
+    uint32_t       rank = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups / WAVES; ++i)
     {
+        const int      j     = (int)WaveOfGroup() * (kGroups / WAVES) + i;
         const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
         rank += other > mine || (other == mine && j < (int)(threadIdx.x & 63)) ? 1 : 0;
     }
-    const uint32_t least = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)__builtin_ctzll(__ballot(rank == a.top - 1)));
-    if (OrderOf(own) >= least && s == s)
+    if constexpr (WAVES > 1)
     {
-        for (int r = (int)threadIdx.x; r < runs; r += kLanes)
-        {
-            Logits<T, N> l;
-            l.get(in, a.columns, r);
+        atomicAdd(&s_top.rank[threadIdx.x & 63], rank);
+        __syncthreads();
+        rank = s_top.rank[threadIdx.x & 63];
+    }
+    const uint32_t least = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)__builtin_ctzll(__ballot((int)rank == a.top - 1)));
+    auto           look  = [&](const Logits<T, N> &l)
+    {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i)
+        {
+            const float v = (float)l.run.v[i];
+            if (i >= l.skip && OrderOf(v) >= least)
             {
-                const float v = (float)l.run.v[i];
-                if (i >= l.skip && OrderOf(v) >= least)
+                const uint32_t at = atomicAdd(&s_top.count, 1u);
+                if (at < kCandidates)
                 {
-                    const uint32_t at = atomicAdd(&s_top.count, 1u);
-                    if (at < kCandidates)
+                    s_top.key[at] = KeyOf(v, l.from + i);
+                }
+            }
+        }
+    };
+    if (OrderOf(sums.top) >= least && s == s)
+    {
+        if constexpr (HELD)
+        {
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+            {
+                if ((int)threadIdx.x + k * kLanes < runs)
+                {
+                    look(x[k]);
+                }
+            }
+        }
+        else
+        {
+            for (int r = (int)threadIdx.x; r < runs; r += AHEAD * kLanes)
+            {
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+                {
+                    x[k].get(in, a.columns, min(r + k * kLanes, runs - 1));
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+                {
+                    if (r + k * kLanes < runs)
                     {
-                        s_top.key[at] = KeyOf(v, l.from + i);
+                        look(x[k]);
                     }
                 }
             }
@@ -286,7 +384,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
             }
             if (above < a.top)
             {
-                PutTop(a, row, above, ColumnOf(key), (float)in[ColumnOf(key)], m, logSum, nothing);
+                PutTop(a, row, above, key, total);
             }
         }
         return;
@@ -309,7 +407,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         before = LargestKey<WAVES>(best, s_key);
         if (threadIdx.x == 0)
         {
-            PutTop(a, row, k, ColumnOf(before), (float)in[ColumnOf(before)], m, logSum, nothing);
+            PutTop(a, row, k, before, total);
         }
     }
 }
@@ -384,14 +482,25 @@ __global__ __launch_bounds__(kGradThreads) void LogProbsGradKernel(const LogProb
     }
 }
 
+constexpr int kAhead = 4; // runs of a lane on their way
+
 template<class T, int N, int WAVES>
 void LaunchRows(LogProbsArgs a, hipStream_t stream)
 {
     constexpr int most = INT32_MAX / (64 * WAVES);
+    const bool    held = a.columns <= kAhead * 64 * WAVES * N;
     for (int64_t first = 0; first < a.rows; first += most)
     {
-        a.firstRow = (int32_t)first;
-        LogProbsKernel<T, N, WAVES><<<(uint32_t)std::min<int64_t>(most, a.rows - first), 64 * WAVES, 0, stream>>>(a);
+        const uint32_t blocks = (uint32_t)std::min<int64_t>(most, a.rows - first);
+        a.firstRow            = (int32_t)first;
+        if (held)
+        {
+            LogProbsKernel<T, N, WAVES, kAhead, true><<<blocks, 64 * WAVES, 0, stream>>>(a);
+        }
+        else
+        {
+            LogProbsKernel<T, N, WAVES, kAhead, false><<<blocks, 64 * WAVES, 0, stream>>>(a);
+        }
         CheckLaunch("log probabilities");
     }
 }
