@@ -309,28 +309,28 @@ __device__ __forceinline__ uint32_t WaveTotal(uint32_t v)
 // sequences (up to 64 of them), so that the workgroups that begin last are short ones (long_attention_grad 863 us, 835 with it).
 __device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, uint32_t t, uint32_t most, int size, int each, bool ofKeys, bool causal)
 {
-    const int lane    = (int)(threadIdx.x & 63);
-    auto      tilesOf = [&](int b)
+    const int lane = (int)(threadIdx.x & 63);
+    // the lane's sequence, with all that a tile needs of it, and its tiles
+    SequenceTile own;
+    uint32_t     tiles;
+    auto         look = [&](int base)
     {
-        const int first = ofKeys ? s.firstKey(b) : s.firstRow(b);
-        return ((uint32_t)(ofKeys ? s.keysOf(b, first) : s.rowsOf(b, first)) * (uint32_t)each + (uint32_t)size - 1) / (uint32_t)size;
+        const int b = min(base + lane, s.count - 1);
+        own.firstRow = s.firstRow(b), own.rows = s.rowsOf(b, own.firstRow);
+        own.firstKey = s.firstKey(b), own.keys = s.keysOf(b, own.firstKey);
+        tiles = base + lane < s.count ? ((uint32_t)(ofKeys ? own.keys : own.rows) * (uint32_t)each + (uint32_t)size - 1) / (uint32_t)size : 0;
     };
-    auto found = [&](int b, uint32_t tile)
+    auto found = [&](int at, uint32_t tile)
     {
-        SequenceTile r;
-        r.tile     = (int)tile;
-        r.firstRow = s.firstRow(b);
-        r.rows     = s.rowsOf(b, r.firstRow);
-        r.firstKey = s.firstKey(b);
-        r.keys     = s.keysOf(b, r.firstKey);
-        return r;
+        return SequenceTile{__builtin_amdgcn_readlane(own.firstRow, at), __builtin_amdgcn_readlane(own.rows, at), __builtin_amdgcn_readlane(own.firstKey, at),
+                            __builtin_amdgcn_readlane(own.keys, at), (int)tile};
     };
     if (causal && s.count <= 64)
     {
-        const uint32_t tiles = tilesOf(min(lane, s.count - 1)), own = lane < s.count ? tiles : 0;
+        look(0);
         // of the tiles that have at least `low` less heavy ones in their sequence there are more than t
-        auto     of  = [&](uint32_t less) { return WaveTotal(own > less ? own - less : 0); };
-        uint32_t low = 0, high = WaveLargest(own);
+        auto     of  = [&](uint32_t less) { return WaveTotal(tiles > less ? tiles - less : 0); };
+        uint32_t low = 0, high = WaveLargest(tiles);
         if (of(0) <= t)
         {
             return {0, 0, 0, 0, -1};
@@ -341,18 +341,17 @@ __device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, ui
             of(middle) > t ? low = middle : high = middle;
         }
         const uint32_t rank = t - of(low + 1);
-        const uint64_t some = __ballot(own > low);
+        const uint64_t some = __ballot(tiles > low);
         const uint32_t at   = __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
-        const int      b    = (int)__builtin_ctzll(__ballot(own > low && at == rank));
-        return found(b, ofKeys ? (uint32_t)__builtin_amdgcn_readlane((int)own, b) - 1 - low : low);
+        const int      b    = (int)__builtin_ctzll(__ballot(tiles > low && at == rank));
+        return found(b, ofKeys ? (uint32_t)__builtin_amdgcn_readlane((int)tiles, b) - 1 - low : low);
     }
     t               = causal && !ofKeys ? most - 1 - t : t;
     uint32_t before = 0; // tiles of the sequences that were looked at
     for (int base = 0; base < s.count; base += 64)
     {
-        const int      b = base + lane;
-        const uint32_t all = tilesOf(min(b, s.count - 1)), tiles = b < s.count ? all : 0;
-        uint32_t       upTo = tiles; // this sequence's and those of the lanes before
+        look(base);
+        uint32_t upTo = tiles; // this sequence's and those of the lanes before
 #pragma unroll
         for (int d = 1; d < 64; d *= 2)
         {
@@ -363,8 +362,7 @@ __device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, ui
         if (behind != 0)
         {
             const int at = (int)__builtin_ctzll(behind);
-            return found(base + at,
-                         t - before - ((uint32_t)__builtin_amdgcn_readlane((int)upTo, at) - (uint32_t)__builtin_amdgcn_readlane((int)tiles, at)));
+            return found(at, t - before - ((uint32_t)__builtin_amdgcn_readlane((int)upTo, at) - (uint32_t)__builtin_amdgcn_readlane((int)tiles, at)));
         }
         before += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
     }

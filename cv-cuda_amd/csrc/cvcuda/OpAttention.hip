@@ -137,13 +137,21 @@ __device__ __forceinline__ float LseOf(float top, float sum)
 }
 
 // ---- prompts: 128 rows to a workgroup, 32 to a wave ------------------------------------------------------------------
-constexpr int kManyRows = 128, kManyKeys = 64, kManyThreads = 256;
+constexpr int kManyRows = 128, kManyThreads = 256;
+
+// Keys of a tile, and waves to a SIMD.
+template<int DP>
+constexpr int kManyKeys = DP > 64 ? 32 : 64;
+template<int DP>
+constexpr int kManyWaves = DP > 64 ? 3 : 4;
+
 
 template<class T, int DP>
-__global__ __launch_bounds__(kManyThreads, 2) void AttentionKernel(const AttentionArgs a)
+__global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(const AttentionArgs a)
 {
-    __shared__ __attribute__((aligned(256))) uint8_t s_k0[kManyKeys * DP * 2], s_k1[kManyKeys * DP * 2];
-    __shared__ __attribute__((aligned(256))) uint8_t s_v0[kManyKeys * DP * 2], s_v1[kManyKeys * DP * 2];
+    constexpr int kKeys = kManyKeys<DP>;
+    __shared__ __attribute__((aligned(256))) uint8_t s_k0[kKeys * DP * 2], s_k1[kKeys * DP * 2];
+    __shared__ __attribute__((aligned(256))) uint8_t s_v0[kKeys * DP * 2], s_v1[kKeys * DP * 2];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
     const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
     const SequenceTile s       = FindTile(a.sequences, t, a.tiles, kManyRows, a.rows.size(), false, a.causal);
@@ -158,14 +166,14 @@ __global__ __launch_bounds__(kManyThreads, 2) void AttentionKernel(const Attenti
     auto       limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
     const int  tileKeys = max(limitAt(first + kManyRows - 1) + 1, 0), waveKeys = ownFirst < all ? limitAt(ownFirst + 31) + 1 : 0;
     const int  seenKeys = limitAt(ownFirst) + 1;
-    const int  parts    = (tileKeys + kManyKeys - 1) / kManyKeys;
+    const int  parts    = (tileKeys + kKeys - 1) / kKeys;
     const int  from = (int)((int64_t)parts * blockIdx.y / a.splits), to = (int)((int64_t)parts * (blockIdx.y + 1) / a.splits);
     const uint8_t *k = a.k + s.firstKey * a.kToken + keyHead * a.kHead, *v = a.v + s.firstKey * a.vToken + keyHead * a.vHead;
 
-    using Copy = TileCopy<kManyKeys, DP, kManyThreads / 64>;
+    using Copy = TileCopy<kKeys, DP, kManyThreads / 64>;
     auto load  = [&](int part, uint8_t *toK, uint8_t *toV)
     {
-        const int key = part * kManyKeys;
+        const int key = part * kKeys;
         Copy::rows(wave, toK, k + key * a.kToken, (uint32_t)a.kToken, s.keys - key, a.dims);
         Copy::rows(wave, toV, v + key * a.vToken, (uint32_t)a.vToken, s.keys - key, a.dims);
     };
@@ -178,7 +186,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void AttentionKernel(const Attenti
     Running<T, DP> run;
     auto           take = [&](int part, const uint8_t *fromK, const uint8_t *fromV, uint8_t *nextK, uint8_t *nextV)
     {
-        const int key = part * kManyKeys;
+        const int key = part * kKeys;
         CopiesAndBarrier(); // (all have done the part before: its place may be written over)
         if (part + 1 < to)
         {
@@ -186,9 +194,9 @@ __global__ __launch_bounds__(kManyThreads, 2) void AttentionKernel(const Attenti
         }
         if (key < waveKeys)
         {
-            Acc16 scores[kManyKeys / 32];
-            Scores<T, DP>(scores, fromK, q, key, row.limit, key + kManyKeys > seenKeys);
-            run.template add<kManyKeys>(scores, fromV, a.scale);
+            Acc16 scores[kKeys / 32];
+            Scores<T, DP>(scores, fromK, q, key, row.limit, key + kKeys > seenKeys);
+            run.template add<kKeys>(scores, fromV, a.scale);
         }
     };
     // (by turns of their own, so that the compiler sees that what is read is not what is on its way)
