@@ -125,49 +125,6 @@ __device__ __forceinline__ int RowOf(int i)
     return (i >> 2) * 8 + (int)((threadIdx.x & 63) >> 5) * 4 + (i & 3);
 }
 
-// A workgroup's part of a tile of ROWS rows on its way from memory to LDS: 16 bytes a piece, zeros for rows from `count` on and
-// elements from `dims` on. THREADS threads.
-template<int ROWS, int DP, int THREADS>
-struct TileLoad
-{
-    static constexpr int kUnits = DP / 8, kPieces = ROWS * kUnits / THREADS;
-    static_assert(ROWS * kUnits % THREADS == 0, "whole pieces");
-
-    uint4 piece[kPieces];
-
-    // `thread`: the caller's number among the THREADS. rowAt(r): where row r of the tile begins.
-    template<class F>
-    __device__ __forceinline__ void get(uint32_t thread, int count, int dims, F &&rowAt)
-    {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-        {
-            const int at = (int)thread + i * THREADS, row = at / kUnits, unit = at % kUnits;
-            piece[i] = make_uint4(0, 0, 0, 0);
-            if (row < count && unit * 8 < dims)
-            {
-                piece[i] = *reinterpret_cast<const uint4 *>(rowAt(row) + unit * 16);
-            }
-        }
-    }
-
-    // The same of rows at one distance from each other.
-    __device__ __forceinline__ void get(uint32_t thread, const uint8_t *base, int64_t rowStride, int count, int dims)
-    {
-        get(thread, count, dims, [&](int row) { return base + row * rowStride; });
-    }
-
-    __device__ __forceinline__ void put(uint32_t thread, uint8_t *tile) const
-    {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-        {
-            const int at = (int)thread + i * THREADS, row = at / kUnits, unit = at % kUnits;
-            *reinterpret_cast<uint4 *>(tile + TileAt<DP>(row, unit)) = piece[i];
-        }
-    }
-};
-
 // ROWS rows from memory to a tile in LDS, without a stop in registers, by WAVES waves. Each instruction moves 64 units to 64 places that
 // follow one another: the lanes' addresses make the exchange of units. The buffer ends behind the last row, and what lies behind
 // a buffer's end reads as zeros; lanes of units behind `dims` read there too.
@@ -216,6 +173,40 @@ struct TileCopy
             const int      row  = rowOf(wave, i) - i * WAVES * kOfOne;
             const uint32_t unit = unitOf(rowOf(wave, i));
             copy(wave, i, tile, from, (int)unit * 8 < dims ? (uint32_t)row * stride + unit * 16 : kNowhere, (uint32_t)(i * WAVES * kOfOne) * stride);
+        }
+    }
+};
+
+// A wave's tile of ROWS rows on its way to LDS in registers: where tiles follow one another without a barrier, and LDS holds one of them.
+template<int ROWS, int DP>
+struct TileLoad
+{
+    using Copy = TileCopy<ROWS, DP, 1>;
+    using Unit = uint32_t __attribute__((ext_vector_type(4)));
+
+    Unit unit[Copy::kCount];
+
+    // As TileCopy::rows.
+    __device__ __forceinline__ void get(const uint8_t *base, uint32_t stride, int count, int dims)
+    {
+        const uint32_t lane = threadIdx.x & 63, row = lane / Copy::kUnits, part = lane % Copy::kUnits;
+        const uint32_t bytes = (uint32_t)(min(count, ROWS) - 1) * stride + (uint32_t)dims * 2;
+        const uint32_t at    = (int)part * 8 < dims ? row * stride + part * 16 : Copy::kNowhere;
+        const auto     from  = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, (int)bytes, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < Copy::kCount; ++i)
+        {
+            unit[i] = __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, (int)((uint32_t)(i * Copy::kOfOne) * stride), 0);
+        }
+    }
+
+    __device__ __forceinline__ void put(uint8_t *tile) const
+    {
+        const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < Copy::kCount; ++i)
+        {
+            *reinterpret_cast<Unit *>(tile + TileAt<DP>((uint32_t)(i * Copy::kOfOne) + lane / Copy::kUnits, lane % Copy::kUnits)) = unit[i];
         }
     }
 };

@@ -24,7 +24,7 @@ struct AttentionArgs
     float             *partial, *partialLse; // [splits][heads][rows][dims], [splits][heads][rows]: where keys are split
     GroupRows          rows;                 // of a key head
     DivBy              keyHeads;
-    int32_t            heads, dims, splits;
+    int32_t            heads, dims, splits, chunkKeys;
     uint32_t           tiles;
     float              scale; // to the base 2
     bool               causal;
@@ -245,17 +245,18 @@ __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(
     }
 }
 
-// ---- few rows to a sequence (single tokens): 32 rows to a workgroup, every fourth 32 keys to each of its waves ------------
-constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4, kFewThreads = 64 * kFewWaves;
+// ---- few rows to a sequence (single tokens): 32 rows to a workgroup, of whose waves each takes every WAVES-th 32 keys -----------
+constexpr int kFewRows = 32, kFewKeys = 32;
 
-template<class T, int DP>
-__global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const AttentionArgs a)
+template<class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void AttentionFewKernel(const AttentionArgs a)
 {
     // each wave's keys and values, later its weighted values in 32 bits
-    __shared__ __attribute__((aligned(256))) uint8_t s_tile[kFewWaves][2 * kFewKeys * DP * 2];
-    __shared__ float                                 s_top[kFewWaves][kFewRows], s_sum[kFewWaves][kFewRows];
-    const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
-    const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
+    __shared__ __attribute__((aligned(256))) uint8_t s_tile[WAVES][2 * kFewKeys * DP * 2];
+    __shared__ float                                 s_top[WAVES][kFewRows], s_sum[WAVES][kFewRows];
+    // (a sequence's key heads next to each other on one XCD: what they read lies side by side. 88 us with one of eight heads to each XCD, 85)
+    const int          keyHead = (int)(blockIdx.x / a.tiles);
+    const uint32_t     t       = blockIdx.x - (uint32_t)keyHead * a.tiles;
     const SequenceTile s       = FindTile(a.sequences, t, a.tiles, kFewRows, a.rows.size(), false, false);
     if (s.tile < 0)
     {
@@ -267,16 +268,19 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
     auto           limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
     const int      tileKeys = max(limitAt(first + kFewRows - 1) + 1, 0), seenKeys = limitAt(first) + 1;
     const int      parts    = (tileKeys + kFewKeys - 1) / kFewKeys;
-    const int      from = (int)((int64_t)parts * blockIdx.y / a.splits) + (int)wave, to = (int)((int64_t)parts * (blockIdx.y + 1) / a.splits);
+    // its keys in as many pieces as have chunkKeys of them, all of about one length; the call's other pieces are empty
+    const int      pieces = min((max(tileKeys, 1) - 1) / a.chunkKeys + 1, a.splits), piece = (int)blockIdx.y;
+    const int      from = piece < pieces ? (int)((int64_t)parts * piece / pieces) + (int)wave : 0;
+    const int      to   = piece < pieces ? (int)((int64_t)parts * (piece + 1) / pieces) : 0;
     const uint8_t *k = a.k + s.firstKey * a.kToken + keyHead * a.kHead, *v = a.v + s.firstKey * a.vToken + keyHead * a.vHead;
     uint8_t       *keys = s_tile[wave], *values = keys + kFewKeys * DP * 2;
 
-    TileLoad<kFewKeys, DP, 64> nextK, nextV;
+    TileLoad<kFewKeys, DP> nextK, nextV;
     auto load = [&](int part)
     {
         const int key = part * kFewKeys;
-        nextK.get(lane, k + key * a.kToken, a.kToken, s.keys - key, a.dims);
-        nextV.get(lane, v + key * a.vToken, a.vToken, s.keys - key, a.dims);
+        nextK.get(k + key * a.kToken, (uint32_t)a.kToken, s.keys - key, a.dims);
+        nextV.get(v + key * a.vToken, (uint32_t)a.vToken, s.keys - key, a.dims);
     };
     if (from < to)
     {
@@ -285,17 +289,17 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
     Vec8<T> q[DP / 16];
     LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
     Running<T, DP> run;
-    for (int part = from; part < to; part += kFewWaves)
+    for (int part = from; part < to; part += WAVES)
     {
         const int key = part * kFewKeys;
         // (a wave's reads and writes of LDS take place in their order; the compiler is kept from changing it)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        nextK.put(lane, keys);
-        nextV.put(lane, values);
+        nextK.put(keys);
+        nextV.put(values);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (part + kFewWaves < to)
+        if (part + WAVES < to)
         {
-            load(part + kFewWaves);
+            load(part + WAVES);
         }
         Acc16 scores[1];
         Scores<T, DP>(scores, keys, q, key, row.limit, key + kFewKeys > seenKeys);
@@ -320,15 +324,19 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
         s_sum[wave][lane] = sum;
     }
     __syncthreads();
+    if (threadIdx.x >= 256)
+    {
+        return;
+    }
     const uint32_t r = threadIdx.x % kFewRows, d0 = threadIdx.x / kFewRows * (DP / 8);
-    float          top = -INFINITY, total = 0, weight[kFewWaves];
+    float          top = -INFINITY, total = 0, weight[WAVES];
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w)
+    for (int w = 0; w < WAVES; ++w)
     {
         top = fmaxf(top, s_top[w][r]);
     }
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w)
+    for (int w = 0; w < WAVES; ++w)
     {
         weight[w] = s_top[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_top[w][r] - top);
         total += weight[w] * s_sum[w][r];
@@ -349,7 +357,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
         {
             v8[i] = 0;
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w)
+            for (int w = 0; w < WAVES; ++w)
             {
                 v8[i] += weight[w] * reinterpret_cast<const float *>(s_tile[w])[(d0 + d + i) * kFewRows + r];
             }
@@ -390,7 +398,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
 }
 
 // The parts of the keys joined: 16 lanes to a row, 8 elements to a lane.
-constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 16;
+constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 16, kMostSplits = 64;
 
 template<class T>
 __global__ __launch_bounds__(kJoinThreads) void AttentionJoinKernel(const AttentionArgs a)
@@ -403,28 +411,58 @@ __global__ __launch_bounds__(kJoinThreads) void AttentionJoinKernel(const Attent
     }
     // (rows of no sequence have no parts)
     const int begin = a.sequences.firstRow(0), end = begin + a.sequences.rowsOf(a.sequences.count - 1, begin);
-    if (token < begin || token >= end || d >= a.dims)
+    if (token < begin || token >= end)
     {
         return;
     }
-    float top = -INFINITY, total = 0, out[8] = {};
-    for (int p = 0; p < a.splits; ++p)
-    {
-        top = fmaxf(top, a.partialLse[p * rows + number]);
-    }
-    for (int p = 0; p < a.splits; ++p)
-    {
-        const float lse = a.partialLse[p * rows + number], weight = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - top);
-        if (lse != -INFINITY)
-        {
-            const float *part = a.partial + (p * rows + number) * a.dims + d;
+    // lane l of the row has the lse of its pieces l, l + 16 ...
+    float lse[kMostSplits / 16], top = -INFINITY, total = 0, out[8] = {};
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kMostSplits / 16; ++i)
+    {
+        const int p = (int)(threadIdx.x % 16) + 16 * i;
+        lse[i]      = p < a.splits ? a.partialLse[p * rows + number] : -INFINITY;
+        top         = fmaxf(top, lse[i]);
+    }
+#pragma unroll
+    for (int n = 1; n < 16; n *= 2)
+    {
+        top = fmaxf(top, __shfl_xor(top, n));
+    }
+#pragma unroll
+    for (int i = 0; i < kMostSplits / 16; ++i)
+    {
+        const float weight = lse[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse[i] - top);
+        for (int l = 0; l < 16 && 16 * i + l < a.splits; l += 4)
+        {
+            // (pieces that are empty hold anything)
+            float4 part[4][2];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
             {
-                out[i] += weight * part[i];
+                const float4 *from = reinterpret_cast<const float4 *>(a.partial + (min(16 * i + l + n, a.splits - 1) * rows + number) * a.dims + min(d, a.dims - 8));
+                part[n][0] = from[0], part[n][1] = from[1];
             }
-            total += weight;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+            {
+                const float w = __shfl(weight, l + n, 16);
+                if (w != 0)
+                {
+                    const float v[8] = {part[n][0].x, part[n][0].y, part[n][0].z, part[n][0].w, part[n][1].x, part[n][1].y, part[n][1].z, part[n][1].w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                    {
+                        out[k] += w * v[k];
+                    }
+                    total += w;
+                }
+            }
         }
+    }
+    if (d >= a.dims)
+    {
+        return;
     }
     const float factor = total == 0 ? 0.f : 1.f / total;
     Run<T, 8>   made;
@@ -444,8 +482,8 @@ __global__ __launch_bounds__(kJoinThreads) void AttentionJoinKernel(const Attent
 struct Plan
 {
     bool     few;
-    int32_t  splits;
-    uint32_t tiles; // at most, of a key head
+    int32_t  splits, chunkKeys; // pieces of a sequence's keys at most, and keys of one where there are few rows
+    uint32_t tiles;             // at most, of a key head
 
     Plan(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t keyHeads)
     {
@@ -453,9 +491,22 @@ struct Plan
         few                  = matrix <= 48 * most;
         const int64_t size = few ? kFewRows : kManyRows, whole = (matrix + size - 1) / size;
         tiles              = (uint32_t)(whole + std::min(sequences, rows));
-        // as many workgroups as fill the card's CUs twice, each with 256 keys at least
         const int64_t groups = std::max<int64_t>(std::max(whole, std::min(sequences, rows)) * keyHeads, 1), each = keys / most;
-        splits               = (int32_t)std::max<int64_t>(std::min<int64_t>({512 / groups, each / 256, 64}), 1);
+        if (few)
+        {
+            // Pieces of one length whatever the sequences' lengths, so that no workgroup has much more to do than the others, and as many as
+            // the card holds at once where all caches are full (tokens_attention 83 us, with twice as many 85, with four times 101).
+            // Up to 1024 keys are not worth the second launch that joins pieces (700 keys: 17.7 us, 14.5 in one piece of eight waves).
+            const int64_t chunk = std::max<int64_t>(groups * each / 512, 256);
+            splits    = each <= 1024 ? 1 : (int32_t)std::max<int64_t>(std::min<int64_t>((2 * each + chunk - 1) / chunk, kMostSplits), 1);
+            chunkKeys = (int32_t)std::min<int64_t>(chunk, INT32_MAX / 2);
+        }
+        else
+        {
+            // as many workgroups as fill the card's CUs twice, each with 256 keys at least
+            splits    = (int32_t)std::max<int64_t>(std::min<int64_t>({512 / groups, each / 256, kMostSplits}), 1);
+            chunkKeys = 0;
+        }
     }
 
     int64_t partials(int64_t rows, int64_t heads) const
@@ -473,9 +524,14 @@ template<class T, int DP>
 void Launch(const AttentionArgs &a, bool few, hipStream_t stream)
 {
     const dim3 grid(a.tiles * a.keyHeads.d, (uint32_t)a.splits);
-    if (few)
+    // few workgroups: each with as many waves as LDS has room for
+    if (few && grid.x * grid.y <= 256)
     {
-        AttentionFewKernel<T, DP><<<grid, kFewThreads, 0, stream>>>(a);
+        AttentionFewKernel<T, DP, 8><<<grid, 512, 0, stream>>>(a);
+    }
+    else if (few)
+    {
+        AttentionFewKernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
     }
     else
     {
@@ -512,7 +568,7 @@ struct Attention
         const AttentionArgs a = {in.q.base, in.k.base, in.v.base, out.base, in.q.tokenStride, in.q.headStride, in.k.tokenStride, in.k.headStride,
                                  in.v.tokenStride, in.v.headStride, out.tokenStride, out.headStride, in.sequences, in.lse, partial,
                                  partial + plan.partials(in.q.tokens, in.q.heads) * in.q.dims, {DivBy((uint32_t)(in.q.heads / in.k.heads))},
-                                 DivBy((uint32_t)in.k.heads), in.q.heads, in.q.dims, plan.splits, plan.tiles, scale * kLog2E, causal};
+                                 DivBy((uint32_t)in.k.heads), in.q.heads, in.q.dims, plan.splits, plan.chunkKeys, plan.tiles, scale * kLog2E, causal};
         auto                launch = [&](auto t)
         {
             using T = decltype(t);

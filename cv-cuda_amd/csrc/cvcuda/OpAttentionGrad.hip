@@ -378,18 +378,22 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
         }
     };
     const RowsPlace<DP> place0 = {s_q0, s_grad0, s_base0, s_delta0}, place1 = {s_q1, s_grad1, s_base1, s_delta1};
+    // From the last tile to the first: with `causal` workgroups of one sequence see the same last rows, which all but one read from L2.
+    // (Four of five of long_attention_grad's
+    // reads missed L2 the other way round, 44 of 100 do now: 621 us and 614.)
+    const int last = begin + (max(all - begin, 1) - 1) / kOfRows * kOfRows;
     if (begin < all)
     {
         places(begin);
-        load(begin, place0);
+        load(last, place0);
     }
     Acc16 sumK[DP / 32] = {}, sumV[DP / 32] = {};
     auto  take = [&](int at, const RowsPlace<DP> &place, const RowsPlace<DP> &next)
     {
         CopiesAndBarrier(); // (all have done the tile before: its place may be written over)
-        if (at + kOfRows < all)
+        if (at > begin)
         {
-            load(at + kOfRows, next);
+            load(at - kOfRows, next);
         }
 #pragma unroll
         for (int part = 0; part < (kInPairs<DP> ? 1 : 2); ++part)
@@ -450,12 +454,12 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
             }
         }
     };
-    for (int at = begin; at < all; at += 2 * kOfRows)
+    for (int at = last; at >= begin && begin < all; at -= 2 * kOfRows)
     {
         take(at, place0, place1);
-        if (at + kOfRows < all)
+        if (at > begin)
         {
-            take(at + kOfRows, place1, place0);
+            take(at - kOfRows, place1, place0);
         }
     }
     if constexpr (kInPairs<DP>)
