@@ -5,8 +5,8 @@
 // b is the lane's first large z, and grows, the sums being rescaled, where a z lies more than kSlack above it: the sums have room for
 // e^kSlack, and most lanes never do. The workgroup joins its lanes' afterwards. The entropy is log(s) - t / s, in which nothing
 // large is left to cancel. The top tokens come from what the pass has
-// anyway: of the lanes' largest logits, by 64 groups, the K-th largest is one that K logits of the row reach, so that the lanes
-// which reach it, few in most rows, look through theirs again for those that do. Where too many do, or the row has NaN, the whole row is
+// anyway: a number that K of the lanes' largest logits, by 64 groups, reach is one that K logits of the row reach, so that the lanes
+// which reach it, few in most rows, look through theirs again for those that do (4096 rows of 128000 BF16 with the top 5 192 us). Where too many do, or the row has NaN, the whole row is
 // gone over K times.
 #include "RowOps.hpp"
 
@@ -29,7 +29,7 @@ __device__ __forceinline__ float Exp(float x)
 {
     return __builtin_amdgcn_exp2f(x * kLog2E);
 }
-constexpr int   kGroups = 64, kCandidates = 512;
+constexpr int   kGroups = 64, kCandidates = 512, kFewMore = 5;
 static_assert(CVCUDAX_LOG_PROBS_MOST_TOP <= kGroups, "as many groups as top tokens");
 
 struct LogProbsArgs
@@ -88,7 +88,7 @@ struct Logits
 
 struct TopRoom
 {
-    uint32_t group[kGroups], rank[kGroups];
+    uint32_t group[kGroups];
     uint64_t key[kCandidates];
     uint32_t count;
 };
@@ -279,10 +279,6 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         {
             s_top.group[threadIdx.x / WAVES] = OrderOf(g);
         }
-        if (threadIdx.x < kGroups)
-        {
-            s_top.rank[threadIdx.x] = 0;
-        }
         if (threadIdx.x == 0)
         {
             s_top.count = 0;
@@ -312,40 +308,50 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     {
         return;
     }
-    // the K-th largest of the groups' largest logits: each wave counts for some of them how many groups they lie before
+    // A logit that K groups' largest ones reach, and not many more: between the smallest and the largest of them, by halves.
     const uint32_t mine = s_top.group[threadIdx.x & 63];
-    uint32_t       rank = 0;
-#pragma unroll
-    for (int i = 0; i < kGroups / WAVES; ++i)
+    uint32_t       low = ~WaveLargest(~mine), high = s == s ? WaveLargest(mine) + 1 : low;
+    while (high - low > 1)
     {
-        const int      j     = (int)WaveOfGroup() * (kGroups / WAVES) + i;
-        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
-        rank += other > mine || (other == mine && j < (int)(threadIdx.x & 63)) ? 1 : 0;
+        const uint32_t middle = low + (high - low) / 2;
+        const int      reach  = __popcll(__ballot(mine >= middle));
+        reach >= a.top ? low = middle : high = middle;
+        if (reach >= a.top && reach < a.top + kFewMore)
+        {
+            break;
+        }
     }
-    if constexpr (WAVES > 1)
+    const float least = ValueOf(low);
+    auto        look  = [&](const Logits<T, N> &l)
     {
-        atomicAdd(&s_top.rank[threadIdx.x & 63], rank);
-        __syncthreads();
-        rank = s_top.rank[threadIdx.x & 63];
-    }
-    const uint32_t least = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)__builtin_ctzll(__ballot((int)rank == a.top - 1)));
-    auto           look  = [&](const Logits<T, N> &l)
-    {
+        float v[N], largest = -INFINITY;
 #pragma unroll
         for (int i = 0; i < N; ++i)
         {
-            const float v = (float)l.run.v[i];
-            if (i >= l.skip && OrderOf(v) >= least)
+            v[i] = (float)l.run.v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; i += 2)
+        {
+            largest = Largest(largest, v[i], v[std::min(i + 1, N - 1)]);
+        }
+        if (largest >= least)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
             {
-                const uint32_t at = atomicAdd(&s_top.count, 1u);
-                if (at < kCandidates)
+                if (i >= l.skip && v[i] >= least)
                 {
-                    s_top.key[at] = KeyOf(v, l.from + i);
+                    const uint32_t at = atomicAdd(&s_top.count, 1u);
+                    if (at < kCandidates)
+                    {
+                        s_top.key[at] = KeyOf(v[i], l.from + i);
+                    }
                 }
             }
         }
     };
-    if (OrderOf(sums.top) >= least && s == s)
+    if (sums.top >= least && s == s)
     {
         if constexpr (HELD)
         {
@@ -380,6 +386,25 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     }
     __syncthreads();
     const int count = (int)s_top.count;
+    if (s == s && count >= a.top && count <= 64)
+    {
+        if (threadIdx.x < 64)
+        {
+            const uint64_t key   = (int)threadIdx.x < count ? s_top.key[threadIdx.x] : 0;
+            int            above = 0;
+            for (int j = 0; j < count; ++j)
+            {
+                const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), j) << 32) |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, j);
+                above += other > key ? 1 : 0;
+            }
+            if ((int)threadIdx.x < count && above < a.top)
+            {
+                PutTop(a, row, above, key, total);
+            }
+        }
+        return;
+    }
     if (s == s && count >= a.top && count <= kCandidates)
     {
         for (int i = (int)threadIdx.x; i < count; i += kLanes)
@@ -490,7 +515,8 @@ __global__ __launch_bounds__(kGradThreads) void LogProbsGradKernel(const LogProb
     }
 }
 
-constexpr int kAhead = 4; // runs of a lane on their way
+// runs of a lane on their way (4096 rows of 128000 BF16, eight waves: with two 264 us, four 249, six 250, eight 262)
+constexpr int kAhead = 4;
 
 template<class T, int N, int WAVES>
 void LaunchRows(LogProbsArgs a, hipStream_t stream)
@@ -516,10 +542,34 @@ void LaunchRows(LogProbsArgs a, hipStream_t stream)
 template<class T, int N>
 void LaunchLogProbs(const LogProbsArgs &a, hipStream_t stream)
 {
-    a.columns <= 2048    ? LaunchRows<T, N, 1>(a, stream)
-    : a.columns <= 16384 ? LaunchRows<T, N, 4>(a, stream)
-    : a.columns <= 65536 && a.rows > 512 ? LaunchRows<T, N, 8>(a, stream)
-                                         : LaunchRows<T, N, 16>(a, stream);
+    if constexpr (N == 1)
+    {
+        LaunchRows<T, N, 1>(a, stream);
+    }
+    else
+    {
+        // Where rows fill the card, waves of 8 runs to a lane and more, so that joining lanes is little beside them: 20000 rows of 4000
+        // BF16 with the top 20 59 us with one wave, 82 with two; 2600 of 32000 45 with eight, 92 with sixteen; 1300 of 64000 46 and 49, 660 of
+        // 128000 48 and 44. Where there are fewer, more waves, until there are 4096: 64 rows of 2000 8.3 us with one, 6.5 with four; of 16000
+        // 10.3 with four, 8.5 with eight; of 64000 15.1 with eight, 12.7 with sixteen. A row of more than
+        // 32 runs has more than 32 groups of lanes with logits in all of them: with fewer than top tokens the whole row would be gone over.
+        const int runs = (a.columns + N - 1) / N;
+        const int many = runs <= 512 ? 1 : runs <= 1024 ? 2 : runs <= 2048 ? 4 : runs <= 8192 ? 8 : 16;
+        const int few  = runs <= 64 ? 1 : runs <= 128 ? 2 : runs <= 512 ? 4 : runs <= 2048 ? 8 : 16;
+        switch (std::max(many, std::min(few, 4096 / a.rows)))
+        {
+        case 0:
+        case 1: LaunchRows<T, N, 1>(a, stream); break;
+        case 2:
+        case 3: LaunchRows<T, N, 2>(a, stream); break;
+        case 4:
+        case 5:
+        case 6:
+        case 7: LaunchRows<T, N, 4>(a, stream); break;
+        case 16: LaunchRows<T, N, 16>(a, stream); break;
+        default: LaunchRows<T, N, 8>(a, stream); break;
+        }
+    }
 }
 
 template<class T, int N, bool ENTROPY>
