@@ -1,12 +1,15 @@
 #include "AttentionOps.hpp"
 
-#include <cmath>
+#include <algorithm>
 
 namespace cvamd {
 
 namespace {
 
 constexpr int kMostDims = 128, kAlign = 16;
+
+// Numbers of rows and keys, and what is added to them, stay below 2^31, and a launch's threads below 2^32.
+constexpr int64_t kMostRows = 1 << 29, kMostSequences = 1 << 21;
 
 const int32_t *TakeNumbers(NVCVTensorHandle h, const char *what, int64_t count)
 {
@@ -25,7 +28,7 @@ HeadsView TakeHeads(NVCVTensorHandle h, const char *what)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must hold F16 or BF16 values", what);
     }
-    if (v.tokenStride > kMostStride || v.headStride * v.heads > kMostStride)
+    if (v.tokenStride > kMostStride || v.headStride > kMostStride / std::max(v.heads, 1))
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "%s must have tokens, and all heads, within %ld bytes of one another", what, (long)kMostStride);
     }
@@ -36,13 +39,13 @@ HeadsView TakeHeads(NVCVTensorHandle h, const char *what)
 
 void RequireAttentionSizes(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t keyHeads, int64_t dims)
 {
-    if (rows < 0 || keys < 0 || sequences < 0 || sequences >= INT32_MAX || heads < 1 || keyHeads < 1 || heads % keyHeads != 0)
+    if (rows < 0 || keys < 0 || sequences < 0 || heads < 1 || keyHeads < 1 || heads % keyHeads != 0)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT,
                       "Rows, keys and sequences must not be negative, heads a multiple of the key heads, not %ld, %ld, %ld, %ld and %ld", (long)rows,
                       (long)keys, (long)sequences, (long)heads, (long)keyHeads);
     }
-    if (rows > INT32_MAX / heads || keys > INT32_MAX / keyHeads || sequences > INT32_MAX / keyHeads)
+    if (rows > (kMostRows - 1) / heads || keys > (kMostRows - 1) / keyHeads || sequences > (kMostSequences - 1) / keyHeads)
     {
         throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Too many rows, keys or sequences");
     }
@@ -97,9 +100,9 @@ AttentionInputs TakeAttention(NVCVTensorHandle hq, NVCVTensorHandle hk, NVCVTens
         }
         in.lse = reinterpret_cast<float *>(lse.base);
     }
-    if (!(scale > 0) || !std::isfinite(scale))
+    if (!(scale > 0) || !(scale <= 1e30f))
     {
-        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Scale must be finite and positive, not %g", (double)scale);
+        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Scale must be positive, at most 1e30, not %g", (double)scale);
     }
     return in;
 }

@@ -560,10 +560,6 @@ struct Attention
         {
             return;
         }
-        if ((int64_t)plan.tiles * in.k.heads > INT32_MAX / kManyThreads * 2)
-        {
-            throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Too many rows");
-        }
         float              *partial = reinterpret_cast<float *>(room);
         const AttentionArgs a = {in.q.base, in.k.base, in.v.base, out.base, in.q.tokenStride, in.q.headStride, in.k.tokenStride, in.k.headStride,
                                  in.v.tokenStride, in.v.headStride, out.tokenStride, out.headStride, in.sequences, in.lse, partial,

@@ -540,10 +540,6 @@ void SubmitGrad(hipStream_t stream, NVCVTensorHandle hgrad, NVCVTensorHandle hq,
     const int64_t group = in.q.heads / in.k.heads, rows = in.q.tokens, keys = in.k.tokens, sequences = in.sequences.count;
     const int64_t tiles    = (rows * group + kGradRows - 1) / kGradRows + std::min(sequences, rows);
     const int64_t keyTiles = (keys + kOfKeys - 1) / kOfKeys + std::min(sequences, keys);
-    if (std::max(tiles, keyTiles) * in.k.heads > INT32_MAX / kGradThreads * 2)
-    {
-        throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Too many rows or keys");
-    }
     const int64_t  bounds = (std::max(rows, keys) + kBoundTokens * kBoundThreads / 64 - 1) / (kBoundTokens * kBoundThreads / 64);
     float2        *largest = reinterpret_cast<float2 *>(room);
     const AttentionGradArgs a = {

@@ -18,15 +18,16 @@
  * end lies before its begin as empty.
  *
  * q, out, gradOut, gradQ  : [Tq, Hq, D]; k, v, gradK, gradV: [Tk, Hk, D]; F16 or BF16 (NVCVX_DATA_TYPE_BF16), one type for all. Hk
- *                           divides Hq. D: a multiple of 8, at most 128. A row's elements follow one another, tokens and heads may lie
- *                           at any distances of whole 16 bytes, aligned to 16 bytes (such as parts of one projection's result).
+ *                           divides Hq. D: a multiple of 8, at most 128. A row's elements follow one another; tokens
+ *                           and heads lie at any distances of whole 16 bytes, aligned to 16 bytes (such as parts of one projection's
+ *                           result), a token's heads within 2^24 bytes, and the next token as well.
  *                           Outputs must not overlap inputs nor each other.
  * offsets, keyOffsets     : S32, dense, B + 1 elements each, ascending; keyLengths: S32, B elements, only beside keyOffsets.
  * lse                     : F32, [Hq, Tq], dense. NULL if not wanted; an input of the gradient.
  * workspace               : U8, dense, at least as many elements as cvcudaxAttentionWorkspace or ...GradWorkspace gives (for any lengths of
  *                           the sequences), aligned to 16 bytes. It belongs to the call until the stream has passed it; NULL
  *                           where 0 bytes are needed.
- * scale: finite, positive. Tq * Hq and Tk * Hk below 2^31; tensors may be larger than 2^32 bytes.
+ * scale: positive, at most 1e30. Tq * Hq and Tk * Hk below 2^29, B * Hk below 2^21; tensors may be larger than 2^32 bytes.
  * Status: INVALID_ARGUMENT for any type / shape / stride problem. */
 #ifndef CVCUDA_ATTENTION_H
 #define CVCUDA_ATTENTION_H

@@ -178,3 +178,33 @@ def test_native_calls_are_handed_on(cv):
         api.rotary(None, None)
     with pytest.raises((api.Error, TypeError, ValueError, AttributeError)):
         api.log_probs(None, None)
+
+
+@pytest.mark.parametrize("gradient", [False, True])
+def test_attention_refuses_what_its_addresses_do_not_reach(cv, gradient):
+    op = cv.AttentionGrad() if gradient else cv.Attention()
+    good = attention_parts(cv)
+    if gradient:
+        room = cv.AttentionGrad.workspace(6, 6, 2, 4, 2, 16)
+        good.update(grad=good["out"], grad_q=good["out"], grad_k=good["k"], grad_v=good["v"], workspace=fake(cv, [room], np.uint8))
+
+    def no(**change):
+        refused(cv, op, 0, **dict(good, **change))
+
+    far = (1 << 23) + 8                                                        # elements: 2^24 bytes and 16
+    no(k=fake(cv, [6, 2, 16], BF16, "TWE", strides=[far, 16, 1]))
+    no(v=fake(cv, [6, 2, 16], BF16, "TWE", strides=[far, 16, 1]))
+    no(out=fake(cv, [6, 4, 16], BF16, "TWE", strides=[far, 16, 1]))
+    # a single token, whose heads alone lie too far from one another
+    one = attention_parts(cv, rows=1, keys=1, sequences=1)
+    refused(cv, cv.Attention(), 0, **dict(one, q=fake(cv, [1, 4, 16], BF16, "TWE", strides=[4 * ((1 << 21) + 8), (1 << 21) + 8, 1])))
+    no(scale=2e30)
+
+
+@pytest.mark.parametrize("name", ["Attention", "AttentionGrad"])
+def test_sizes_that_kernels_cannot_count(cv, name):
+    workspace = getattr(cv, name).workspace
+    for sizes in ((1 << 27, 1, 1, 4, 2, 16), (1, 1 << 28, 1, 4, 2, 16), (1, 1, 1 << 20, 4, 2, 16), (1 << 62, 1, 1, 4, 2, 16), (1, 1 << 62, 1, 4, 2, 16),
+                  (1, 1, 1 << 62, 4, 2, 16)):
+        refused(cv, workspace, *sizes)
+    assert workspace((1 << 27) - 1, (1 << 28) - 1, (1 << 20) - 1, 4, 2, 16) >= 0
