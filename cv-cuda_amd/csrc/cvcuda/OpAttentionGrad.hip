@@ -24,12 +24,10 @@ struct AttentionGradArgs
     AttentionSequences sequences;
     const float       *lse;
     float             *base, *delta; // [rows][heads]: ShareBase and gradOut . out
-    float2            *largest; // F16: of each of the first kernel's workgroups, the largest squares of rows of gradOut and of v
-    int32_t            largestCount;
     GroupRows          rows; // of a key head
-    DivBy              keyHeads, queryHeads;
+    DivBy              keyHeads;
     int32_t            heads, dims;
-    uint32_t           tiles, keyTiles, boundTiles;
+    uint32_t           tiles, keyTiles;
     float              scale;
     bool               causal;
 
@@ -51,106 +49,49 @@ __device__ __forceinline__ float ShareBase(float lse)
     return lse == -INFINITY ? INFINITY : __builtin_fmaf(lse, kLog2E, -kShareShift<T>);
 }
 
-// ---- F16: what bounds the shares' gradients ------------------------------------------------------------------------------
-constexpr int kBoundThreads = 1024, kBoundBlocks = 512, kBoundTokens = 4; // the last: of keys, to a wave
-
-// The larger of two sums of squares; one that is not finite (its sequence's gradients aren't either) counts for nothing.
-__device__ __forceinline__ float Larger(float a, float b)
+// The larger of a and the magnitudes of b and c.
+__device__ __forceinline__ float LargestMagnitude(float a, float b, float c)
 {
-    return b < INFINITY ? fmaxf(a, b) : a;
+    float r;
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
 }
 
-// The largest square of rows of `tokens` tokens from `base` on, of which the wave takes every `step`-th LANES-th of a wave from `first` on. LANES
-// lanes to a row, 8 elements to a lane.
-template<class T, int LANES>
-__device__ __forceinline__ float LargestSquare(const uint8_t *base, int64_t tokenStride, int64_t headStride, const DivBy &heads, uint32_t tokens, int dims,
-                                               uint32_t first, uint32_t step)
-{
-    const uint32_t lane = threadIdx.x & 63, rows = tokens * heads.d;
-    const int      d       = (int)(lane % LANES) * 8, from = min(d, dims - 8);
-    float          largest = 0;
-#pragma unroll 4
-    for (uint32_t r = first * (64 / LANES) + lane / LANES; r < rows; r += step * (64 / LANES))
-    {
-        const uint32_t  token = heads.Quotient(r), head = r - token * heads.d;
-        const Run<T, 8> x      = *reinterpret_cast<const Run<T, 8> *>(base + token * tokenStride + head * headStride + from * 2);
-        float           square = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-        {
-            square = __builtin_fmaf((float)x.v[i], (float)x.v[i], square);
-        }
-        square = d < dims ? square : 0.f;
-#pragma unroll
-        for (int n = 1; n < LANES; n *= 2)
-        {
-            square += __shfl_xor(square, n);
-        }
-        largest = Larger(largest, square);
-    }
-    return largest;
-}
-
-template<class T, int DP>
-__global__ __launch_bounds__(kBoundThreads) void AttentionBoundKernel(const AttentionGradArgs a)
-{
-    __shared__ float2 s_largest[kBoundThreads / 64];
-    const uint32_t    wave = blockIdx.x * (kBoundThreads / 64) + WaveOfGroup(), waves = gridDim.x * (kBoundThreads / 64);
-    // the sequences' rows lie one behind the other, their keys may lie in places of a cache, which hold anything behind them
-    const int begin = a.sequences.firstRow(0), end = begin + a.sequences.rowsOf(a.sequences.count - 1, begin);
-    float     ofGrad = LargestSquare<T, DP / 8>(a.grad + begin * a.gradToken, a.gradToken, a.gradHead, a.queryHeads, (uint32_t)(end - begin), a.dims, wave,
-                                            waves);
-    float     ofValues = 0;
-    for (uint32_t t = wave; t < a.boundTiles; t += waves)
-    {
-        const SequenceTile s = FindTile(a.sequences, t, 0, kBoundTokens, 1, true, false);
-        if (s.tile < 0)
-        {
-            break;
-        }
-        const int first = s.tile * kBoundTokens;
-        ofValues = fmaxf(ofValues, LargestSquare<T, DP / 8>(a.v + (s.firstKey + first) * a.vToken, a.vToken, a.vHead, a.keyHeads,
-                                                            (uint32_t)min(s.keys - first, kBoundTokens), a.dims, 0, 1));
-    }
-    ofGrad                     = __uint_as_float(WaveLargest(__float_as_uint(ofGrad)));
-    ofValues                   = __uint_as_float(WaveLargest(__float_as_uint(ofValues)));
-    if ((threadIdx.x & 63) == 0)
-    {
-        s_largest[WaveOfGroup()] = make_float2(ofGrad, ofValues);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0)
-    {
-        float2 largest = s_largest[0];
-        for (int w = 1; w < kBoundThreads / 64; ++w)
-        {
-            largest = make_float2(Larger(largest.x, s_largest[w].x), Larger(largest.y, s_largest[w].y));
-        }
-        a.largest[blockIdx.x] = largest;
-    }
-}
-
-// The power of two by which the shares' gradients t are multiplied before they are rounded to T. In F16 small ones would be lost (its
-// smallest number is 2^-24) and large ones have no bound in T, but |t| <= 2 |gradOut| |v| (out is a mean of values): with the longest of
-// these rows it stays below 2^14, and what is 2^-28 of that keeps all of its bits.
+// What the shares' gradients t are multiplied with before they are rounded to T. In F16 small ones would be lost (its smallest number is 2^-24)
+// and large ones are not bounded, so it is a power of two that follows the largest that the wave has met: at first one that no
+// small t is lost with, and lowered, with the sums so far, where a t passes 2^15, so that the largest is at 2^12 to 2^13 again. What is
+// 2^-26 of the largest keeps all of its bits. (Taken from the largest rows of gradOut and v, by a kernel that reads both before, it cost
+// pairs_attention_grad 13 us.)
 template<class T>
-__device__ __forceinline__ float GradFactor(const AttentionGradArgs &a)
+struct GradScale
 {
-    if constexpr (!std::is_same<T, Half>::value)
+    static constexpr bool kNeeded = std::is_same<T, Half>::value;
+
+    float factor = kNeeded ? 0x1p60f : 1.f;
+
+    // The products t of a tile, times `factor`, and what goes with them: delta, and the sums so far.
+    template<class F>
+    __device__ __forceinline__ void fit(Acc16 &t, F &&lower)
     {
-        return 1.f;
+        if constexpr (kNeeded)
+        {
+            float most = 0;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+            {
+                most = LargestMagnitude(most, t[i], t[i + 1]);
+            }
+            if (__any(most > 0x1p15f))
+            {
+                const uint32_t exponent = WaveLargest(__float_as_uint(most)) >> 23; // (127: 1 to 2; 255: not finite)
+                const float    less     = __uint_as_float((127u - min(exponent - (127u + 12u), 100u)) << 23);
+                factor *= less;
+                t *= less;
+                lower(less);
+            }
+        }
     }
-    float ofGrad = 0, ofValues = 0;
-    for (int i = (int)(threadIdx.x & 63); i < a.largestCount; i += 64)
-    {
-        ofGrad   = Larger(ofGrad, a.largest[i].x);
-        ofValues = Larger(ofValues, a.largest[i].y);
-    }
-    ofGrad            = __uint_as_float(WaveLargest(__float_as_uint(ofGrad)));
-    ofValues          = __uint_as_float(WaveLargest(__float_as_uint(ofValues)));
-    const float bound = sqrtf(ofGrad) * sqrtf(ofValues); // below 2^(ilogb + 1)
-    return bound == 0 ? 1.f : ldexpf(1.f, min(max(12 - ilogbf(bound), -100), 100));
-}
+};
 
 // ---- the queries' gradient: 128 rows to a workgroup, 32 to a wave --------------------------------------------------------
 constexpr int kGradRows = 128, kGradKeys = 64, kGradThreads = 256;
@@ -189,8 +130,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
     Vec8<T> q[DP / 16], grad[DP / 16];
     LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
     LoadColumn<T, DP>(grad, a.grad + row.token * a.gradToken + row.head * a.gradHead, a.dims);
-    const float factor = GradFactor<T>(a), base = ShareBase<T>(a.lse[(int64_t)row.head * a.sequences.rows + row.token]);
-    const float scale = a.scale * kLog2E, of = factor * __builtin_amdgcn_exp2f(-kShareShift<T>);
+    const float base = ShareBase<T>(a.lse[(int64_t)row.head * a.sequences.rows + row.token]), scale = a.scale * kLog2E;
     // gradOut . out, here and for the other kernel
     float dot = 0;
     {
@@ -212,9 +152,10 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
         a.base[a.number(row)]  = base;
         a.delta[a.number(row)] = dot;
     }
-    const float delta = dot * of;
-    Acc16       sum[DP / 32] = {};
-    auto        take = [&](int part, const uint8_t *fromK, const uint8_t *fromV, uint8_t *nextK, uint8_t *nextV)
+    GradScale<T> grow;
+    float        of = grow.factor * __builtin_amdgcn_exp2f(-kShareShift<T>), delta = dot * of;
+    Acc16        sum[DP / 32] = {};
+    auto         take = [&](int part, const uint8_t *fromK, const uint8_t *fromV, uint8_t *nextK, uint8_t *nextV)
     {
         const int key = part * kGradKeys;
         CopiesAndBarrier(); // (all have done the part before: its place may be written over)
@@ -252,6 +193,16 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
                     grads[i] = key + 32 * half + RowOf(i) <= row.limit ? grads[i] : 0.f;
                 }
             }
+            grow.fit(grads,
+                     [&](float less)
+                     {
+                         of *= less, delta *= less;
+#pragma unroll
+                         for (int p = 0; p < DP / 32; ++p)
+                         {
+                             sum[p] *= less;
+                         }
+                     });
 #pragma unroll
             for (int k16 = 0; k16 < 2; ++k16)
             {
@@ -273,7 +224,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
             take(part + 1, s_k1, s_v1, s_k0, s_v0);
         }
     }
-    StoreColumn<T, DP>(sum, a.scale / factor, a.gradQ + row.token * a.gradQToken + row.head * a.gradQHead, row.there, a.dims);
+    StoreColumn<T, DP>(sum, a.scale / grow.factor, a.gradQ + row.token * a.gradQToken + row.head * a.gradQHead, row.there, a.dims);
 }
 
 // ---- the keys' and values' gradients: 128 keys to a workgroup, 32 to a wave ------------------------------------------------
@@ -334,7 +285,9 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
     }
     auto keyOperand = [&](int step) { return kInPairs<DP> ? RowsOperand<T, DP>(s_k, 32 * ofKeys, step) : k[kInPairs<DP> ? 0 : step]; };
     auto valueOperand = [&](int step) { return kInPairs<DP> ? RowsOperand<T, DP>(s_v, 32 * ofKeys, step) : v[kInPairs<DP> ? 0 : step]; };
-    const float factor = GradFactor<T>(a), of = factor * __builtin_amdgcn_exp2f(-kShareShift<T>), scale = a.scale * kLog2E;
+    GradScale<T> grow;
+    float        of = grow.factor * __builtin_amdgcn_exp2f(-kShareShift<T>);
+    const float  scale = a.scale * kLog2E;
 
     // the lane's places in a tile, from its first token's on
     uint32_t placeQ[Copy::kCount], placeGrad[Copy::kCount], placeValue;
@@ -441,6 +394,16 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
             {
                 grads[i] = shares[i] * (std::is_same<T, Half>::value ? grads[i] * of : grads[i]);
             }
+            grow.fit(grads,
+                     [&](float less)
+                     {
+                         of *= less;
+#pragma unroll
+                         for (int p = 0; p < DP / 32; ++p)
+                         {
+                             sumK[p] *= less;
+                         }
+                     });
 #pragma unroll
             for (int r16 = 0; r16 < 2; ++r16)
             {
@@ -461,6 +424,12 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
         {
             take(at - kOfRows, place1, place0);
         }
+    }
+    // (here, since two waves that go together may have other factors)
+#pragma unroll
+    for (int p = 0; p < DP / 32; ++p)
+    {
+        sumK[p] *= a.scale / grow.factor;
     }
     if constexpr (kInPairs<DP>)
     {
@@ -494,14 +463,14 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
             return;
         }
     }
-    StoreColumn<T, DP>(sumK, a.scale / factor, a.gradK + (s.firstKey + key) * a.gradKToken + keyHead * a.gradKHead, there, a.dims);
+    StoreColumn<T, DP>(sumK, 1.f, a.gradK + (s.firstKey + key) * a.gradKToken + keyHead * a.gradKHead, there, a.dims);
     StoreColumn<T, DP>(sumV, __builtin_amdgcn_exp2f(-kShareShift<T>), a.gradV + (s.firstKey + key) * a.gradVToken + keyHead * a.gradVHead, there,
                        a.dims);
 }
 
 int64_t GradBytes(int64_t rows, int64_t heads)
 {
-    return kBoundBlocks * (int64_t)sizeof(float2) + 2 * rows * heads * (int64_t)sizeof(float);
+    return 2 * rows * heads * (int64_t)sizeof(float);
 }
 
 template<class T, int DP>
@@ -509,11 +478,6 @@ void Launch(const AttentionGradArgs &a, hipStream_t stream)
 {
     if (a.tiles > 0)
     {
-        if (std::is_same<T, Half>::value)
-        {
-            AttentionBoundKernel<T, DP><<<(uint32_t)a.largestCount, kBoundThreads, 0, stream>>>(a);
-            CheckLaunch("attention's gradient (bounds)");
-        }
         AttentionGradQKernel<T, DP><<<a.tiles * a.keyHeads.d, kGradThreads, 0, stream>>>(a);
         CheckLaunch("attention's gradient (queries)");
     }
@@ -540,16 +504,13 @@ void SubmitGrad(hipStream_t stream, NVCVTensorHandle hgrad, NVCVTensorHandle hq,
     const int64_t group = in.q.heads / in.k.heads, rows = in.q.tokens, keys = in.k.tokens, sequences = in.sequences.count;
     const int64_t tiles    = (rows * group + kGradRows - 1) / kGradRows + std::min(sequences, rows);
     const int64_t keyTiles = (keys + kOfKeys - 1) / kOfKeys + std::min(sequences, keys);
-    const int64_t  bounds = (std::max(rows, keys) + kBoundTokens * kBoundThreads / 64 - 1) / (kBoundTokens * kBoundThreads / 64);
-    float2        *largest = reinterpret_cast<float2 *>(room);
+    float *base = reinterpret_cast<float *>(room);
     const AttentionGradArgs a = {
         in.q.base, in.k.base, in.v.base, out.base, grad.base, gradQ.base, gradK.base, gradV.base, in.q.tokenStride, in.q.headStride,
         in.k.tokenStride, in.k.headStride, in.v.tokenStride, in.v.headStride, out.tokenStride, out.headStride, grad.tokenStride, grad.headStride,
         gradQ.tokenStride, gradQ.headStride, gradK.tokenStride, gradK.headStride, gradV.tokenStride, gradV.headStride, in.sequences, in.lse,
-        reinterpret_cast<float *>(largest + kBoundBlocks), reinterpret_cast<float *>(largest + kBoundBlocks) + rows * in.q.heads, largest,
-        (int32_t)std::max<int64_t>(std::min<int64_t>(bounds, kBoundBlocks), 1), {DivBy((uint32_t)group)}, DivBy((uint32_t)in.k.heads), DivBy((uint32_t)in.q.heads),
-        in.q.heads, in.q.dims, (uint32_t)tiles, (uint32_t)keyTiles,
-        (uint32_t)((keys + kBoundTokens - 1) / kBoundTokens + std::min(sequences, keys)), scale, causal};
+        base, base + rows * in.q.heads, {DivBy((uint32_t)group)}, DivBy((uint32_t)in.k.heads), in.q.heads, in.q.dims, (uint32_t)tiles,
+        (uint32_t)keyTiles, scale, causal};
     auto launch = [&](auto t)
     {
         using T = decltype(t);
