@@ -1148,12 +1148,13 @@ def _untouched_workspace():
     return _untouched[device]
 
 
-def _workspace(workspace, size, stream):
+def _workspace(workspace, size, stream, untouched=0):
     """The caller's workspace, or one for this call alone (None where none is needed). Not for a call that is captured: a graph
-    writes there in every replay, when others have the memory of what this call made."""
+    writes there in every replay, when others have the memory of what this call made. Of up to `untouched` bytes it is not written to,
+    and calls share one."""
     if workspace is not None or size == 0:
         return workspace
-    if size <= _UNTOUCHED_BYTES:
+    if size <= untouched:
         return _untouched_workspace()
     if _capturing(stream):
         raise Error(4, "a captured call of this kind needs workspace=, a tensor of %d bytes that lives as long as the graph" % size)  # INVALID_OPERATION
@@ -1188,7 +1189,7 @@ def layer_norm_grad_into(grad_src, grad_gamma, grad_beta, grad, src, gamma, mean
     (unless it is one of few rows, which touches none)."""
     sums = grad_gamma is not None or grad_beta is not None
     need = _layer_norm_workspace(*_rows_of(src)) if sums else 0
-    workspace = _workspace(workspace, need, stream)
+    workspace = _workspace(workspace, need, stream, _UNTOUCHED_BYTES)
     written = workspace if need > _UNTOUCHED_BYTES else None
     _run(stream, _given(grad, src, gamma, mean, rstd), _given(grad_src, grad_gamma, grad_beta, written), _op(LayerNormGrad), grad, src,
          gamma, mean, rstd, grad_src, grad_gamma, grad_beta, workspace)
@@ -1198,7 +1199,7 @@ def layer_norm_grad_into(grad_src, grad_gamma, grad_beta, grad, src, gamma, mean
 def layer_norm_grad(grad, src, gamma, mean, rstd, *, workspace=None, stream=None):
     """(gradient of src, of gamma, of beta); the latter have gamma's type, F32 without one."""
     kind = np.dtype(np.float32) if gamma is None else gamma.dtype
-    workspace = _workspace(workspace, _layer_norm_workspace(*_rows_of(src)), stream)  # (before anything is made)
+    workspace = _workspace(workspace, _layer_norm_workspace(*_rows_of(src)), stream, _UNTOUCHED_BYTES)  # (before anything is made)
     made = [_result((src.shape[-1],), kind, None, stream) for _ in range(2)]
     return layer_norm_grad_into(_like(src, stream), made[0], made[1], grad, src, gamma, mean, rstd, workspace=workspace, stream=stream)
 
@@ -1223,7 +1224,7 @@ def embedding_grad_into(grad_table, grad, tokens, scale=1.0, *, padding=None, ac
     if padding is not None and padding < 0:
         raise ValueError("padding is a token, or None")
     rows, columns = _rows_of(grad)
-    workspace = _workspace(workspace, _embedding_workspace(rows, _rows_of(grad_table)[0], columns), stream)
+    workspace = _workspace(workspace, _embedding_workspace(rows, _rows_of(grad_table)[0], columns), stream, _UNTOUCHED_BYTES)
     reads, writes = [grad, tokens], _given(grad_table, workspace)
     _run(stream, reads, writes, _op(EmbeddingGrad), grad, tokens, grad_table, workspace, float(scale), -1 if padding is None else int(padding),
          bool(accumulate))
@@ -1233,7 +1234,7 @@ def embedding_grad_into(grad_table, grad, tokens, scale=1.0, *, padding=None, ac
 def embedding_grad(grad, tokens, rows, scale=1.0, *, padding=None, dtype=None, workspace=None, stream=None):
     """The gradient of a table of `rows` rows, of `dtype` (none: grad's)."""
     count, columns = _rows_of(grad)
-    workspace = _workspace(workspace, _embedding_workspace(count, int(rows), columns), stream)  # (before anything is made)
+    workspace = _workspace(workspace, _embedding_workspace(count, int(rows), columns), stream, _UNTOUCHED_BYTES)  # (before anything is made)
     dst = _result((int(rows), grad.shape[-1]), grad.dtype if dtype is None else _np_dtype(dtype), None, stream)
     return embedding_grad_into(dst, grad, tokens, scale, padding=padding, workspace=workspace, stream=stream)
 

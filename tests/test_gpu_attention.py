@@ -390,3 +390,26 @@ def test_two_calls_at_once(api):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+def test_gradients_of_one_row_in_a_graph_and_beside_others(api):
+    """What the smallest call works with is its own: it needs a workspace when it is captured, and changes nobody else's."""
+    calls = [Call([(1, 1)], 1, 1, 8, BF16, 30 + i) for i in range(2)]
+    made = [c.run(api) for c in calls]
+    assert api.AttentionGrad.workspace(1, 1, 1, 1, 1, 8) > 0
+    api.layer_norm_grad(*[api.as_tensor(t) for t in (random((4, 8), BF16, 1), random((4, 8), BF16, 2))], None,
+                        *[api.as_tensor(torch.ones(4, device="cuda")) for _ in range(2)])
+    torch.cuda.synchronize()
+    before = {d: t.torch().clone() for d, t in api._untouched.items()}
+    for c, m in zip(calls, made):
+        c.check_gradients(api, *m)
+    torch.cuda.synchronize()
+    assert all(torch.equal(api._untouched[d].torch(), t) for d, t in before.items())
+    graph = torch.cuda.CUDAGraph()
+    t = {n: api.as_tensor(getattr(calls[0], n)) for n in ("q", "k", "v", "grad", "offsets")}
+    outs, lse = [api.as_tensor(torch.empty_like(calls[0].q)) for _ in range(4)], api.as_tensor(torch.empty((1, 1), device="cuda"))
+    with torch.cuda.graph(graph):
+        s = api.as_stream(torch.cuda.current_stream())
+        api.attention_into(outs[3], t["q"], t["k"], t["v"], t["offsets"], lse=lse, stream=s)
+        with pytest.raises(api.Error):
+            api.attention_grad_into(*outs[:3], t["grad"], t["q"], t["k"], t["v"], outs[3], lse, t["offsets"], stream=s)
