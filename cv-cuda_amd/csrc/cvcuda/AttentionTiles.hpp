@@ -275,6 +275,26 @@ __device__ __forceinline__ void StoreColumn(const Acc16 (&acc)[DP / 32], float f
     }
 }
 
+// The same to a row of F32, which is joined with those of other pieces.
+template<int DP>
+__device__ __forceinline__ void StorePiece(const Acc16 (&acc)[DP / 32], float factor, float *row, bool there, int dims)
+{
+#pragma unroll
+    for (int p = 0; p < DP / 32; ++p)
+    {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+        {
+            const int d = 32 * p + RowOf(i);
+            if (there && d < dims)
+            {
+                *reinterpret_cast<float4 *>(row + d) =
+                    make_float4(acc[p][i] * factor, acc[p][i + 1] * factor, acc[p][i + 2] * factor, acc[p][i + 3] * factor);
+            }
+        }
+    }
+}
+
 // ---- sequences -----------------------------------------------------------------------------------------------------
 // A sequence and one of its tiles.
 struct SequenceTile

@@ -221,27 +221,10 @@ __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(
         return;
     }
     const int64_t at = (int64_t)blockIdx.y * a.heads * a.sequences.rows + number;
-    if (row.there)
+    StorePiece<DP>(run.out, factor, a.partial + at * a.dims, row.there, a.dims);
+    if (row.there && (threadIdx.x & 32) == 0)
     {
-        float *partial = a.partial + at * a.dims;
-#pragma unroll
-        for (int p = 0; p < DP / 32; ++p)
-        {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-            {
-                const int d = 32 * p + RowOf(i);
-                if (d < a.dims)
-                {
-                    *reinterpret_cast<float4 *>(partial + d) = make_float4(run.out[p][i] * factor, run.out[p][i + 1] * factor,
-                                                                           run.out[p][i + 2] * factor, run.out[p][i + 3] * factor);
-                }
-            }
-        }
-        if ((threadIdx.x & 32) == 0)
-        {
-            a.partialLse[at] = lse;
-        }
+        a.partialLse[at] = lse;
     }
 }
 

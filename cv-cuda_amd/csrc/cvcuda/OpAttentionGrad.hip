@@ -24,10 +24,12 @@ struct AttentionGradArgs
     AttentionSequences sequences;
     const float       *lse;
     float             *base, *delta; // [rows][heads]: ShareBase and gradOut . out
+    float             *pieces;       // [pieces][tokens][heads][dims], of keys once more for values: where a kernel's work is split
     GroupRows          rows; // of a key head
     DivBy              keyHeads;
     int32_t            heads, dims;
     uint32_t           tiles, keyTiles;
+    int32_t            splits, keySplits; // pieces, at most, of the keys that a row's gradient is summed over, and of the rows for a key's
     float              scale;
     bool               causal;
 
@@ -93,8 +95,36 @@ struct GradScale
     }
 };
 
+// Tiles: rows and keys of a workgroup of the first kernel and its steps, keys and rows of the second's.
+constexpr int kGradRows = 128, kGradKeys = 64, kOfKeys = 128, kOfRows = 64;
+
+// Of how many pieces a sum over `all` keys or rows is made, and where piece `n` begins among its tiles: pieces differ by one tile at most.
+constexpr int kPiece = 256;
+
+__device__ __forceinline__ int PiecesOf(int all, int most)
+{
+    return min((max(all, 1) - 1) / kPiece + 1, most);
+}
+
+__device__ __forceinline__ int PieceBegin(int tiles, int n, int pieces)
+{
+    return (int)((int64_t)tiles * n / pieces);
+}
+
+// The keys that a tile's rows see, and the first row, of a key head's, that sees one of a tile's keys.
+__device__ __forceinline__ int KeysOfTile(const AttentionGradArgs &a, const SequenceTile &s)
+{
+    const int last = min((s.tile + 1) * kGradRows, s.rows * a.rows.size()) - 1;
+    return max(LimitOf(a.causal, s, a.rows.token(last)) + 1, 0);
+}
+
+__device__ __forceinline__ int FirstRowOfTile(const AttentionGradArgs &a, const SequenceTile &s)
+{
+    return a.causal ? min(max(s.tile * kOfKeys - (s.keys - s.rows), 0), s.rows) * a.rows.size() : 0;
+}
+
 // ---- the queries' gradient: 128 rows to a workgroup, 32 to a wave --------------------------------------------------------
-constexpr int kGradRows = 128, kGradKeys = 64, kGradThreads = 256;
+constexpr int kGradThreads = 256;
 
 template<class T, int DP>
 __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const AttentionGradArgs a)
@@ -112,8 +142,14 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
     const int      first = s.tile * kGradRows, ownFirst = first + (int)wave * 32, all = s.rows * a.rows.size();
     const AttentionRow row(a.rows, a.causal, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
     auto               limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
-    const int          tileKeys = max(limitAt(first + kGradRows - 1) + 1, 0), waveKeys = ownFirst < all ? limitAt(ownFirst + 31) + 1 : 0;
+    const int          tileKeys = KeysOfTile(a, s), waveKeys = ownFirst < all ? limitAt(ownFirst + 31) + 1 : 0;
     const int          seenKeys = limitAt(ownFirst) + 1, parts = (tileKeys + kGradKeys - 1) / kGradKeys;
+    const int          pieces = PiecesOf(tileKeys, a.splits), piece = (int)blockIdx.y;
+    const int          from = PieceBegin(parts, piece, pieces), to = PieceBegin(parts, piece + 1, pieces);
+    if (piece >= pieces)
+    {
+        return;
+    }
     const uint8_t     *k = a.k + s.firstKey * a.kToken + keyHead * a.kHead, *v = a.v + s.firstKey * a.vToken + keyHead * a.vHead;
 
     using Copy = TileCopy<kGradKeys, DP, kGradThreads / 64>;
@@ -123,9 +159,9 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
         Copy::rows(wave, toK, k + key * a.kToken, (uint32_t)a.kToken, s.keys - key, a.dims);
         Copy::rows(wave, toV, v + key * a.vToken, (uint32_t)a.vToken, s.keys - key, a.dims);
     };
-    if (parts > 0)
+    if (from < to)
     {
-        load(0, s_k0, s_v0);
+        load(from, s_k0, s_v0);
     }
     Vec8<T> q[DP / 16], grad[DP / 16];
     LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
@@ -147,7 +183,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
         }
         dot = BothSum(dot);
     }
-    if (row.there && (threadIdx.x & 32) == 0)
+    if (row.there && (threadIdx.x & 32) == 0 && piece == 0)
     {
         a.base[a.number(row)]  = base;
         a.delta[a.number(row)] = dot;
@@ -159,7 +195,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
     {
         const int key = part * kGradKeys;
         CopiesAndBarrier(); // (all have done the part before: its place may be written over)
-        if (part + 1 < parts)
+        if (part + 1 < to)
         {
             load(part + 1, nextK, nextV);
         }
@@ -216,20 +252,26 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
         }
     };
     // (by turns of their own, so that the compiler sees that what is read is not what is on its way)
-    for (int part = 0; part < parts; part += 2)
+    for (int part = from; part < to; part += 2)
     {
         take(part, s_k0, s_v0, s_k1, s_v1);
-        if (part + 1 < parts)
+        if (part + 1 < to)
         {
             take(part + 1, s_k1, s_v1, s_k0, s_v0);
         }
     }
-    StoreColumn<T, DP>(sum, a.scale / grow.factor, a.gradQ + row.token * a.gradQToken + row.head * a.gradQHead, row.there, a.dims);
+    if (a.splits == 1)
+    {
+        StoreColumn<T, DP>(sum, a.scale / grow.factor, a.gradQ + row.token * a.gradQToken + row.head * a.gradQHead, row.there, a.dims);
+    }
+    else
+    {
+        const int64_t at = (int64_t)piece * a.sequences.rows * a.heads + a.number(row);
+        StorePiece<DP>(sum, a.scale / grow.factor, a.pieces + at * a.dims, row.there, a.dims);
+    }
 }
 
 // ---- the keys' and values' gradients: 128 keys to a workgroup, 32 to a wave ------------------------------------------------
-constexpr int kOfKeys = 128, kOfRows = 64;
-
 // With heads of 128 elements two gradients, keys and values would be 192 registers of the 256 that two waves to a SIMD have: keys and values
 // stay in LDS, and eight waves go with them, of which two have the same keys and halves of each tile of rows, so that the
 // workgroup of a long sequence's first keys, which all rows see, is done in half the time. (With 64 elements such pairs are slower:
@@ -266,8 +308,14 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
     const int      first = s.tile * kOfKeys, ownFirst = first + (int)ofKeys * 32, key = ownFirst + (int)(threadIdx.x & 31);
     const bool     there = key < s.keys;
     const int      group = a.rows.size(), all = s.rows * group;
-    // the first row that sees one of these keys
-    const int begin = a.causal ? min(max(first - (s.keys - s.rows), 0), s.rows) * group : 0;
+    // the first row that sees one of these keys, and this piece's tiles of rows from there on
+    const int seen   = FirstRowOfTile(a, s), tiles = (all - seen + kOfRows - 1) / kOfRows;
+    const int pieces = PiecesOf(all - seen, a.keySplits), piece = (int)blockIdx.y;
+    const int begin = seen + PieceBegin(tiles, piece, pieces) * kOfRows, last = seen + (PieceBegin(tiles, piece + 1, pieces) - 1) * kOfRows;
+    if (piece >= pieces)
+    {
+        return;
+    }
     auto      limitAt = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
 
     Vec8<T> k[kInPairs<DP> ? 1 : DP / 16], v[kInPairs<DP> ? 1 : DP / 16];
@@ -334,8 +382,7 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
     // From the last tile to the first: with `causal` workgroups of one sequence see the same last rows, which all but one read from L2.
     // (Four of five of long_attention_grad's
     // reads missed L2 the other way round, 44 of 100 do now: 621 us and 614.)
-    const int last = begin + (max(all - begin, 1) - 1) / kOfRows * kOfRows;
-    if (begin < all)
+    if (begin <= last)
     {
         places(begin);
         load(last, place0);
@@ -417,7 +464,7 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
             }
         }
     };
-    for (int at = last; at >= begin && begin < all; at -= 2 * kOfRows)
+    for (int at = last; at >= begin; at -= 2 * kOfRows)
     {
         take(at, place0, place1);
         if (at > begin)
@@ -463,28 +510,138 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
             return;
         }
     }
-    StoreColumn<T, DP>(sumK, 1.f, a.gradK + (s.firstKey + key) * a.gradKToken + keyHead * a.gradKHead, there, a.dims);
-    StoreColumn<T, DP>(sumV, __builtin_amdgcn_exp2f(-kShareShift<T>), a.gradV + (s.firstKey + key) * a.gradVToken + keyHead * a.gradVHead, there,
-                       a.dims);
+    const float ofValues = __builtin_amdgcn_exp2f(-kShareShift<T>);
+    if (a.keySplits == 1)
+    {
+        StoreColumn<T, DP>(sumK, 1.f, a.gradK + (s.firstKey + key) * a.gradKToken + keyHead * a.gradKHead, there, a.dims);
+        StoreColumn<T, DP>(sumV, ofValues, a.gradV + (s.firstKey + key) * a.gradVToken + keyHead * a.gradVHead, there, a.dims);
+    }
+    else
+    {
+        const int64_t keys = (int64_t)a.sequences.keys * a.keyHeads.d, at = piece * keys + (int64_t)(s.firstKey + key) * a.keyHeads.d + keyHead;
+        StorePiece<DP>(sumK, 1.f, a.pieces + at * a.dims, there, a.dims);
+        StorePiece<DP>(sumV, ofValues, a.pieces + (a.keySplits * keys + at) * a.dims, there, a.dims);
+    }
 }
 
-int64_t GradBytes(int64_t rows, int64_t heads)
+// ---- pieces joined: a tile of tokens to kJoinGroups workgroups, 8 elements of a row to a thread -----------------------------
+constexpr int kJoinThreads = 256, kJoinGroups = 8;
+
+template<class T, bool KEYS>
+__global__ __launch_bounds__(kJoinThreads) void AttentionGradJoinKernel(const AttentionGradArgs a)
 {
-    return 2 * rows * heads * (int64_t)sizeof(float);
+    const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
+    const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d), size = KEYS ? kOfKeys : kGradRows, units = a.dims / 8;
+    const SequenceTile s       = FindTile(a.sequences, t, KEYS ? a.keyTiles : a.tiles, size, KEYS ? 1 : a.rows.size(), KEYS, a.causal);
+    if (s.tile < 0)
+    {
+        return;
+    }
+    const int      first = s.tile * size, count = min((KEYS ? s.keys : s.rows * a.rows.size()) - first, size);
+    const int64_t  rows = KEYS ? (int64_t)a.sequences.keys * a.keyHeads.d : (int64_t)a.sequences.rows * a.heads;
+    const int      pieces = KEYS ? PiecesOf(s.rows * a.rows.size() - FirstRowOfTile(a, s), a.keySplits) : PiecesOf(KeysOfTile(a, s), a.splits);
+    for (int i = (int)(blockIdx.y * kJoinThreads + threadIdx.x); i < count * units; i += kJoinGroups * kJoinThreads)
+    {
+        const int          r = i / units, d = (i - r * units) * 8;
+        const AttentionRow row(a.rows, false, s, keyHead, first + r);
+        const int          token = KEYS ? s.firstKey + first + r : row.token, head = KEYS ? keyHead : row.head;
+        const int64_t      at    = KEYS ? (int64_t)token * a.keyHeads.d + head : a.number(row);
+        auto               join  = [&](const float *from, uint8_t *to)
+        {
+            float sum[8] = {};
+#pragma unroll 4
+            for (int p = 0; p < pieces; ++p)
+            {
+                const Run<float, 8> piece = *reinterpret_cast<const Run<float, 8> *>(from + (p * rows + at) * a.dims + d);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                {
+                    sum[k] += piece.v[k];
+                }
+            }
+            Run<T, 8> made;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+            {
+                made.v[k] = FromFloat<T>(sum[k]);
+            }
+            *reinterpret_cast<Run<T, 8> *>(to + d * 2) = made;
+        };
+        if (KEYS)
+        {
+            join(a.pieces, a.gradK + token * a.gradKToken + head * a.gradKHead);
+            join(a.pieces + a.keySplits * rows * a.dims, a.gradV + token * a.gradVToken + head * a.gradVHead);
+        }
+        else
+        {
+            join(a.pieces, a.gradQ + token * a.gradQToken + head * a.gradQHead);
+        }
+    }
 }
+
+// How a call is made, by its sizes alone: the sequences' lengths are on the device.
+struct GradPlan
+{
+    int64_t rows, keys, heads, keyHeads, dims; // rows, keys: of all heads
+    int64_t tiles, keyTiles;                   // at most, of a key head
+    int64_t splits, keySplits;
+
+    GradPlan(int64_t tokens, int64_t keyTokens, int64_t sequences, int64_t heads_, int64_t keyHeads_, int64_t dims_)
+        : rows(tokens * heads_)
+        , keys(keyTokens * keyHeads_)
+        , heads(heads_)
+        , keyHeads(keyHeads_)
+        , dims(dims_)
+    {
+        const int64_t matrix = rows / keyHeads, most = std::max<int64_t>(sequences, 1), some = std::min(sequences, tokens), someKeys = std::min(sequences, keyTokens);
+        const int64_t whole = (matrix + kGradRows - 1) / kGradRows, wholeKeys = (keyTokens + kOfKeys - 1) / kOfKeys;
+        tiles     = whole + some;
+        keyTiles  = wholeKeys + someKeys;
+        // As many workgroups as fill the card's CUs twice; sequences of twice the mean length still have pieces of kPiece. (1200 rows of a
+        // head that see 166 keys, 8 workgroups: the keys' kernel 54 us, 17.7 and 4.7 to join them; 151 rows before 6300 keys the queries' 106 us, 18.9
+        // and 6.7; with up to 400 keys and rows, 72 workgroups, 19 and 22 us, 15 and 18 in pieces that take 5 each to join.)
+        auto split = [](int64_t groups, int64_t each)
+        { return each <= 2 * kPiece ? 1 : std::max<int64_t>(std::min({512 / std::max<int64_t>(groups, 1), (2 * each + kPiece - 1) / kPiece, kMostPieces}), 1); };
+        splits    = split(std::max(whole, some) * keyHeads, keyTokens / most);
+        keySplits = split(std::max(wholeKeys, someKeys) * keyHeads, matrix / most);
+    }
+
+    int64_t sums() const
+    {
+        return (2 * rows + 3) / 4 * 4; // (what follows is aligned)
+    }
+
+    int64_t bytes() const
+    {
+        const int64_t ofRows = splits > 1 ? splits * rows * dims : 0, ofKeys = keySplits > 1 ? 2 * keySplits * keys * dims : 0;
+        return (sums() + std::max(ofRows, ofKeys)) * (int64_t)sizeof(float);
+    }
+
+    static constexpr int64_t kMostPieces = 32;
+};
 
 template<class T, int DP>
 void Launch(const AttentionGradArgs &a, hipStream_t stream)
 {
     if (a.tiles > 0)
     {
-        AttentionGradQKernel<T, DP><<<a.tiles * a.keyHeads.d, kGradThreads, 0, stream>>>(a);
+        AttentionGradQKernel<T, DP><<<dim3(a.tiles * a.keyHeads.d, (uint32_t)a.splits), kGradThreads, 0, stream>>>(a);
         CheckLaunch("attention's gradient (queries)");
+        if (a.splits > 1)
+        {
+            AttentionGradJoinKernel<T, false><<<dim3(a.tiles * a.keyHeads.d, kJoinGroups), kJoinThreads, 0, stream>>>(a);
+            CheckLaunch("attention's gradient (queries' pieces)");
+        }
     }
     if (a.keyTiles > 0)
     {
-        AttentionGradKVKernel<T, DP><<<a.keyTiles * a.keyHeads.d, kOfThreads<DP>, 0, stream>>>(a);
+        AttentionGradKVKernel<T, DP><<<dim3(a.keyTiles * a.keyHeads.d, (uint32_t)a.keySplits), kOfThreads<DP>, 0, stream>>>(a);
         CheckLaunch("attention's gradient (keys)");
+        if (a.keySplits > 1)
+        {
+            AttentionGradJoinKernel<T, true><<<dim3(a.keyTiles * a.keyHeads.d, kJoinGroups), kJoinThreads, 0, stream>>>(a);
+            CheckLaunch("attention's gradient (keys' pieces)");
+        }
     }
 }
 
@@ -496,21 +653,19 @@ void SubmitGrad(hipStream_t stream, NVCVTensorHandle hgrad, NVCVTensorHandle hq,
     const HeadsView out = TakeHeadsLike(hout, in.q, "Output"), grad = TakeHeadsLike(hgrad, in.q, "Output's gradient");
     const HeadsView gradQ = TakeHeadsLike(hgradQ, in.q, "Queries' gradient"), gradK = TakeHeadsLike(hgradK, in.k, "Keys' gradient");
     const HeadsView gradV = TakeHeadsLike(hgradV, in.k, "Values' gradient");
-    uint8_t        *room  = RequireWorkspace(hworkspace, GradBytes(in.q.tokens, in.q.heads));
+    const GradPlan plan(in.q.tokens, in.k.tokens, in.sequences.count, in.q.heads, in.k.heads, in.q.dims);
+    uint8_t *room = RequireWorkspace(hworkspace, plan.bytes());
     if (in.sequences.count == 0)
     {
         return;
     }
-    const int64_t group = in.q.heads / in.k.heads, rows = in.q.tokens, keys = in.k.tokens, sequences = in.sequences.count;
-    const int64_t tiles    = (rows * group + kGradRows - 1) / kGradRows + std::min(sequences, rows);
-    const int64_t keyTiles = (keys + kOfKeys - 1) / kOfKeys + std::min(sequences, keys);
     float *base = reinterpret_cast<float *>(room);
     const AttentionGradArgs a = {
         in.q.base, in.k.base, in.v.base, out.base, grad.base, gradQ.base, gradK.base, gradV.base, in.q.tokenStride, in.q.headStride,
         in.k.tokenStride, in.k.headStride, in.v.tokenStride, in.v.headStride, out.tokenStride, out.headStride, grad.tokenStride, grad.headStride,
         gradQ.tokenStride, gradQ.headStride, gradK.tokenStride, gradK.headStride, gradV.tokenStride, gradV.headStride, in.sequences, in.lse,
-        base, base + rows * in.q.heads, {DivBy((uint32_t)group)}, DivBy((uint32_t)in.k.heads), in.q.heads, in.q.dims, (uint32_t)tiles,
-        (uint32_t)keyTiles, scale, causal};
+        base, base + plan.rows, base + plan.sums(), {DivBy((uint32_t)(in.q.heads / in.k.heads))}, DivBy((uint32_t)in.k.heads), in.q.heads, in.q.dims,
+        (uint32_t)plan.tiles, (uint32_t)plan.keyTiles, (int32_t)plan.splits, (int32_t)plan.keySplits, scale, causal};
     auto launch = [&](auto t)
     {
         using T = decltype(t);
@@ -537,7 +692,7 @@ CVCUDA_PUBLIC NVCVStatus cvcudaxAttentionGradWorkspace(int64_t rows, int64_t key
                 throw OpError(NVCV_ERROR_INVALID_ARGUMENT, "Pointer to output must not be NULL");
             }
             RequireAttentionSizes(rows, keys, sequences, heads, keyHeads, dims);
-            *bytes = GradBytes(rows, heads);
+            *bytes = GradPlan(rows, keys, sequences, heads, keyHeads, dims).bytes();
         });
 }
 

@@ -413,3 +413,21 @@ def test_gradients_of_one_row_in_a_graph_and_beside_others(api):
         api.attention_into(outs[3], t["q"], t["k"], t["v"], t["offsets"], lse=lse, stream=s)
         with pytest.raises(api.Error):
             api.attention_grad_into(*outs[:3], t["grad"], t["q"], t["k"], t["v"], outs[3], lse, t["offsets"], stream=s)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,heads,key_heads", [(40, 2, 2), (128, 6, 2), (64, 8, 1)])
+def test_gradients_of_few_rows_and_of_few_keys(api, d, heads, key_heads, causal, dtype):
+    """Where the work of a kernel is split: long caches of few rows, and few keys that many rows see; some sequences have far fewer than others."""
+    few_rows = Call([(5, 3000), (0, 10), (1, 1), (130, 1500), (3, 0)], heads, key_heads, d, dtype, 40, causal, room=3000, before=2, behind=3)
+    few_keys = Call([(1500, 40), (0, 0), (700, 1), (2, 130)], heads, key_heads, d, dtype, 41, causal, room=140, before=1, behind=2)
+    for call in (few_rows, few_keys):
+        for _ in range(2):
+            again = call.check_gradients(api, *call.run(api))
+        first = call.gradients(api, *call.run(api))
+        assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(first, again))
+    # (more than the rows' sums: both are split)
+    sums = lambda rows: (2 * rows * heads + 3) // 4 * 16
+    assert api.AttentionGrad.workspace(few_rows.rows, few_rows.keys, 5, heads, key_heads, d) > sums(few_rows.rows)
+    assert api.AttentionGrad.workspace(few_keys.rows, few_keys.keys, 4, heads, key_heads, d) > sums(few_keys.rows)
