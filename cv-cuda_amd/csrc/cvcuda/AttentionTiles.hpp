@@ -40,13 +40,6 @@ __device__ __forceinline__ void Multiply(Acc16 &acc, Vec8<Half> a, Vec8<Half> b)
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
 }
 
-// The lane that has the same column's other rows.
-__device__ __forceinline__ float OtherHalf(float v)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float((threadIdx.x & 32) != 0 ? r[0] : r[1]);
-}
-
 // Largest and sum of a lane's and the other half's.
 __device__ __forceinline__ float BothMax(float v)
 {

@@ -139,12 +139,12 @@ __device__ __forceinline__ float LseOf(float top, float sum)
 // ---- prompts: 128 rows to a workgroup, 32 to a wave ------------------------------------------------------------------
 constexpr int kManyRows = 128, kManyThreads = 256;
 
-// Keys of a tile, and waves to a SIMD.
+// Keys of a tile, and waves to a SIMD. With heads of 128 elements three waves with tiles of 32 keys hide more of each other's waits than
+// two with 64 do (prompts_attention 290 us, 276); with 64 elements four waves have registers for 64 keys.
 template<int DP>
 constexpr int kManyKeys = DP > 64 ? 32 : 64;
 template<int DP>
 constexpr int kManyWaves = DP > 64 ? 3 : 4;
-
 
 template<class T, int DP>
 __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(const AttentionArgs a)
@@ -228,15 +228,17 @@ __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(
     }
 }
 
-// ---- few rows to a sequence (single tokens): 32 rows to a workgroup, of whose waves each takes every WAVES-th 32 keys -----------
-constexpr int kFewRows = 32, kFewKeys = 32;
+// ---- few rows to a sequence (single tokens): 32 rows to a workgroup, of whose waves each takes every fourth 32 keys -------------
+// Bound by the reads of keys and values: 16 caches of up to 8192 keys, 362 MB, in 75 us, and 5.6 to join the pieces. (Eight waves are slower:
+// 700 keys 13.1 us, 11.6 with four.)
+constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4, kFewThreads = 64 * kFewWaves;
 
-template<class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void AttentionFewKernel(const AttentionArgs a)
+template<class T, int DP>
+__global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const AttentionArgs a)
 {
     // each wave's keys and values, later its weighted values in 32 bits
-    __shared__ __attribute__((aligned(256))) uint8_t s_tile[WAVES][2 * kFewKeys * DP * 2];
-    __shared__ float                                 s_top[WAVES][kFewRows], s_sum[WAVES][kFewRows];
+    __shared__ __attribute__((aligned(256))) uint8_t s_tile[kFewWaves][2 * kFewKeys * DP * 2];
+    __shared__ float                                 s_top[kFewWaves][kFewRows], s_sum[kFewWaves][kFewRows];
     // (a sequence's key heads next to each other on one XCD: what they read lies side by side. 88 us with one of eight heads to each XCD, 85)
     const int          keyHead = (int)(blockIdx.x / a.tiles);
     const uint32_t     t       = blockIdx.x - (uint32_t)keyHead * a.tiles;
@@ -272,7 +274,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void AttentionFewKernel(const Attent
     Vec8<T> q[DP / 16];
     LoadColumn<T, DP>(q, a.q + row.token * a.qToken + row.head * a.qHead, a.dims);
     Running<T, DP> run;
-    for (int part = from; part < to; part += WAVES)
+    for (int part = from; part < to; part += kFewWaves)
     {
         const int key = part * kFewKeys;
         // (a wave's reads and writes of LDS take place in their order; the compiler is kept from changing it)
@@ -280,9 +282,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void AttentionFewKernel(const Attent
         nextK.put(keys);
         nextV.put(values);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (part + WAVES < to)
+        if (part + kFewWaves < to)
         {
-            load(part + WAVES);
+            load(part + kFewWaves);
         }
         Acc16 scores[1];
         Scores<T, DP>(scores, keys, q, key, row.limit, key + kFewKeys > seenKeys);
@@ -307,19 +309,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void AttentionFewKernel(const Attent
         s_sum[wave][lane] = sum;
     }
     __syncthreads();
-    if (threadIdx.x >= 256)
-    {
-        return;
-    }
     const uint32_t r = threadIdx.x % kFewRows, d0 = threadIdx.x / kFewRows * (DP / 8);
-    float          top = -INFINITY, total = 0, weight[WAVES];
+    float          top = -INFINITY, total = 0, weight[kFewWaves];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w)
+    for (int w = 0; w < kFewWaves; ++w)
     {
         top = fmaxf(top, s_top[w][r]);
     }
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w)
+    for (int w = 0; w < kFewWaves; ++w)
     {
         weight[w] = s_top[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_top[w][r] - top);
         total += weight[w] * s_sum[w][r];
@@ -340,7 +338,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void AttentionFewKernel(const Attent
         {
             v8[i] = 0;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w)
+            for (int w = 0; w < kFewWaves; ++w)
             {
                 v8[i] += weight[w] * reinterpret_cast<const float *>(s_tile[w])[(d0 + d + i) * kFewRows + r];
             }
@@ -471,22 +469,25 @@ struct Plan
     Plan(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t keyHeads)
     {
         const int64_t matrix = rows * (heads / keyHeads), most = std::max<int64_t>(sequences, 1);
-        few                  = matrix <= 48 * most;
+        // (4 sequences of 16 rows of a key head that see 1500 keys 14.8 us here, 15.8 where there are many; of 32 rows 21.5 and 16.3; 64 sequences
+        // of 48 rows 120 and 73)
+        few                = matrix <= 16 * most;
         const int64_t size = few ? kFewRows : kManyRows, whole = (matrix + size - 1) / size;
         tiles              = (uint32_t)(whole + std::min(sequences, rows));
         const int64_t groups = std::max<int64_t>(std::max(whole, std::min(sequences, rows)) * keyHeads, 1), each = keys / most;
         if (few)
         {
             // Pieces of one length whatever the sequences' lengths, so that no workgroup has much more to do than the others, and as many as
-            // the card holds at once where all caches are full (tokens_attention 83 us, with twice as many 85, with four times 101).
-            // Up to 1024 keys are not worth the second launch that joins pieces (700 keys: 17.7 us, 14.5 in one piece of eight waves).
-            const int64_t chunk = std::max<int64_t>(groups * each / 512, 256);
+            // the card holds at once where all caches are full (tokens_attention 83 us, with twice as many 85, with four times 101), of 512
+            // keys at least (8000 keys 21 us, with 256 at least 29). Up to 1024 keys are not worth the second launch that joins pieces.
+            const int64_t chunk = std::max<int64_t>(groups * each / 512, 512);
             splits    = each <= 1024 ? 1 : (int32_t)std::max<int64_t>(std::min<int64_t>((2 * each + chunk - 1) / chunk, kMostSplits), 1);
             chunkKeys = (int32_t)std::min<int64_t>(chunk, INT32_MAX / 2);
         }
         else
         {
-            // as many workgroups as fill the card's CUs twice, each with 256 keys at least
+            // as many workgroups as fill the card's CUs twice, each with 256 keys at least (128 rows of 8 heads before 2048 keys 17 us, whole 52;
+            // before 600 16 and 19)
             splits    = (int32_t)std::max<int64_t>(std::min<int64_t>({512 / groups, each / 256, kMostSplits}), 1);
             chunkKeys = 0;
         }
@@ -507,14 +508,9 @@ template<class T, int DP>
 void Launch(const AttentionArgs &a, bool few, hipStream_t stream)
 {
     const dim3 grid(a.tiles * a.keyHeads.d, (uint32_t)a.splits);
-    // few workgroups: each with as many waves as LDS has room for
-    if (few && grid.x * grid.y <= 256)
+    if (few)
     {
-        AttentionFewKernel<T, DP, 8><<<grid, 512, 0, stream>>>(a);
-    }
-    else if (few)
-    {
-        AttentionFewKernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
+        AttentionFewKernel<T, DP><<<grid, kFewThreads, 0, stream>>>(a);
     }
     else
     {
