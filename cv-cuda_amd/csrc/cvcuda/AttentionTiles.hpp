@@ -310,7 +310,8 @@ __device__ __forceinline__ uint32_t WaveTotal(uint32_t v)
 
 // Tile `t` of all sequences' tiles, of `size` rows each, a token having `each` rows (of keys: `ofKeys`). Every wave finds it by itself.
 // With `causal` a sequence's last tiles of rows have the most keys, its first tiles of keys the most rows. They come first, of all
-// sequences (up to 64 of them), so that the workgroups that begin last are short ones (long_attention_grad 863 us, 835 with it).
+// sequences (up to 64 of them), so that the workgroups that begin last are short ones (the gradient of 8 sequences of up to
+// 2048 tokens, 32 heads on 8 of 128 elements, 863 us, 835 with it).
 __device__ __forceinline__ SequenceTile FindTile(const AttentionSequences &s, uint32_t t, uint32_t most, int size, int each, bool ofKeys, bool causal)
 {
     const int lane = (int)(threadIdx.x & 63);
