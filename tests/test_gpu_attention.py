@@ -431,3 +431,26 @@ def test_gradients_of_few_rows_and_of_few_keys(api, d, heads, key_heads, causal,
     sums = lambda rows: (2 * rows * heads + 3) // 4 * 16
     assert api.AttentionGrad.workspace(few_rows.rows, few_rows.keys, 5, heads, key_heads, d) > sums(few_rows.rows)
     assert api.AttentionGrad.workspace(few_keys.rows, few_keys.keys, 4, heads, key_heads, d) > sums(few_keys.rows)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("rows,keys", [(0, 5), (3, 0), (200, 0)])
+def test_no_rows_or_no_keys_at_all(api, rows, keys, causal):
+    call = Call([(rows, keys)], 4, 2, 64, F16, 50, causal, room=keys, before=2)
+    out, lse = call.check(api)
+    for t in call.check_gradients(api, out, lse):
+        assert (t[2:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_one_tensor_in_three_places(api, dtype):
+    """Keys that are values and queries as well: what is read twice counts for both."""
+    call = Call([(70, 70), (9, 9)], 4, 4, 64, dtype, 51)
+    call.k = call.v = call.q
+    out, lse = call.check(api)
+    grads = call.check_gradients(api, out, lse)
+    x, g, o, s, seq = (api.as_tensor(t) for t in (call.q, call.grad, out, lse, call.offsets))
+    again = api.attention(x, x, x, seq, causal=True, scale=call.scale)
+    made = api.attention_grad(g, x, x, x, o, s, seq, causal=True, scale=call.scale)
+    torch.cuda.synchronize()
+    assert torch.equal(again.torch(), out) and all(torch.equal(a.torch(), b) for a, b in zip(made, grads))
