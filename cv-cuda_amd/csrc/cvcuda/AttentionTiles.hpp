@@ -179,7 +179,8 @@ struct TileLoad
 
     Unit unit[Copy::kCount];
 
-    // As TileCopy::rows.
+    // As TileCopy::rows. PAST: as in LoadRun.
+    template<bool PAST>
     __device__ __forceinline__ void get(const uint8_t *base, uint32_t stride, int count, int dims)
     {
         const uint32_t lane = threadIdx.x & 63, row = lane / Copy::kUnits, part = lane % Copy::kUnits;
@@ -189,7 +190,7 @@ struct TileLoad
 #pragma unroll
         for (int i = 0; i < Copy::kCount; ++i)
         {
-            unit[i] = __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, (int)((uint32_t)(i * Copy::kOfOne) * stride), 0);
+            unit[i] = __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, (int)((uint32_t)(i * Copy::kOfOne) * stride), PAST ? 2 : 0);
         }
     }
 

@@ -6,7 +6,7 @@
 //
 // Measured: long prompts (8 sequences of up to 4096 tokens, 32 heads on 8 key heads of 128 BF16 elements, causal) 276 us, 953 TFLOP/s, where a
 // product of two 8192 x 8192 matrices by the library has 1253: exponentials take as long as the products, and overlap those of other waves
-// only. Single tokens (16 before caches of up to 8192, the same heads: 362 MB) 80 us, of them 75 of reading at 4.9 TB/s.
+// only. Single tokens (16 before caches of up to 8192, the same heads: 362 MB) 70 us, of them 65 of reading at 5.6 TB/s.
 #include "AttentionTiles.hpp"
 
 #include <cvcuda/Attention.h>
@@ -233,11 +233,11 @@ __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(
 }
 
 // ---- few rows to a sequence (single tokens): 32 rows to a workgroup, of whose waves each takes every fourth 32 keys -------------
-// Bound by the reads of keys and values: 16 caches of up to 8192 keys, 362 MB, in 75 us, and 5.6 to join the pieces. (Eight waves are slower:
+// Bound by the reads of keys and values: 16 caches of up to 8192 keys, 362 MB, in 65 us, and 5.6 to join the pieces (75 where the caches are to keep them). (Eight waves are slower:
 // 700 keys 13.1 us, 11.6 with four.)
 constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4, kFewThreads = 64 * kFewWaves;
 
-template<class T, int DP>
+template<class T, int DP, bool PAST>
 __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const AttentionArgs a)
 {
     // each wave's keys and values, later its weighted values in 32 bits
@@ -268,8 +268,8 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
     auto load = [&](int part)
     {
         const int key = part * kFewKeys;
-        nextK.get(k + key * a.kToken, (uint32_t)a.kToken, s.keys - key, a.dims);
-        nextV.get(v + key * a.vToken, (uint32_t)a.vToken, s.keys - key, a.dims);
+        nextK.template get<PAST>(k + key * a.kToken, (uint32_t)a.kToken, s.keys - key, a.dims);
+        nextV.template get<PAST>(v + key * a.vToken, (uint32_t)a.vToken, s.keys - key, a.dims);
     };
     if (from < to)
     {
@@ -512,9 +512,13 @@ template<class T, int DP>
 void Launch(const AttentionArgs &a, bool few, hipStream_t stream)
 {
     const dim3 grid(a.tiles * a.keyHeads.d, (uint32_t)a.splits);
-    if (few)
+    if (few && MovesPastCaches(2 * (int64_t)a.sequences.keys * a.keyHeads.d * a.dims * (int64_t)sizeof(T)))
     {
-        AttentionFewKernel<T, DP><<<grid, kFewThreads, 0, stream>>>(a);
+        AttentionFewKernel<T, DP, true><<<grid, kFewThreads, 0, stream>>>(a);
+    }
+    else if (few)
+    {
+        AttentionFewKernel<T, DP, false><<<grid, kFewThreads, 0, stream>>>(a);
     }
     else
     {

@@ -6,8 +6,8 @@
 // e^kSlack, and most lanes never do. The workgroup joins its lanes' afterwards. The entropy is log(s) - t / s, in which nothing
 // large is left to cancel. The top tokens come from what the pass has
 // anyway: a number that K of the lanes' largest logits, by 64 groups, reach is one that K logits of the row reach, so that the lanes
-// which reach it, few in most rows, look through theirs again for those that do (4096 rows of 128000 BF16 with the top 5 192 us). Where too many do, or the row has NaN, the whole row is
-// gone over K times.
+// which reach it, few in most rows, look through theirs again for those that do (4096 rows of 128000 BF16 with the top 5 186 us, 5.6
+// TB/s). Where too many do, or the row has NaN, the whole row is gone over K times.
 #include "RowOps.hpp"
 
 #include <cvcuda/LogProbs.h>
@@ -72,7 +72,7 @@ __device__ __forceinline__ int ColumnOf(uint64_t key)
 }
 
 // Run r of a row: N logits from N * r on, at the row's end the last N of it, of which those from `skip` on are its own.
-template<class T, int N>
+template<class T, int N, bool PAST>
 struct Logits
 {
     Run<T, N> run;
@@ -82,7 +82,7 @@ struct Logits
     {
         from = min(r * N, columns - N);
         skip = r * N - from;
-        run  = *reinterpret_cast<const Run<T, N> *>(row + from);
+        run  = LoadRun<PAST, T, N>(row + from);
     }
 };
 
@@ -188,7 +188,7 @@ struct Sums
 
 // N: logits of a run (1 where rows are narrower than 16 bytes). One workgroup to a row. HELD: the row fits the registers of runs on their
 // way, and is looked through again there.
-template<class T, int N, int WAVES, int AHEAD, bool HELD>
+template<class T, int N, int WAVES, int AHEAD, bool HELD, bool PAST>
 __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs a)
 {
     constexpr int       kLanes = 64 * WAVES;
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     const T       *in   = reinterpret_cast<const T *>(a.logits.at(row));
     const int      runs = (a.columns + N - 1) / N, whole = a.columns / N;
     Sums           sums;
-    Logits<T, N>   x[AHEAD];
+    Logits<T, N, PAST>   x[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
     {
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     const int64_t token = TokenAt(a.tokens, a.wide, row);
     const bool    there = token >= 0 && token < a.columns;
     const float   its   = (float)in[there ? token : 0];
-    auto          take  = [&](const Logits<T, N> &l, int r)
+    auto          take  = [&](const Logits<T, N, PAST> &l, int r)
     {
         float v[N];
 #pragma unroll
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         }
     }
     const float least = ValueOf(low);
-    auto        look  = [&](const Logits<T, N> &l)
+    auto        look  = [&](const Logits<T, N, PAST> &l)
     {
         float v[N], largest = -INFINITY;
 #pragma unroll
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         uint64_t best = 0;
         for (int r = (int)threadIdx.x; r < runs; r += kLanes)
         {
-            Logits<T, N> l;
+            Logits<T, N, PAST> l;
             l.get(in, a.columns, r);
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -456,60 +456,52 @@ struct LogProbsGradArgs
     bool         wide;
 };
 
-constexpr int kGradThreads = 256, kGradRuns = 4; // runs of a lane
+constexpr int kGradThreads = 256;
 
-// A workgroup makes kGradRuns * kGradThreads runs of a row.
-template<class T, int N, bool ENTROPY>
+// A run of a row to a lane (4096 rows of 128000 BF16 320 us, 6.6 TB/s; with two runs 332).
+template<class T, int N, bool ENTROPY, bool PAST>
 __global__ __launch_bounds__(kGradThreads) void LogProbsGradKernel(const LogProbsGradArgs a, uint32_t firstBlock)
 {
     const uint32_t block = firstBlock + blockIdx.x, row = a.parts.Quotient(block), part = block - row * a.parts.d;
     const T       *in    = reinterpret_cast<const T *>(a.logits.at(row));
     T             *out   = reinterpret_cast<T *>(a.out.at(row));
-    const int      runs  = (a.columns + N - 1) / N, first = (int)(part * kGradRuns) * kGradThreads + (int)threadIdx.x;
-    Logits<T, N>   x[kGradRuns];
-#pragma unroll
-    for (int k = 0; k < kGradRuns; ++k)
-    {
-        x[k].get(in, a.columns, min(first + k * kGradThreads, runs - 1));
-    }
+    const int      runs = (a.columns + N - 1) / N, r = (int)(part * kGradThreads + threadIdx.x);
+    Logits<T, N, PAST>   x;
+    x.get(in, a.columns, min(r, runs - 1));
     const int64_t token   = TokenAt(a.tokens, a.wide, row);
     const bool    there   = token >= 0 && token < a.columns;
     const float   lse     = a.lse[row], g = there ? a.grad[row] : 0.f, h = ENTROPY ? a.gradEntropy[row] : 0.f;
     const float   entropy = ENTROPY ? a.entropy[row] : 0.f;
     const bool    nothing = lse == -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kGradRuns; ++k)
+    if (r >= runs)
     {
-        if (first + k * kGradThreads >= runs)
+        return;
+    }
+    Run<T, N> made;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+        const float logp = a.scale * (float)x.run.v[i] - lse, p = __builtin_amdgcn_exp2f(logp * kLog2E);
+        float       v = -g * p;
+        if (ENTROPY)
         {
-            break;
+            v -= p == 0 ? 0.f : h * p * (logp + entropy);
         }
-        Run<T, N> made;
+        v += there && x.from + i == (int)token ? g : 0.f;
+        made.v[i] = FromFloat<T>(nothing ? 0.f : a.scale * v);
+    }
+    if (x.skip == 0)
+    {
+        StoreRun<PAST>(out + x.from, made);
+    }
+    else
+    {
 #pragma unroll
         for (int i = 0; i < N; ++i)
         {
-            const float logp = a.scale * (float)x[k].run.v[i] - lse, p = __builtin_amdgcn_exp2f(logp * kLog2E);
-            float       v = -g * p;
-            if (ENTROPY)
+            if (i >= x.skip)
             {
-                v -= p == 0 ? 0.f : h * p * (logp + entropy);
-            }
-            v += there && x[k].from + i == (int)token ? g : 0.f;
-            made.v[i] = FromFloat<T>(nothing ? 0.f : a.scale * v);
-        }
-        if (x[k].skip == 0)
-        {
-            *reinterpret_cast<Run<T, N> *>(out + x[k].from) = made;
-        }
-        else
-        {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-            {
-                if (i >= x[k].skip)
-                {
-                    out[x[k].from + i] = made.v[i];
-                }
+                out[x.from + i] = made.v[i];
             }
         }
     }
@@ -518,7 +510,7 @@ __global__ __launch_bounds__(kGradThreads) void LogProbsGradKernel(const LogProb
 // runs of a lane on their way (4096 rows of 128000 BF16, eight waves: with two 264 us, four 249, six 250, eight 262)
 constexpr int kAhead = 4;
 
-template<class T, int N, int WAVES>
+template<class T, int N, int WAVES, bool PAST>
 void LaunchRows(LogProbsArgs a, hipStream_t stream)
 {
     constexpr int most = INT32_MAX / (64 * WAVES);
@@ -529,22 +521,22 @@ void LaunchRows(LogProbsArgs a, hipStream_t stream)
         a.firstRow            = (int32_t)first;
         if (held)
         {
-            LogProbsKernel<T, N, WAVES, kAhead, true><<<blocks, 64 * WAVES, 0, stream>>>(a);
+            LogProbsKernel<T, N, WAVES, kAhead, true, PAST><<<blocks, 64 * WAVES, 0, stream>>>(a);
         }
         else
         {
-            LogProbsKernel<T, N, WAVES, kAhead, false><<<blocks, 64 * WAVES, 0, stream>>>(a);
+            LogProbsKernel<T, N, WAVES, kAhead, false, PAST><<<blocks, 64 * WAVES, 0, stream>>>(a);
         }
         CheckLaunch("log probabilities");
     }
 }
 
-template<class T, int N>
+template<class T, int N, bool PAST>
 void LaunchLogProbs(const LogProbsArgs &a, hipStream_t stream)
 {
     if constexpr (N == 1)
     {
-        LaunchRows<T, N, 1>(a, stream);
+        LaunchRows<T, N, 1, PAST>(a, stream);
     }
     else
     {
@@ -559,20 +551,20 @@ void LaunchLogProbs(const LogProbsArgs &a, hipStream_t stream)
         switch (std::max(many, std::min(few, 4096 / a.rows)))
         {
         case 0:
-        case 1: LaunchRows<T, N, 1>(a, stream); break;
+        case 1: LaunchRows<T, N, 1, PAST>(a, stream); break;
         case 2:
-        case 3: LaunchRows<T, N, 2>(a, stream); break;
+        case 3: LaunchRows<T, N, 2, PAST>(a, stream); break;
         case 4:
         case 5:
         case 6:
-        case 7: LaunchRows<T, N, 4>(a, stream); break;
-        case 16: LaunchRows<T, N, 16>(a, stream); break;
-        default: LaunchRows<T, N, 8>(a, stream); break;
+        case 7: LaunchRows<T, N, 4, PAST>(a, stream); break;
+        case 16: LaunchRows<T, N, 16, PAST>(a, stream); break;
+        default: LaunchRows<T, N, 8, PAST>(a, stream); break;
         }
     }
 }
 
-template<class T, int N, bool ENTROPY>
+template<class T, int N, bool ENTROPY, bool PAST>
 void LaunchLogProbsGrad(const LogProbsGradArgs &a, hipStream_t stream)
 {
     const int64_t blocks = (int64_t)a.rows * a.parts.d, most = INT32_MAX / kGradThreads;
@@ -582,7 +574,7 @@ void LaunchLogProbsGrad(const LogProbsGradArgs &a, hipStream_t stream)
     }
     for (int64_t first = 0; first < blocks; first += most)
     {
-        LogProbsGradKernel<T, N, ENTROPY><<<(uint32_t)std::min(most, blocks - first), kGradThreads, 0, stream>>>(a, (uint32_t)first);
+        LogProbsGradKernel<T, N, ENTROPY, PAST><<<(uint32_t)std::min(most, blocks - first), kGradThreads, 0, stream>>>(a, (uint32_t)first);
         CheckLaunch("log probabilities' gradient");
     }
 }
@@ -679,7 +671,9 @@ public:
                  [&](auto t)
                  {
                      using T = decltype(t);
-                     logits.columns >= kRunOf<T> ? LaunchLogProbs<T, kRunOf<T>>(a, stream) : LaunchLogProbs<T, 1>(a, stream);
+                     logits.columns < kRunOf<T>                                                         ? LaunchLogProbs<T, 1, false>(a, stream)
+                     : MovesPastCaches((int64_t)logits.rows * logits.columns * (int64_t)sizeof(T)) ? LaunchLogProbs<T, kRunOf<T>, true>(a, stream)
+                                                                                                        : LaunchLogProbs<T, kRunOf<T>, false>(a, stream);
                  });
     }
 
@@ -704,15 +698,19 @@ public:
                  [&](auto t)
                  {
                      using T              = decltype(t);
-                     const auto run       = [&](auto n)
+                     const auto run       = [&](auto n, auto past)
                      {
                          constexpr int          N     = decltype(n)::value;
-                         const int64_t          parts = ((int64_t)logits.columns + N * kGradRuns * kGradThreads - 1) / (N * kGradRuns * kGradThreads);
+                         constexpr bool         PAST  = decltype(past)::value;
+                         const int64_t          parts = ((int64_t)logits.columns + N * kGradThreads - 1) / (N * kGradThreads);
                          const LogProbsGradArgs a     = {RowPlaces(logits), RowPlaces(out), tokens.base, lse, entropy, grad, gradEntropy, scale,
                                                          logits.rows, logits.columns, DivBy((uint32_t)parts), tokens.dtype == NVCV_DATA_TYPE_S64};
-                         gradEntropy != nullptr ? LaunchLogProbsGrad<T, N, true>(a, stream) : LaunchLogProbsGrad<T, N, false>(a, stream);
+                         gradEntropy != nullptr ? LaunchLogProbsGrad<T, N, true, PAST>(a, stream) : LaunchLogProbsGrad<T, N, false, PAST>(a, stream);
                      };
-                     logits.columns >= kRunOf<T> ? run(std::integral_constant<int, kRunOf<T>>()) : run(std::integral_constant<int, 1>());
+                     const std::integral_constant<int, kRunOf<T>> whole;
+                     logits.columns < kRunOf<T> ? run(std::integral_constant<int, 1>(), std::false_type())
+                     : MovesPastCaches(2 * (int64_t)logits.rows * logits.columns * (int64_t)sizeof(T)) ? run(whole, std::true_type())
+                                                                                                       : run(whole, std::false_type());
                  });
     }
 };
