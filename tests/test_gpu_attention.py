@@ -454,3 +454,12 @@ def test_one_tensor_in_three_places(api, dtype):
     made = api.attention_grad(g, x, x, x, o, s, seq, causal=True, scale=call.scale)
     torch.cuda.synchronize()
     assert torch.equal(again.torch(), out) and all(torch.equal(a.torch(), b) for a, b in zip(made, grads))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,key_heads,d,room", [(8, 8, 128, 20000), (12, 4, 40, 60000), (4, 4, 64, 80000)])
+def test_single_tokens_before_large_caches(api, heads, key_heads, d, room, dtype):
+    """Caches that are larger than what the card keeps near its memory, filled to different lengths; NaN in all other places."""
+    assert 2 * 4 * room * key_heads * d * 2 > 128 << 20
+    Call([(1, 1), (1, 3000), (0, 40), (2, 777)], heads, key_heads, d, dtype, 60, True, room=room).check(api)
+    Call([(1, room), (1, 0), (3, 33), (1, 1025)], heads, key_heads, d, dtype, 61, False, room=room, before=1, behind=1).check(api)

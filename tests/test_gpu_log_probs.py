@@ -258,3 +258,15 @@ def test_whole_interface(api):
         got = out.clone(), stats.clone(), to.clone()
         want = run(api, x, tokens)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[2]) and torch.equal(got[2], gradient(api, x, tokens, want[2], g))
+
+
+@pytest.mark.parametrize("dtype,n", [(F32, 1100), (F16, 2200), (BF16, 2200)])
+def test_many_rows_of_an_odd_width(api, dtype, n):
+    """More logits than the card keeps near its memory; rows begin at odd addresses and end within a run."""
+    v = 32003
+    x = random((n, v), dtype, 13, 3.0)
+    assert x.numel() * x.element_size() > 128 << 20
+    check(api, x, words(n, v, 14), 0.9, 5)
+    tokens = words(n, v, 15)
+    got, both, (lse, g, entropy, h) = check_gradient(api, x, tokens)
+    assert torch.equal(gradient(api, x, tokens, lse, g, 1.0, entropy, h, out=x), both)

@@ -135,3 +135,13 @@ def test_another_stream_and_a_graph(api):
         torch.cuda.synchronize()
         assert torch.equal(out.clone(), run(api, x, positions, 64, inverse=True))
     assert back.isfinite().all()
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype,n,d,dims", [(F32, 9000, 129, 128), (BF16, 12000, 100, 36), (F16, 12000, 128, 128), (F32, 9000, 66, 62)])
+def test_many_tokens(api, dtype, n, d, dims, interleaved):
+    """More than the card keeps near its memory."""
+    x, positions = random((n, 32, d), dtype, 16), places(n, 17)
+    assert 2 * x.numel() * x.element_size() > 128 << 20
+    got = check(api, x, positions, dims, interleaved=interleaved)
+    assert torch.equal(run(api, x, positions, dims, out=x, interleaved=interleaved), got)
