@@ -40,7 +40,7 @@ struct __attribute__((packed, aligned(sizeof(T)))) Run
 
 // Runs of 16 bytes that a kernel reads or writes once. PAST: with the hint that the caches need not keep them, for calls that move more
 // than half of what the memory-side cache holds (256 MB). Their inputs and outputs are gone from there before they are wanted again, and what is
-// kept of them costs places: the gradient of 1 GiB of logits 344 us, 320 with the hint; in buffers that take turns 128 MB of logits 45 and
+// kept of them costs places: the gradient of 512 MB of logits 174 us, 164 with the hint; in buffers that take turns 128 MB of logits 45 and
 // 42, 64 MB 24 and 22. Smaller calls find their inputs there, and their outputs are found: 16 MB 6.8 us, with the hint 7.4.
 inline bool MovesPastCaches(int64_t bytes)
 {
