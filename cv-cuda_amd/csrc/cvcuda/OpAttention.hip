@@ -382,24 +382,26 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
     }
 }
 
-// The parts of the keys joined: 16 lanes to a row, 8 elements to a lane.
+// The parts of the keys joined: a tile of rows to blockIdx.y's workgroups, 16 lanes to a row, 8 elements to a lane. Tiles are found as they were made:
+// rows of no sequence have no parts, and with offsets that go back they may lie anywhere.
 constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 16, kMostSplits = 64;
 
 template<class T>
-__global__ __launch_bounds__(kJoinThreads) void AttentionJoinKernel(const AttentionArgs a)
+__global__ __launch_bounds__(kJoinThreads) void AttentionJoinKernel(const AttentionArgs a, int size)
 {
-    const int64_t rows = (int64_t)a.heads * a.sequences.rows, number = (int64_t)blockIdx.x * kJoinRows + threadIdx.x / 16;
-    const int     head = (int)(number / a.sequences.rows), token = (int)(number - (int64_t)head * a.sequences.rows), d = (int)(threadIdx.x % 16) * 8;
-    if (number >= rows)
+    const int          keyHead = (int)(blockIdx.x / a.tiles);
+    const SequenceTile s       = FindTile(a.sequences, blockIdx.x - (uint32_t)keyHead * a.tiles, a.tiles, size, a.rows.size(), false, false);
+    if (s.tile < 0)
     {
         return;
     }
-    // (rows of no sequence have no parts)
-    const int begin = a.sequences.firstRow(0), end = begin + a.sequences.rowsOf(a.sequences.count - 1, begin);
-    if (token < begin || token >= end)
+    const AttentionRow row(a.rows, false, s, keyHead, s.tile * size + (int)(blockIdx.y * kJoinRows + threadIdx.x / 16));
+    if (!row.there)
     {
         return;
     }
+    const int64_t rows = (int64_t)a.heads * a.sequences.rows, number = a.number(row);
+    const int     d    = (int)(threadIdx.x % 16) * 8;
     // lane l of the row has the lse of its pieces l, l + 16 ...
     float lse[kMostSplits / 16], top = -INFINITY, total = 0, out[8] = {};
 #pragma unroll
@@ -456,7 +458,7 @@ __global__ __launch_bounds__(kJoinThreads) void AttentionJoinKernel(const Attent
     {
         made.v[i] = FromFloat<T>(out[i] * factor);
     }
-    *reinterpret_cast<Run<T, 8> *>(a.out + token * a.outToken + head * a.outHead + d * 2) = made;
+    *reinterpret_cast<Run<T, 8> *>(a.out + row.token * a.outToken + row.head * a.outHead + d * 2) = made;
     if (d == 0 && a.lse != nullptr)
     {
         a.lse[number] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
@@ -527,8 +529,8 @@ void Launch(const AttentionArgs &a, bool few, hipStream_t stream)
     CheckLaunch("attention");
     if (a.splits > 1)
     {
-        const int64_t rows = (int64_t)a.heads * a.sequences.rows;
-        AttentionJoinKernel<T><<<(uint32_t)((rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, stream>>>(a);
+        const int size = few ? kFewRows : kManyRows;
+        AttentionJoinKernel<T><<<dim3(grid.x, (uint32_t)(size / kJoinRows)), kJoinThreads, 0, stream>>>(a, size);
         CheckLaunch("attention's parts");
     }
 }

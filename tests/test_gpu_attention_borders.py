@@ -1,0 +1,46 @@
+"""Attention at the borders of what its header allows: offsets that go back."""
+import importlib
+
+import pytest
+import torch
+
+from test_gpu_attention import BF16, F16, Call, numbers
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def api(cv, gpu):
+    return importlib.import_module("cvcuda_amd.pyapi")
+
+
+@pytest.fixture(autouse=True)
+def no_default_stream_is_followed(api, monkeypatch):
+    monkeypatch.setattr(api, "_followed", {})
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [20, 90])  # (few to a sequence, and many)
+@pytest.mark.parametrize("back", [lambda n: [0, n // 3, n // 4], lambda n: [n // 2, n // 9, n], lambda n: [n // 3, n, n // 2, n // 4],
+                                  lambda n: [n // 2, n // 4, n // 3, 0, n // 8]],
+                         ids=["last", "first", "two", "between"])
+def test_pieces_of_sequences_whose_offsets_go_back(api, cv, back, rows, dtype):
+    """A sequence whose end lies before its begin has no rows; the others' are the same as where it has its end at its begin, whether their
+    keys are in one piece or in several."""
+    offsets = back(rows)
+    sequences = len(offsets) - 1
+    call = Call([(rows, rows)] + [(0, 0)] * (sequences - 1), 4, 4, 64, dtype, rows, room=2100)
+    call.k, call.v = (torch.where(t.isnan(), torch.ones_like(t), t) for t in (call.k, call.v))
+    call.key_lengths = numbers([1100 + 300 * b for b in range(sequences)])
+    assert cv.Attention.workspace(rows, call.keys, sequences, 4, 4, 64) > 0
+    want, stats = torch.full(call.q.shape, 7.0, dtype=dtype, device="cuda"), torch.full((4, rows), 7.0, device="cuda")
+    for b in range(sequences):
+        if offsets[b] < offsets[b + 1]:
+            call.offsets = numbers([offsets[b]] * (b + 1) + [offsets[b + 1]] * (sequences - b))
+            alone, lse = call.run(api)
+            at = slice(offsets[b], offsets[b + 1])
+            want[at], stats[:, at] = alone[at], lse[:, at]
+            assert (alone[at] != 7).any(-1).all() and (lse[:, at] != 7).all()
+    call.offsets = numbers(offsets)
+    out, lse = call.run(api)
+    assert torch.equal(out, want) and torch.equal(lse, stats)
