@@ -1,13 +1,16 @@
 // Log probabilities of tokens with entropy and top alternatives, and their gradient (formulas: cvcuda/LogProbs.h). Bound by memory: the
 // logits are read once.
 //
-// One pass over a row: each lane has a number b that it takes exponentials relative to, and the sums of e = exp(z - b) and of e * (z - b).
-// b is the lane's first large z, and grows, the sums being rescaled, where a z lies more than kSlack above it: the sums have room for
-// e^kSlack, and most lanes never do. The workgroup joins its lanes' afterwards. The entropy is log(s) - t / s, in which nothing
-// large is left to cancel. The top tokens come from what the pass has
-// anyway: a number that K of the lanes' largest logits, by 64 groups, reach is one that K logits of the row reach, so that the lanes
-// which reach it, few in most rows, look through theirs again for those that do (4096 rows of 128000 BF16 with the top 5 186 us, 5.6
-// TB/s). Where too many do, or the row has NaN, the whole row is gone over K times.
+// One pass over a row: each wave has a logit a that it takes exponentials relative to, and the sums r of e = exp(z - z_a) and t of
+// e * (z - z_a) of all its logits but a. a is the largest of its first ones, and then the largest of those that lie more than kSlack above a, the
+// sums being rescaled: few do. The waves' are joined relative to the largest a. Log probabilities are then (x - a) * scale - log(1 + r), the entropy is
+// log(1 + r) - t / (1 + r). Of a row with one logit far above the others that one is a: r is what the others leave of it, in all its digits,
+// and nothing of the size of logits, or of 1, is there to cancel. (A largest logit that isn't a lies at most kSlack above it, so that a has
+// a share of 1 / (1 + e^kSlack) at least beside it.)
+//
+// The top tokens come from what the pass has anyway: a number that K of the lanes' largest logits, by 64 groups, reach is one that K
+// logits of the row reach, so that the lanes which reach it, few in most rows, look through theirs again for those that do (4096 rows of
+// 128000 BF16 with the top 5 189 us, 5.5 TB/s). Where too many do, or the row has NaN, the whole row is gone over K times.
 #include "RowOps.hpp"
 
 #include <cvcuda/LogProbs.h>
@@ -23,7 +26,7 @@ namespace {
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2   = 0.6931471805599453f;
 constexpr float kFar   = -1e30f; // below any difference whose exponential isn't 0; a sum of 2^31 of it is finite
-constexpr float kSlack = 20.f;
+constexpr float kSlack = 2.f; // (4096 rows of 128000 BF16 189.5 us, with 20 187.7, and 1 - p of likely tokens known to 5e-6 only)
 
 __device__ __forceinline__ float Exp(float x)
 {
@@ -38,7 +41,7 @@ struct LogProbsArgs
     const void *tokens;
     float      *out, *entropy, *lse, *topValues; // all but out: nullptr where not wanted
     int32_t    *topTokens;
-    float       scale;
+    float       scale, slack; // slack: kSlack / scale
     int32_t     rows, columns, top, firstRow;
     bool        wide; // tokens of 64 bits
 };
@@ -117,15 +120,15 @@ __device__ __forceinline__ uint64_t LargestKey(uint64_t v, uint64_t (&part)[WAVE
     return v;
 }
 
-// What the row's log probabilities are taken relative to: that of x is scale * x - base - logSum.
+// What the row's log probabilities are taken relative to: that of x is scale * (x - at) - logSum.
 struct Total
 {
-    float scale, base, logSum;
+    float scale, at, logSum;
     bool  nothing; // all logits are -infinity
 
     __device__ __forceinline__ float of(float x) const
     {
-        return nothing ? -INFINITY : __builtin_fmaf(x, scale, -base) - logSum;
+        return nothing ? -INFINITY : (x - at) * scale - logSum;
     }
 };
 
@@ -146,45 +149,142 @@ __device__ __forceinline__ float Largest(float a, float b, float c)
     return r;
 }
 
-// A lane's sums on their way through the row.
+// The largest of N logits and of `top`. (A NaN among them is left out.)
+template<int N>
+__device__ __forceinline__ float LargestOf(float top, const float (&v)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+    {
+        top = Largest(top, v[i], v[std::min(i + 1, N - 1)]);
+    }
+    return top;
+}
+
+// The sums r of e and t of e * (z - z_a) over some logits but `at`, the logit a (-infinity: all were).
 struct Sums
 {
-    float base, s, t, top; // top: the largest logit
+    float at, r, t;
+};
 
-    __device__ __forceinline__ explicit Sums()
-        : base(-INFINITY)
-        , s(0)
+// A wave's lanes on their way through the row.
+struct Running
+{
+    float at, base, limit; // the same in all lanes: scale * at, rounded, and the logit above which the sums are rescaled
+    float r, t, top;       // the lane's, relative to `base`; its largest logit
+
+    __device__ __forceinline__ explicit Running()
+        : at(-INFINITY)
+        , base(-INFINITY)
+        , limit(-INFINITY)
+        , r(0)
         , t(0)
         , top(-INFINITY)
     {
     }
 
-    // N logits; (a NaN among them is left out of `top`, and reaches the sums)
+    // Sums from now on relative to `to`, the largest of the lanes' `top` and one of their next logits v: the first lane that has it
+    // takes it out of them.
     template<int N>
-    __device__ __forceinline__ void add(const float (&v)[N], float scale)
+    __device__ __forceinline__ void begin(float to, float (&v)[N], float scale, float slack)
     {
-#pragma unroll
-        for (int i = 0; i < N; i += 2)
-        {
-            top = Largest(top, v[i], v[std::min(i + 1, N - 1)]);
-        }
-        if (top * scale > base + kSlack)
-        {
-            const float to = top * scale, less = fmaxf(base - to, kFar), r = Exp(less);
-            t    = r * __builtin_fmaf(s, less, t);
-            s    = s * r;
-            base = to;
-        }
-        const float from = base == -INFINITY ? 0.f : base; // (all were -infinity so far)
+        const uint64_t some = __ballot(top == to);
+        bool           mine = some != 0 && (int)(threadIdx.x & 63) == (int)__builtin_ctzll(some);
+        base  = to * scale;
+        at    = base == -INFINITY ? base : to;
+        limit = at == -INFINITY ? at : at + slack;
 #pragma unroll
         for (int i = 0; i < N; ++i)
         {
-            const float d = __builtin_fmaf(v[i], scale, -from), e = Exp(d);
-            s += e;
-            t = __builtin_fmaf(e, fmaxf(d, kFar), t); // (e is 0 where d is -infinity)
+            const bool its = mine && v[i] == to;
+            v[i]           = its ? -INFINITY : v[i];
+            mine           = mine && !its;
         }
     }
+
+    // The lanes' next N logits (-infinity where one has none).
+    template<int N>
+    __device__ __forceinline__ void next(float (&v)[N], float scale, float slack)
+    {
+        top = LargestOf(top, v);
+        if (__any(top > limit))
+        {
+            const float to = ValueOf(WaveLargest(OrderOf(top)));
+            if (at != -INFINITY)
+            {
+                // the logit `at` is one of the first lane's from here on
+                const float its = rounding(scale), e = (threadIdx.x & 63) == 0 ? Exp(its) : 0.f;
+                const float less = fmaxf(base - to * scale, kFar), share = Exp(less);
+                r += e;
+                t = share * __builtin_fmaf(r, less, __builtin_fmaf(e, its, t));
+                r = share * r;
+            }
+            begin(to, v, scale, slack);
+        }
+        add(v, scale);
+    }
+
+    template<int N>
+    __device__ __forceinline__ void add(const float (&v)[N], float scale)
+    {
+        const float from = base == -INFINITY ? 0.f : base; // (all were -infinity so far)
+        float       e[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const float d = __builtin_fmaf(v[i], scale, -from);
+            e[i]          = Exp(d);
+            t             = __builtin_fmaf(e[i], fmaxf(d, kFar), t); // (e is 0 where d is -infinity)
+        }
+#pragma unroll
+        for (int w = N / 2; w > 0; w /= 2)
+        {
+#pragma unroll
+            for (int i = 0; i < w; ++i)
+            {
+                e[i] += e[i + w];
+            }
+        }
+        r += e[0];
+    }
+
+    // What scale * at is above `base`.
+    __device__ __forceinline__ float rounding(float scale) const
+    {
+        return base == -INFINITY ? 0.f : __builtin_fmaf(at, scale, -base);
+    }
+
+    // The wave's, relative to `at` itself.
+    __device__ __forceinline__ Sums sums(float scale) const
+    {
+        Sums        s    = {at, WaveSum(r), WaveSum(t)};
+        const float less = -rounding(scale);
+        if (less != 0)
+        {
+            const float share = Exp(less);
+            s.t = share * __builtin_fmaf(s.r, less, s.t);
+            s.r = share * s.r;
+        }
+        return s;
+    }
 };
+
+// log(1 + r), to its own last bits: 1 + r is u and what was lost when that was rounded, whose share of u is what the logarithm lacks.
+__device__ __forceinline__ float Log1(float r)
+{
+    const float u = 1.f + r;
+    return __builtin_fmaf(__builtin_amdgcn_logf(u), kLn2, (r - (u - 1.f)) * __builtin_amdgcn_rcpf(u));
+}
+
+// The sums that a wave's lanes have as one.
+__device__ __forceinline__ Sums Joined(const Sums &s, float scale)
+{
+    const float    at   = ValueOf(WaveLargest(OrderOf(s.at)));
+    const uint64_t some = __ballot(s.at == at);
+    const bool     its  = some != 0 && (int)(threadIdx.x & 63) == (int)__builtin_ctzll(some);
+    const float    less = s.at == at ? 0.f : fmaxf((s.at - at) * scale, kFar), share = Exp(less), all = s.r + (its || s.at == -INFINITY ? 0.f : 1.f);
+    return {at, WaveSum(share * all), WaveSum(share * __builtin_fmaf(all, less, s.t))};
+}
 
 // N: logits of a run (1 where rows are narrower than 16 bytes). One workgroup to a row. HELD: the row fits the registers of runs on their
 // way, and is looked through again there.
@@ -192,13 +292,13 @@ template<class T, int N, int WAVES, int AHEAD, bool HELD, bool PAST>
 __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs a)
 {
     constexpr int       kLanes = 64 * WAVES;
-    __shared__ float    s_base[WAVES], s_s[WAVES], s_t[WAVES];
+    __shared__ Sums     s_sums[WAVES];
     __shared__ uint64_t s_key[WAVES];
     __shared__ TopRoom  s_top;
     const uint32_t row  = a.firstRow + blockIdx.x;
     const T       *in   = reinterpret_cast<const T *>(a.logits.at(row));
     const int      runs = (a.columns + N - 1) / N, whole = a.columns / N;
-    Sums           sums;
+    Running        run;
     Logits<T, N, PAST>   x[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
@@ -209,7 +309,9 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     const int64_t token = TokenAt(a.tokens, a.wide, row);
     const bool    there = token >= 0 && token < a.columns;
     const float   its   = (float)in[there ? token : 0];
-    auto          take  = [&](const Logits<T, N, PAST> &l, int r)
+    // runs of the wave's lanes from `at` on
+    const int lane = (int)(threadIdx.x & 63);
+    auto      take = [&](const Logits<T, N, PAST> &l, int at)
     {
         float v[N];
 #pragma unroll
@@ -217,59 +319,44 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         {
             v[i] = (float)l.run.v[i];
         }
-        if (r >= whole) // (the row's last run, where it is not a whole one)
+        if (at + 64 > whole) // (the row's last run, where it is not a whole one, or none)
         {
             asm volatile(""); // (or the compiler makes what follows for every run, and chooses afterwards)
 #pragma unroll
             for (int i = 0; i < N; ++i)
             {
-                v[i] = i >= l.skip ? v[i] : -INFINITY;
+                v[i] = at + lane < whole || (i >= l.skip && at + lane < runs) ? v[i] : -INFINITY;
             }
         }
-        sums.add(v, a.scale);
+        run.next(v, a.scale, a.slack);
     };
-    for (int r = (int)threadIdx.x; r < runs; r += AHEAD * kLanes)
+    for (int at = (int)WaveOfGroup() * 64; at < runs; at += AHEAD * kLanes)
     {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
         {
-            if (r + k * kLanes < runs)
+            if (at + k * kLanes < runs)
             {
-                take(x[k], r + k * kLanes);
+                take(x[k], at + k * kLanes);
             }
             if (!HELD)
             {
-                x[k].get(in, a.columns, min(r + (k + AHEAD) * kLanes, runs - 1));
+                x[k].get(in, a.columns, min(at + lane + (k + AHEAD) * kLanes, runs - 1));
             }
         }
     }
-    // the workgroup's sums; a lane that has met nothing but -infinity, or nothing, has s = 0
-    auto join = [&](float &base, float &s, float &t, float to)
-    {
-        const float less = fmaxf(base - to, kFar), r = Exp(less);
-        t    = s != 0 ? r * __builtin_fmaf(s, less, t) : 0.f;
-        s    = s != 0 ? r * s : 0.f;
-        base = to;
-    };
-    float base, s, t;
-    auto  ofWave = [&](float b, float sb, float tb)
-    {
-        base = ValueOf(WaveLargest(OrderOf(b)));
-        join(b, sb, tb, base);
-        s = WaveSum(sb), t = WaveSum(tb);
-    };
-    ofWave(sums.base, sums.s, sums.t);
+    Sums sums = run.sums(a.scale);
     if constexpr (WAVES > 1)
     {
         if ((threadIdx.x & 63) == 0)
         {
-            s_base[WaveOfGroup()] = base, s_s[WaveOfGroup()] = s, s_t[WaveOfGroup()] = t;
+            s_sums[WaveOfGroup()] = sums;
         }
     }
     if (a.top > 0)
     {
         // groups of WAVES lanes that follow one another
-        float g = sums.top;
+        float g = run.top;
 #pragma unroll
         for (int d = 1; d < WAVES; d *= 2)
         {
@@ -285,23 +372,35 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         }
     }
     __syncthreads();
+    bool sound = sums.r == sums.r; // (the row has neither NaN nor +infinity)
     if constexpr (WAVES > 1)
     {
-        const uint32_t w = threadIdx.x % 64 % WAVES;
-        const bool     one = threadIdx.x % 64 < WAVES;
-        ofWave(one ? s_base[w] : -INFINITY, one ? s_s[w] : 0.f, one ? s_t[w] : 0.f);
+        const Sums none = {-INFINITY, 0, 0};
+        sums            = lane < WAVES ? s_sums[lane] : none;
+        sound           = !__any(sums.r != sums.r);
     }
-    const Total total = {a.scale, base, s == 0 ? 0.f : __builtin_amdgcn_logf(s) * kLn2, s == 0};
-    if (threadIdx.x == 0)
+    // (by the first wave, and by all where all need it)
+    Total total;
+    auto  join = [&]()
     {
-        a.out[row] = there ? total.of(its) : 0.f;
-        if (a.entropy != nullptr)
+        const Sums all = WAVES > 1 ? Joined(sums, a.scale) : sums;
+        total          = {a.scale, all.at, Log1(all.r), all.at == -INFINITY && all.r == 0};
+        return all;
+    };
+    if (threadIdx.x < 64)
+    {
+        const Sums all = join();
+        if (threadIdx.x == 0)
         {
-            a.entropy[row] = total.nothing ? 0.f : total.logSum - t / s;
-        }
-        if (a.lse != nullptr)
-        {
-            a.lse[row] = total.nothing ? -INFINITY : base + total.logSum;
+            a.out[row] = there ? total.of(its) : 0.f;
+            if (a.entropy != nullptr)
+            {
+                a.entropy[row] = total.nothing ? 0.f : total.logSum - all.t / (1.f + all.r);
+            }
+            if (a.lse != nullptr)
+            {
+                a.lse[row] = total.nothing ? -INFINITY : __builtin_fmaf(all.at, a.scale, total.logSum);
+            }
         }
     }
     if (a.top == 0)
@@ -310,7 +409,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     }
     // A logit that K groups' largest ones reach, and not many more: between the smallest and the largest of them, by halves.
     const uint32_t mine = s_top.group[threadIdx.x & 63];
-    uint32_t       low = ~WaveLargest(~mine), high = s == s ? WaveLargest(mine) + 1 : low;
+    uint32_t       low = ~WaveLargest(~mine), high = sound ? WaveLargest(mine) + 1 : low;
     while (high - low > 1)
     {
         const uint32_t middle = low + (high - low) / 2;
@@ -351,7 +450,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
             }
         }
     };
-    if (sums.top >= least && s == s)
+    if (run.top >= least && sound)
     {
         if constexpr (HELD)
         {
@@ -386,7 +485,7 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     }
     __syncthreads();
     const int count = (int)s_top.count;
-    if (s == s && count >= a.top && count <= 64)
+    if (sound && count >= a.top && count <= 64)
     {
         if (threadIdx.x < 64)
         {
@@ -405,8 +504,12 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
         }
         return;
     }
-    if (s == s && count >= a.top && count <= kCandidates)
+    if (sound && count >= a.top && count <= kCandidates)
     {
+        if (threadIdx.x >= 64)
+        {
+            join();
+        }
         for (int i = (int)threadIdx.x; i < count; i += kLanes)
         {
             const uint64_t key   = s_top.key[i];
@@ -665,7 +768,7 @@ public:
         {
             return;
         }
-        const LogProbsArgs a = {RowPlaces(logits), tokens.base, out, entropy, lse, topValues, topTokens, scale, logits.rows, logits.columns,
+        const LogProbsArgs a = {RowPlaces(logits), tokens.base, out, entropy, lse, topValues, topTokens, scale, kSlack / scale, logits.rows, logits.columns,
                                 (int32_t)top, 0, tokens.dtype == NVCV_DATA_TYPE_S64};
         Dispatch(logits.elem,
                  [&](auto t)
