@@ -63,11 +63,11 @@ __device__ __forceinline__ float LargestMagnitude(float a, float b, float c)
     return r;
 }
 
-// What the shares' gradients t are multiplied with before they are rounded to T. In F16 small ones would be lost (its smallest number is 2^-24)
-// and large ones are not bounded, so it is a power of two that follows the largest that the wave has met: at first one that no
-// small t is lost with, and lowered, with the sums so far, where a t passes 2^15, so that the largest is at 2^12 to 2^13 again. What is
-// 2^-26 of the largest keeps all of its bits. (Taken from the largest rows of gradOut and v, by a kernel that reads both before, it cost
-// short sequences 13 us.)
+// What a column's gradients t of shares are multiplied with before they are rounded to T. In F16 small ones would be lost (its smallest number is
+// 2^-24) and large ones are not bounded, so it is a power of two that follows the largest that the column, a row's or a key's, has met: at first one
+// that no small t is lost with, and lowered, with the sums so far, where a t passes 2^15, so that the largest is at 2^11 to 2^12 again. What is 2^-25 of
+// the largest keeps all of its bits. (Taken from the largest rows of gradOut and v, by a kernel that reads both before, it cost short sequences
+// 13 us.)
 template<class T>
 struct GradScale
 {
@@ -89,8 +89,9 @@ struct GradScale
             }
             if (__any(most > 0x1p15f))
             {
-                const uint32_t exponent = WaveLargest(__float_as_uint(most)) >> 23; // (127: 1 to 2; 255: not finite)
-                const float    less     = __uint_as_float((127u - min(exponent - (127u + 12u), 100u)) << 23);
+                most                    = BothMax(most); // (the column's other half)
+                const uint32_t exponent = __float_as_uint(most) >> 23; // (127: 1 to 2; 255: not finite)
+                const float    less     = most > 0x1p15f ? __uint_as_float((127u - min(exponent - (127u + 11u), 100u)) << 23) : 1.f;
                 factor *= less;
                 t *= less;
                 lower(less);

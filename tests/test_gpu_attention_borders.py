@@ -44,3 +44,23 @@ def test_pieces_of_sequences_whose_offsets_go_back(api, cv, back, rows, dtype):
     call.offsets = numbers(offsets)
     out, lse = call.run(api)
     assert torch.equal(out, want) and torch.equal(lse, stats)
+
+
+def test_small_gradients_beside_large_ones_in_f16(api):
+    """A row's gradient of q, and that of keys which only rows of small gradients see, depend on no other row: bit for bit the same where those beside
+    them have gradients larger by 2^28."""
+    for d, heads, key_heads in ((64, 2, 2), (128, 4, 2)):
+        call = Call([(150, 150)], heads, key_heads, d, F16, d)
+        call.grad = (call.grad.float() * 2.0 ** -16).half()
+        out, lse = call.run(api)
+        small = call.gradients(api, out, lse)
+        last, alone = slice(140, 150), slice(40, 43)
+        large = call.grad.float() * 2.0 ** 28
+        large[last], large[alone] = call.grad[last].float(), call.grad[alone].float()
+        call.grad = large.half()
+        assert call.grad.isfinite().all() and call.grad.abs().max() > 2.0 ** 13
+        got = call.gradients(api, out, lse)
+        for rows in (last, alone):
+            assert torch.equal(got[0][rows], small[0][rows]) and (got[0][rows] != 0).any()
+        for a, b in zip(got[1:], small[1:]):
+            assert torch.equal(a[last], b[last]) and (a[last] != 0).any()
