@@ -53,6 +53,13 @@ __device__ __forceinline__ float BothSum(float v)
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A number that the compiler takes for another one than v: what is made of it once more doesn't wait in registers.
+__device__ __forceinline__ uint32_t Again(uint32_t v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // Keeps the compiler from making what stands in a branch in every case, and choosing afterwards.
 __device__ __forceinline__ void KeepBranch()
 {
@@ -113,9 +120,14 @@ __device__ __forceinline__ Vec8<T> RoundedHalf(const Acc16 &v, int half)
 }
 
 // The row that a lane's number i of a product lies in.
+__device__ __forceinline__ int RowOf(int i, int lane)
+{
+    return (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3);
+}
+
 __device__ __forceinline__ int RowOf(int i)
 {
-    return (i >> 2) * 8 + (int)((threadIdx.x & 63) >> 5) * 4 + (i & 3);
+    return RowOf(i, (int)(threadIdx.x & 63));
 }
 
 // ROWS rows from memory to a tile in LDS, without a stop in registers, by WAVES waves. Each instruction moves 64 units to 64 places that
@@ -217,9 +229,9 @@ __device__ __forceinline__ void CopiesAndBarrier()
 // A row of a matrix as the right operand's column: elements 16 * step + 8 * (l / 32) to + 7 of it, zeros behind `dims`. Loads stand
 // under no condition.
 template<class T, int DP>
-__device__ __forceinline__ void LoadColumn(Vec8<T> (&to)[DP / 16], const uint8_t *row, int dims)
+__device__ __forceinline__ void LoadColumn(Vec8<T> (&to)[DP / 16], const uint8_t *row, int dims, uint32_t thread = threadIdx.x)
 {
-    const int first = (int)((threadIdx.x & 63) >> 5) * 8;
+    const int first = (int)((thread & 63) >> 5) * 8;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
     {
@@ -232,59 +244,168 @@ __device__ __forceinline__ void LoadColumn(Vec8<T> (&to)[DP / 16], const uint8_t
     }
 }
 
-// A transposed product's columns to rows of memory: lane l's column is the row at `row`, times `factor`, rounded. Lanes exchange what they
-// have, so that each stores whole 16 bytes.
-template<class T, int DP>
-__device__ __forceinline__ void StoreColumn(const Acc16 (&acc)[DP / 32], float factor, uint8_t *row, bool there, int dims)
+// 32 numbers of a transposed product's columns, from 32 * part on, to rows of memory: lane l's column is the row at `row`, times `factor`, rounded.
+// Lanes exchange what they have, so that each stores whole 16 bytes.
+template<class T>
+__device__ __forceinline__ void StoreColumnPart(const Acc16 &acc, int part, float factor, uint8_t *row, bool there, int dims)
 {
-    const int upper = (int)((threadIdx.x & 63) >> 5);
+    const int upper = (int)((Again(threadIdx.x) & 63) >> 5);
 #pragma unroll
-    for (int part = 0; part < DP / 32; ++part)
+    for (int p = 0; p < 2; ++p)
     {
+        uint32_t words[2][2]; // of the elements 16 * p + 4 * upper to + 3, and 8 + that
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
+        for (int k = 0; k < 2; ++k)
         {
-            uint32_t words[2][2]; // of the elements 16 * p + 4 * upper to + 3, and 8 + that
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int w = 0; w < 2; ++w)
             {
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
+                struct
                 {
-                    struct
-                    {
-                        T a, b;
-                    } two = {(T)(acc[part][8 * p + 4 * k + 2 * w] * factor), (T)(acc[part][8 * p + 4 * k + 2 * w + 1] * factor)};
-                    words[k][w] = __builtin_bit_cast(uint32_t, two);
-                }
+                    T a, b;
+                } two = {(T)(acc[8 * p + 4 * k + 2 * w] * factor), (T)(acc[8 * p + 4 * k + 2 * w + 1] * factor)};
+                words[k][w] = __builtin_bit_cast(uint32_t, two);
             }
-            const auto     x = __builtin_amdgcn_permlane32_swap(words[0][0], words[1][0], false, false);
-            const auto     y = __builtin_amdgcn_permlane32_swap(words[0][1], words[1][1], false, false);
-            const int      first = part * 32 + 16 * p + 8 * upper;
-            if (there && first < dims)
-            {
-                *reinterpret_cast<uint4 *>(row + first * 2) = make_uint4(x[0], y[0], x[1], y[1]);
-            }
+        }
+        const auto x     = __builtin_amdgcn_permlane32_swap(words[0][0], words[1][0], false, false);
+        const auto y     = __builtin_amdgcn_permlane32_swap(words[0][1], words[1][1], false, false);
+        const int  first = part * 32 + 16 * p + 8 * upper;
+        if (there && first < dims)
+        {
+            *reinterpret_cast<uint4 *>(row + first * 2) = make_uint4(x[0], y[0], x[1], y[1]);
         }
     }
 }
 
+template<class T, int DP>
+__device__ __forceinline__ void StoreColumn(const Acc16 (&acc)[DP / 32], float factor, uint8_t *row, bool there, int dims)
+{
+#pragma unroll
+    for (int part = 0; part < DP / 32; ++part)
+    {
+        StoreColumnPart<T>(acc[part], part, factor, row, there, dims);
+    }
+}
+
 // The same to a row of F32, which is joined with those of other pieces.
+__device__ __forceinline__ void StorePiecePart(const Acc16 &acc, int part, float factor, float *row, bool there, int dims)
+{
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+    {
+        const int d = 32 * part + RowOf(i);
+        if (there && d < dims)
+        {
+            *reinterpret_cast<float4 *>(row + d) = make_float4(acc[i] * factor, acc[i + 1] * factor, acc[i + 2] * factor, acc[i + 3] * factor);
+        }
+    }
+}
+
 template<int DP>
 __device__ __forceinline__ void StorePiece(const Acc16 (&acc)[DP / 32], float factor, float *row, bool there, int dims)
 {
 #pragma unroll
     for (int p = 0; p < DP / 32; ++p)
     {
+        StorePiecePart(acc[p], p, factor, row, there, dims);
+    }
+}
+
+// ---- values that are not finite ----------------------------------------------------------------------------------------------
+// A tile's products give what a row does not see a weight of 0, and 0 times an infinity or NaN is NaN. So where a result is not finite, and something
+// in its tiles that not all of its rows or keys see isn't either, its wave makes it once more, by itself and from memory, 32 numbers of the
+// columns at a time (few registers): where something is hidden each row of the matrix has a product of its own, which only the columns that see it
+// take. Finite inputs pay a sum over the results (long prompts 271.4 us, 272.4 before); a call whose inputs are all NaN takes up to 40 times
+// as long.
+template<int N>
+__device__ __forceinline__ bool AnyNotFinite(const Acc16 (&sum)[N])
+{
+    Acc16 all = sum[0];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
+    for (int p = 1; p < N; ++p)
+    {
+        all += sum[p];
+    }
+    float one = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+    {
+        one += all[i];
+    }
+    return __any(!(fabsf(one) < INFINITY)); // (a sum of these that overflows costs time alone)
+}
+
+// Rows of a matrix in memory, the row at `row` being the lane's and that of the lane 32 from it, times columns(step).
+template<class T, int DP, class F>
+__device__ __forceinline__ void MultiplyRows(Acc16 &sum, const uint8_t *row, int dims, F &&columns)
+{
+    const int first = (int)((Again(threadIdx.x) & 63) >> 5) * 8;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+    {
+        const Vec8<T> part = *reinterpret_cast<const Vec8<T> *>(row + min(16 * s + first, dims - 8) * 2);
+        Multiply(sum, 16 * s + first < dims ? part : Vec8<T>{}, columns(s));
+        __builtin_amdgcn_sched_barrier(0); // (one after the other: few registers)
+    }
+}
+
+// Whether `count` rows, in memory at rowAt(n), hold a number that is not finite.
+template<class T, class R>
+__device__ __forceinline__ bool RowsNotFinite(int dims, int count, R &&rowAt)
+{
+    constexpr uint32_t kExponent = std::is_same<T, Half>::value ? 0x7C00 : 0x7F80;
+    const int          at        = (int)(Again(threadIdx.x) & 63) * 2;
+    bool               some      = false;
+    for (int n = 0; n < count; ++n)
+    {
+        const uint32_t two = at < dims ? *reinterpret_cast<const uint32_t *>(rowAt(n) + at * 2) : 0;
+        some |= (two & kExponent) == kExponent || (two >> 16 & kExponent) == kExponent;
+    }
+    return __any(some);
+}
+
+// `count` rows of a matrix, up to 32, their columns 32 * part on times the columns of `weights`, to `sum`: row n, in memory at rowAt(n), to
+// the columns of which seen(n); `all`: to all of them.
+template<class T, class R, class F>
+__device__ __forceinline__ void MultiplySeen(Acc16 &sum, const Acc16 &weights, int part, int dims, int count, bool all, R &&rowAt, F &&seen)
+{
+    using Words           = uint32_t __attribute__((ext_vector_type(4)));
+    const uint32_t lane   = Again(threadIdx.x) & 63;
+    const int      column = 32 * part + (int)(lane & 31);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+        const Words packed = __builtin_bit_cast(Words, RoundedHalf<T>(weights, half));
+        Words       values = {};
+#pragma unroll 1
+        for (int n = 0; n < min(16, count - 16 * half); ++n)
         {
-            const int d = 32 * p + RowOf(i);
-            if (there && d < dims)
+            // the half wave and the element that have row n of 16
+            const bool     own     = lane >> 5 == (uint32_t)(n >> 2 & 1);
+            const int      element = (n >> 3) * 4 + (n & 3), shift = 16 * (element & 1);
+            const uint32_t value   = own && column < dims ? (uint32_t)reinterpret_cast<const uint16_t *>(rowAt(16 * half + n))[column] << shift : 0;
+            Words          weight;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
             {
-                *reinterpret_cast<float4 *>(row + d) =
-                    make_float4(acc[p][i] * factor, acc[p][i + 1] * factor, acc[p][i + 2] * factor, acc[p][i + 3] * factor);
+                values[i] = (all ? values[i] : 0) | (i == element / 2 ? value : 0);
+                weight[i] = own && i == element / 2 ? packed[i] & 0xFFFFu << shift : 0;
             }
+            if (!all)
+            {
+                const bool takes = seen(16 * half + n);
+                Acc16      one   = {};
+                Multiply(one, __builtin_bit_cast(Vec8<T>, values), __builtin_bit_cast(Vec8<T>, weight));
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    sum[i] = takes ? sum[i] + one[i] : sum[i];
+                }
+            }
+        }
+        if (all)
+        {
+            Multiply(sum, __builtin_bit_cast(Vec8<T>, values), __builtin_bit_cast(Vec8<T>, packed));
         }
     }
 }

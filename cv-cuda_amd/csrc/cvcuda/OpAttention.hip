@@ -133,6 +133,30 @@ __device__ __forceinline__ void Scores(Acc16 (&scores)[N], const uint8_t *keys, 
     }
 }
 
+// Numbers 32 * part on of a row's weighted values from keys firstKey to behindKey, `step` of them after the other, made from memory, those
+// that the row doesn't see left out.
+template<class T, int DP>
+__device__ __forceinline__ Acc16 SeenPart(const AttentionArgs &a, const Vec8<T> (&q)[DP / 16], const uint8_t *k, const uint8_t *v, int firstKey,
+                                          int behindKey, int step, int keys, int limit, float top, int part)
+{
+    const float shift = kExpShift<T> - (top == -INFINITY ? 0.f : top);
+    Acc16       out   = {};
+    const int   lane  = (int)Again(threadIdx.x) & 63;
+    for (int key = firstKey; key < behindKey; key += step)
+    {
+        Acc16 scores = {};
+        MultiplyRows<T, DP>(scores, k + min(key + (lane & 31), keys - 1) * a.kToken, a.dims, [&](int s) { return q[s]; });
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            scores[i] = key + RowOf(i, lane) <= limit ? __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i], a.scale, shift)) : 0.f;
+        }
+        MultiplySeen<T>(out, scores, part, a.dims, keys - key, !__any(key + 31 > limit),
+                        [&](int n) { return v + (key + n) * a.vToken; }, [&](int n) { return key + n <= limit; });
+    }
+    return out;
+}
+
 // What a row has at the end: lse to the base 2.
 template<class T>
 __device__ __forceinline__ float LseOf(float top, float sum)
@@ -150,7 +174,9 @@ constexpr int kManyKeys = DP > 64 ? 32 : 64;
 template<int DP>
 constexpr int kManyWaves = DP > 64 ? 3 : 4;
 
-template<class T, int DP>
+// (CAUSAL: calls of the other kind hide nothing, and their kernels need fewer registers without what that takes: pairs 21.6 us, with one kernel for
+// both 21.9, their gradient 69.4 and 73.)
+template<class T, int DP, bool CAUSAL>
 __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(const AttentionArgs a)
 {
     constexpr int kKeys = kManyKeys<DP>;
@@ -158,16 +184,16 @@ __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(
     __shared__ __attribute__((aligned(256))) uint8_t s_v0[kKeys * DP * 2], s_v1[kKeys * DP * 2];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
     const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
-    const SequenceTile s       = FindTile(a.sequences, t, a.tiles, kManyRows, a.rows.size(), false, a.causal);
+    const SequenceTile s       = FindTile(a.sequences, t, a.tiles, kManyRows, a.rows.size(), false, CAUSAL);
     if (s.tile < 0)
     {
         return;
     }
     const uint32_t wave = WaveOfGroup();
     const int  first = s.tile * kManyRows, ownFirst = first + (int)wave * 32, all = s.rows * a.rows.size();
-    const AttentionRow row(a.rows, a.causal, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
+    const AttentionRow row(a.rows, CAUSAL, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
     // keys of the tile, of the wave and those that all of the wave's rows see; this workgroup's part of the tile's
-    auto       limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
+    auto       limitAt  = [&](int r) { return LimitOf(CAUSAL, s, a.rows.token(min(r, all - 1))); };
     const int  tileKeys = max(limitAt(first + kManyRows - 1) + 1, 0), waveKeys = ownFirst < all ? limitAt(ownFirst + 31) + 1 : 0;
     const int  seenKeys = limitAt(ownFirst) + 1;
     const int  parts    = (tileKeys + kKeys - 1) / kKeys;
@@ -214,21 +240,48 @@ __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(
     }
     const float   sum = BothSum(run.sum), factor = sum == 0 ? 0.f : 1.f / sum;
     const float   lse = LseOf<T>(run.top, sum);
-    const int64_t number = a.number(row);
-    if (a.splits == 1)
+    // 32 numbers of the results, from 32 * part on
+    auto store = [&](int part, const Acc16 &made, const AttentionRow &its)
     {
-        StoreColumn<T, DP>(run.out, factor, a.out + row.token * a.outToken + row.head * a.outHead, row.there, a.dims);
-        if (a.lse != nullptr && row.there && (threadIdx.x & 32) == 0)
+        if (a.splits == 1)
+        {
+            StoreColumnPart<T>(made, part, factor, a.out + its.token * a.outToken + its.head * a.outHead, its.there, a.dims);
+        }
+        else
+        {
+            const int64_t at = (int64_t)blockIdx.y * a.heads * a.sequences.rows + a.number(its);
+            StorePiecePart(made, part, factor, a.partial + at * a.dims, its.there, a.dims);
+        }
+    };
+    const AttentionRow its(a.rows, CAUSAL, s, keyHead, ownFirst + (int)(Again(threadIdx.x) & 31));
+    if (its.there && (threadIdx.x & 32) == 0)
+    {
+        const int64_t number = a.number(its);
+        if (a.splits > 1)
+        {
+            a.partialLse[(int64_t)blockIdx.y * a.heads * a.sequences.rows + number] = lse;
+        }
+        else if (a.lse != nullptr)
         {
             a.lse[number] = lse * kLn2;
         }
+    }
+    auto hidden = [&](int n) { return v + (max(seenKeys, 0) + n) * a.vToken; };
+    if (CAUSAL && AnyNotFinite(run.out) &&
+        RowsNotFinite<T>(a.dims, min((waveKeys + kKeys - 1) / kKeys * kKeys, s.keys) - max(seenKeys, 0), hidden))
+    {
+        const AttentionRow again(a.rows, CAUSAL, s, keyHead, ownFirst + (int)(Again(threadIdx.x) & 31));
+        LoadColumn<T, DP>(q, a.q + again.token * a.qToken + again.head * a.qHead, a.dims, Again(threadIdx.x));
+        for (int part = 0; part * 32 < a.dims; ++part)
+        {
+            store(part, SeenPart<T, DP>(a, q, k, v, from * kKeys, min(to * kKeys, waveKeys), 32, s.keys, again.limit, run.top, part), again);
+        }
         return;
     }
-    const int64_t at = (int64_t)blockIdx.y * a.heads * a.sequences.rows + number;
-    StorePiece<DP>(run.out, factor, a.partial + at * a.dims, row.there, a.dims);
-    if (row.there && (threadIdx.x & 32) == 0)
+#pragma unroll
+    for (int p = 0; p < DP / 32; ++p)
     {
-        a.partialLse[at] = lse;
+        store(p, run.out[p], its);
     }
 }
 
@@ -238,7 +291,7 @@ __global__ __launch_bounds__(kManyThreads, kManyWaves<DP>) void AttentionKernel(
 constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4, kFewThreads = 64 * kFewWaves;
 
 template<class T, int DP, bool PAST>
-__global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const AttentionArgs a)
+__global__ __launch_bounds__(kFewThreads, DP > 64 ? 2 : 4) void AttentionFewKernel(const AttentionArgs a)
 {
     // each wave's keys and values, later its weighted values in 32 bits
     __shared__ __attribute__((aligned(256))) uint8_t s_tile[kFewWaves][2 * kFewKeys * DP * 2];
@@ -298,13 +351,30 @@ __global__ __launch_bounds__(kFewThreads, 2) void AttentionFewKernel(const Atten
     const float sum = BothSum(run.sum);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     float *own = reinterpret_cast<float *>(s_tile[wave]); // [DP][32]
-#pragma unroll
-    for (int p = 0; p < DP / 32; ++p)
+    auto   put = [&](const Acc16 &made, int part)
     {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
         {
-            own[(32 * p + RowOf(i)) * kFewRows + (lane & 31)] = run.out[p][i];
+            own[(32 * part + RowOf(i)) * kFewRows + (lane & 31)] = made[i];
+        }
+    };
+    auto hidden = [&](int n) { return v + (max(seenKeys, 0) + n) * a.vToken; };
+    if (a.causal && AnyNotFinite(run.out) && RowsNotFinite<T>(a.dims, min(parts * kFewKeys, s.keys) - max(seenKeys, 0), hidden))
+    {
+        const AttentionRow again(a.rows, a.causal, s, keyHead, first + (int)(Again(threadIdx.x) & 31));
+        LoadColumn<T, DP>(q, a.q + again.token * a.qToken + again.head * a.qHead, a.dims, Again(threadIdx.x));
+        for (int part = 0; part * 32 < a.dims; ++part)
+        {
+            put(SeenPart<T, DP>(a, q, k, v, from * kFewKeys, to * kFewKeys, kFewWaves * kFewKeys, s.keys, again.limit, run.top, part), part);
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int p = 0; p < DP / 32; ++p)
+        {
+            put(run.out[p], p);
         }
     }
     if (lane < 32)
@@ -522,9 +592,13 @@ void Launch(const AttentionArgs &a, bool few, hipStream_t stream)
     {
         AttentionFewKernel<T, DP, false><<<grid, kFewThreads, 0, stream>>>(a);
     }
+    else if (a.causal)
+    {
+        AttentionKernel<T, DP, true><<<grid, kManyThreads, 0, stream>>>(a);
+    }
     else
     {
-        AttentionKernel<T, DP><<<grid, kManyThreads, 0, stream>>>(a);
+        AttentionKernel<T, DP, false><<<grid, kManyThreads, 0, stream>>>(a);
     }
     CheckLaunch("attention");
     if (a.splits > 1)

@@ -131,22 +131,22 @@ __device__ __forceinline__ int FirstRowOfTile(const AttentionGradArgs &a, const 
 // ---- the queries' gradient: 128 rows to a workgroup, 32 to a wave --------------------------------------------------------
 constexpr int kGradThreads = 256;
 
-template<class T, int DP>
+template<class T, int DP, bool CAUSAL>
 __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const AttentionGradArgs a)
 {
     __shared__ __attribute__((aligned(256))) uint8_t s_k0[kGradKeys * DP * 2], s_k1[kGradKeys * DP * 2];
     __shared__ __attribute__((aligned(256))) uint8_t s_v0[kGradKeys * DP * 2], s_v1[kGradKeys * DP * 2];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
     const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
-    const SequenceTile s       = FindTile(a.sequences, t, a.tiles, kGradRows, a.rows.size(), false, a.causal);
+    const SequenceTile s       = FindTile(a.sequences, t, a.tiles, kGradRows, a.rows.size(), false, CAUSAL);
     if (s.tile < 0)
     {
         return;
     }
     const uint32_t wave = WaveOfGroup();
     const int      first = s.tile * kGradRows, ownFirst = first + (int)wave * 32, all = s.rows * a.rows.size();
-    const AttentionRow row(a.rows, a.causal, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
-    auto               limitAt  = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
+    const AttentionRow row(a.rows, CAUSAL, s, keyHead, ownFirst + (int)(threadIdx.x & 31));
+    auto               limitAt  = [&](int r) { return LimitOf(CAUSAL, s, a.rows.token(min(r, all - 1))); };
     const int          tileKeys = KeysOfTile(a, s), waveKeys = ownFirst < all ? limitAt(ownFirst + 31) + 1 : 0;
     const int          seenKeys = limitAt(ownFirst) + 1, parts = (tileKeys + kGradKeys - 1) / kGradKeys;
     const int          pieces = PiecesOf(tileKeys, a.splits), piece = (int)blockIdx.y;
@@ -265,14 +265,48 @@ __global__ __launch_bounds__(kGradThreads, 2) void AttentionGradQKernel(const At
             take(part + 1, s_k1, s_v1, s_k0, s_v0);
         }
     }
-    if (a.splits == 1)
+    const AttentionRow its(a.rows, CAUSAL, s, keyHead, ownFirst + (int)(Again(threadIdx.x) & 31));
+    const float        factor = a.scale / grow.factor;
+    uint8_t           *result = a.gradQ + its.token * a.gradQToken + its.head * a.gradQHead;
+    float             *pieceOf = a.pieces + ((int64_t)piece * a.sequences.rows * a.heads + a.number(its)) * a.dims;
+    auto hidden = [&](int n) { return k + (max(seenKeys, 0) + n) * a.kToken; };
+    if (CAUSAL && AnyNotFinite(sum) &&
+        RowsNotFinite<T>(a.dims, min((waveKeys + kGradKeys - 1) / kGradKeys * kGradKeys, s.keys) - max(seenKeys, 0), hidden))
     {
-        StoreColumn<T, DP>(sum, a.scale / grow.factor, a.gradQ + row.token * a.gradQToken + row.head * a.gradQHead, row.there, a.dims);
+        // once more, without what the rows don't see (MultiplySeen)
+        const uint32_t thread = Again(threadIdx.x);
+        const int      lane   = (int)(thread & 63);
+        LoadColumn<T, DP>(q, a.q + its.token * a.qToken + its.head * a.qHead, a.dims, thread);
+        LoadColumn<T, DP>(grad, a.grad + its.token * a.gradToken + its.head * a.gradHead, a.dims, thread);
+        for (int part = 0; part * 32 < a.dims; ++part)
+        {
+            Acc16 made = {};
+            for (int key = from * kGradKeys; key < min(to * kGradKeys, waveKeys); key += 32)
+            {
+                const int own = min(key + (lane & 31), s.keys - 1);
+                Acc16     shares = {}, grads = {};
+                MultiplyRows<T, DP>(shares, k + own * a.kToken, a.dims, [&](int step) { return q[step]; });
+                MultiplyRows<T, DP>(grads, v + own * a.vToken, a.dims, [&](int step) { return grad[step]; });
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    const float share = __builtin_amdgcn_exp2f(__builtin_fmaf(shares[i], scale, -base));
+                    grads[i] = key + RowOf(i, lane) <= its.limit ? share * __builtin_fmaf(grads[i], of, -delta) : 0.f;
+                }
+                MultiplySeen<T>(made, grads, part, a.dims, s.keys - key, !__any(key + 31 > its.limit),
+                                [&](int n) { return k + (key + n) * a.kToken; }, [&](int n) { return key + n <= its.limit; });
+            }
+            a.splits == 1 ? StoreColumnPart<T>(made, part, factor, result, its.there, a.dims)
+                          : StorePiecePart(made, part, factor, pieceOf, its.there, a.dims);
+        }
+    }
+    else if (a.splits == 1)
+    {
+        StoreColumn<T, DP>(sum, factor, result, its.there, a.dims);
     }
     else
     {
-        const int64_t at = (int64_t)piece * a.sequences.rows * a.heads + a.number(row);
-        StorePiece<DP>(sum, a.scale / grow.factor, a.pieces + at * a.dims, row.there, a.dims);
+        StorePiece<DP>(sum, factor, pieceOf, its.there, a.dims);
     }
 }
 
@@ -294,7 +328,7 @@ struct RowsPlace
     float   *base, *delta;
 };
 
-template<class T, int DP>
+template<class T, int DP, bool CAUSAL>
 __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const AttentionGradArgs a)
 {
     constexpr int kWaves = kOfThreads<DP> / 64, kBytes = kOfRows * DP * 2;
@@ -304,7 +338,7 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
     __shared__ __attribute__((aligned(256))) uint8_t s_k[kInPairs<DP> ? kOfKeys * DP * 2 : 16], s_v[kInPairs<DP> ? kOfKeys * DP * 2 : 16];
     const uint32_t     t       = a.keyHeads.Quotient(blockIdx.x);
     const int          keyHead = (int)(blockIdx.x - t * a.keyHeads.d);
-    const SequenceTile s       = FindTile(a.sequences, t, a.keyTiles, kOfKeys, 1, true, a.causal);
+    const SequenceTile s       = FindTile(a.sequences, t, a.keyTiles, kOfKeys, 1, true, CAUSAL);
     if (s.tile < 0)
     {
         return;
@@ -321,7 +355,7 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
     {
         return;
     }
-    auto      limitAt = [&](int r) { return LimitOf(a.causal, s, a.rows.token(min(r, all - 1))); };
+    auto      limitAt = [&](int r) { return LimitOf(CAUSAL, s, a.rows.token(min(r, all - 1))); };
 
     Vec8<T> k[kInPairs<DP> ? 1 : DP / 16], v[kInPairs<DP> ? 1 : DP / 16];
     if constexpr (kInPairs<DP>)
@@ -426,15 +460,6 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
                     grads[i + n]  = -d[n];
                 }
             }
-            if (limitAt(from) < ownFirst + 31)
-            {
-                KeepBranch();
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                {
-                    shares[i] = key <= limitAt(from + RowOf(i)) ? shares[i] : 0.f;
-                }
-            }
 #pragma unroll
             for (int step = 0; step < DP / 16; ++step)
             {
@@ -444,6 +469,17 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
             for (int i = 0; i < 16; ++i)
             {
                 grads[i] = shares[i] * (std::is_same<T, Half>::value ? grads[i] * of : grads[i]);
+            }
+            if (limitAt(from) < ownFirst + 31)
+            {
+                KeepBranch();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    const bool takes = key <= limitAt(from + RowOf(i));
+                    shares[i] = takes ? shares[i] : 0.f;
+                    grads[i]  = takes ? grads[i] : 0.f;
+                }
             }
             grow.fit(grads,
                      [&](float less)
@@ -514,17 +550,81 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
             return;
         }
     }
-    const float ofValues = __builtin_amdgcn_exp2f(-kShareShift<T>);
-    if (a.keySplits == 1)
+    const float   ofValues = __builtin_amdgcn_exp2f(-kShareShift<T>);
+    const int     its      = ownFirst + (int)(Again(threadIdx.x) & 31), place = s.firstKey + its;
+    const bool    stored   = its < s.keys;
+    // 32 numbers of both gradients, from 32 * part on
+    auto store = [&](int part, const Acc16 &ofK, float factorK, const Acc16 &ofV)
     {
-        StoreColumn<T, DP>(sumK, 1.f, a.gradK + (s.firstKey + key) * a.gradKToken + keyHead * a.gradKHead, there, a.dims);
-        StoreColumn<T, DP>(sumV, ofValues, a.gradV + (s.firstKey + key) * a.gradVToken + keyHead * a.gradVHead, there, a.dims);
+        if (a.keySplits == 1)
+        {
+            StoreColumnPart<T>(ofK, part, factorK, a.gradK + place * a.gradKToken + keyHead * a.gradKHead, stored, a.dims);
+            StoreColumnPart<T>(ofV, part, ofValues, a.gradV + place * a.gradVToken + keyHead * a.gradVHead, stored, a.dims);
+        }
+        else
+        {
+            const int64_t keys = (int64_t)a.sequences.keys * a.keyHeads.d, at = piece * keys + (int64_t)place * a.keyHeads.d + keyHead;
+            StorePiecePart(ofK, part, factorK, a.pieces + at * a.dims, stored, a.dims);
+            StorePiecePart(ofV, part, ofValues, a.pieces + (a.keySplits * keys + at) * a.dims, stored, a.dims);
+        }
+    };
+    const int lane  = (int)(Again(threadIdx.x) & 63);
+    auto      rowAt = [&](int row, int64_t tokenStride, int64_t headStride)
+    {
+        const int i = a.rows.token(row);
+        return (int64_t)(s.firstRow + i) * tokenStride + (int64_t)(keyHead * group + row - i * group) * headStride;
+    };
+    auto queryAt = [&](int row) { return a.q + rowAt(row, a.qToken, a.qHead); };
+    auto gradAt  = [&](int row) { return a.grad + rowAt(row, a.gradToken, a.gradHead); };
+    // whether rows that don't see all of the wave's keys hold something that isn't finite
+    auto hidden = [&]()
+    {
+        const int end   = min(min(last + kOfRows, all), max(min(ownFirst + 31 - (s.keys - s.rows), s.rows), 0) * group);
+        const int count = end - begin;
+        return RowsNotFinite<T>(a.dims, count, [&](int n) { return queryAt(begin + n); }) ||
+               RowsNotFinite<T>(a.dims, count, [&](int n) { return gradAt(begin + n); });
+    };
+    if (CAUSAL && (AnyNotFinite(sumK) || AnyNotFinite(sumV)) && hidden())
+    {
+        // once more, of all rows here, without those that don't see a key (MultiplySeen)
+        for (int part = 0; part * 32 < a.dims; ++part)
+        {
+            GradScale<T> grow;
+            float        of = grow.factor * __builtin_amdgcn_exp2f(-kShareShift<T>);
+            Acc16        madeK = {}, madeV = {};
+            for (int from = begin; from < min(last + kOfRows, all); from += 32)
+            {
+                if (limitAt(from + 31) < ownFirst)
+                {
+                    continue;
+                }
+                const int own = min(from + (lane & 31), all - 1);
+                Acc16     shares = {}, grads = {};
+                MultiplyRows<T, DP>(shares, queryAt(own), a.dims, keyOperand);
+                MultiplyRows<T, DP>(grads, gradAt(own), a.dims, valueOperand);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    const int     row = from + RowOf(i, lane);
+                    const int64_t number = rowAt(min(row, all - 1), a.heads, 1);
+                    const bool    takes = row < all && its <= limitAt(row);
+                    shares[i] = takes ? __builtin_amdgcn_exp2f(__builtin_fmaf(shares[i], scale, -a.base[number])) : 0.f;
+                    grads[i]  = takes ? shares[i] * ((grads[i] - a.delta[number]) * of) : 0.f;
+                }
+                grow.fit(grads, [&](float less) { of *= less, madeK *= less; });
+                auto seen = [&](int n) { return its <= limitAt(from + n); };
+                const bool every = limitAt(from) >= ownFirst + 31;
+                MultiplySeen<T>(madeV, shares, part, a.dims, all - from, every, [&](int n) { return gradAt(from + n); }, seen);
+                MultiplySeen<T>(madeK, grads, part, a.dims, all - from, every, [&](int n) { return queryAt(from + n); }, seen);
+            }
+            store(part, madeK, a.scale / grow.factor, madeV);
+        }
+        return;
     }
-    else
+#pragma unroll
+    for (int p = 0; p < DP / 32; ++p)
     {
-        const int64_t keys = (int64_t)a.sequences.keys * a.keyHeads.d, at = piece * keys + (int64_t)(s.firstKey + key) * a.keyHeads.d + keyHead;
-        StorePiece<DP>(sumK, 1.f, a.pieces + at * a.dims, there, a.dims);
-        StorePiece<DP>(sumV, ofValues, a.pieces + (a.keySplits * keys + at) * a.dims, there, a.dims);
+        store(p, sumK[p], 1.f, sumV[p]);
     }
 }
 
@@ -629,7 +729,15 @@ void Launch(const AttentionGradArgs &a, hipStream_t stream)
 {
     if (a.tiles > 0)
     {
-        AttentionGradQKernel<T, DP><<<dim3(a.tiles * a.keyHeads.d, (uint32_t)a.splits), kGradThreads, 0, stream>>>(a);
+        const dim3 grid(a.tiles * a.keyHeads.d, (uint32_t)a.splits);
+        if (a.causal)
+        {
+            AttentionGradQKernel<T, DP, true><<<grid, kGradThreads, 0, stream>>>(a);
+        }
+        else
+        {
+            AttentionGradQKernel<T, DP, false><<<grid, kGradThreads, 0, stream>>>(a);
+        }
         CheckLaunch("attention's gradient (queries)");
         if (a.splits > 1)
         {
@@ -639,7 +747,15 @@ void Launch(const AttentionGradArgs &a, hipStream_t stream)
     }
     if (a.keyTiles > 0)
     {
-        AttentionGradKVKernel<T, DP><<<dim3(a.keyTiles * a.keyHeads.d, (uint32_t)a.keySplits), kOfThreads<DP>, 0, stream>>>(a);
+        const dim3 grid(a.keyTiles * a.keyHeads.d, (uint32_t)a.keySplits);
+        if (a.causal)
+        {
+            AttentionGradKVKernel<T, DP, true><<<grid, kOfThreads<DP>, 0, stream>>>(a);
+        }
+        else
+        {
+            AttentionGradKVKernel<T, DP, false><<<grid, kOfThreads<DP>, 0, stream>>>(a);
+        }
         CheckLaunch("attention's gradient (keys)");
         if (a.keySplits > 1)
         {

@@ -13,8 +13,8 @@
  * Every result is the same in every call.
  *
  * Rows of no sequence, and keys' places that none of them has, are left as they are in out, lse, gradQ, gradK and gradV, and not read
- * elsewhere. Values that are not finite reach the rows that see them, and in a sequence that has such a value in k, v or gradOut its other
- * rows and keys too. Offsets are read on the device: those below 0 or beyond the tensors count as the border, a sequence whose
+ * elsewhere. Values that are not finite reach the rows that see them, and in the gradient the rows and keys that these are summed over; no
+ * others. (Such calls take longer.) Offsets are read on the device: those below 0 or beyond the tensors count as the border, a sequence whose
  * end lies before its begin as empty.
  *
  * q, out, gradOut, gradQ  : [Tq, Hq, D]; k, v, gradK, gradV: [Tk, Hk, D]; F16 or BF16 (NVCVX_DATA_TYPE_BF16), one type for all. Hk
