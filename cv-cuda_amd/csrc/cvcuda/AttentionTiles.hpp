@@ -20,10 +20,13 @@ namespace cvamd {
 
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Exponentials are kept in F16 times a power of two: a share of 2^-20 of the largest keeps all of its bits, one of 2^-30 one bit.
-// (BF16 has the exponents of F32.)
+// How far scores, to the base 2, may lie above what exponentials are taken relative to.
+constexpr float kSlack = 8.f;
+
+// Exponentials are kept in F16 times a power of two: a share of 2^-20 of the largest keeps all of its bits, one of 2^-30 one bit, and the largest reaches
+// 2^14. BF16 has the exponents of F32: there none is above 1, so that its products with values stay as finite as these.
 template<class T>
-constexpr float kExpShift = std::is_same<T, Half>::value ? 6.f : 0.f;
+constexpr float kExpShift = std::is_same<T, Half>::value ? 6.f : -kSlack;
 
 template<class T>
 using Vec8 = T __attribute__((ext_vector_type(8)));

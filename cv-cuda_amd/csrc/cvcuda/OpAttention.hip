@@ -40,9 +40,6 @@ struct AttentionArgs
     }
 };
 
-// How far scores, to the base 2, may lie above what exponentials are taken relative to: F16 reaches 2^16, from 2^kExpShift on.
-constexpr float kSlack = 8.f;
-
 // A lane's row on its way through the keys: a score to the base 2, near the largest so far, that exponentials are taken relative to, the sum of its
 // own keys' exponentials (the other half wave has the other keys') and the weighted values.
 template<class T, int DP>

@@ -64,3 +64,18 @@ def test_small_gradients_beside_large_ones_in_f16(api):
             assert torch.equal(got[0][rows], small[0][rows]) and (got[0][rows] != 0).any()
         for a, b in zip(got[1:], small[1:]):
             assert torch.equal(a[last], b[last]) and (a[last] != 0).any()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_large_values_behind_growing_scores(api, rows):
+    """Values of 1e37 at a key whose score lies above those of the keys before it, by less than makes the sums' reference follow."""
+    for d in (64, 128):
+        call = Call([(rows, 200)], 2, 2, d, BF16, 31, causal=False, room=200, scale=1.0)
+        call.q.zero_(), call.k.zero_()
+        call.q[..., 0] = 1
+        call.k[:, :, 0] = torch.arange(200, device="cuda").div(50, rounding_mode="floor").mul(1.7).to(BF16)[:, None]
+        for key in (49, 99, 120, 199):
+            v = call.v.clone()
+            call.v[key] = 1e37
+            assert call.check(api)[0].abs().max() > 5e32  # (shares are e^-5.1 / 62 = 1e-4 at least)
+            call.v = v
