@@ -6,7 +6,8 @@
 
 namespace cvamd {
 
-// [T, H, D]: the row of a token's head begins at base + token * tokenStride + head * headStride bytes.
+// [T, H, D]: the row of a token's head begins at base + token * tokenStride + head * headStride bytes. A token lies behind all heads of the one before,
+// as the library's tensors have no smaller pitch than what lies within it (nvcvTensorWrapDataConstruct).
 struct HeadsView
 {
     uint8_t *base;

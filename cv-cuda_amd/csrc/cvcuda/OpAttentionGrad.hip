@@ -393,7 +393,8 @@ __global__ __launch_bounds__(kOfThreads<DP>, 2) void AttentionGradKVKernel(const
         const int r = (int)(threadIdx.x & 63), i = a.rows.token(at + r);
         placeValue  = ((uint32_t)(i - i0) * (uint32_t)a.heads + (uint32_t)(at + r - i * group)) * 4;
     };
-    // Rows from `at` on to LDS. Their buffers end with the sequence: rows behind it are zeros, which add nothing to any sum.
+    // Rows from `at` on to LDS. Their buffers end with the sequence: rows behind it are zeros, which add nothing to any sum. (A token lies behind all
+    // heads of the one before, or rows of the next sequence would stand there: tensors are wrapped in no other order, RequireHeads.)
     auto load = [&](int at, const RowsPlace<DP> &to)
     {
         using Place = __attribute__((address_space(3))) void;

@@ -18,9 +18,9 @@
  * end lies before its begin as empty.
  *
  * q, out, gradOut, gradQ  : [Tq, Hq, D]; k, v, gradK, gradV: [Tk, Hk, D]; F16 or BF16 (NVCVX_DATA_TYPE_BF16), one type for all. Hk
- *                           divides Hq. D: a multiple of 8, at most 128. A row's elements follow one another; tokens
- *                           and heads lie at any distances of whole 16 bytes, aligned to 16 bytes (such as parts of one projection's
- *                           result), a token's heads within 2^24 bytes, and the next token as well.
+ *                           divides Hq. D: a multiple of 8, at most 128. A row's elements follow one another; heads, and
+ *                           tokens, lie at distances of whole 16 bytes, aligned to 16 bytes, each token behind all heads of the one before (such
+ *                           as parts of one projection's result), within 2^24 bytes of it.
  *                           Outputs must not overlap inputs nor each other.
  * offsets, keyOffsets     : S32, dense, B + 1 elements each, ascending; keyLengths: S32, B elements, only beside keyOffsets.
  * lse                     : F32, [Hq, Tq], dense. NULL if not wanted; an input of the gradient.

@@ -15,7 +15,7 @@
  * position below 2^31; results are computed in float32 and rounded once.
  *
  * in, out   : [T, H, D], F32, F16 or BF16 (NVCVX_DATA_TYPE_BF16), of one type and shape; a row's elements follow one another, tokens
- *             and heads may have gaps. out may be in, or must not overlap it.
+ *             and heads may have gaps, each token lies behind all heads of the one before. out may be in, or must not overlap it.
  * positions : S32 or S64, dense, T elements, any numbers.
  * dims      : even, 2 to 256, at most D. base, factor, magnitude: finite and positive. original >= 0; with it 0 <= low < high.
  * T * H below 2^31, D at most 2^20; tensors may be larger than 2^32 bytes.
