@@ -11,8 +11,8 @@
  * a and b being elements 2 i and 2 i + 1 (`interleaved`) or i and i + dims / 2. Elements from `dims` on are copied. `inverse` takes -s
  * for s: the gradient of in from that of out.
  *
- * An angle's whole turns are taken off in 64-bit arithmetic before the sine and cosine, which have errors of some 2^-24 at any
- * position below 2^31; results are computed in float32 and rounded once.
+ * An angle's whole turns are taken off in 64-bit arithmetic before the sine and cosine, which have errors of some 2^-24, and of up to
+ * position * 2^-52 for the 64 bits of a frequency (2^-24 at 2^28, 2^-21 at 2^31); results are computed in float32 and rounded once.
  *
  * in, out   : [T, H, D], F32, F16 or BF16 (NVCVX_DATA_TYPE_BF16), of one type and shape; a row's elements follow one another, tokens
  *             and heads may have gaps, each token lies behind all heads of the one before. out may be in, or must not overlap it.
