@@ -26,7 +26,7 @@ namespace {
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2   = 0.6931471805599453f;
 constexpr float kFar   = -1e30f; // below any difference whose exponential isn't 0; a sum of 2^31 of it is finite
-constexpr float kSlack = 2.f; // (4096 rows of 128000 BF16 189.5 us, with 20 187.7, and 1 - p of likely tokens known to 5e-6 only)
+constexpr float kSlack = 2.f; // (4096 rows of 128000 BF16 189.5 us; with 20 187.7, and what is within that of a likely token's logit lies in its digits)
 
 __device__ __forceinline__ float Exp(float x)
 {
@@ -120,15 +120,15 @@ __device__ __forceinline__ uint64_t LargestKey(uint64_t v, uint64_t (&part)[WAVE
     return v;
 }
 
-// What the row's log probabilities are taken relative to: that of x is scale * (x - at) - logSum.
+// What the row's log probabilities are taken relative to: that of x is scale * x - scale * at - logSum.
 struct Total
 {
-    float scale, at, logSum;
-    bool  nothing; // all logits are -infinity
+    float scale, base, rounding, logSum; // base: scale * at, rounded; rounding: what it is short of that
+    bool  nothing;                       // all logits are -infinity
 
     __device__ __forceinline__ float of(float x) const
     {
-        return nothing ? -INFINITY : (x - at) * scale - logSum;
+        return nothing ? -INFINITY : (__builtin_fmaf(x, scale, -base) - rounding) - logSum;
     }
 };
 
@@ -383,8 +383,9 @@ __global__ __launch_bounds__(64 * WAVES) void LogProbsKernel(const LogProbsArgs 
     Total total;
     auto  join = [&]()
     {
-        const Sums all = WAVES > 1 ? Joined(sums, a.scale) : sums;
-        total          = {a.scale, all.at, Log1(all.r), all.at == -INFINITY && all.r == 0};
+        const Sums  all  = WAVES > 1 ? Joined(sums, a.scale) : sums;
+        const float base = all.at * a.scale;
+        total            = {a.scale, base, __builtin_fmaf(all.at, a.scale, -base), Log1(all.r), all.at == -INFINITY && all.r == 0};
         return all;
     };
     if (threadIdx.x < 64)

@@ -135,3 +135,14 @@ def test_near_certain_tokens_keep_their_digits(api):
     out = check(api, x, tokens, 1.0)
     rest = (v - 1) * torch.exp(-peaks.double())
     assert ((out.double() + torch.log1p(rest)).abs() <= 2e-3 * torch.log1p(rest)).all() and (out < 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logits_at_both_ends_of_the_type(api, dtype):
+    """Of logits that lie further apart than the type reaches, scaled down: log probabilities are finite."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = torch.full((3, 1000), low, device="cuda").to(dtype)
+    x[0, 5], x[1, 900], x[2, 0] = high, high, 1.0
+    tokens = torch.tensor([7, 900, 999], device="cuda")
+    out = check(api, x, tokens, 0.25, 3)
+    assert out.isfinite().all() and out[0] < -1e38 and out[1] == 0
