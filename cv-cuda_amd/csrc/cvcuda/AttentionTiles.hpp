@@ -109,7 +109,10 @@ __device__ __forceinline__ Vec8<T> ColumnsOperand(const uint8_t *tile, uint32_t 
     return __builtin_bit_cast(Vec8<T>, both);
 }
 
-// Eight of a lane's 16 numbers, rounded: rows 16 * half to + 15 of a product as the next one's right operand.
+// Eight of a lane's 16 numbers, rounded: rows 16 * half to + 15 of a product as the next one's right operand. (Rounded, since a matrix instruction takes
+// both operands in the 16 bits of the values or keys: each is off by half a step at most, and the sum by that of the magnitudes that are added, where
+// the result's own rounding is half a step of it. Measured over a call, 0.0021 of BF16 results, of which 0.0016 are their rounding. A second
+// product, for what the rounding took off, would take as long as the first.)
 template<class T>
 __device__ __forceinline__ Vec8<T> RoundedHalf(const Acc16 &v, int half)
 {

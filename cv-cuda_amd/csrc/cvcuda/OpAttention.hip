@@ -4,7 +4,7 @@
 // rows that a key head serves (all heads of its group, token by token) are one matrix, so that its keys and values are read once for
 // them, whatever the group.
 //
-// Measured: long prompts (8 sequences of up to 4096 tokens, 32 heads on 8 key heads of 128 BF16 elements, causal) 276 us, 953 TFLOP/s, where a
+// Measured: long prompts (8 sequences of up to 4096 tokens, 32 heads on 8 key heads of 128 BF16 elements, causal) 272 us, 967 TFLOP/s, where a
 // product of two 8192 x 8192 matrices by the library has 1253: exponentials take as long as the products, and overlap those of other waves
 // only. Single tokens (16 before caches of up to 8192, the same heads: 362 MB) 70 us, of them 65 of reading at 5.6 TB/s.
 #include "AttentionTiles.hpp"

@@ -5,9 +5,9 @@
 // twice (seven products of a pair where five would do), but every sum stays in the registers of one wave and is made in one
 // order: there is nothing to add up by atomics in memory, and no gradient in 32 bits to write and read.
 //
-// Measured: long sequences (8 of up to 2048 tokens, 32 heads on 8 key heads of 128 BF16 elements, causal) 610 us, seven products at 0.67 of the
+// Measured: long sequences (8 of up to 2048 tokens, 32 heads on 8 key heads of 128 BF16 elements, causal) 612 us, seven products at 0.67 of the
 // 1253 TFLOP/s of a library's product of two 8192 x 8192 matrices: what bounds it are the phases of products, exponentials and reads of LDS between
-// two barriers. Short ones (64 of up to 273 tokens, 12 heads of 64 F16 elements, not causal) 71 us, waits of workgroups of four or five tiles.
+// two barriers. Short ones (64 of up to 273 tokens, 12 heads of 64 F16 elements, not causal) 69.7 us, waits of workgroups of four or five tiles.
 #include "AttentionTiles.hpp"
 
 #include <cvcuda/Attention.h>
