@@ -33,10 +33,14 @@ CALLS = {  # lengths, heads, key heads, elements, room
     "pieces": ([(6, 4000)], 4, 4, 128, 4096),
     "many pieces": ([(200, 3001)], 2, 1, 64, 3001),
 }
+LONG = {  # rows in pieces, for the gradient alone
+    "rows in pieces": ([(1200, 1200)], 2, 1, 64, None),
+    "wide rows in pieces": ([(700, 900), (40, 60)], 3, 1, 128, 900),
+}
 
 
 def made(name, dtype, seed=0):
-    lengths, heads, key_heads, d, room = CALLS[name]
+    lengths, heads, key_heads, d, room = {**CALLS, **LONG}[name]
     return Call(lengths, heads, key_heads, d, dtype, 21 + seed, room=room)
 
 
@@ -118,7 +122,7 @@ def gradients(call, out, lse):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("name", list(CALLS))
+@pytest.mark.parametrize("name", list(CALLS) + list(LONG))
 @pytest.mark.parametrize("into", ["q", "k", "v", "grad"])
 def test_gradients_beside_what_is_not_finite(api, name, into, dtype):
     """With one row, or one key, of each sequence not finite in one input."""
@@ -153,3 +157,31 @@ def test_gradients_beside_what_is_not_finite(api, name, into, dtype):
             assert (a[~kept] == 7).all()
             if math.isnan(value):
                 assert a[met].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("name", list(CALLS))
+@pytest.mark.parametrize("into", ["out", "lse"])
+def test_gradients_of_results_that_are_not_finite(api, name, into, dtype):
+    """A row's result, or its lse, is NaN: its gradient, and those of the keys that it sees, and no others."""
+    call = made(name, dtype, 3)
+    out, lse = call.check(api)
+    want, errors = gradients(call, out, lse)
+    rows_met = torch.zeros(call.rows, dtype=torch.bool, device="cuda")
+    keys_met = torch.zeros(call.keys, dtype=torch.bool, device="cuda")
+    for rows, keys in call.parts():
+        n, m = rows.stop - rows.start, keys.stop - keys.start
+        row = n // 2
+        rows_met[rows.start + row] = True
+        keys_met[keys.start:keys.start + m - n + row + 1] = True
+    if into == "out":
+        out = torch.where(rows_met[:, None, None], torch.full_like(out, NAN), out)
+    else:
+        lse = torch.where(rows_met, torch.full_like(lse, NAN), lse)
+    values_met = keys_met if into == "lse" else torch.zeros_like(keys_met)
+    got = call.gradients(api, out, lse)
+    for what, a, b, e, kept, met in zip(("gradient of q", "of k", "of v"), got, want, errors, (call.kept_q, call.kept_k, call.kept_k),
+                                        (rows_met, keys_met, values_met)):
+        fine = kept & ~met
+        close(a[fine], b[fine], e[fine], what)
+        assert a[met].isnan().all()
