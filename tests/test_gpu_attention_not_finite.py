@@ -185,3 +185,17 @@ def test_gradients_of_results_that_are_not_finite(api, name, into, dtype):
         fine = kept & ~met
         close(a[fine], b[fine], e[fine], what)
         assert a[met].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_other_sequences_to_the_last_bit(api, causal, dtype):
+    call = Call([(40, 40), (50, 50), (60, 60)], 4, 2, 64, dtype, 41, causal)
+    clean, clean_lse = call.run(api)
+    grads = call.gradients(api, clean, clean_lse)
+    call.k[45], call.v[60], call.grad[50], call.q[70] = NAN, INF, NAN, -INF
+    out, lse = call.run(api)
+    got = call.gradients(api, out, lse)
+    for rows in (slice(0, 40), slice(90, 150)):
+        assert torch.equal(out[rows], clean[rows]) and torch.equal(lse[:, rows], clean_lse[:, rows])
+        assert all(torch.equal(a[rows], b[rows]) for a, b in zip(got, grads))
